@@ -26,6 +26,9 @@
  *   nsfps_gather_points, nsfps_ball_query (and _device)
  *                        no counterpart: the grouping step the reference's
  *                        callers run on its output (see their declarations)
+ *   nsfps_embed_*, nsfps_conv_*, nsfps_scan_*
+ *                        no counterpart: sequence operators over the samples
+ *                        (see "Sequence operators")
  *   nsfps_fps_device_noalloc
  *                        no counterpart: nsfps_fps_device for callers that
  *                        cannot allocate device memory (see its declaration)
@@ -50,7 +53,8 @@ typedef enum {
                             needing more than 4096 level-1 nodes when the tree
                             engine is asked for (NSFPS_ENGINE=tree; the default
                             engine has no such limit), or a layout beyond the
-                            allocation-free entry point's array */
+                            allocation-free entry point's array, or a sequence
+                            operator's size beyond its limits */
 } nsfps_status;
 
 /* The nine primary SpaceRange fields (src/yuezu_fps.h:56-60).  Derived fields
@@ -268,6 +272,167 @@ nsfps_status nsfps_ball_query(const float *xyz, uint64_t n, const float *centers
 nsfps_status nsfps_ball_query_device(const float *d_xyz, uint64_t n, const float *d_centers,
                                      uint64_t m, float radius, uint32_t nsample, int32_t *d_out,
                                      void *stream);
+
+/* ------------------------------------------------------------------------
+ * Sequence operators: what follows sampling in a model that reads a cloud's
+ * samples as tokens.  The samples in the order of their grid cells are a
+ * sequence; a sample's cell is its token (a vocabulary of total_blocks rows);
+ * a selective state space scan with its short causal convolution mixes the
+ * sequence.  No counterpart in the reference, which stops at the indices.
+ *
+ * All pointers are device pointers of the current device (d_..., and the p
+ * of nsfps_rows); the argument structs live in host memory and are read
+ * during the call only.  The calls only enqueue kernels on the stream (a
+ * hipStream_t, NULL = default stream): they do not wait, allocate or copy, so
+ * they can be captured into a HIP graph, and calls on several streams run
+ * side by side.  Work that the kernels need beside their outputs is the
+ * caller's: a call with a _workspace_bytes companion needs that many bytes
+ * at workspace (aligned to 256), whose contents need not be kept, and which
+ * calls that may overlap must not share.  A workspace that is too small, a
+ * size or stride that does not fit and a null pointer are NSFPS_EINVAL;
+ * sizes beyond the limits named below are NSFPS_EUNSUPPORTED.  Nothing is
+ * enqueued by a refused call.
+ *
+ * Types: NSFPS_F32 and NSFPS_BF16 for inputs and outputs; sums, states and
+ * the gradients of parameters are float32 with both.  Results do not depend
+ * on the order in which workgroups run: the same call gives the same bits. */
+typedef enum { NSFPS_F32 = 0, NSFPS_BF16 = 1 } nsfps_dtype;
+
+/* A tensor of batch x length rows: row t of sequence b starts at
+ * p + (b * batch_stride + t * row_stride) elements.  A row's elements are
+ * contiguous.  Any strides that keep rows apart will do; the widest loads
+ * need rows aligned to 16 bytes. */
+typedef struct {
+  void *p;
+  uint64_t batch_stride, row_stride;
+} nsfps_rows;
+
+/* Embedding lookup: out[i] = scale * table[tokens[i]], tokens x width; a
+ * token outside [0, rows) gives a row of zeros (the -1 that pads a batch's
+ * index rows, say).
+ *
+ * Its gradient (d_out is then the input and d_table the output): every row v
+ * of d_table is written, scale times the sum of the rows of d_out whose
+ * token is v, zeros where no token is.  The tokens are sorted, and each
+ * row's terms are added in float32 in an order that the tokens alone decide.
+ * d_out has type dtype, d_table grad_dtype.  At most 2^31 - 1 tokens and
+ * rows (both calls), width at most 65,536. */
+typedef struct {
+  uint64_t tokens, rows;
+  uint32_t width;
+  uint32_t dtype;      /* lookup: table and out; gradient: out */
+  uint32_t grad_dtype; /* gradient: table */
+  float scale;
+  uint64_t table_stride, out_stride; /* elements from row to row, >= width */
+  void *d_table;
+  const int32_t *d_tokens;
+  void *d_out;
+  void *workspace; /* gradient only */
+  uint64_t workspace_bytes;
+} nsfps_embed_args;
+nsfps_status nsfps_embed_device(const nsfps_embed_args *args, void *stream);
+nsfps_status nsfps_embed_grad_workspace_bytes(const nsfps_embed_args *args, uint64_t *bytes);
+nsfps_status nsfps_embed_grad_device(const nsfps_embed_args *args, void *stream);
+
+/* Ragged batches and caches, for the convolution and the scan alike:
+ *   d_lengths    tokens of each sequence, at most length (NULL: all length);
+ *                more count as length, fewer than 0 as 0.  Input rows past
+ *                them are not read, output rows past them are zeros.
+ *   d_positions  tokens that each sequence has had before this call (NULL:
+ *                none).  0 starts it anew, whatever its caches hold; above 0
+ *                continues from them.
+ *   d_slots      each sequence's place in the caches (NULL: b); a negative
+ *                one has none: it starts anew and leaves nothing.  No two
+ *                sequences of a call may have the same place.
+ * Convolution cache: [slots][width][channels] of type dtype; the input of
+ * the token at position t is entry t modulo width.  Scan cache: [slots]
+ * [heads][head_dim][state_dim] float32, the state after the last token. */
+
+/* Short causal convolution over time with SiLU, each channel on its own:
+ * y[t] = silu(bias + sum over k < width of weight[k] * x[t - (width-1) + k]).
+ * width 2 to 4, weight [channels][width], bias [channels] (or NULL) of type
+ * dtype.  d_cache (or NULL) is read where positions are above 0 and receives
+ * the last inputs.  batch * length at most 2^31 - 1, channels at most 2^24.
+ * x and y must not overlap.
+ *
+ * The gradient starts every sequence anew (d_positions, d_slots, d_cache
+ * must be NULL; y is not read): dx of type dtype, d_dweight [channels][width]
+ * and d_dbias [channels] (or NULL) in float32, all written. */
+typedef struct {
+  uint64_t batch, length;
+  uint32_t channels, width, dtype;
+  nsfps_rows x, y;
+  const void *d_weight, *d_bias;
+  const int32_t *d_lengths, *d_positions, *d_slots;
+  void *d_cache;
+  void *workspace; /* gradient only */
+  uint64_t workspace_bytes;
+} nsfps_conv_args;
+typedef struct {
+  nsfps_rows dy, dx;
+  float *d_dweight, *d_dbias;
+} nsfps_conv_grads;
+nsfps_status nsfps_conv_device(const nsfps_conv_args *args, void *stream);
+nsfps_status nsfps_conv_grad_workspace_bytes(const nsfps_conv_args *args, uint64_t *bytes);
+nsfps_status nsfps_conv_grad_device(const nsfps_conv_args *args, const nsfps_conv_grads *grads,
+                                    void *stream);
+
+/* Selective state space scan.  Per head, with step = softplus(dt + dt_bias):
+ *   state = exp(step * a) * state + step * x b^T   (head_dim x state_dim)
+ *   y     = state c + d * x
+ * x and y: rows of heads * head_dim; b and c: rows of groups * state_dim
+ * (group g serves heads g * heads / groups onwards); dt: rows of heads; all
+ * of type dtype; a, d and dt_bias: [heads] float32 (d and dt_bias may be
+ * NULL).  a is not positive: exp(step * a) is a decay.  A dt of -infinity is
+ * a step of 0: the token leaves the state as it is.  Non-finite inputs
+ * elsewhere spoil their sequence, and no other.  d_state (or NULL) is the
+ * scan cache.  groups divides heads; head_dim and state_dim at most 128;
+ * batch * heads at most 2^20; batch * length at most 2^31 - 1.
+ *
+ * The gradient starts every sequence anew (d_positions, d_slots and d_state
+ * must be NULL; y is not read) and takes no gradient of the last state.  All
+ * of dx, db, dc, ddt (type dtype) and d_da, d_dd, d_ddt_bias ([heads] float32;
+ * the last two may be NULL) are written. */
+typedef struct {
+  uint64_t batch, length;
+  uint32_t heads, groups, head_dim, state_dim, dtype;
+  nsfps_rows x, b, c, dt, y;
+  const float *d_a, *d_d, *d_dt_bias;
+  const int32_t *d_lengths, *d_positions, *d_slots;
+  float *d_state;
+  void *workspace;
+  uint64_t workspace_bytes;
+} nsfps_scan_args;
+typedef struct {
+  nsfps_rows dy, dx, db, dc, ddt;
+  float *d_da, *d_dd, *d_ddt_bias;
+} nsfps_scan_grads;
+nsfps_status nsfps_scan_workspace_bytes(const nsfps_scan_args *args, uint64_t *bytes);
+nsfps_status nsfps_scan_device(const nsfps_scan_args *args, void *stream);
+nsfps_status nsfps_scan_grad_workspace_bytes(const nsfps_scan_args *args, uint64_t *bytes);
+nsfps_status nsfps_scan_grad_device(const nsfps_scan_args *args, const nsfps_scan_grads *grads,
+                                    void *stream);
+
+/* One token of every request, convolution and scan in one launch over the
+ * caches that both leave: xbc (rows of heads * head_dim + 2 * groups *
+ * state_dim channels: x, b, c) goes through the convolution, and x, b, c of
+ * its result with dt through one step of the scan.  Between the two nothing
+ * is rounded.  d_positions (required): tokens that each request has had; the
+ * caller adds one after the call.  d_slots as above (NULL: b); a request
+ * whose slot is negative gets a row of zeros and touches no cache.  width 2
+ * to 4; head_dim and state_dim at most 128. */
+typedef struct {
+  uint64_t batch;
+  uint32_t heads, groups, head_dim, state_dim, width, dtype;
+  uint64_t xbc_stride, dt_stride, y_stride; /* elements from request to request */
+  const void *d_xbc, *d_weight, *d_bias, *d_dt;
+  const float *d_a, *d_d, *d_dt_bias;
+  const int32_t *d_positions, *d_slots;
+  void *d_cache;
+  float *d_state;
+  void *d_y;
+} nsfps_step_args;
+nsfps_status nsfps_scan_step_device(const nsfps_step_args *args, void *stream);
 
 /* Measurements of the last compute call made on this thread. */
 nsfps_status nsfps_get_stats(nsfps_stats *stats);

@@ -49,6 +49,73 @@ class Stats(ctypes.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_}
 
 
+# nsfps_dtype: the types of the sequence operators' tensors
+F32, BF16 = 0, 1
+
+
+class Rows(ctypes.Structure):
+    """nsfps_rows: (pointer, elements from sequence to sequence, from row to row)."""
+    _fields_ = [("p", ctypes.c_void_p), ("batch_stride", ctypes.c_uint64),
+                ("row_stride", ctypes.c_uint64)]
+
+
+class EmbedArgs(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_uint64), ("rows", ctypes.c_uint64),
+                ("width", ctypes.c_uint32), ("dtype", ctypes.c_uint32),
+                ("grad_dtype", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("table_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64),
+                ("d_table", ctypes.c_void_p), ("d_tokens", ctypes.c_void_p),
+                ("d_out", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class ConvArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("length", ctypes.c_uint64),
+                ("channels", ctypes.c_uint32), ("width", ctypes.c_uint32),
+                ("dtype", ctypes.c_uint32), ("x", Rows), ("y", Rows),
+                ("d_weight", ctypes.c_void_p), ("d_bias", ctypes.c_void_p),
+                ("d_lengths", ctypes.c_void_p), ("d_positions", ctypes.c_void_p),
+                ("d_slots", ctypes.c_void_p), ("d_cache", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class ConvGrads(ctypes.Structure):
+    _fields_ = [("dy", Rows), ("dx", Rows), ("d_dweight", ctypes.c_void_p),
+                ("d_dbias", ctypes.c_void_p)]
+
+
+class ScanArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("length", ctypes.c_uint64),
+                ("heads", ctypes.c_uint32), ("groups", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("state_dim", ctypes.c_uint32),
+                ("dtype", ctypes.c_uint32), ("x", Rows), ("b", Rows), ("c", Rows), ("dt", Rows),
+                ("y", Rows), ("d_a", ctypes.c_void_p), ("d_d", ctypes.c_void_p),
+                ("d_dt_bias", ctypes.c_void_p), ("d_lengths", ctypes.c_void_p),
+                ("d_positions", ctypes.c_void_p), ("d_slots", ctypes.c_void_p),
+                ("d_state", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class ScanGrads(ctypes.Structure):
+    _fields_ = [("dy", Rows), ("dx", Rows), ("db", Rows), ("dc", Rows), ("ddt", Rows),
+                ("d_da", ctypes.c_void_p), ("d_dd", ctypes.c_void_p),
+                ("d_ddt_bias", ctypes.c_void_p)]
+
+
+class StepArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("heads", ctypes.c_uint32),
+                ("groups", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("state_dim", ctypes.c_uint32), ("width", ctypes.c_uint32),
+                ("dtype", ctypes.c_uint32), ("xbc_stride", ctypes.c_uint64),
+                ("dt_stride", ctypes.c_uint64), ("y_stride", ctypes.c_uint64),
+                ("d_xbc", ctypes.c_void_p), ("d_weight", ctypes.c_void_p),
+                ("d_bias", ctypes.c_void_p), ("d_dt", ctypes.c_void_p), ("d_a", ctypes.c_void_p),
+                ("d_d", ctypes.c_void_p), ("d_dt_bias", ctypes.c_void_p),
+                ("d_positions", ctypes.c_void_p), ("d_slots", ctypes.c_void_p),
+                ("d_cache", ctypes.c_void_p), ("d_state", ctypes.c_void_p),
+                ("d_y", ctypes.c_void_p)]
+
+
 class NsfpsError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"nsfps status {status}: {msg}")
@@ -66,6 +133,17 @@ class Lib:
         self.lib = ctypes.CDLL(path)
         self.lib.nsfps_last_error.restype = ctypes.c_char_p
         self.lib.nsfps_version.restype = ctypes.c_char_p
+        # the sequence operators' calls are short: declared once, their
+        # arguments are not converted one by one
+        for name, structs in (("embed", [EmbedArgs]), ("embed_grad", [EmbedArgs]),
+                              ("conv", [ConvArgs]), ("conv_grad", [ConvArgs, ConvGrads]),
+                              ("scan", [ScanArgs]), ("scan_grad", [ScanArgs, ScanGrads]),
+                              ("scan_step", [StepArgs])):
+            pointers = [ctypes.POINTER(t) for t in structs]
+            getattr(self.lib, f"nsfps_{name}_device").argtypes = pointers + [_vp]
+            if name in ("embed_grad", "conv_grad", "scan", "scan_grad"):
+                getattr(self.lib, f"nsfps_{name}_workspace_bytes").argtypes = \
+                    pointers[:1] + [ctypes.POINTER(_u64)]
 
     def _check(self, rc):
         if rc != NSFPS_OK:
@@ -216,6 +294,53 @@ class Lib:
                                                      ctypes.c_float(radius),
                                                      ctypes.c_uint32(int(nsample)), _vp(d_out),
                                                      _vp(stream)))
+
+    # The sequence operators: args (and grads) are the structs above, filled
+    # once and reused with other pointers; everything they point to is device
+    # memory, and the calls only enqueue on the stream.
+
+    def _workspace_bytes(self, call, args):
+        n = _u64()
+        self._check(call(args, n))
+        return n.value
+
+    def embed_device(self, args, stream=None):
+        """nsfps_embed_device: scaled rows of a table by token."""
+        self._check(self.lib.nsfps_embed_device(args, stream))
+
+    def embed_grad_workspace_bytes(self, args):
+        return self._workspace_bytes(self.lib.nsfps_embed_grad_workspace_bytes, args)
+
+    def embed_grad_device(self, args, stream=None):
+        """nsfps_embed_grad_device: the table's gradient (d_table) from the rows' (d_out)."""
+        self._check(self.lib.nsfps_embed_grad_device(args, stream))
+
+    def conv_device(self, args, stream=None):
+        """nsfps_conv_device: short causal convolution and SiLU."""
+        self._check(self.lib.nsfps_conv_device(args, stream))
+
+    def conv_grad_workspace_bytes(self, args):
+        return self._workspace_bytes(self.lib.nsfps_conv_grad_workspace_bytes, args)
+
+    def conv_grad_device(self, args, grads, stream=None):
+        self._check(self.lib.nsfps_conv_grad_device(args, grads, stream))
+
+    def scan_workspace_bytes(self, args):
+        return self._workspace_bytes(self.lib.nsfps_scan_workspace_bytes, args)
+
+    def scan_device(self, args, stream=None):
+        """nsfps_scan_device: selective state space scan over prompts."""
+        self._check(self.lib.nsfps_scan_device(args, stream))
+
+    def scan_grad_workspace_bytes(self, args):
+        return self._workspace_bytes(self.lib.nsfps_scan_grad_workspace_bytes, args)
+
+    def scan_grad_device(self, args, grads, stream=None):
+        self._check(self.lib.nsfps_scan_grad_device(args, grads, stream))
+
+    def scan_step_device(self, args, stream=None):
+        """nsfps_scan_step_device: convolution and scan of one token a request."""
+        self._check(self.lib.nsfps_scan_step_device(args, stream))
 
     def stats(self):
         return self.stats_raw().as_dict()

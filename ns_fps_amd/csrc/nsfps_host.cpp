@@ -32,15 +32,12 @@
 
 #include "nsfps_internal.h"
 #include "nsfps_launch.h"
+#include "nsfps_sequence.h"
+#include "nsfps_status.h"
 
 namespace nsfps {
-namespace {
 
-constexpr float kBoundaryEps = 1e-6f;  // BOUNDARY_EPS, src/yuezu_fps.h:43-45
-
-thread_local std::string g_err;
-thread_local nsfps_stats g_stats;
-thread_local uint64_t g_prof[kProfWords];
+static thread_local std::string g_err;
 
 nsfps_status fail(nsfps_status s, const char *fmt, ...) {
   char buf[512];
@@ -62,9 +59,8 @@ nsfps_status fail(nsfps_status s, const char *fmt, ...) {
 // each call gets its own countdown and a call after the variable is removed
 // runs normally.  The error paths this reaches (status, message, the
 // workspace left usable, the stream drained) are tested on the GPU.
-enum InjectKind : int { kInjNone = 0, kInjAlloc, kInjLaunch, kInjCopy, kInjSync, kInjAny };
 thread_local int g_inj_kind = kInjNone;
-thread_local uint64_t g_inj_left = 0;
+static thread_local uint64_t g_inj_left = 0;
 
 void arm_injection() {
   g_inj_kind = kInjNone;
@@ -97,18 +93,12 @@ hipError_t injected(int kind) {
   return kind == kInjAlloc ? hipErrorOutOfMemory : hipErrorLaunchFailure;
 }
 
-#define HIP_TRY(expr)                                                                        \
-  do {                                                                                       \
-    hipError_t e_ = g_inj_kind ? injected(op_kind(#expr)) : hipSuccess;                      \
-    const bool inj_ = e_ != hipSuccess;                                                      \
-    if (!inj_) {                                                                             \
-      e_ = (expr);                                                                           \
-    }                                                                                        \
-    if (e_ != hipSuccess)                                                                    \
-      return fail(e_ == hipErrorOutOfMemory ? NSFPS_ENOMEM : NSFPS_EDEVICE, "%s: %s (%s:%d)", \
-                  #expr, inj_ ? "injected failure (NSFPS_INJECT)" : hipGetErrorString(e_),   \
-                  __FILE__, __LINE__);                                                       \
-  } while (0)
+namespace {
+
+constexpr float kBoundaryEps = 1e-6f;  // BOUNDARY_EPS, src/yuezu_fps.h:43-45
+
+thread_local nsfps_stats g_stats;
+thread_local uint64_t g_prof[kProfWords];
 
 // ---------------------------------------------------------------- range ----
 
@@ -2181,26 +2171,6 @@ struct nsfps_plan_s {
 
 using namespace nsfps;
 
-namespace {
-
-// No C++ exception crosses the C ABI: host allocation failures and any other
-// exception become a status with a message.
-template <class F>
-nsfps_status guarded(F &&f) {
-  try {
-    arm_injection();
-    return f();
-  } catch (const std::bad_alloc &) {
-    return fail(NSFPS_ENOMEM, "host allocation failed");
-  } catch (const std::exception &e) {
-    return fail(NSFPS_EDEVICE, "internal error: %s", e.what());
-  } catch (...) {
-    return fail(NSFPS_EDEVICE, "internal error");
-  }
-}
-
-}  // namespace
-
 extern "C" {
 
 const char *nsfps_last_error(void) { return g_err.c_str(); }
@@ -2211,7 +2181,13 @@ nsfps_status nsfps_init_device(void) {
   return guarded([&]() -> nsfps_status {
     std::lock_guard<std::mutex> lk(g_mu);
     Arena *ap = nullptr;
-    return arena_for_device(&ap);
+    const nsfps_status rc = arena_for_device(&ap);
+    if (rc) return rc;
+    HIP_TRY(preload_embed_kernels());
+    HIP_TRY(preload_conv_kernels());
+    HIP_TRY(preload_scan_kernels());
+    HIP_TRY(preload_scan_grad_kernels());
+    return NSFPS_OK;
   });
 }
 

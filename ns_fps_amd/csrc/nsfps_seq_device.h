@@ -1,0 +1,152 @@
+// Device helpers of the sequence operators: the two storage types, vectors of
+// them, and the exponential.  Contraction to FMA is wanted here (a sum of
+// products has no order of operations to reproduce, and an FMA rounds once),
+// so the operators' files switch it on.
+#pragma once
+
+#include "nsfps_sequence.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#if defined(__HIP_DEVICE_COMPILE__)
+#define NSFPS_GLOBAL_SEQ __attribute__((address_space(1)))
+#else
+#define NSFPS_GLOBAL_SEQ
+#endif
+
+namespace nsfps {
+namespace seq {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct bf16 {
+  uint16_t u;
+};
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(bf16 v) { return __uint_as_float((uint32_t)v.u << 16); }
+
+// Nearest even, as the hardware converts (NaN stays NaN).
+__device__ __forceinline__ uint16_t bf16_bits(float v) {
+  const __bf16 h = (__bf16)v;
+  return __builtin_bit_cast(uint16_t, h);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ bf16 from_f32<bf16>(float v) {
+  return bf16{bf16_bits(v)};
+}
+
+// V elements at p, p aligned to V elements.
+template <typename T, int V>
+struct Vec {
+  T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ void load_f32(const T *p, float (&o)[V]) {
+  const NSFPS_GLOBAL_SEQ T *g = (const NSFPS_GLOBAL_SEQ T *)p;
+  constexpr int kWords = V * (int)sizeof(T) / 4;
+  if constexpr (kWords >= 1) {
+    uint32_t w[kWords];
+    if constexpr (kWords == 4) {
+      const u32x4 t = *(const NSFPS_GLOBAL_SEQ u32x4 *)g;
+      w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+    } else if constexpr (kWords == 2) {
+      const u32x2 t = *(const NSFPS_GLOBAL_SEQ u32x2 *)g;
+      w[0] = t.x, w[1] = t.y;
+    } else {
+      static_assert(kWords == 1, "vector width");
+      w[0] = *(const NSFPS_GLOBAL_SEQ uint32_t *)g;
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        o[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16));
+    }
+  } else {
+    static_assert(V == 1, "vector width");
+    T t;
+    if constexpr (sizeof(T) == 4)
+      t = __builtin_bit_cast(T, *(const NSFPS_GLOBAL_SEQ uint32_t *)g);
+    else
+      t = __builtin_bit_cast(T, *(const NSFPS_GLOBAL_SEQ uint16_t *)g);
+    o[0] = to_f32(t);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_f32(T *p, const float (&o)[V]) {
+  NSFPS_GLOBAL_SEQ T *g = (NSFPS_GLOBAL_SEQ T *)p;
+  constexpr int kWords = V * (int)sizeof(T) / 4;
+  if constexpr (kWords >= 1) {
+    uint32_t w[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (sizeof(T) == 4)
+        w[i] = __float_as_uint(o[i]);
+      else
+        w[i] = (uint32_t)bf16_bits(o[2 * i]) | ((uint32_t)bf16_bits(o[2 * i + 1]) << 16);
+    }
+    if constexpr (kWords == 4) {
+      u32x4 t;
+      t.x = w[0], t.y = w[1], t.z = w[2], t.w = w[3];
+      *(NSFPS_GLOBAL_SEQ u32x4 *)g = t;
+    } else if constexpr (kWords == 2) {
+      u32x2 t;
+      t.x = w[0], t.y = w[1];
+      *(NSFPS_GLOBAL_SEQ u32x2 *)g = t;
+    } else {
+      *(NSFPS_GLOBAL_SEQ uint32_t *)g = w[0];
+    }
+  } else {
+    if constexpr (sizeof(T) == 4)
+      *(NSFPS_GLOBAL_SEQ uint32_t *)g = __float_as_uint(o[0]);
+    else
+      *(NSFPS_GLOBAL_SEQ uint16_t *)g = bf16_bits(o[0]);
+  }
+}
+
+// Elements of a 16-byte load.
+template <typename T>
+constexpr int kWide = 16 / (int)sizeof(T);
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// 2^x (v_exp_f32: within an ulp; results below the normal range become 0)
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
+// 1 / (1 + exp(-x)): the exponential's infinity gives 0, its zero gives 1
+__device__ __forceinline__ float sigmoid(float x) {
+  return rcp_fast(1.f + exp2_fast(-x * kLog2e));
+}
+// log(1 + exp(x)) without overflow; -infinity gives 0
+__device__ __forceinline__ float softplus(float x) {
+  const float e = exp2_fast(-fabsf(x) * kLog2e);
+  return fmaxf(x, 0.f) + log1pf(e);
+}
+
+__device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
+
+}  // namespace seq
+
+inline uint64_t host_ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+// Rows whose start and strides keep 16-byte loads of `size`-byte elements aligned.
+inline bool rows_wide(const nsfps_rows &r, uint32_t size) {
+  const uint64_t v = 16 / size;
+  return (uintptr_t)r.p % 16 == 0 && r.batch_stride % v == 0 && r.row_stride % v == 0;
+}
+
+}  // namespace nsfps
