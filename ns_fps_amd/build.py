@@ -15,6 +15,7 @@ Run ``python -m ns_fps_amd.build`` (or ``__graft_entry__.build()``);
 ``python -m ns_fps_amd.build sanitize`` builds the sanitized pair.
 """
 
+import concurrent.futures
 import os
 import re
 import subprocess
@@ -57,9 +58,12 @@ DEVICE_FLAGS = [
     "-fno-gpu-flush-denormals-to-zero",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-mllvm", "-amdgpu-atomic-optimizer-strategy=None",
-    "-mllvm", "-amdgpu-sched-strategy=max-ilp",
     "-Wall", "-Wno-unused-result",
 ]
+MAX_ILP = ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
+# The scan's kernels are bound by registers: the default scheduler, which
+# counts them.
+DEFAULT_SCHEDULER = ("nsfps_scan.hip", "nsfps_scan_grad.hip")
 HOST_PASS_WARNING = "'-packed-fp32-ops' is not a recognized feature for this target"
 PACKED_FP32 = re.compile(r"\bv_pk_(add|mul|fma)_f32\b")
 
@@ -111,13 +115,23 @@ SAN_HOST_FLAGS = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitiz
 
 
 def build_lib(out=LIB, extra=()):
-    srcs = [os.path.join(CSRC, f) for f in SOURCES]
+    """Every source on its own, several at a time, then one link."""
     os.makedirs(os.path.dirname(out), exist_ok=True)
     tmp = out + ".tmp"
     with tempfile.TemporaryDirectory(prefix="nsfps_build_") as td:
-        # -save-temps keeps each translation unit's gfx950 assembly in td
-        _run([HIPCC, *DEVICE_FLAGS, *extra, "-save-temps", "-shared", "-I", INCLUDE, "-I", CSRC,
-              *srcs, "-o", tmp], cwd=td)
+        def compile_one(name):
+            # -save-temps keeps the source's gfx950 assembly in td
+            flags = [] if name in DEFAULT_SCHEDULER else MAX_ILP
+            lang = ["-x", "hip"] if name.endswith(".cpp") else []
+            obj = os.path.join(td, name + ".o")
+            _run([HIPCC, *DEVICE_FLAGS, *flags, *extra, "-save-temps", "-I", INCLUDE, "-I", CSRC,
+                  *lang, "-c", os.path.join(CSRC, name), "-o", obj], cwd=td)
+            return obj
+
+        jobs = max(1, min(8, int(os.environ.get("MAX_JOBS") or os.cpu_count() or 1)))
+        with concurrent.futures.ThreadPoolExecutor(jobs) as pool:
+            objs = list(pool.map(compile_one, SOURCES))
+        _run([HIPCC, f"--offload-arch={ARCH}", "-fPIC", "-shared", *extra, *objs, "-o", tmp], cwd=td)
         check_no_packed_fp32(td)
     os.replace(tmp, out)
     return out

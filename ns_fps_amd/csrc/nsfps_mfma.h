@@ -92,54 +92,117 @@ __device__ __forceinline__ Terms<T, N> split(f32x4 v) {
 }
 
 // LDS tiles: rows of `ld` elements, padded by 16 bytes so that the 16 rows a
-// quarter of a wave reads at once start in different banks.
+// quarter of a wave reads at once start in different banks.  In bfloat16 the
+// columns of every 32 are stored with a lane's two quads next to each other
+// (column 16a + 4g + r at 8g + 4a + r), so that both come in one 16-byte read.
 template <typename T, int COLS>
 constexpr int kLd = COLS + 16 / (int)sizeof(T);
 
-// terms along the row: row r, terms k .. k+3
 template <typename T>
-__device__ __forceinline__ Quad<T> quad_row(const T *tile, int ld, int r, int k) {
-  return *(const Quad<T> *)(tile + r * ld + k);
-}
-// terms down the column: column c, terms (rows) k .. k+3
-template <typename T>
-__device__ __forceinline__ Quad<T> quad_col(const T *tile, int ld, int k, int c) {
-  Quad<T> q;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4)
-      q[i] = tile[(k + i) * ld + c];
-    else
-      q[i] = __builtin_bit_cast(__bf16, tile[(k + i) * ld + c].u);
-  }
-  return q;
+__device__ __forceinline__ int column_at(int c) {
+  return sizeof(T) == 4 ? c : (c & ~31) | ((c & 12) << 1) | ((c & 16) >> 2) | (c & 3);
 }
 
-// A tile of 64 rows x COLS columns from global rows, zeros from row `rows` and
-// column `cols` on; 256 threads.  wide: rows start at 16-byte boundaries and
-// cols is a multiple of the elements in 16 bytes.
-template <typename T, int COLS>
-__device__ __forceinline__ void load_tile(T *tile, const T *g, uint64_t row_stride, uint32_t rows,
-                                          uint32_t cols, bool wide) {
-  constexpr int V = kWide<T>, kVecs = COLS / V, ld = kLd<T, COLS>;
-  if (wide) {
+// Both quads of an operand of 32 terms.
+template <typename T>
+struct Pair {
+  Quad<T> q0, q1;
+};
+template <typename T>
+__device__ __forceinline__ void mma(f32x4 &sum, const Pair<T> &a, const Pair<T> &b) {
+  mma(sum, a.q0, a.q1, b.q0, b.q1);
+}
+template <typename T>
+__device__ __forceinline__ void mma_apart(f32x4 &sum, const Pair<T> &a, const Pair<T> &b) {
+  mma_apart(sum, a.q0, a.q1, b.q0, b.q1);
+}
+
+// terms along the row: row r, terms 32 kb + this lane's
+__device__ __forceinline__ Pair<float> pair_row(const float *tile, int ld, int r, int kb, int g) {
+  const float *at = tile + r * ld + 32 * kb + 4 * g;
+  return Pair<float>{*(const f32x4 *)at, *(const f32x4 *)(at + 16)};
+}
+__device__ __forceinline__ Pair<bf16> pair_row(const bf16 *tile, int ld, int r, int kb, int g) {
+  const bf16x8 v = *(const bf16x8 *)(tile + r * ld + 32 * kb + 8 * g);
+  return Pair<bf16>{__builtin_shufflevector(v, v, 0, 1, 2, 3), __builtin_shufflevector(v, v, 4, 5, 6, 7)};
+}
+// one quad of a row: columns c .. c+3, c a multiple of four
+template <typename T>
+__device__ __forceinline__ Quad<T> quad_row(const T *tile, int ld, int r, int c) {
+  return *(const Quad<T> *)(tile + r * ld + column_at<T>(c));
+}
+template <typename T>
+__device__ __forceinline__ void put_quad(T *tile, int ld, int r, int c, Quad<T> q) {
+  *(Quad<T> *)(tile + r * ld + column_at<T>(c)) = q;
+}
+
+// terms down the column: columns c .. c+15 (this lane's: c + l), terms (rows)
+// k .. k+3 with k the lane's own (a multiple of four plus 4g).  bfloat16: the
+// transposing LDS read, in which the 16 lanes of a quarter read four rows of
+// 16 elements and each receives a column; the whole wave takes part.
+__device__ __forceinline__ f32x4 quad_col(const float *tile, int ld, int k, int c, int l) {
+  f32x4 q;
 #pragma unroll
-    for (uint32_t e = threadIdx.x; e < 64 * kVecs; e += 256) {
-      const uint32_t r = e / kVecs, c = (e % kVecs) * V;
-      u32x4 v = {0, 0, 0, 0};
-      if (r < rows && c < cols)
-        v = *(const NSFPS_GLOBAL_SEQ u32x4 *)(g + r * row_stride + c);
-      *(u32x4 *)(tile + r * ld + c) = v;
-    }
-  } else {
-    for (uint32_t e = threadIdx.x; e < 64 * COLS; e += 256) {
-      const uint32_t r = e / COLS, c = e % COLS;
-      float v[1] = {0.f};
-      if (r < rows && c < cols) load_f32<T, 1>(g + r * row_stride + c, v);
-      tile[r * ld + c] = from_f32<T>(v[0]);
+  for (int i = 0; i < 4; ++i) q[i] = tile[(k + i) * ld + c + l];
+  return q;
+}
+__device__ __forceinline__ bf16x4 quad_col(const bf16 *tile, int ld, int k, int c, int l) {
+  typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+  const bf16 *at = tile + (k + l / 4) * ld + (c & ~31) + 8 * (l % 4) + ((c & 16) >> 2);
+  return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at));
+}
+// terms 32 kb + this lane's, down the column
+template <typename T>
+__device__ __forceinline__ Pair<T> pair_col(const T *tile, int ld, int kb, int c, int g, int l) {
+  return Pair<T>{quad_col(tile, ld, 32 * kb + 4 * g, c, l),
+                 quad_col(tile, ld, 32 * kb + 16 + 4 * g, c, l)};
+}
+
+// A tile of 64 rows x COLS columns on its way from global memory to LDS, in
+// the registers of 256 threads: fetched while the tile before it is worked on.
+// Zeros from row `rows` and column `cols` on.  kWideRows: rows start at 16-byte
+// boundaries and cols is a multiple of the elements in 16 bytes.
+template <typename T, int COLS, bool kWideRows>
+struct Tile {
+  static constexpr int V = kWide<T>, kVecs = COLS / V, kPer = 64 * kVecs / 256;
+  static_assert(kPer >= 1, "tile too small");
+  u32x4 v[kPer];
+
+  __device__ __forceinline__ void fetch(const T *g, uint64_t row_stride, uint32_t rows,
+                                        uint32_t cols) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + 256 * i, r = e / kVecs, c = (e % kVecs) * V;
+      v[i] = u32x4{0, 0, 0, 0};
+      const NSFPS_GLOBAL_SEQ T *at = (const NSFPS_GLOBAL_SEQ T *)(g + r * row_stride + c);
+      if constexpr (kWideRows) {
+        if (r < rows && c < cols) v[i] = *(const NSFPS_GLOBAL_SEQ u32x4 *)at;
+      } else if (r < rows) {
+#pragma unroll
+        for (uint32_t k = 0; k < V; ++k) {
+          if (c + k >= cols) break;
+          if constexpr (sizeof(T) == 4)
+            v[i][k] = *(const NSFPS_GLOBAL_SEQ uint32_t *)(at + k);
+          else
+            v[i][k / 2] |= (uint32_t) * (const NSFPS_GLOBAL_SEQ uint16_t *)(at + k) << (16 * (k % 2));
+        }
+      }
     }
   }
-}
+  __device__ __forceinline__ void put(T *tile) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + 256 * i;
+      const int r = e / kVecs, c = (e % kVecs) * V;
+      if constexpr (sizeof(T) == 4) {
+        *(u32x4 *)(tile + r * kLd<T, COLS> + c) = v[i];
+      } else {
+        *(u32x2 *)(tile + r * kLd<T, COLS> + column_at<T>(c)) = u32x2{v[i].x, v[i].y};
+        *(u32x2 *)(tile + r * kLd<T, COLS> + column_at<T>(c + 4)) = u32x2{v[i].z, v[i].w};
+      }
+    }
+  }
+};
 
 }  // namespace seq
 }  // namespace nsfps

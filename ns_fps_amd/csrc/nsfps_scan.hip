@@ -6,9 +6,7 @@
 //   y_i = sum_{j<=i} exp(s_i - s_j) delta_j (c_i . b_j) x_j + exp(s_i) state_in c_i + d x_i
 //   state_out = exp(s_last) state_in + sum_j exp(s_last - s_j) delta_j x_j b_j^T
 // so the work is on the matrix cores and the sequence is only walked from
-// chunk to chunk: the chunks' own sums are found side by side (k_scan_sums),
-// a pass over them gives the state each chunk starts from (k_scan_pass), and
-// the outputs are found side by side again (k_scan_out).
+// chunk to chunk (k_scan_sweep).
 #include "nsfps_launch.h"
 #include "nsfps_scan_device.h"
 
@@ -23,137 +21,357 @@ using namespace seq;
 
 namespace {
 
-// LDS of k_scan_out, in elements of T
-template <typename T, int NT>
-struct OutLds {
-  static constexpr int kTerms = Terms<T, 2>::kN;
-  T x[kChunk * kLd<T, (int)kPTile>];
-  T b[kChunk * kLd<T, NT>], c[kChunk * kLd<T, NT>];
-  T h[kTerms][kPTile * kLd<T, NT>];
-  Steps st;
+// ---- the sweep over a sequence's chunks
+//
+// One workgroup walks a segment of a sequence's chunks with a head's state (64
+// rows of it) in registers, wave w holding rows 16w .. 16w+15 as the sum tiles
+// [n][p] that the state's own update
+//   state = decay(chunk) state + sum over tokens of weight u v^T
+// accumulates into.  Forward: u = x, v = b, weight = delta_j * decay from j to
+// the chunk's end.  Reversed, for the gradient: u = dy, v = c, weight = decay
+// from the chunk's start through i, from the last chunk to the first.  The
+// weighted u is split into three bfloat16 terms: states are float32 and keep
+// float32 accuracy.
+//
+// kOut: the chunk's outputs too (forward).  The four waves share the ten
+// 16 x 16 tiles of c b^T that the causal order leaves, weigh them and leave
+// them in LDS as rows of operands; then each wave has its 16 columns of y from
+// them and x, and from its rows of the state, which in its registers already
+// are an operand.  Scores and states enter there as two bfloat16 terms (16
+// bits): the output's own rounding to 8 bits stays the only one that shows.
+//
+// Few sequences: segments run side by side, a first sweep over them finding
+// what each adds to the state (ends), k_scan_carry turning that into the state
+// each starts from (starts).
+struct SweepDev {
+  nsfps_rows u, v;
+  float *starts;  // [batch][heads][segs][head_dim][state_dim], or null: from the cache, or zero
+  float *ends;    // the same shape: the segment's state after its chunks, or null
+  float *totals;  // [batch][heads][segs], with ends: log2 of the segment's decay
+  float *store;   // [batch][heads][chunks][head_dim][state_dim]: the state each chunk finds, or null
 };
 
-// The outputs of a chunk, one wave per 16 tokens.  A wave finds its rows of
-// c.b^T transposed, so that the weighted scores are, in its registers, the
-// operand of the product with x.  Scores and states enter as two bfloat16
-// terms (16 bits): the output's own rounding to 8 bits stays the only one
-// that shows.
-template <typename T, int NT>
-__global__ __launch_bounds__(256) void k_scan_out(ScanDev s, uint64_t work) {
-  extern __shared__ __attribute__((aligned(16))) char s_raw[];
-  OutLds<T, NT> &m = *(OutLds<T, NT> *)s_raw;
-  constexpr int ldx = kLd<T, (int)kPTile>, ldn = kLd<T, NT>, kTerms = OutLds<T, NT>::kTerms;
-  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, l = lane & 15u;
-  for (uint64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const uint32_t hp = (uint32_t)(w % (s.heads * s.ptiles));
-    const uint64_t bc = w / (s.heads * s.ptiles);
-    const uint32_t h = hp / s.ptiles, p0 = (hp % s.ptiles) * kPTile;
-    const uint32_t c = (uint32_t)(bc % s.chunks), b = (uint32_t)(bc / s.chunks);
-    const uint32_t len = scan_length(s, b), t0 = c * kChunk, pn = s.head_dim - p0;
-    T *yr = (T *)s.y.p + (uint64_t)b * s.y.batch_stride + (uint64_t)t0 * s.y.row_stride +
-            h * s.head_dim + p0;
-    const uint32_t out_rows = min(kChunk, s.length - t0);
-    if (t0 >= len) {  // past the sequence's end
-      for (uint32_t e = threadIdx.x; e < kChunk * kPTile; e += 256) {
-        const float z[1] = {0.f};
-        if (e / kPTile < out_rows && e % kPTile < pn)
-          store_f32<T, 1>(yr + (uint64_t)(e / kPTile) * s.y.row_stride + e % kPTile, z);
+constexpr int kStepAhead = 4;  // chunks whose steps are found together, one by each wave
+
+template <typename T, int NT, bool kOut>
+struct SweepLds {
+  static constexpr int kTerms = kOut ? Terms<T, 2>::kN : 1;
+  T u[kChunk * kLd<T, (int)kPTile>], v[kChunk * kLd<T, NT>];
+  T c[kOut ? kChunk * kLd<T, NT> : 16];
+  T m[kTerms][kOut ? kChunk * kLd<T, (int)kChunk> : 16];  // weighted scores, rows i
+  Steps st[kStepAhead];
+};
+
+// XCD-aware order of work: workgroups are dealt to the 8 XCDs in turn, so that
+// item w is given to the XCD whose L2 already holds its neighbours' b and c.
+__device__ __forceinline__ uint32_t xcd_item(uint32_t id, uint32_t work) {
+  const uint32_t per = (work + 7) / 8;
+  return (id % 8) * per + id / 8;
+}
+
+// This lane's part of a state: row p, columns 16nt + 4g .. + 3.
+template <int kNt, bool kWideRows, bool kStore>
+__device__ __forceinline__ void state_io(float *state, f32x4 (&v)[kNt], uint32_t p, uint32_t rows,
+                                         uint32_t cols, uint32_t g) {
+  if (p >= rows) return;
+  NSFPS_GLOBAL_SEQ float *row = (NSFPS_GLOBAL_SEQ float *)(state + (uint64_t)p * cols);
+#pragma unroll
+  for (int nt = 0; nt < kNt; ++nt) {
+    const uint32_t at = 16 * nt + 4 * g;
+    if constexpr (kWideRows) {
+      if (at < cols) {
+        if constexpr (kStore)
+          *(NSFPS_GLOBAL_SEQ f32x4 *)(row + at) = v[nt];
+        else
+          v[nt] = *(const NSFPS_GLOBAL_SEQ f32x4 *)(row + at);
       }
-      continue;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (at + r < cols) {
+          if constexpr (kStore)
+            row[at + r] = v[nt][r];
+          else
+            v[nt][r] = row[at + r];
+        }
     }
-    const uint32_t rows = min(kChunk, len - t0), grp = h / (s.heads / s.groups);
-    load_tile<T, (int)kPTile>(m.x, (const T *)s.x.p + (uint64_t)b * s.x.batch_stride +
-                                       (uint64_t)t0 * s.x.row_stride + h * s.head_dim + p0,
-                              s.x.row_stride, rows, pn, s.wide_x);
-    load_tile<T, NT>(m.b, (const T *)s.b.p + (uint64_t)b * s.b.batch_stride +
-                              (uint64_t)t0 * s.b.row_stride + grp * s.state_dim,
-                     s.b.row_stride, rows, s.state_dim, s.wide_bc);
-    load_tile<T, NT>(m.c, (const T *)s.c.p + (uint64_t)b * s.c.batch_stride +
-                              (uint64_t)t0 * s.c.row_stride + grp * s.state_dim,
-                     s.c.row_stride, rows, s.state_dim, s.wide_bc);
-    if (wave == 0) chunk_steps<T>(s, m.st, b, h, t0, len);
-    const float *st = s.states +
-                      (((uint64_t)b * s.heads + h) * s.chunks + c) * s.head_dim * s.state_dim +
-                      (uint64_t)p0 * s.state_dim;
-    for (uint32_t e = threadIdx.x; e < kPTile * (NT / 4); e += 256) {
-      const uint32_t p = e / (NT / 4), n = (e % (NT / 4)) * 4;
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (p < pn)
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-          if (n + i < s.state_dim) v[i] = st[p * s.state_dim + n + i];
-      const Terms<T, 2> t = split<T, 2>(v);
-#pragma unroll
-      for (int k = 0; k < kTerms; ++k) *(Quad<T> *)(m.h[k] + p * ldn + n) = t.q[k];
+  }
+}
+
+// Two workgroups a CU where their LDS allows it (160 KB): the compiler may then
+// use 256 registers.
+template <typename T, int NT, bool kOut>
+constexpr int kSweepGroups = sizeof(SweepLds<T, NT, kOut>) <= 80 * 1024 ? 2 : 1;
+
+template <typename T, int NT, bool kOut, bool kRev, bool kWideRows>
+__global__ __launch_bounds__(256, (kSweepGroups<T, NT, kOut>)) void k_scan_sweep(ScanDev s,
+                                                                                 SweepDev d,
+                                                                                 uint32_t work) {
+  extern __shared__ __attribute__((aligned(16))) char s_raw[];
+  SweepLds<T, NT, kOut> &m = *(SweepLds<T, NT, kOut> *)s_raw;
+  constexpr int ldu = kLd<T, (int)kPTile>, ldn = kLd<T, NT>, ldm = kLd<T, (int)kChunk>,
+                kNt = NT / 16, kT2 = Terms<T, 2>::kN, kT3 = Terms<T, 3>::kN;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
+                 g = lane >> 4, l = lane & 15u;
+  const uint32_t hps = s.heads * s.ptiles;
+  if constexpr (kOut) {  // the tiles above the diagonal that a product of 32 terms takes along
+    for (uint32_t e = threadIdx.x; e < SweepLds<T, NT, kOut>::kTerms * kChunk * ldm; e += 256)
+      (&m.m[0][0])[e] = from_f32<T>(0.f);
+  }
+  const uint32_t w = xcd_item(blockIdx.x, work);
+  if (w >= work) return;
+  const uint32_t hp = w % hps, sg = w / hps % s.segs, b = w / hps / s.segs;
+  const uint32_t h = hp / s.ptiles, p0 = (hp % s.ptiles) * kPTile, pn = s.head_dim - p0;
+  const uint32_t grp = h / (s.heads / s.groups), sn = s.state_dim;
+  const uint32_t len = scan_length(s, b), n = (len + kChunk - 1) / kChunk;
+  const uint32_t first = sg * s.seg, last = min(first + s.seg, s.chunks);  // chunks
+  const uint32_t mine = n > first ? min(n, last) - first : 0;              // with tokens in them
+  const uint64_t bh = (uint64_t)b * s.heads + h, pn_all = (uint64_t)s.head_dim * sn;
+  const uint32_t p = 16 * wave + l;  // this lane's row of the state
+  const bool works = 16 * wave < pn;
+  f32x4 st[kNt] = {};
+  float *cache = nullptr;
+  if (kOut && s.state) {
+    const int32_t slot = s.slots ? s.slots[b] : (int32_t)b;
+    if (slot >= 0)
+      cache = s.state + ((uint64_t)slot * s.heads + h) * pn_all + (uint64_t)p0 * sn;
+  }
+  const uint64_t seg_at = (bh * s.segs + sg) * pn_all + (uint64_t)p0 * sn;
+  if (d.starts)
+    state_io<kNt, kWideRows, false>(d.starts + seg_at, st, p, pn, sn, g);
+  else if (cache && s.positions && s.positions[b] > 0)
+    state_io<kNt, kWideRows, false>(cache, st, p, pn, sn, g);
+
+  const T *const ub = (const T *)d.u.p + (uint64_t)b * d.u.batch_stride + h * s.head_dim + p0;
+  const T *const vb = (const T *)d.v.p + (uint64_t)b * d.v.batch_stride + grp * sn;
+  const T *const cb = (const T *)s.c.p + (uint64_t)b * s.c.batch_stride + grp * sn;
+  T *const yb = (T *)s.y.p + (uint64_t)b * s.y.batch_stride + h * s.head_dim + p0;
+  const auto chunk_at = [&](uint32_t k) { return kRev ? first + mine - 1 - k : first + k; };
+  Tile<T, (int)kPTile, kWideRows> tu;
+  Tile<T, NT, kWideRows> tv, tc;
+  const auto fetch = [&](uint32_t k) {
+    const uint32_t t0 = chunk_at(k) * kChunk, rows = len - t0;
+    tu.fetch(ub + t0 * d.u.row_stride, d.u.row_stride, rows, pn);
+    tv.fetch(vb + t0 * d.v.row_stride, d.v.row_stride, rows, sn);
+    if constexpr (kOut) tc.fetch(cb + t0 * s.c.row_stride, s.c.row_stride, rows, sn);
+  };
+  // the raw step of the chunk this wave finds the steps of, one group ahead
+  float raw = 0.f;
+  const auto fetch_raw = [&](uint32_t k) {
+    raw = 0.f;
+    if (k + wave < mine) {
+      const uint32_t t = chunk_at(k + wave) * kChunk + lane;
+      if (t < len) raw = raw_step<T>(s, b, h, t);
+    }
+  };
+  float total = 0.f;
+  if (mine) {
+    fetch(0);
+    fetch_raw(0);
+  }
+  for (uint32_t k = 0; k < mine; ++k) {
+    const uint32_t c = chunk_at(k);
+    const Steps &sp = m.st[k % kStepAhead];
+    __syncthreads();  // the tiles of the chunk before are done with
+    tu.put(m.u);
+    tv.put(m.v);
+    if constexpr (kOut) tc.put(m.c);
+    if (k % kStepAhead == 0) {
+      if (k + wave < mine)
+        chunk_steps(m.st[wave], raw, chunk_at(k + wave) * kChunk + lane < len, s.a[h]);
+      fetch_raw(k + kStepAhead);
     }
     __syncthreads();
+    if (k + 1 < mine) fetch(k + 1);
+    if (d.store)
+      state_io<kNt, kWideRows, true>(d.store + (bh * s.chunks + c) * pn_all + (uint64_t)p0 * sn,
+                                     st, p, pn, sn, g);
 
-    const int i = 16 * wave + l;  // this lane's token
-    f32x4 from[kPTile / 16] = {}, own[kPTile / 16] = {};
-    Quad<T> cq[NT / 16];
-#pragma unroll
-    for (int nt = 0; nt < NT / 16; ++nt) cq[nt] = quad_row<T>(m.c, ldn, i, 16 * nt + 4 * g);
-    // state_in c_i
-#pragma unroll
-    for (int pt = 0; pt < (int)kPTile / 16; ++pt)
-#pragma unroll
-      for (int k = 0; k < kTerms; ++k)
-#pragma unroll
-        for (int nt = 0; nt < NT / 16; nt += 2)
-          mma(from[pt], quad_row<T>(m.h[k], ldn, 16 * pt + l, 16 * nt + 4 * g),
-              quad_row<T>(m.h[k], ldn, 16 * pt + l, 16 * nt + 16 + 4 * g), cq[nt], cq[nt + 1]);
-    // the chunk's own tokens, 32 at a time
-    for (uint32_t jj = 0; jj <= wave / 2; ++jj) {
-      Terms<T, 2> sc[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int jt = 2 * jj + half;
+    if constexpr (kOut) {
+      // tiles (i, j) of the lower triangle: 3, 3, 2, 2 a wave
+      const int from = wave < 2 ? 3 * (int)wave : 2 + 2 * (int)wave, upto = from + (wave < 2 ? 3 : 2);
+      for (int t = from; t < upto; ++t) {
+        const int it = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, jt = t - it * (it + 1) / 2;
         f32x4 q = {0.f, 0.f, 0.f, 0.f};
-        if (jt <= (int)wave) {
 #pragma unroll
-          for (int nt = 0; nt < NT / 16; nt += 2)
-            mma(q, quad_row<T>(m.b, ldn, 16 * jt + l, 16 * nt + 4 * g),
-                quad_row<T>(m.b, ldn, 16 * jt + l, 16 * nt + 16 + 4 * g), cq[nt], cq[nt + 1]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = 16 * jt + 4 * g + r;
-            q[r] = j <= i ? q[r] * m.st.delta[j] * decay_between(m.st, i, j) : 0.f;
-          }
-        }
-        sc[half] = split<T, 2>(q);
-      }
-#pragma unroll
-      for (int pt = 0; pt < (int)kPTile / 16; ++pt) {
-        const Quad<T> a0 = quad_col<T>(m.x, ldx, 32 * jj + 4 * g, 16 * pt + l);
-        const Quad<T> a1 = quad_col<T>(m.x, ldx, 32 * jj + 16 + 4 * g, 16 * pt + l);
-#pragma unroll
-        for (int k = 0; k < kTerms; ++k) mma(own[pt], a0, a1, sc[0].q[k], sc[1].q[k]);
-      }
-    }
-    const float ei = exp2_fast(m.st.hi[i] + m.st.lo[i]), dh = s.d ? s.d[h] : 0.f;
-    if ((uint32_t)i < out_rows) {
-#pragma unroll
-      for (int pt = 0; pt < (int)kPTile / 16; ++pt) {
-        const int p = 16 * pt + 4 * g;
-        const f32x4 xv = quad_f32(quad_row<T>(m.x, ldx, i, p));
-        float o[4];
+        for (int kb = 0; kb < NT / 32; ++kb)
+          mma(q, pair_row(m.v, ldn, 16 * jt + l, kb, g), pair_row(m.c, ldn, 16 * it + l, kb, g));
+        const int i = 16 * it + l, j0 = 16 * jt + 4 * g;
+        const f32x4 dj = quad_of(sp.delta, j0), hj = quad_of(sp.hi, j0), lj = quad_of(sp.lo, j0);
+        const float hi = sp.hi[i], lo = sp.lo[i];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          o[r] = t0 + i < len ? fmaf(dh, xv[r], fmaf(ei, from[pt][r], own[pt][r])) : 0.f;
-        T *dst = yr + (uint64_t)i * s.y.row_stride + p;
-        if (s.wide_y) {
-          if ((uint32_t)p < pn) store_f32<T, 4>(dst, o);
-        } else {
+          q[r] = j0 + r <= i ? q[r] * dj[r] * exp2_fast((hi - hj[r]) + (lo - lj[r])) : 0.f;
+        const Terms<T, 2> sc = split<T, 2>(q);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float o1[1] = {o[r]};
-            if ((uint32_t)(p + r) < pn) store_f32<T, 1>(dst + r, o1);
+        for (int e = 0; e < kT2; ++e) put_quad(m.m[e], ldm, i, j0, sc.q[e]);
+      }
+      __syncthreads();
+    }
+    if (works) {
+      // x transposed: rows p, terms j (operand A of y, and times the weights B of the update)
+      Pair<T> uq[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) uq[kb] = pair_col(m.u, ldu, kb, 16 * wave, g, l);
+      if constexpr (kOut) {
+        f32x4 own[4] = {}, carried[4] = {};
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+#pragma unroll
+          for (int kb = 0; kb <= it / 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < kT2; ++e)
+              mma(own[it], uq[kb], pair_row(m.m[e], ldm, 16 * it + l, kb, g));
+#pragma unroll
+        for (int kb = 0; kb < NT / 32; ++kb) {
+          const Terms<T, 2> h0 = split<T, 2>(st[2 * kb]), h1 = split<T, 2>(st[2 * kb + 1]);
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const Pair<T> cq = pair_row(m.c, ldn, 16 * it + l, kb, g);
+#pragma unroll
+            for (int e = 0; e < kT2; ++e) mma(carried[it], Pair<T>{h0.q[e], h1.q[e]}, cq);
+          }
+        }
+        const float skip = s.d ? s.d[h] : 0.f;
+        const uint32_t t0 = c * kChunk, out_rows = s.length - t0, rows = len - t0;
+        const uint32_t po = 16 * wave + 4 * g;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const uint32_t i = 16 * it + l;
+          const f32x4 xv = quad_f32(quad_row(m.u, ldu, i, po));
+          const float e = sp.e[i];
+          float o[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            o[r] = i < rows ? fmaf(skip, xv[r], fmaf(e, carried[it][r], own[it][r])) : 0.f;
+          T *dst = yb + (t0 + i) * s.y.row_stride + po;
+          if (i < out_rows) {
+            if constexpr (kWideRows) {
+              if (po < pn) store_f32<T, 4>(dst, o);
+            } else {
+#pragma unroll
+              for (uint32_t r = 0; r < 4; ++r) {
+                const float o1[1] = {o[r]};
+                if (po + r < pn) store_f32<T, 1>(dst + r, o1);
+              }
+            }
           }
         }
       }
+      // the state's update
+      const float keep = exp2_fast(sp.total);
+#pragma unroll
+      for (int nt = 0; nt < kNt; ++nt) st[nt] *= keep;
+      f32x4 low[kNt] = {};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const int j = 32 * kb + 4 * g;
+        f32x4 q0 = quad_f32(uq[kb].q0), q1 = quad_f32(uq[kb].q1);
+        if constexpr (kRev) {
+          q0 *= quad_of(sp.e, j);
+          q1 *= quad_of(sp.e, j + 16);
+        } else {
+          q0 *= quad_of(sp.delta, j) * quad_of(sp.end, j);
+          q1 *= quad_of(sp.delta, j + 16) * quad_of(sp.end, j + 16);
+        }
+        const Terms<T, 3> u0 = split<T, 3>(q0), u1 = split<T, 3>(q1);
+#pragma unroll
+        for (int nt = 0; nt < kNt; ++nt) {
+          const Pair<T> vq = pair_col(m.v, ldn, kb, 16 * nt, g, l);
+#pragma unroll
+          for (int e = kT3 - 1; e > 0; --e) mma(low[nt], vq, Pair<T>{u0.q[e], u1.q[e]});
+          mma_apart(st[nt], vq, Pair<T>{u0.q[0], u1.q[0]});
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < kNt; ++nt) st[nt] += low[nt];
     }
-    __syncthreads();
+    total += sp.total;
   }
+  if (d.ends) {
+    state_io<kNt, kWideRows, true>(d.ends + seg_at, st, p, pn, sn, g);
+    if (threadIdx.x == 0 && p0 == 0) d.totals[bh * s.segs + sg] = total;
+  }
+  if (cache && mine && n <= last)  // the sequence's last chunk
+    state_io<kNt, kWideRows, true>(cache, st, p, pn, sn, g);
+  if constexpr (kOut) {  // rows past the sequence's end
+    const uint32_t from = max(n, first) * kChunk, upto = min(last * kChunk, s.length);
+    const float z[1] = {0.f};
+    const uint32_t cols = min(pn, kPTile);
+    for (uint64_t e = threadIdx.x; from < upto && e < (uint64_t)(upto - from) * kPTile; e += 256)
+      if (e % kPTile < cols)
+        store_f32<T, 1>(yb + (from + e / kPTile) * s.y.row_stride + e % kPTile, z);
+  }
+}
+
+// What each segment adds becomes the state each starts from (reversed: the
+// gradient each ends with), in place; one thread per state value walks the
+// sequence's segments, kRun of them loaded ahead.
+template <bool kRev>
+__global__ __launch_bounds__(256) void k_scan_carry(ScanDev s, float *__restrict__ states,
+                                                    const float *__restrict__ totals,
+                                                    uint64_t values) {
+  constexpr uint32_t kRun = 8;
+  const uint32_t pn = s.head_dim * s.state_dim, n = s.segs;
+  for (uint64_t e = (uint64_t)blockIdx.x * 256 + threadIdx.x; e < values;
+       e += (uint64_t)gridDim.x * 256) {
+    const uint64_t bh = e / pn;
+    const uint32_t b = (uint32_t)(bh / s.heads), at = (uint32_t)(e % pn);
+    float run = 0.f;
+    if (!kRev && s.state && s.positions && s.positions[b] > 0) {
+      const int32_t slot = s.slots ? s.slots[b] : (int32_t)b;
+      if (slot >= 0) run = s.state[((uint64_t)slot * s.heads + bh % s.heads) * pn + at];
+    }
+    float *st = states + bh * n * pn + at;
+    const float *tot = totals + bh * n;
+    for (uint32_t c0 = 0; c0 < n; c0 += kRun) {
+      float v[kRun], t[kRun];
+#pragma unroll
+      for (uint32_t k = 0; k < kRun; ++k) {
+        const uint32_t i = min(c0 + k, n - 1), c = kRev ? n - 1 - i : i;
+        v[k] = st[(uint64_t)c * pn];
+        t[k] = tot[c];
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < kRun; ++k) {
+        if (c0 + k >= n) break;
+        const uint32_t c = kRev ? n - 1 - (c0 + k) : c0 + k;
+        st[(uint64_t)c * pn] = run;
+        run = fmaf(exp2_fast(t[k]), run, v[k]);
+      }
+    }
+  }
+}
+
+template <typename T, int NT, bool kOut, bool kRev, bool kWideRows>
+hipError_t launch_sweep(const ScanDev &s, const SweepDev &d, hipStream_t st) {
+  constexpr size_t lds = sizeof(SweepLds<T, NT, kOut>);
+  static_assert(lds <= 160 * 1024, "LDS");
+  const hipError_t e = hipFuncSetAttribute((const void *)k_scan_sweep<T, NT, kOut, kRev, kWideRows>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (e != hipSuccess) return e;
+  // at most 2^22: sequences are split only while they are few
+  const uint32_t work = s.batch * s.segs * s.heads * s.ptiles;
+  k_scan_sweep<T, NT, kOut, kRev, kWideRows><<<(work + 7) / 8 * 8, 256, lds, st>>>(s, d, work);
+  return hipGetLastError();
+}
+
+// The whole sweep: over segments first where there are several.  ws: carry_bytes.
+template <typename T, int NT, bool kOut, bool kRev, bool kWideRows>
+hipError_t run_sweep(const ScanDev &s, SweepDev d, char *ws, hipStream_t st) {
+  if (s.segs > 1) {
+    SweepDev first = d;
+    first.store = nullptr;
+    first.ends = (float *)ws;
+    first.totals = (float *)(ws + carry_states_bytes(s));
+    hipError_t e = launch_sweep<T, NT, false, kRev, kWideRows>(s, first, st);
+    if (e != hipSuccess) return e;
+    const uint64_t values = (uint64_t)s.batch * s.heads * s.head_dim * s.state_dim;
+    k_scan_carry<kRev><<<scan_grid(host_ceil_div(values, 256)), 256, 0, st>>>(
+        s, first.ends, first.totals, values);
+    d.starts = first.ends;
+  }
+  return launch_sweep<T, NT, kOut, kRev, kWideRows>(s, d, st);
 }
 
 // ---- one token
@@ -238,28 +456,37 @@ __global__ __launch_bounds__(256) void k_scan_step(nsfps_step_args a, uint32_t p
 
 }  // namespace
 
+// Never 0, though a call of many sequences needs none: what a caller has to
+// bring does not hang on how the work is split.
 uint64_t scan_bytes(const nsfps_scan_args &a) {
-  return scan_states_bytes(a) + scan_totals_bytes(a);
+  return std::max<uint64_t>(256, carry_bytes(scan_dev(a)));
 }
 
 hipError_t launch_scan(const nsfps_scan_args &a, hipStream_t st) {
-  ScanDev s = scan_dev(a);
-  s.states = (float *)a.workspace;
-  s.totals = (float *)((char *)a.workspace + scan_states_bytes(a));
-  const uint64_t work = a.batch * s.chunks * s.heads * s.ptiles;
-  const uint64_t values = a.batch * s.heads * (uint64_t)s.head_dim * s.state_dim;
-  return scan_by_type(a.dtype, a.state_dim, [&](auto t, auto n) {
+  const ScanDev s = scan_dev(a);
+  SweepDev d = {};
+  d.u = s.x;
+  d.v = s.b;
+  const bool wide = scan_wide(a, {&a.x, &a.b, &a.c, &a.y});
+  return scan_by_type(a.dtype, a.state_dim, wide, [&](auto t, auto n, auto w) {
+    return run_sweep<decltype(t), decltype(n)::value, true, false, decltype(w)::value>(
+        s, d, (char *)a.workspace, st);
+  });
+}
+
+hipError_t launch_states(const nsfps_scan_args &a, const ScanDev &s, const nsfps_rows &u,
+                         const nsfps_rows &v, float *store, bool reversed, char *ws,
+                         hipStream_t st) {
+  SweepDev d = {};
+  d.u = u;
+  d.v = v;
+  d.store = store;
+  return scan_by_type(a.dtype, a.state_dim, scan_wide(a, {&u, &v}), [&](auto t, auto n, auto w) {
     using T = decltype(t);
     constexpr int NT = decltype(n)::value;
-    k_scan_sums<T, NT, false><<<scan_grid(work), 256, 0, st>>>(s, s.x, s.b, s.wide_x, s.wide_bc,
-                                                               s.states, work);
-    k_scan_pass<false><<<scan_grid(host_ceil_div(values, 256)), 256, 0, st>>>(s, s.states, values);
-    constexpr size_t lds = sizeof(OutLds<T, NT>);
-    const hipError_t e = hipFuncSetAttribute((const void *)k_scan_out<T, NT>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-    k_scan_out<T, NT><<<scan_grid(work), 256, lds, st>>>(s, work);
-    return hipGetLastError();
+    constexpr bool kWideRows = decltype(w)::value;
+    return reversed ? run_sweep<T, NT, false, true, kWideRows>(s, d, ws, st)
+                    : run_sweep<T, NT, false, false, kWideRows>(s, d, ws, st);
   });
 }
 
@@ -279,7 +506,8 @@ hipError_t launch_scan_step(const nsfps_step_args &a, hipStream_t st) {
 }
 
 hipError_t preload_scan_kernels() {
-  return func_attributes(k_scan_out<bf16, 64>, k_scan_step<bf16, 4>, k_scan_pass<false>);
+  return func_attributes(k_scan_sweep<bf16, 64, true, false, true>, k_scan_step<bf16, 4>,
+                         k_scan_carry<false>);
 }
 
 }  // namespace nsfps

@@ -13,8 +13,8 @@
 // all terms from inside the chunk, so nothing cancels over the sequence.  Then
 // ddelta_t = a da_t + (what came through delta_t itself), ddt = ddelta sigmoid(raw).
 //
-// H and dH come from the forward's chunk sums and pass, and from the same two
-// kernels run over dy and c from the sequence's end (nothing is kept from the
+// H and dH come from the forward's sweep over the chunks, and from the same
+// kernel run over dy and c from the sequence's end (nothing is kept from the
 // forward call); then every chunk is done by itself, one workgroup per chunk
 // and group: a wave owns 16 tokens, as rows i for dc and as columns j for dx
 // and db, finds S and W in both orientations so that the weighted tiles are
@@ -36,10 +36,13 @@ namespace {
 
 struct GradDev {
   nsfps_rows dy, dx, db, dc, ddt;
-  const float *ends;   // dH: [batch][heads][chunks][head_dim][state_dim]
-  float *part;         // [3][heads][batch * chunks]: da, dd, ddt_bias
-  uint32_t wide_dy, wide_dx, wide_dbc;
+  // [batch][heads][chunks][head_dim][state_dim]: H, the state each chunk starts
+  // from, and dH, the gradient of the state it ends with
+  const float *states, *ends;
+  float *part;  // [3][heads][batch * chunks * 4]: da, dd, ddt_bias, one per wave
 };
+
+constexpr int kHeadAhead = 4;  // heads whose steps are found together, one by each wave
 
 template <typename T, int NT>
 struct GradLds {
@@ -47,36 +50,59 @@ struct GradLds {
   T x[kChunk * kLd<T, (int)kPTile>], dy[kChunk * kLd<T, (int)kPTile>];
   T b[kChunk * kLd<T, NT>], c[kChunk * kLd<T, NT>];
   T h[kTerms][kPTile * kLd<T, NT>];  // H, then dH
-  Steps st;
-  // by token: T's sums over j < i and (without delta_j) over i > j, its
-  // diagonal (without delta), c_i . e_i H^T dy_i, x_j . dH b_j to the chunk's end
-  double row_t[kChunk], col_u[kChunk];
-  float diag[kChunk], from[kChunk], thru[kChunk];
-  float red[8];  // per wave: <dH, H>, sum dy.x
+  Steps st[kHeadAhead];
+  // Sums over tokens that da needs, by wave: what is added from a token on
+  // (cancelling, not cancelling) and before it; <dH, H>
+  double after[4], from[4], before[4];
+  float whole[4];
 };
 
-// 64 x NT values of a state, head_dim rows from p0 on, as three terms each
-// (float32: one).  With H given too, returns this thread's part of <v, H>.
-template <typename T, int NT>
-__device__ __forceinline__ float load_state(GradLds<T, NT> &m, const float *v, const float *with,
-                                            uint32_t rows, uint32_t cols) {
-  float dot = 0.f;
-  for (uint32_t e = threadIdx.x; e < kPTile * (NT / 4); e += 256) {
-    const uint32_t p = e / (NT / 4), n = (e % (NT / 4)) * 4;
-    f32x4 q = {0.f, 0.f, 0.f, 0.f};
-    if (p < rows)
+// 64 x NT values of a state on their way from global memory to LDS.
+template <int NT, bool kWideRows>
+struct StateTile {
+  static constexpr int kPer = 64 * (NT / 4) / 256;
+  f32x4 v[kPer];
+  __device__ __forceinline__ void fetch(const float *g, uint32_t rows, uint32_t cols) {
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-        if (n + i < cols) {
-          q[i] = v[p * cols + n + i];
-          if (with) dot = fmaf(q[i], with[p * cols + n + i], dot);
-        }
-    const Terms<T, 3> t = split<T, 3>(q);
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + 256 * i, p = e / (NT / 4), n = (e % (NT / 4)) * 4;
+      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const NSFPS_GLOBAL_SEQ float *at = (const NSFPS_GLOBAL_SEQ float *)(g + p * cols + n);
+      if constexpr (kWideRows) {
+        if (p < rows && n < cols) v[i] = *(const NSFPS_GLOBAL_SEQ f32x4 *)at;
+      } else if (p < rows) {
 #pragma unroll
-    for (int k = 0; k < Terms<T, 3>::kN; ++k)
-      *(Quad<T> *)(m.h[k] + p * kLd<T, NT> + n) = t.q[k];
+        for (uint32_t k = 0; k < 4; ++k)
+          if (n + k < cols) v[i][k] = at[k];
+      }
+    }
   }
-  return dot;
+  template <typename T>
+  __device__ __forceinline__ void put(GradLds<T, NT> &m) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + 256 * i, p = e / (NT / 4), n = (e % (NT / 4)) * 4;
+      const Terms<T, 3> t = split<T, 3>(v[i]);
+#pragma unroll
+      for (int k = 0; k < Terms<T, 3>::kN; ++k) put_quad(m.h[k], kLd<T, NT>, p, n, t.q[k]);
+    }
+  }
+  __device__ __forceinline__ float dot(const StateTile &o) const {
+    float d = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d = fmaf(v[i][k], o.v[i][k], d);
+    return d;
+  }
+};
+
+// Keeps what is read from LDS on its side of this point: without it the
+// compiler reads the next products' operands ahead of these ones' until no
+// register is left.
+__device__ __forceinline__ void phase() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -91,10 +117,26 @@ __device__ __forceinline__ V column_sum(V v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+// v of lane l - K of the same 16 lanes, 0 where there is none (DPP row shift)
+template <int K>
+__device__ __forceinline__ double row_shift(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0u, (uint32_t)u, 0x110 + K, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(u >> 32), 0x110 + K, 0xf, 0xf, true);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+// inclusive sum over lanes 0 .. l of each 16
+__device__ __forceinline__ double row_scan(double v) {
+  v += row_shift<1>(v);
+  v += row_shift<2>(v);
+  v += row_shift<4>(v);
+  return v + row_shift<8>(v);
+}
+
 // Four values of a lane's column to a row of global memory.
-template <typename T>
-__device__ __forceinline__ void store_quad(T *dst, f32x4 v, uint32_t at, uint32_t cols, bool wide) {
-  if (wide) {
+template <typename T, bool kWideRows>
+__device__ __forceinline__ void store_quad(T *dst, f32x4 v, uint32_t at, uint32_t cols) {
+  if constexpr (kWideRows) {
     const float o[4] = {v[0], v[1], v[2], v[3]};
     if (at < cols) store_f32<T, 4>(dst + at, o);
   } else {
@@ -107,316 +149,340 @@ __device__ __forceinline__ void store_quad(T *dst, f32x4 v, uint32_t at, uint32_
 }
 
 template <typename T, int NT>
-__global__ __launch_bounds__(256) void k_scan_grad(ScanDev s, GradDev gr, uint64_t work) {
+constexpr int kGradGroups = 1;
+
+// Work item w: chunk bc = w / groups of all sequences' and group w % groups.
+template <typename T, int NT, bool kWideRows>
+__global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev s, GradDev gr,
+                                                                         uint64_t first_item,
+                                                                         uint32_t work) {
   extern __shared__ __attribute__((aligned(16))) char s_raw[];
   GradLds<T, NT> &m = *(GradLds<T, NT> *)s_raw;
   constexpr int ldx = kLd<T, (int)kPTile>, ldn = kLd<T, NT>, kT3 = Terms<T, 3>::kN,
-                kT2 = Terms<T, 2>::kN, kNt = NT / 16;
-  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, l = lane & 15u;
+                kT2 = Terms<T, 2>::kN, kNt = NT / 16, kNb = NT / 32, kPb = (int)kPTile / 32;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
+                 g = lane >> 4, l = lane & 15u;
   const uint32_t each = s.heads / s.groups;  // heads of a group
   const int own = 16 * wave + l;             // this lane's token, as i and as j
-  for (uint64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const uint32_t grp = (uint32_t)(w % s.groups);
-    const uint64_t bc = w / s.groups;
-    const uint32_t c = (uint32_t)(bc % s.chunks), b = (uint32_t)(bc / s.chunks);
-    const uint32_t len = scan_length(s, b), t0 = c * kChunk;
-    const uint32_t out_rows = min(kChunk, s.length - t0);
-    const uint32_t rows = t0 < len ? min(kChunk, len - t0) : 0u;
-    const bool writes = (uint32_t)own < out_rows;
-    const auto rows_at = [&](const nsfps_rows &r) {
-      return (T *)r.p + (uint64_t)b * r.batch_stride + (uint64_t)t0 * r.row_stride;
-    };
-    T *const db_row = rows_at(gr.db) + (uint64_t)own * gr.db.row_stride + grp * s.state_dim;
-    T *const dc_row = rows_at(gr.dc) + (uint64_t)own * gr.dc.row_stride + grp * s.state_dim;
-    if (rows == 0) {  // past the sequence's end: zeros
-      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-      if (writes) {
-        for (uint32_t nt = 0; nt < kNt; ++nt) {
-          store_quad<T>(db_row, z, 16 * nt + 4 * g, s.state_dim, false);
-          store_quad<T>(dc_row, z, 16 * nt + 4 * g, s.state_dim, false);
-        }
-        T *dx_row = rows_at(gr.dx) + (uint64_t)own * gr.dx.row_stride;
-        T *ddt_row = rows_at(gr.ddt) + (uint64_t)own * gr.ddt.row_stride;
-        for (uint32_t p = grp * each * s.head_dim + g; p < (grp + 1) * each * s.head_dim; p += 4)
-          store_quad<T>(dx_row + p, z, 0, 1, false);
-        for (uint32_t h = grp * each + g; h < (grp + 1) * each; h += 4)
-          store_quad<T>(ddt_row + h, z, 0, 1, false);
+  if (blockIdx.x >= work) return;
+  const uint64_t w = first_item + blockIdx.x, bc = w / s.groups;
+  const uint32_t grp = (uint32_t)(w % s.groups), h0 = grp * each, h1 = h0 + each;
+  const uint32_t c = (uint32_t)(bc % s.chunks), b = (uint32_t)(bc / s.chunks);
+  const uint32_t len = scan_length(s, b), t0 = c * kChunk, sn = s.state_dim;
+  const uint32_t out_rows = min(kChunk, s.length - t0);
+  const uint32_t rows = t0 < len ? min(kChunk, len - t0) : 0u;
+  const bool writes = (uint32_t)own < out_rows;
+  const uint64_t parts = (uint64_t)s.batch * s.chunks * 4;
+  const auto rows_at = [&](const nsfps_rows &r) {
+    return (T *)r.p + (uint64_t)b * r.batch_stride + (uint64_t)t0 * r.row_stride;
+  };
+  T *const db_row = rows_at(gr.db) + (uint64_t)own * gr.db.row_stride + grp * sn;
+  T *const dc_row = rows_at(gr.dc) + (uint64_t)own * gr.dc.row_stride + grp * sn;
+  T *const dx_row = rows_at(gr.dx) + (uint64_t)own * gr.dx.row_stride;
+  T *const ddt_row = rows_at(gr.ddt) + (uint64_t)own * gr.ddt.row_stride;
+  if (rows == 0) {  // past the sequence's end: zeros
+    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
+    if (writes) {
+      for (uint32_t nt = 0; nt < kNt; ++nt) {
+        store_quad<T, kWideRows>(db_row, z, 16 * nt + 4 * g, sn);
+        store_quad<T, kWideRows>(dc_row, z, 16 * nt + 4 * g, sn);
       }
-      if (threadIdx.x < 3)
-        for (uint32_t h = grp * each; h < (grp + 1) * each; ++h)
-          gr.part[((uint64_t)threadIdx.x * s.heads + h) * s.batch * s.chunks + bc] = 0.f;
-      continue;
+      for (uint32_t p = h0 * s.head_dim + 4 * g; p < h1 * s.head_dim; p += 16)
+        store_quad<T, kWideRows>(dx_row, z, p, h1 * s.head_dim);
+      for (uint32_t h = h0 + 4 * g; h < h1; h += 16) store_quad<T, false>(ddt_row, z, h, h1);
     }
-    load_tile<T, NT>(m.b, rows_at(s.b) + grp * s.state_dim, s.b.row_stride, rows, s.state_dim,
-                     s.wide_bc);
-    load_tile<T, NT>(m.c, rows_at(s.c) + grp * s.state_dim, s.c.row_stride, rows, s.state_dim,
-                     s.wide_bc);
-    __syncthreads();
+    if (threadIdx.x < 12)
+      for (uint32_t h = h0; h < h1; ++h)
+        gr.part[((uint64_t)(threadIdx.x >> 2) * s.heads + h) * parts + bc * 4 + (threadIdx.x & 3)] =
+            0.f;
+    return;
+  }
+  const bool one = s.ptiles == 1;  // the whole head in one tile: its loads run ahead
+  const T *const x_at = rows_at(s.x), *const dy_at = rows_at(gr.dy);
+  Tile<T, (int)kPTile, kWideRows> tx, tdy;
+  StateTile<NT, kWideRows> th, tdh;
+  const auto fetch_xdy = [&](uint32_t h, uint32_t pt) {
+    const uint32_t at = h * s.head_dim + pt * kPTile, cols = s.head_dim - pt * kPTile;
+    tx.fetch(x_at + at, s.x.row_stride, rows, cols);
+    tdy.fetch(dy_at + at, gr.dy.row_stride, rows, cols);
+  };
+  const auto state_at = [&](uint32_t h, uint32_t pt) {
+    return ((((uint64_t)b * s.heads + h) * s.chunks + c) * s.head_dim + pt * kPTile) * sn;
+  };
+  const auto fetch_h = [&](uint32_t h, uint32_t pt) {
+    th.fetch(gr.states + state_at(h, pt), s.head_dim - pt * kPTile, sn);
+  };
+  const auto fetch_dh = [&](uint32_t h, uint32_t pt) {
+    tdh.fetch(gr.ends + state_at(h, pt), s.head_dim - pt * kPTile, sn);
+  };
+  float raw = 0.f;  // of the head this wave finds the steps of
+  const auto fetch_raw = [&](uint32_t h) {
+    raw = 0.f;
+    if (h + wave < h1 && lane < rows) raw = raw_step<T>(s, b, h + wave, t0 + lane);
+  };
+  {
+    Tile<T, NT, kWideRows> tb, tc;
+    tb.fetch(rows_at(s.b) + grp * sn, s.b.row_stride, rows, sn);
+    tc.fetch(rows_at(s.c) + grp * sn, s.c.row_stride, rows, sn);
+    fetch_xdy(h0, 0);
+    if (one) fetch_h(h0, 0);
+    fetch_raw(h0);
+    tb.put(m.b);
+    tc.put(m.c);
+  }
+  __syncthreads();
 
-    // S with this wave's tokens as columns j (tiles of rows i >= its own) and,
-    // transposed, as columns i (tiles of rows j <= its own)
-    f32x4 s_j[4] = {}, s_i[4] = {};
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int nt = 0; nt < kNt; nt += 2) {
-        const int k0 = 16 * nt + 4 * g, k1 = k0 + 16;
-        if (t >= (int)wave)
-          mma_apart(s_j[t], quad_row<T>(m.c, ldn, 16 * t + l, k0), quad_row<T>(m.c, ldn, 16 * t + l, k1),
-              quad_row<T>(m.b, ldn, own, k0), quad_row<T>(m.b, ldn, own, k1));
-        if (t <= (int)wave)
-          mma_apart(s_i[t], quad_row<T>(m.b, ldn, 16 * t + l, k0), quad_row<T>(m.b, ldn, 16 * t + l, k1),
-              quad_row<T>(m.c, ldn, own, k0), quad_row<T>(m.c, ldn, own, k1));
+  // S with this wave's tokens as columns j (tiles of rows i >= its own) and,
+  // transposed, as columns i (tiles of rows j <= its own)
+  f32x4 s_j[4] = {}, s_i[4] = {};
+  unrolled<kNb>([&](auto kb) __attribute__((always_inline)) {
+    const Pair<T> bo = pair_row(m.b, ldn, own, kb, g), co = pair_row(m.c, ldn, own, kb, g);
+    unrolled<4>([&](auto t) __attribute__((always_inline)) {
+      if (t >= (int)wave) mma_apart(s_j[t], pair_row(m.c, ldn, 16 * t + l, kb, g), bo);
+      if (t <= (int)wave) mma_apart(s_i[t], pair_row(m.b, ldn, 16 * t + l, kb, g), co);
+    });
+  });
+
+  f32x4 db[kNt] = {}, dc[kNt] = {};
+  for (uint32_t h = h0; h < h1; ++h) {
+    const Steps &sp = m.st[(h - h0) % kHeadAhead];
+    phase();
+    // ---- W in both orientations, over head_dim
+    f32x4 w_j[4] = {}, w_i[4] = {};
+    for (uint32_t pt = 0; pt < s.ptiles; ++pt) {
+      if (pt || (!one && h > h0)) fetch_xdy(h, pt);
+      __syncthreads();  // all are done with the head (or tile) before
+      tx.put(m.x);
+      tdy.put(m.dy);
+      if (one) th.put(m);
+      if (pt == 0 && (h - h0) % kHeadAhead == 0) {
+        if (h + wave < h1) chunk_steps(m.st[wave], raw, lane < rows, s.a[h + wave]);
+        fetch_raw(h + kHeadAhead);
       }
+      __syncthreads();
+      if (one) fetch_dh(h, 0);
+      unrolled<kPb>([&](auto kb) __attribute__((always_inline)) {
+        const Pair<T> xo = pair_row(m.x, ldx, own, kb, g), go = pair_row(m.dy, ldx, own, kb, g);
+        unrolled<4>([&](auto t) __attribute__((always_inline)) {
+          if (t >= (int)wave) mma_apart(w_j[t], pair_row(m.dy, ldx, 16 * t + l, kb, g), xo);
+          if (t <= (int)wave) mma_apart(w_i[t], pair_row(m.x, ldx, 16 * t + l, kb, g), go);
+        });
+      });
     }
 
-    f32x4 db[kNt] = {}, dc[kNt] = {};
-    for (uint32_t h = grp * each; h < (grp + 1) * each; ++h) {
-      // ---- W in both orientations, over head_dim
-      f32x4 w_j[4] = {}, w_i[4] = {};
-      const auto load_xdy = [&](uint32_t p0) {
-        load_tile<T, (int)kPTile>(m.x, rows_at(s.x) + h * s.head_dim + p0, s.x.row_stride, rows,
-                                  s.head_dim - p0, s.wide_x);
-        load_tile<T, (int)kPTile>(m.dy, rows_at(gr.dy) + h * s.head_dim + p0, gr.dy.row_stride,
-                                  rows, s.head_dim - p0, gr.wide_dy);
-      };
-      for (uint32_t pt = 0; pt < s.ptiles; ++pt) {
-        load_xdy(pt * kPTile);
-        if (pt == 0 && wave == 0) chunk_steps<T>(s, m.st, b, h, t0, len);
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-          for (int kt = 0; kt < (int)kPTile / 16; kt += 2) {
-            const int k0 = 16 * kt + 4 * g, k1 = k0 + 16;
-            if (t >= (int)wave)
-              mma_apart(w_j[t], quad_row<T>(m.dy, ldx, 16 * t + l, k0),
-                  quad_row<T>(m.dy, ldx, 16 * t + l, k1), quad_row<T>(m.x, ldx, own, k0),
-                  quad_row<T>(m.x, ldx, own, k1));
-            if (t <= (int)wave)
-              mma_apart(w_i[t], quad_row<T>(m.x, ldx, 16 * t + l, k0),
-                  quad_row<T>(m.x, ldx, 16 * t + l, k1), quad_row<T>(m.dy, ldx, own, k0),
-                  quad_row<T>(m.dy, ldx, own, k1));
-          }
-        }
-        if (s.ptiles > 1) __syncthreads();  // the tiles are loaded again
-      }
-
-      // ---- the weighted tiles: M and G as columns j, G as columns i; sums of T
-      Terms<T, 2> m_j[4], g_j[4], g_i[4];
-      // L_ij S_ij W_ij without the diagonal, which counts nowhere: sums over i
-      // (u_off) and, times delta_j, over j (rt).  In float64, from products
-      // rounded alike in both orientations: below, sums over rows are taken
-      // from sums over columns, and what is in both must go.
-      double u_off = 0.0, rt = 0.0;
-      float diag = 0.f, dd = 0.f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        f32x4 mj = {0.f, 0.f, 0.f, 0.f}, gj = mj, gi = mj;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int o = 16 * t + 4 * g + r;  // the tile's other token
-          if (t >= (int)wave && o >= own) {
-            const float lw = decay_between(m.st, o, own);
-            const float ls = lw * s_j[t][r];
-            mj[r] = ls * m.st.delta[own];
-            gj[r] = lw * m.st.delta[own] * w_j[t][r];
-            if (o == own) {
-              dd = w_j[t][r];
-              diag = ls * dd;
-            } else {
-              u_off += (double)(ls * w_j[t][r]);
+    phase();
+    // ---- as rows i: G, and T's sums over j < i.  L_ij S_ij W_ij is summed in
+    // float64 and rounded alike in both orientations: below, sums over rows are
+    // taken from sums over columns, and what is in both must go.
+    double rt = 0.0;
+    {
+      Terms<T, 2> g_i[4];
+      const float hi = sp.hi[own], lo = sp.lo[own];
+      unrolled<4>([&](auto t) __attribute__((always_inline)) {
+        f32x4 gi = {0.f, 0.f, 0.f, 0.f};
+        if (t <= (int)wave) {
+          const int j0 = 16 * t + 4 * g;
+          const f32x4 dj = quad_of(sp.delta, j0), hj = quad_of(sp.hi, j0), lj = quad_of(sp.lo, j0);
+          unrolled<4>([&](auto r_) __attribute__((always_inline)) {
+              constexpr int r = decltype(r_)::value;
+            if (j0 + r <= own) {
+              const float lw = exp2_fast((hi - hj[r]) + (lo - lj[r]));
+              gi[r] = lw * dj[r] * w_i[t][r];
+              if (j0 + r != own)
+                rt = fma((double)((lw * s_i[t][r]) * w_i[t][r]), (double)dj[r], rt);
             }
-          }
-          if (t <= (int)wave && o <= own) {
-            const float lw = decay_between(m.st, own, o);
-            gi[r] = lw * m.st.delta[o] * w_i[t][r];
-            if (o != own) rt = fma((double)((lw * s_i[t][r]) * w_i[t][r]), (double)m.st.delta[o], rt);
-          }
+          });
+        }
+        g_i[t] = split<T, 2>(gi);
+      });
+      rt = column_sum(rt);
+      unrolled<2>([&](auto kb) __attribute__((always_inline)) {
+        if (2 * kb <= (int)wave) {
+          unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
+            const Pair<T> a = pair_col(m.b, ldn, kb, 16 * nt, g, l);
+            unrolled<kT2>([&](auto k) __attribute__((always_inline)) {
+              mma(dc[nt], a, Pair<T>{g_i[2 * kb].q[k], g_i[2 * kb + 1].q[k]});
+            });
+          });
+        }
+      });
+    }
+    phase();
+    // ---- as columns j: M and G, and T's sums over i > j without delta_j
+    Terms<T, 2> m_j[4];
+    double u_off = 0.0;
+    float diag = 0.f, dd = 0.f;
+    const float delta = sp.delta[own];
+    {
+      Terms<T, 2> g_j[4];
+      const float hj = sp.hi[own], lj = sp.lo[own];
+      unrolled<4>([&](auto t) __attribute__((always_inline)) {
+        f32x4 mj = {0.f, 0.f, 0.f, 0.f}, gj = mj;
+        if (t >= (int)wave) {
+          const int i0 = 16 * t + 4 * g;
+          const f32x4 hi = quad_of(sp.hi, i0), lo = quad_of(sp.lo, i0);
+          unrolled<4>([&](auto r_) __attribute__((always_inline)) {
+              constexpr int r = decltype(r_)::value;
+            if (i0 + r >= own) {
+              const float lw = exp2_fast((hi[r] - hj) + (lo[r] - lj));
+              const float ls = lw * s_j[t][r];
+              mj[r] = ls * delta;
+              gj[r] = lw * delta * w_j[t][r];
+              if (i0 + r == own) {
+                dd = w_j[t][r];
+                diag = ls * dd;
+              } else {
+                u_off += (double)(ls * w_j[t][r]);
+              }
+            }
+          });
         }
         m_j[t] = split<T, 2>(mj);
         g_j[t] = split<T, 2>(gj);
-        g_i[t] = split<T, 2>(gi);
-      }
+      });
       u_off = column_sum(u_off);
-      rt = column_sum(rt);
       diag = column_sum(diag);
-      dd = wave_sum(dd);
-
-      // ---- db and dc inside the chunk
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt) {
-#pragma unroll
-        for (int tt = 0; tt < 2; ++tt) {
-          const int k0 = 32 * tt + 4 * g, k1 = k0 + 16;
-          if (2 * tt + 1 >= (int)wave) {
-            const Quad<T> a0 = quad_col<T>(m.c, ldn, k0, 16 * nt + l);
-            const Quad<T> a1 = quad_col<T>(m.c, ldn, k1, 16 * nt + l);
-#pragma unroll
-            for (int k = 0; k < kT2; ++k) mma(db[nt], a0, a1, g_j[2 * tt].q[k], g_j[2 * tt + 1].q[k]);
-          }
-          if (2 * tt <= (int)wave) {
-            const Quad<T> a0 = quad_col<T>(m.b, ldn, k0, 16 * nt + l);
-            const Quad<T> a1 = quad_col<T>(m.b, ldn, k1, 16 * nt + l);
-#pragma unroll
-            for (int k = 0; k < kT2; ++k) mma(dc[nt], a0, a1, g_i[2 * tt].q[k], g_i[2 * tt + 1].q[k]);
-          }
+      unrolled<2>([&](auto kb) __attribute__((always_inline)) {
+        if (2 * kb + 1 >= (int)wave) {
+          unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
+            const Pair<T> a = pair_col(m.c, ldn, kb, 16 * nt, g, l);
+            unrolled<kT2>([&](auto k) __attribute__((always_inline)) {
+              mma(db[nt], a, Pair<T>{g_j[2 * kb].q[k], g_j[2 * kb + 1].q[k]});
+            });
+          });
         }
-      }
-
-      // ---- what passes through the states, 64 rows of them at a time
-      const float e_i = exp2_fast(m.st.hi[own] + m.st.lo[own]);
-      const float to_end = decay_between(m.st, kChunk - 1, own), w_end = m.st.delta[own] * to_end;
-      float thru = 0.f, dot = 0.f;
-      f32x4 dci[kNt] = {};
-      for (uint32_t pt = 0; pt < s.ptiles; ++pt) {
-        const uint32_t p0 = pt * kPTile, pn = min(kPTile, s.head_dim - p0);
-        const uint64_t at = ((((uint64_t)b * s.heads + h) * s.chunks + c) * s.head_dim + p0) *
-                            s.state_dim;
-        if (s.ptiles > 1) load_xdy(p0);
-        load_state<T, NT>(m, s.states + at, nullptr, pn, s.state_dim);
-        __syncthreads();
-        // H^T dy_i
-#pragma unroll
-        for (int nt = 0; nt < kNt; ++nt) {
-          f32x4 low = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kt = 0; kt < (int)kPTile / 16; kt += 2) {
-            const int k0 = 16 * kt + 4 * g, k1 = k0 + 16;
-            const Quad<T> b0 = quad_row<T>(m.dy, ldx, own, k0), b1 = quad_row<T>(m.dy, ldx, own, k1);
-#pragma unroll
-            for (int k = kT3 - 1; k > 0; --k)
-              mma(low, quad_col<T>(m.h[k], ldn, k0, 16 * nt + l),
-                  quad_col<T>(m.h[k], ldn, k1, 16 * nt + l), b0, b1);
-            mma_apart(dci[nt], quad_col<T>(m.h[0], ldn, k0, 16 * nt + l),
-                      quad_col<T>(m.h[0], ldn, k1, 16 * nt + l), b0, b1);
-          }
-          dci[nt] += low;
-        }
-        __syncthreads();
-        dot += load_state<T, NT>(m, gr.ends + at, s.states + at, pn, s.state_dim);
-        __syncthreads();
-        // dH^T x_j
-#pragma unroll
-        for (int nt = 0; nt < kNt; ++nt) {
-          f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int kt = 0; kt < (int)kPTile / 16; kt += 2) {
-            const int k0 = 16 * kt + 4 * g, k1 = k0 + 16;
-#pragma unroll
-            for (int k = 0; k < kT3; ++k)
-              mma(v, quad_col<T>(m.h[k], ldn, k0, 16 * nt + l),
-                  quad_col<T>(m.h[k], ldn, k1, 16 * nt + l), quad_row<T>(m.x, ldx, own, k0),
-                  quad_row<T>(m.x, ldx, own, k1));
-          }
-          db[nt] += v * w_end;
-        }
-        // dx: through the chunk, and dH b_j
-        const float dskip = s.d ? s.d[h] : 0.f;
-        T *const dx_row = rows_at(gr.dx) + (uint64_t)own * gr.dx.row_stride + h * s.head_dim + p0;
-#pragma unroll
-        for (int q = 0; q < (int)kPTile / 16; ++q) {
-          f32x4 in = {0.f, 0.f, 0.f, 0.f}, thr = in, low = in;
-#pragma unroll
-          for (int tt = 0; tt < 2; ++tt)
-            if (2 * tt + 1 >= (int)wave) {
-              const Quad<T> a0 = quad_col<T>(m.dy, ldx, 32 * tt + 4 * g, 16 * q + l);
-              const Quad<T> a1 = quad_col<T>(m.dy, ldx, 32 * tt + 16 + 4 * g, 16 * q + l);
-#pragma unroll
-              for (int k = 0; k < kT2; ++k) mma(in, a0, a1, m_j[2 * tt].q[k], m_j[2 * tt + 1].q[k]);
-            }
-#pragma unroll
-          for (int nt = 0; nt < kNt; nt += 2) {
-            const int k0 = 16 * nt + 4 * g, k1 = k0 + 16;
-            const Quad<T> b0 = quad_row<T>(m.b, ldn, own, k0), b1 = quad_row<T>(m.b, ldn, own, k1);
-#pragma unroll
-            for (int k = kT3 - 1; k > 0; --k)
-              mma(low, quad_row<T>(m.h[k], ldn, 16 * q + l, k0),
-                  quad_row<T>(m.h[k], ldn, 16 * q + l, k1), b0, b1);
-            mma_apart(thr, quad_row<T>(m.h[0], ldn, 16 * q + l, k0),
-                      quad_row<T>(m.h[0], ldn, 16 * q + l, k1), b0, b1);
-          }
-          thr += low;
-          const f32x4 xv = quad_f32(quad_row<T>(m.x, ldx, own, 16 * q + 4 * g));
-          const f32x4 gv = quad_f32(quad_row<T>(m.dy, ldx, own, 16 * q + 4 * g));
-          f32x4 o;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            thru = fmaf(xv[r], thr[r], thru);
-            o[r] = (uint32_t)own < rows ? fmaf(dskip, gv[r], fmaf(w_end, thr[r], in[r])) : 0.f;
-          }
-          if (writes) store_quad<T>(dx_row, o, 16 * q + 4 * g, pn, gr.wide_dx);
-        }
-        if (pt + 1 < s.ptiles) __syncthreads();
-      }
-      thru = column_sum(thru) * to_end;  // per delta_j
-      // dc through the states, and its part of the exponents' gradient
-      float ri = 0.f;
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt) {
-        const f32x4 cv = quad_f32(quad_row<T>(m.c, ldn, own, 16 * nt + 4 * g));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ri = fmaf(cv[r], dci[nt][r], ri);
-        dc[nt] += dci[nt] * e_i;
-      }
-      if (g == 0) {
-        m.row_t[own] = rt;
-        m.col_u[own] = u_off;
-        m.thru[own] = thru;
-      }
-      ri = column_sum(ri) * e_i;
-      if (g == 1) {
-        m.from[own] = ri;
-        m.diag[own] = diag;
-      }
-      dot = wave_sum(dot);
-      if (lane == 0) {
-        m.red[wave] = dot;
-        m.red[4 + wave] = dd;
-      }
-      __syncthreads();
-      // ---- the exponents: sums over the chunk's tokens from each on, and before it
-      if (wave == 0) {
-        const float delta = m.st.delta[lane];
-        double after = m.row_t[lane] - (double)delta * m.col_u[lane];  // cancels, so first
-        double from = m.from[lane];
-        const double mine = (double)delta * m.thru[lane];
-        double before = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-          const double a2 = __shfl_down(after, off, 64), b2 = __shfl_up(before, off, 64);
-          const double f2 = __shfl_down(from, off, 64);
-          if (lane + off < 64) after += a2, from += f2;
-          if (lane >= (uint32_t)off) before += b2;
-        }
-        const float whole = exp2_fast(m.st.hi[kChunk - 1] + m.st.lo[kChunk - 1]) *
-                            (m.red[0] + m.red[1] + m.red[2] + m.red[3]);
-        const float da = (float)(after + from + (before - mine)) + whole;
-        float ddt = 0.f;
-        if (lane < rows)
-          ddt = fmaf(s.a[h], da, (float)m.col_u[lane] + m.diag[lane] + m.thru[lane]) *
-                sigmoid(raw_step<T>(s, b, h, t0 + lane));
-        const float o[1] = {ddt};
-        if (lane < out_rows)
-          store_f32<T, 1>(rows_at(gr.ddt) + (uint64_t)lane * gr.ddt.row_stride + h, o);
-        const float sda = wave_sum(delta * da), sdt = wave_sum(ddt);
-        if (lane == 0) {
-          const uint64_t per = (uint64_t)s.batch * s.chunks;
-          gr.part[(uint64_t)h * per + bc] = sda;
-          gr.part[((uint64_t)s.heads + h) * per + bc] = m.red[4] + m.red[5] + m.red[6] + m.red[7];
-          gr.part[((uint64_t)2 * s.heads + h) * per + bc] = sdt;
-        }
-      }
-      __syncthreads();
+      });
     }
-    if (writes) {
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt) {
-        store_quad<T>(db_row, db[nt], 16 * nt + 4 * g, s.state_dim, gr.wide_dbc);
-        store_quad<T>(dc_row, dc[nt], 16 * nt + 4 * g, s.state_dim, gr.wide_dbc);
+
+    phase();
+    // ---- what passes through the states, 64 rows of them at a time
+    const float e_i = sp.e[own], to_end = sp.end[own], w_end = delta * to_end;
+    float thru = 0.f, dot = 0.f, from = 0.f;
+    for (uint32_t pt = 0; pt < s.ptiles; ++pt) {
+      const uint32_t p0 = pt * kPTile, pn = s.head_dim - p0;
+      if (!one) {
+        fetch_xdy(h, pt);
+        fetch_h(h, pt);
+        __syncthreads();
+        tx.put(m.x);
+        tdy.put(m.dy);
+        th.put(m);
+        __syncthreads();
+        fetch_dh(h, pt);
       }
+      // H^T dy_i
+      unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
+        phase();
+        f32x4 v = {0.f, 0.f, 0.f, 0.f}, low = v;
+        unrolled<kPb>([&](auto kb) __attribute__((always_inline)) {
+          const Pair<T> go = pair_row(m.dy, ldx, own, kb, g);
+#pragma unroll
+          for (int k = kT3 - 1; k > 0; --k) mma(low, pair_col(m.h[k], ldn, kb, 16 * nt, g, l), go);
+          mma_apart(v, pair_col(m.h[0], ldn, kb, 16 * nt, g, l), go);
+        });
+        v += low;
+        const f32x4 cv = quad_f32(quad_row(m.c, ldn, own, 16 * nt + 4 * g));
+        unrolled<4>([&](auto r_) __attribute__((always_inline)) {
+              constexpr int r = decltype(r_)::value; from = fmaf(cv[r], v[r], from);
+        });
+        dc[nt] += v * e_i;
+      });
+      __syncthreads();
+      tdh.put(m);
+      dot += tdh.dot(th);
+      __syncthreads();
+      if (one && h + 1 < h1) {
+        fetch_xdy(h + 1, 0);
+        fetch_h(h + 1, 0);
+      }
+      // dH^T x_j
+      unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
+        phase();
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        unrolled<kPb>([&](auto kb) __attribute__((always_inline)) {
+          const Pair<T> xo = pair_row(m.x, ldx, own, kb, g);
+#pragma unroll
+          for (int k = kT2 - 1; k >= 0; --k) mma(v, pair_col(m.h[k], ldn, kb, 16 * nt, g, l), xo);
+        });
+        db[nt] += v * w_end;
+      });
+      // dx: through the chunk, and dH b_j
+      const float skip = s.d ? s.d[h] : 0.f;
+      unrolled<(int)kPTile / 16>([&](auto q) __attribute__((always_inline)) {
+        phase();
+        f32x4 in = {0.f, 0.f, 0.f, 0.f}, thr = in, low = in;
+        unrolled<2>([&](auto kb) __attribute__((always_inline)) {
+          if (2 * kb + 1 >= (int)wave) {
+            const Pair<T> a = pair_col(m.dy, ldx, kb, 16 * q, g, l);
+            unrolled<kT2>([&](auto k) __attribute__((always_inline)) {
+              mma(in, a, Pair<T>{m_j[2 * kb].q[k], m_j[2 * kb + 1].q[k]});
+            });
+          }
+        });
+        unrolled<kNb>([&](auto kb) __attribute__((always_inline)) {
+          const Pair<T> bo = pair_row(m.b, ldn, own, kb, g);
+#pragma unroll
+          for (int k = kT3 - 1; k > 0; --k) mma(low, pair_row(m.h[k], ldn, 16 * q + l, kb, g), bo);
+          mma_apart(thr, pair_row(m.h[0], ldn, 16 * q + l, kb, g), bo);
+        });
+        thr += low;
+        const f32x4 xv = quad_f32(quad_row(m.x, ldx, own, 16 * q + 4 * g));
+        const f32x4 gv = quad_f32(quad_row(m.dy, ldx, own, 16 * q + 4 * g));
+        f32x4 o;
+        unrolled<4>([&](auto r_) __attribute__((always_inline)) {
+              constexpr int r = decltype(r_)::value;
+          thru = fmaf(xv[r], thr[r], thru);
+          o[r] = (uint32_t)own < rows ? fmaf(skip, gv[r], fmaf(w_end, thr[r], in[r])) : 0.f;
+        });
+        if (writes) store_quad<T, kWideRows>(dx_row + h * s.head_dim + p0, o, 16 * q + 4 * g, pn);
+      });
     }
+    phase();
+    thru = column_sum(thru) * to_end;  // per delta_j
+    from = column_sum(from) * e_i;
+    dot = wave_sum(dot);
+
+    // ---- the exponents: sums over the chunk's tokens from each on, and before
+    // it.  The 16 tokens of a wave are lanes l of each quarter, so the quarters
+    // take one of the sums each.
+    const double after = rt - (double)delta * u_off;  // cancels over the tokens
+    const double mine = (double)delta * thru;
+    const double sum = row_scan(g == 0 ? after : g == 1 ? (double)from : mine);
+    if (l == 15) {
+      if (g == 0) m.after[wave] = sum;
+      if (g == 1) m.from[wave] = sum;
+      if (g == 2) m.before[wave] = sum;
+      if (g == 3) m.whole[wave] = dot;
+    }
+    const double sum_after = __shfl(sum, l, 64), sum_from = __shfl(sum, 16 + l, 64),
+                 sum_before = __shfl(sum, 32 + l, 64);
     __syncthreads();
+    double a_on = after - sum_after, f_on = (double)from - sum_from, before = sum_before - mine;
+    unrolled<4>([&](auto o) __attribute__((always_inline)) {
+      if (o >= (int)wave) a_on += m.after[o], f_on += m.from[o];
+      if (o < (int)wave) before += m.before[o];
+    });
+    const float whole =
+        exp2_fast(sp.total) * (m.whole[0] + m.whole[1] + m.whole[2] + m.whole[3]);
+    const float da = (float)(a_on + f_on + before) + whole;
+    const float ddt = fmaf(s.a[h], da, (float)u_off + diag + thru) * sp.sig[own];
+    const float o[1] = {ddt};
+    if (writes && g == 0) store_f32<T, 1>(ddt_row + h, o);
+    // one quarter each: da, ddt_bias; dd is on the diagonal's lanes
+    const float sums = (float)row_scan(g == 0 ? (double)delta * da : (double)ddt);
+    dd = wave_sum(dd);
+    float *part = gr.part + (uint64_t)h * parts + bc * 4 + wave;
+    if (l == 15) {
+      if (g == 0) part[0] = sums;
+      if (g == 1) part[2 * s.heads * parts] = sums;
+      if (g == 2) part[s.heads * parts] = dd;
+    }
+  }
+  if (writes) {
+    unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
+      store_quad<T, kWideRows>(db_row, db[nt], 16 * nt + 4 * g, sn);
+      store_quad<T, kWideRows>(dc_row, dc[nt], 16 * nt + 4 * g, sn);
+    });
   }
 }
 
@@ -438,65 +504,67 @@ __global__ __launch_bounds__(256) void k_scan_grad_join(const float *__restrict_
 }
 
 uint64_t part_bytes(const nsfps_scan_args &a) {
-  return (12 * a.batch * a.heads * host_ceil_div(a.length, kChunk) + 255) & ~255ull;
+  return round256(48 * a.batch * a.heads * host_ceil_div(a.length, kChunk));
 }
 
 }  // namespace
 
+namespace {
+uint64_t chunk_states_bytes(const ScanDev &s) {
+  return round256(4ull * s.batch * s.heads * s.chunks * s.head_dim * s.state_dim);
+}
+}  // namespace
+
 uint64_t scan_grad_bytes(const nsfps_scan_args &a) {
-  return 2 * scan_states_bytes(a) + scan_totals_bytes(a) + part_bytes(a);
+  const ScanDev s = scan_dev(a);
+  return 2 * chunk_states_bytes(s) + part_bytes(a) + carry_bytes(s);
 }
 
 hipError_t launch_scan_grad(const nsfps_scan_args &a, const nsfps_scan_grads &g, hipStream_t st) {
-  ScanDev s = scan_dev(a);
+  const ScanDev s = scan_dev(a);
   char *const ws = (char *)a.workspace;
-  s.states = (float *)ws;
-  float *const ends = (float *)(ws + scan_states_bytes(a));
-  s.totals = (float *)(ws + 2 * scan_states_bytes(a));
+  float *const states = (float *)ws, *const ends = (float *)(ws + chunk_states_bytes(s));
+  char *const carry = ws + 2 * chunk_states_bytes(s) + part_bytes(a);
   GradDev d = {};
   d.dy = g.dy;
   d.dx = g.dx;
   d.db = g.db;
   d.dc = g.dc;
   d.ddt = g.ddt;
+  d.states = states;
   d.ends = ends;
-  d.part = (float *)(ws + 2 * scan_states_bytes(a) + scan_totals_bytes(a));
-  const uint32_t size = a.dtype == NSFPS_F32 ? 4 : 2, v = 16 / size;
-  d.wide_dy = rows_wide(g.dy, size) && a.head_dim % v == 0;
-  d.wide_dx = rows_wide(g.dx, size) && a.head_dim % v == 0;
-  d.wide_dbc = rows_wide(g.db, size) && rows_wide(g.dc, size) && a.state_dim % v == 0;
-  const uint64_t parts = a.batch * s.chunks, sums = parts * s.heads * s.ptiles,
-                 work = parts * s.groups;
-  const uint64_t values = a.batch * s.heads * (uint64_t)s.head_dim * s.state_dim;
-  const auto run = [&](auto t, auto n) {
-    using T = decltype(t);
-    constexpr int NT = decltype(n)::value;
-    k_scan_sums<T, NT, false><<<scan_grid(sums), 256, 0, st>>>(s, s.x, s.b, s.wide_x, s.wide_bc,
-                                                               s.states, sums);
-    k_scan_sums<T, NT, true><<<scan_grid(sums), 256, 0, st>>>(s, d.dy, s.c, d.wide_dy, s.wide_bc,
-                                                              ends, sums);
-    const uint32_t pass = scan_grid(host_ceil_div(values, 256));
-    k_scan_pass<false><<<pass, 256, 0, st>>>(s, s.states, values);
-    k_scan_pass<true><<<pass, 256, 0, st>>>(s, ends, values);
-    constexpr size_t lds = sizeof(GradLds<T, NT>);
-    static_assert(lds <= 160 * 1024, "LDS");
-    const hipError_t e = hipFuncSetAttribute((const void *)k_scan_grad<T, NT>,
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) return e;
-    k_scan_grad<T, NT><<<scan_grid(work), 256, lds, st>>>(s, d, work);
-    return hipGetLastError();
-  };
+  d.part = (float *)(ws + 2 * chunk_states_bytes(s));
+  const uint64_t parts = a.batch * s.chunks, work = parts * s.groups;
   if (work) {
-    const hipError_t e = scan_by_type(a.dtype, a.state_dim, run);
+    hipError_t e = launch_states(a, s, s.x, s.b, states, false, carry, st);
+    if (e == hipSuccess) e = launch_states(a, s, d.dy, s.c, ends, true, carry, st);
+    if (e != hipSuccess) return e;
+    const bool wide = scan_wide(a, {&a.x, &a.b, &a.c, &g.dy, &g.dx, &g.db, &g.dc});
+    e = scan_by_type(a.dtype, a.state_dim, wide, [&](auto t, auto n, auto w) {
+      using T = decltype(t);
+      constexpr int NT = decltype(n)::value;
+      constexpr bool kWideRows = decltype(w)::value;
+      constexpr size_t lds = sizeof(GradLds<T, NT>);
+      static_assert(lds <= 160 * 1024, "LDS");
+      const hipError_t e2 = hipFuncSetAttribute((const void *)k_scan_grad<T, NT, kWideRows>,
+                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e2 != hipSuccess) return e2;
+      constexpr uint64_t kLaunch = 1u << 23;  // workgroups of a launch: fewer than 2^32 threads
+      for (uint64_t at = 0; at < work; at += kLaunch) {
+        const uint32_t some = (uint32_t)std::min(kLaunch, work - at);
+        k_scan_grad<T, NT, kWideRows><<<some, 256, lds, st>>>(s, d, at, some);
+      }
+      return hipGetLastError();
+    });
     if (e != hipSuccess) return e;
   }
-  k_scan_grad_join<<<dim3(a.heads, 3), 256, 0, st>>>(d.part, parts, a.heads, g.d_da, g.d_dd,
+  k_scan_grad_join<<<dim3(a.heads, 3), 256, 0, st>>>(d.part, 4 * parts, a.heads, g.d_da, g.d_dd,
                                                      g.d_ddt_bias);
   return hipGetLastError();
 }
 
 hipError_t preload_scan_grad_kernels() {
-  return func_attributes(k_scan_grad<bf16, 64>, k_scan_grad_join);
+  return func_attributes(k_scan_grad<bf16, 64, true>, k_scan_grad_join);
 }
 
 }  // namespace nsfps

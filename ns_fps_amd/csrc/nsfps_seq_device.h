@@ -9,6 +9,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+#include <utility>
+
 #if defined(__HIP_DEVICE_COMPILE__)
 #define NSFPS_GLOBAL_SEQ __attribute__((address_space(1)))
 #else
@@ -135,6 +138,19 @@ __device__ __forceinline__ float sigmoid(float x) {
 __device__ __forceinline__ float softplus(float x) {
   const float e = exp2_fast(-fabsf(x) * kLog2e);
   return fmaxf(x, 0.f) + log1pf(e);
+}
+
+// f(0), f(1) .. f(N - 1) with the index a constant: arrays of registers are
+// indexed by constants whatever the optimizer's order of passes.  (A loop that
+// is unrolled late leaves its arrays to be merged into one wide value, which
+// is then copied whole for every element that changes.)
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  unrolled_of(f, std::make_integer_sequence<int, N>());
 }
 
 __device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
