@@ -16,6 +16,7 @@
 #include "nsfps_seq_device.h"
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #pragma clang fp contract(fast)
@@ -26,9 +27,11 @@ using namespace seq;
 
 namespace {
 
-constexpr uint32_t kTile = 16;      // tokens of a thread's walk (>= W - 1: only tile 0 reads history)
+constexpr uint32_t kTile = 32;      // tokens of a thread's walk (>= W - 1: only tile 0 reads history)
 constexpr uint32_t kGradTile = 32;  // the same of the gradient's
 constexpr uint32_t kAhead = 4;      // rows loaded together
+constexpr int kVec = 8;      // bfloat16 channels of a thread
+constexpr int kGradVec = 8;  // the same of the gradient's (4: as fast, but twice the sums to join)
 
 // A launch's sequences, as the kernels see them.
 struct Seqs {
@@ -63,14 +66,14 @@ __device__ __forceinline__ void load_weights(const T *__restrict__ weight, uint3
   }
 }
 
-// cvb: channel vectors a workgroup holds (a power of two <= 64); the other
-// threads take further tiles of tokens.
+// A workgroup holds cvb channel vectors of `per` tiles of tokens, in its first
+// cvb * per threads.
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void k_conv(nsfps_rows x, nsfps_rows y, Seqs s,
                                               const T *__restrict__ weight,
                                               const T *__restrict__ bias, T *cache, uint32_t vecs,
-                                              uint32_t cvb, uint32_t tiles, uint64_t work) {
-  const uint32_t cgroups = ceil_div(vecs, cvb), per = 256 / cvb;
+                                              uint32_t cvb, uint32_t per, uint32_t tiles, uint64_t work) {
+  const uint32_t cgroups = ceil_div(vecs, cvb);
   const uint32_t cl = threadIdx.x % cvb, tl = threadIdx.x / cvb;
   const uint32_t tgroups = ceil_div(tiles, per);
   for (uint64_t i = blockIdx.x; i < work; i += gridDim.x) {
@@ -79,9 +82,8 @@ __global__ __launch_bounds__(256) void k_conv(nsfps_rows x, nsfps_rows y, Seqs s
     const uint64_t r = i / cgroups;
     const uint32_t tile = (uint32_t)(r % tgroups) * per + tl;
     const uint32_t b = (uint32_t)(r / tgroups);
-    if (c >= vecs || tile >= tiles) continue;
+    if (c >= vecs || tl >= per || tile >= tiles) continue;
     const uint32_t len = seq_length(s, b), t0 = tile * kTile;
-    const uint32_t t1 = min((uint64_t)t0 + kTile, s.length);
     const T *xr = (const T *)x.p + (uint64_t)b * x.batch_stride + (uint64_t)c * V;
     T *yr = (T *)y.p + (uint64_t)b * y.batch_stride + (uint64_t)c * V;
     float w[V * W], bs[V] = {};
@@ -105,34 +107,47 @@ __global__ __launch_bounds__(256) void k_conv(nsfps_rows x, nsfps_rows y, Seqs s
         load_f32<T, V>(ring + (uint64_t)((pos + t) % W) * ring_row, win[k]);
       }
     }
-    for (uint32_t t = t0; t < t1; t += kAhead) {
-      float in[kAhead][V];
+    // kFull: the whole tile lies inside the sequence
+    const auto walk = [&](auto full) {
+      constexpr bool kFull = decltype(full)::value;
+      Raw<T, V> in[kAhead], next[kAhead];
+      const auto load = [&](uint32_t t, Raw<T, V>(&o)[kAhead]) {
 #pragma unroll
-      for (uint32_t a = 0; a < kAhead; ++a) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) in[a][j] = 0.f;
-        if (t + a < len) load_f32<T, V>(xr + (uint64_t)(t + a) * x.row_stride, in[a]);
-      }
-#pragma unroll
-      for (uint32_t a = 0; a < kAhead; ++a) {
-        if (t + a >= t1) break;
-#pragma unroll
-        for (int j = 0; j < V; ++j) win[W - 1][j] = in[a][j];
-        float o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float pre = bs[j];
-#pragma unroll
-          for (int k = 0; k < W; ++k) pre = fmaf(w[j * W + k], win[k][j], pre);
-          o[j] = t + a < len ? pre * sigmoid(pre) : 0.f;
+        for (uint32_t a = 0; a < kAhead; ++a) {
+          o[a] = zero_raw<T, V>();
+          if (kFull || t + a < len) o[a] = load_raw<T, V>(xr + (uint64_t)(t + a) * x.row_stride);
         }
-        store_f32<T, V>(yr + (uint64_t)(t + a) * y.row_stride, o);
+      };
+      load(t0, in);
+#pragma unroll 1
+      for (uint32_t i = 0; i < kTile; i += kAhead) {
+        if (i + kAhead < kTile) load(t0 + i + kAhead, next);
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k)
+        for (uint32_t a = 0; a < kAhead; ++a) {
+          const uint32_t t = t0 + i + a;
+          numbers<T, V>(in[a], win[W - 1]);
+          float o[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) win[k][j] = win[k + 1][j];
+          for (int j = 0; j < V; ++j) {
+            float pre = bs[j];
+#pragma unroll
+            for (int k = 0; k < W; ++k) pre = fmaf(w[j * W + k], win[k][j], pre);
+            o[j] = kFull || t < len ? pre * sigmoid(pre) : 0.f;
+          }
+          if (kFull || t < s.length) store_f32<T, V>(yr + (uint64_t)t * y.row_stride, o);
+#pragma unroll
+          for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) win[k][j] = win[k + 1][j];
+        }
+#pragma unroll
+        for (uint32_t a = 0; a < kAhead; ++a) in[a] = next[a];
       }
-    }
+    };
+    if ((uint64_t)t0 + kTile <= len)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
     // The thread that read the ring's history writes its new entries.
     if (tile == 0 && slot >= 0) {
 #pragma unroll
@@ -153,10 +168,10 @@ __global__ __launch_bounds__(256) void k_conv_grad(nsfps_rows x, nsfps_rows dy, 
                                                    Seqs s, const T *__restrict__ weight,
                                                    const T *__restrict__ bias,
                                                    float *__restrict__ part, uint32_t vecs,
-                                                   uint32_t cvb, uint32_t tiles, uint64_t work) {
+                                                   uint32_t cvb, uint32_t per, uint32_t tiles, uint64_t work) {
   constexpr int kSums = V * (W + 1);
   __shared__ float s_sum[kSums][256];
-  const uint32_t cgroups = ceil_div(vecs, cvb), per = 256 / cvb;
+  const uint32_t cgroups = ceil_div(vecs, cvb);
   const uint32_t cl = threadIdx.x % cvb, tl = threadIdx.x / cvb;
   const uint32_t tgroups = ceil_div(tiles, per);
   for (uint64_t i = blockIdx.x; i < work; i += gridDim.x) {
@@ -164,12 +179,10 @@ __global__ __launch_bounds__(256) void k_conv_grad(nsfps_rows x, nsfps_rows dy, 
     const uint64_t r = i / cgroups;
     const uint32_t tile = (uint32_t)(r % tgroups) * per + tl;
     const uint32_t b = (uint32_t)(r / tgroups);
-    const bool mine = c < vecs && tile < tiles;
+    const bool mine = c < vecs && tl < per && tile < tiles;
     float dw[V][W] = {}, db[V] = {};
     if (mine) {
       const uint32_t len = seq_length(s, b), t0 = tile * kGradTile;
-      const uint32_t t1 = min((uint64_t)t0 + kGradTile, s.length);
-      const uint32_t tend = min((uint64_t)t1 + W - 1, (uint64_t)len);  // g is zero from len on
       const T *xr = (const T *)x.p + (uint64_t)b * x.batch_stride + (uint64_t)c * V;
       const T *gr = (const T *)dy.p + (uint64_t)b * dy.batch_stride + (uint64_t)c * V;
       T *dr = (T *)dx.p + (uint64_t)b * dx.batch_stride + (uint64_t)c * V;
@@ -184,54 +197,71 @@ __global__ __launch_bounds__(256) void k_conv_grad(nsfps_rows x, nsfps_rows dy, 
         for (int j = 0; j < V; ++j) win[k][j] = 0.f;
         if (t >= 0 && t < len) load_f32<T, V>(xr + t * x.row_stride, win[k]);
       }
-      for (uint32_t t = t0; t < t1 + W - 1; t += kAhead) {
-        float in[kAhead][V], gi[kAhead][V];
+      // kFull: the tile and the W - 1 tokens after it lie inside the sequence
+      constexpr uint32_t kSteps = (kGradTile + W - 1 + kAhead - 1) / kAhead * kAhead;
+      const auto walk = [&](auto full) {
+        constexpr bool kFull = decltype(full)::value;
+        Raw<T, V> in[kAhead], gi[kAhead], next[kAhead], gnext[kAhead];
+        const auto load = [&](uint32_t t, Raw<T, V>(&o)[kAhead], Raw<T, V>(&go)[kAhead]) {
 #pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a) {
-#pragma unroll
-          for (int j = 0; j < V; ++j) in[a][j] = gi[a][j] = 0.f;
-          if (t + a < tend) {
-            load_f32<T, V>(xr + (uint64_t)(t + a) * x.row_stride, in[a]);
-            load_f32<T, V>(gr + (uint64_t)(t + a) * dy.row_stride, gi[a]);
-          }
-        }
-#pragma unroll
-        for (uint32_t a = 0; a < kAhead; ++a) {
-          const uint32_t ta = t + a;
-          if (ta >= t1 + W - 1) break;
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            win[W - 1][j] = in[a][j];
-            float pre = bs[j];
-#pragma unroll
-            for (int k = 0; k < W; ++k) pre = fmaf(w[j * W + k], win[k][j], pre);
-            const float sig = sigmoid(pre);
-            const float gt = ta < tend ? gi[a][j] * sig * fmaf(pre, 1.f - sig, 1.f) : 0.f;
-#pragma unroll
-            for (int k = W - 1; k > 0; --k) g[k][j] = g[k - 1][j];
-            g[0][j] = gt;
-            if (ta < t1) {
-              db[j] += gt;
-#pragma unroll
-              for (int k = 0; k < W; ++k) dw[j][k] = fmaf(gt, win[k][j], dw[j][k]);
+          for (uint32_t a = 0; a < kAhead; ++a) {
+            o[a] = go[a] = zero_raw<T, V>();
+            if (kFull || t + a < len) {
+              o[a] = load_raw<T, V>(xr + (uint64_t)(t + a) * x.row_stride);
+              go[a] = load_raw<T, V>(gr + (uint64_t)(t + a) * dy.row_stride);
             }
-#pragma unroll
-            for (int k = 0; k < W - 1; ++k) win[k][j] = win[k + 1][j];
           }
-          if (ta >= t0 + W - 1) {  // g[ta - (W-1) .. ta] are known
-            const uint32_t to = ta - (W - 1);
-            float o[V];
+        };
+        load(t0, in, gi);
+#pragma unroll 1
+        for (uint32_t i = 0; i < kSteps; i += kAhead) {
+          if (i + kAhead < kSteps) load(t0 + i + kAhead, next, gnext);
+#pragma unroll
+          for (uint32_t a = 0; a < kAhead; ++a) {
+            const uint32_t t = t0 + i + a;
+            const bool counts = i + a < kGradTile;  // the tile's own tokens
+            float gv[V];
+            numbers<T, V>(in[a], win[W - 1]);
+            numbers<T, V>(gi[a], gv);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-              o[j] = 0.f;
+              float pre = bs[j];
 #pragma unroll
-              for (int k = 0; k < W; ++k) o[j] = fmaf(w[j * W + k], g[k][j], o[j]);
-              if (to >= len) o[j] = 0.f;
+              for (int k = 0; k < W; ++k) pre = fmaf(w[j * W + k], win[k][j], pre);
+              const float sig = sigmoid(pre);
+              // past the sequence's end dy was not read: zero
+              const float gt = gv[j] * sig * fmaf(pre, 1.f - sig, 1.f);
+#pragma unroll
+              for (int k = W - 1; k > 0; --k) g[k][j] = g[k - 1][j];
+              g[0][j] = gt;
+              if (counts) {
+                db[j] += gt;
+#pragma unroll
+                for (int k = 0; k < W; ++k) dw[j][k] = fmaf(gt, win[k][j], dw[j][k]);
+              }
+#pragma unroll
+              for (int k = 0; k < W - 1; ++k) win[k][j] = win[k + 1][j];
             }
-            store_f32<T, V>(dr + (uint64_t)to * dx.row_stride, o);
+            if (i + a >= W - 1 && i + a < kGradTile + W - 1) {  // g[t - (W-1) .. t] are known
+              const uint32_t to = t - (W - 1);
+              float o[V];
+#pragma unroll
+              for (int j = 0; j < V; ++j) {
+                o[j] = 0.f;
+#pragma unroll
+                for (int k = 0; k < W; ++k) o[j] = fmaf(w[j * W + k], g[k][j], o[j]);
+              }
+              if (kFull || to < s.length) store_f32<T, V>(dr + (uint64_t)to * dx.row_stride, o);
+            }
           }
+#pragma unroll
+          for (uint32_t a = 0; a < kAhead; ++a) in[a] = next[a], gi[a] = gnext[a];
         }
-      }
+      };
+      if ((uint64_t)t0 + kSteps <= len)
+        walk(std::true_type());
+      else
+        walk(std::false_type());
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -241,7 +271,7 @@ __global__ __launch_bounds__(256) void k_conv_grad(nsfps_rows x, nsfps_rows dy, 
     }
     __syncthreads();
     // sums of a channel vector: kSums floats next to each other in part
-    for (uint32_t e = threadIdx.x; e < cvb * kSums; e += 256) {
+    for (uint32_t e = threadIdx.x; e < cvb * kSums; e += blockDim.x) {
       const uint32_t lc = e / kSums, k = e % kSums;
       const uint32_t cc = (uint32_t)(i % cgroups) * cvb + lc;
       if (cc >= vecs) continue;
@@ -291,17 +321,20 @@ __global__ __launch_bounds__(1024) void k_conv_join(const float *__restrict__ pa
 }
 
 struct Shape {
-  uint32_t vecs, cvb, tiles;
+  uint32_t vecs, cvb, per, threads, tiles;
   uint64_t rows, work;  // (sequence, tile group) pairs; times channel groups
 };
 
+// All channel vectors in one workgroup where 256 threads hold them, else equal
+// parts of them; then as many tiles of tokens as fit.
 Shape shape_of(const nsfps_conv_args &a, uint32_t v, uint32_t tile) {
   Shape s;
   s.vecs = a.channels / v;
-  s.cvb = 1;
-  while (s.cvb < 64 && s.cvb < s.vecs) s.cvb *= 2;
+  s.cvb = (uint32_t)host_ceil_div(s.vecs, host_ceil_div(s.vecs, 256));
   s.tiles = (uint32_t)host_ceil_div(a.length, tile);
-  s.rows = a.batch * host_ceil_div(s.tiles, 256 / s.cvb);
+  s.per = std::max(1u, std::min(256 / s.cvb, s.tiles));
+  s.threads = (s.cvb * s.per + 63) & ~63u;
+  s.rows = a.batch * host_ceil_div(s.tiles, s.per);
   s.work = s.rows * host_ceil_div(s.vecs, s.cvb);
   return s;
 }
@@ -313,7 +346,7 @@ Seqs seqs_of(const nsfps_conv_args &a) {
 uint32_t grid_of(uint64_t blocks) { return (uint32_t)std::min<uint64_t>(blocks, 1u << 20); }
 
 // f(element type, elements a vector, width)
-template <typename F>
+template <int kBf16, typename F>
 hipError_t by_type(uint32_t dtype, bool wide, uint32_t width, F f) {
   const auto by_width = [&](auto t, auto v) {
     switch (width) {
@@ -324,54 +357,55 @@ hipError_t by_type(uint32_t dtype, bool wide, uint32_t width, F f) {
   };
   constexpr std::integral_constant<int, 1> one;
   constexpr std::integral_constant<int, 4> four;
+  constexpr std::integral_constant<int, kBf16> many;
   if (dtype == NSFPS_F32) return wide ? by_width(float(), four) : by_width(float(), one);
-  return wide ? by_width(bf16(), four) : by_width(bf16(), one);
+  return wide ? by_width(bf16(), many) : by_width(bf16(), one);
 }
 
-// Rows that 4 elements a lane can be loaded from at once.
-bool conv_wide(const nsfps_conv_args &a) {
-  const uint32_t size = a.dtype == NSFPS_F32 ? 4 : 2;
-  const auto at = [&](const void *p) { return (uintptr_t)p % (4 * size) == 0; };
-  return a.channels % 4 == 0 && at(a.d_weight) && at(a.d_bias) && at(a.d_cache);
-}
-bool rows_four(const nsfps_rows &r, uint32_t dtype) {
-  const uint32_t size = dtype == NSFPS_F32 ? 4 : 2;
-  return (uintptr_t)r.p % (4 * size) == 0 && r.batch_stride % 4 == 0 && r.row_stride % 4 == 0;
+// Vectors of a lane fit the channels, the parameters and the rows.
+bool conv_wide(const nsfps_conv_args &a, uint32_t bf16s, std::initializer_list<const nsfps_rows *> rows) {
+  const uint32_t size = a.dtype == NSFPS_F32 ? 4 : 2, v = a.dtype == NSFPS_F32 ? 4 : bf16s;
+  const auto at = [&](const void *p) { return (uintptr_t)p % (v * size) == 0; };
+  bool ok = a.channels % v == 0 && at(a.d_weight) && at(a.d_bias) && at(a.d_cache);
+  for (const nsfps_rows *r : rows)
+    ok = ok && at(r->p) && r->batch_stride % v == 0 && r->row_stride % v == 0;
+  return ok;
 }
 
 }  // namespace
 
 hipError_t launch_conv(const nsfps_conv_args &a, hipStream_t st) {
-  const bool wide = conv_wide(a) && rows_four(a.x, a.dtype) && rows_four(a.y, a.dtype);
-  return by_type(a.dtype, wide, a.width, [&](auto t, auto v, auto w) {
+  const bool wide = conv_wide(a, kVec, {&a.x, &a.y});
+  return by_type<kVec>(a.dtype, wide, a.width, [&](auto t, auto v, auto w) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value, W = decltype(w)::value;
     const Shape s = shape_of(a, V, kTile);
-    k_conv<T, V, W><<<grid_of(s.work), 256, 0, st>>>(
+    k_conv<T, V, W><<<grid_of(s.work), s.threads, 0, st>>>(
         a.x, a.y, seqs_of(a), (const T *)a.d_weight, (const T *)a.d_bias, (T *)a.d_cache, s.vecs,
-        s.cvb, s.tiles, s.work);
+        s.cvb, s.per, s.tiles, s.work);
     return hipGetLastError();
   });
 }
 
 uint64_t conv_grad_bytes(const nsfps_conv_args &a) {
-  // the narrow form has the fewer tiles a workgroup and so the more rows
-  const uint64_t rows = std::max(shape_of(a, 1, kGradTile).rows, shape_of(a, 4, kGradTile).rows);
+  // what the strides allow is not known here: the most of the forms
+  uint64_t rows = 0;
+  for (uint32_t v : {1u, 4u, (uint32_t)kGradVec})
+    if (a.channels % v == 0) rows = std::max(rows, shape_of(a, v, kGradTile).rows);
   return rows * a.channels * (a.width + 1) * 4;
 }
 
 hipError_t launch_conv_grad(const nsfps_conv_args &a, const nsfps_conv_grads &g, hipStream_t st) {
-  const bool wide = conv_wide(a) && rows_four(a.x, a.dtype) && rows_four(g.dy, a.dtype) &&
-                    rows_four(g.dx, a.dtype);
-  return by_type(a.dtype, wide, a.width, [&](auto t, auto v, auto w) {
+  const bool wide = conv_wide(a, kGradVec, {&a.x, &g.dy, &g.dx});
+  return by_type<kGradVec>(a.dtype, wide, a.width, [&](auto t, auto v, auto w) {
     using T = decltype(t);
     constexpr int V = decltype(v)::value, W = decltype(w)::value;
     const Shape s = shape_of(a, V, kGradTile);
     float *const part = (float *)a.workspace;
     if (s.work)
-      k_conv_grad<T, V, W><<<grid_of(s.work), 256, 0, st>>>(
+      k_conv_grad<T, V, W><<<grid_of(s.work), s.threads, 0, st>>>(
           a.x, g.dy, g.dx, seqs_of(a), (const T *)a.d_weight, (const T *)a.d_bias, part, s.vecs,
-          s.cvb, s.tiles, s.work);
+          s.cvb, s.per, s.tiles, s.work);
     const uint64_t cols = (uint64_t)a.channels * (W + 1);
     k_conv_join<<<(uint32_t)host_ceil_div(cols, 64), 1024, 0, st>>>(part, s.rows, cols, W + 1,
                                                                    g.d_dweight, g.d_dbias);
@@ -380,7 +414,7 @@ hipError_t launch_conv_grad(const nsfps_conv_args &a, const nsfps_conv_grads &g,
 }
 
 hipError_t preload_conv_kernels() {
-  return func_attributes(k_conv<bf16, 4, 4>, k_conv_grad<bf16, 4, 4>, k_conv_join);
+  return func_attributes(k_conv<bf16, kVec, 4>, k_conv_grad<bf16, kGradVec, 4>, k_conv_join);
 }
 
 }  // namespace nsfps

@@ -55,39 +55,51 @@ template <typename T, int V>
 struct Vec {
   T v[V];
 };
+// As loaded (a load whose values are converted where it stands is waited for there) ...
+template <typename T, int V>
+struct Raw {
+  static constexpr int kBytes = V * (int)sizeof(T), kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+};
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_raw(const T *p) {
+  const NSFPS_GLOBAL_SEQ T *g = (const NSFPS_GLOBAL_SEQ T *)p;
+  Raw<T, V> o;
+  if constexpr (Raw<T, V>::kBytes == 16) {
+    const u32x4 t = *(const NSFPS_GLOBAL_SEQ u32x4 *)g;
+    o.w[0] = t.x, o.w[1] = t.y, o.w[2] = t.z, o.w[3] = t.w;
+  } else if constexpr (Raw<T, V>::kBytes == 8) {
+    const u32x2 t = *(const NSFPS_GLOBAL_SEQ u32x2 *)g;
+    o.w[0] = t.x, o.w[1] = t.y;
+  } else if constexpr (Raw<T, V>::kBytes == 4) {
+    o.w[0] = *(const NSFPS_GLOBAL_SEQ uint32_t *)g;
+  } else {
+    static_assert(Raw<T, V>::kBytes == 2, "vector width");
+    o.w[0] = *(const NSFPS_GLOBAL_SEQ uint16_t *)g;
+  }
+  return o;
+}
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> zero_raw() {
+  Raw<T, V> o;
+#pragma unroll
+  for (int i = 0; i < Raw<T, V>::kWords; ++i) o.w[i] = 0u;
+  return o;
+}
+// ... and as numbers
+template <typename T, int V>
+__device__ __forceinline__ void numbers(const Raw<T, V> &r, float (&o)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (sizeof(T) == 4)
+      o[i] = __uint_as_float(r.w[i]);
+    else
+      o[i] = __uint_as_float((i & 1) ? (r.w[i / 2] & 0xffff0000u) : (r.w[i / 2] << 16));
+  }
+}
 template <typename T, int V>
 __device__ __forceinline__ void load_f32(const T *p, float (&o)[V]) {
-  const NSFPS_GLOBAL_SEQ T *g = (const NSFPS_GLOBAL_SEQ T *)p;
-  constexpr int kWords = V * (int)sizeof(T) / 4;
-  if constexpr (kWords >= 1) {
-    uint32_t w[kWords];
-    if constexpr (kWords == 4) {
-      const u32x4 t = *(const NSFPS_GLOBAL_SEQ u32x4 *)g;
-      w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
-    } else if constexpr (kWords == 2) {
-      const u32x2 t = *(const NSFPS_GLOBAL_SEQ u32x2 *)g;
-      w[0] = t.x, w[1] = t.y;
-    } else {
-      static_assert(kWords == 1, "vector width");
-      w[0] = *(const NSFPS_GLOBAL_SEQ uint32_t *)g;
-    }
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        o[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16));
-    }
-  } else {
-    static_assert(V == 1, "vector width");
-    T t;
-    if constexpr (sizeof(T) == 4)
-      t = __builtin_bit_cast(T, *(const NSFPS_GLOBAL_SEQ uint32_t *)g);
-    else
-      t = __builtin_bit_cast(T, *(const NSFPS_GLOBAL_SEQ uint16_t *)g);
-    o[0] = to_f32(t);
-  }
+  numbers<T, V>(load_raw<T, V>(p), o);
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_f32(T *p, const float (&o)[V]) {
@@ -152,6 +164,11 @@ template <int N, typename F>
 __device__ __forceinline__ void unrolled(F f) {
   unrolled_of(f, std::make_integer_sequence<int, N>());
 }
+
+// Waits for this wave's loads.  Before a loop that fetches ahead: values loaded
+// before it would else be waited for at their first use inside, every time
+// round, and the loads ahead with them.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 __device__ __forceinline__ uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
