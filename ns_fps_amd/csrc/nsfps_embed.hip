@@ -5,9 +5,9 @@
 //
 // Gradient: dtable[v] = scale * sum of dout[i] over tok[i] = v.  The tokens
 // are sorted with their positions (stable, so a row's positions are in
-// order), start[v] is found at the sorted tokens' boundaries, and one wave
-// per table row adds that row's terms in float32, in that order, and writes
-// the row once: no atomics on values, the same bits every time, and rows
+// order), start[v] is found at the sorted tokens' boundaries, and each table
+// row's terms are added in float32, in that order, by the lanes that hold its
+// columns, and the row is written once: no atomics on values, the same bits every time, and rows
 // without a token cost their zeros.  A crowded row (more than kLong terms:
 // grid cells near an object) is cut into pieces of kPiece terms, a wave each,
 // whose sums (in float64: the
@@ -27,8 +27,8 @@ using namespace seq;
 
 namespace {
 
-constexpr uint32_t kLong = 64;    // terms of one wave's row
-constexpr uint32_t kPiece = 256;  // terms of a piece of a longer one
+constexpr uint32_t kLong = 16;   // terms that a row adds by itself
+constexpr uint32_t kPiece = 64;  // terms of a piece of a longer one
 
 // Workgroups of a grid-stride kernel: a launch holds fewer than 2^32 threads.
 uint32_t grid_of(uint64_t blocks) { return (uint32_t)std::min<uint64_t>(blocks, 1u << 20); }
@@ -66,16 +66,175 @@ __global__ __launch_bounds__(256) void k_embed(const T *__restrict__ table,
 
 // ---- gradient
 
-// keys: the tokens, rows for those outside
-__global__ __launch_bounds__(256) void k_embed_keys(const int32_t *__restrict__ tokens,
-                                                    uint32_t count, uint32_t rows,
-                                                    uint32_t *__restrict__ keys,
-                                                    uint32_t *__restrict__ counters) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i < 2) counters[i] = 0;
-  if (i >= count) return;
+// Stable radix sort of the tokens with their positions, up to kDigitBits bits
+// a pass, so that a vocabulary of 2^20 rows takes two.  A pass: each
+// workgroup's digit counts (hist[tile][digit]); their sums over the tiles
+// ahead, and the digits' totals; the scatter.  A workgroup's kTokTile tokens
+// are four waves' runs of 512 in order; a wave ranks 64 at a time by ballots.
+// (The sampling build's 8-bit sort of 4,096-key tiles took 99 us for 524,288
+// tokens of 19 bits, this one 39; for 16,384 tokens of 14 bits one workgroup
+// in LDS took 34 us.)
+constexpr int kDigitBits = 10;
+constexpr uint32_t kTokTile = 2048;
+constexpr int kTokRounds = kTokTile / 256;
+
+// A token's sort key: itself, or rows when it is outside.
+__device__ __forceinline__ uint32_t token_key(const int32_t *tokens, const uint32_t *keys,
+                                              uint32_t i, uint32_t rows) {
+  if (keys) return keys[i];
   const int32_t t = tokens[i];
-  keys[i] = t >= 0 && (uint32_t)t < rows ? (uint32_t)t : rows;
+  return t >= 0 && (uint32_t)t < rows ? (uint32_t)t : rows;
+}
+
+// keys null: the first pass, from the tokens; it clears the counters too.
+__global__ __launch_bounds__(256) void k_token_hist(const int32_t *__restrict__ tokens,
+                                                    const uint32_t *__restrict__ keys,
+                                                    uint32_t count, uint32_t rows, int shift,
+                                                    int bits, uint32_t *__restrict__ hist,
+                                                    uint32_t *__restrict__ counters) {
+  __shared__ uint32_t s_cnt[1 << kDigitBits];
+  const uint32_t digits = 1u << bits;
+  if (!keys && blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
+  for (uint32_t d = threadIdx.x; d < digits; d += 256) s_cnt[d] = 0;
+  __syncthreads();
+  const uint64_t base = (uint64_t)blockIdx.x * kTokTile;
+  uint32_t key[kTokRounds];
+#pragma unroll
+  for (int r = 0; r < kTokRounds; ++r) {
+    const uint64_t i = base + r * 256 + threadIdx.x;
+    key[r] = i < count ? token_key(tokens, keys, (uint32_t)i, rows) : 0u;
+  }
+#pragma unroll
+  for (int r = 0; r < kTokRounds; ++r)
+    if (base + r * 256 + threadIdx.x < count)
+      atomicAdd(&s_cnt[(key[r] >> shift) & (digits - 1)], 1u);
+  __syncthreads();
+  for (uint32_t d = threadIdx.x; d < digits; d += 256)
+    hist[(uint64_t)blockIdx.x * digits + d] = s_cnt[d];
+}
+
+// hist[tile][digit] becomes the digit's count in the tiles ahead; totals[digit].
+// 64 digits a workgroup, its 16 waves a run of the tiles each.
+__global__ __launch_bounds__(1024) void k_token_scan(uint32_t *__restrict__ hist, uint32_t tiles,
+                                                     int bits, uint32_t *__restrict__ totals) {
+  __shared__ uint32_t s_sum[16][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, digits = 1u << bits;
+  const uint32_t d = blockIdx.x * 64 + lane, run = ceil_div(tiles, 16);
+  const uint32_t a = min(wave * run, tiles), b = min(a + run, tiles);
+  constexpr uint32_t kAhead = 8;
+  uint32_t sum = 0;
+  if (d < digits)
+    for (uint32_t t = a; t < b; t += kAhead) {
+      uint32_t v[kAhead];
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; ++k)
+        v[k] = t + k < b ? hist[(uint64_t)(t + k) * digits + d] : 0u;
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; ++k) sum += v[k];
+    }
+  s_sum[wave][lane] = sum;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < 16; ++w) {
+    before += w < wave ? s_sum[w][lane] : 0u;
+    all += s_sum[w][lane];
+  }
+  if (d >= digits) return;
+  if (wave == 0) totals[d] = all;
+  for (uint32_t t = a; t < b; t += kAhead) {
+    uint32_t v[kAhead];
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k)
+      v[k] = t + k < b ? hist[(uint64_t)(t + k) * digits + d] : 0u;
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k) {
+      if (t + k < b) hist[(uint64_t)(t + k) * digits + d] = before;
+      before += v[k];
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void k_token_scatter(
+    const int32_t *__restrict__ tokens, const uint32_t *__restrict__ kin,
+    const uint32_t *__restrict__ vin, uint32_t *__restrict__ kout, uint32_t *__restrict__ vout,
+    uint32_t count, uint32_t rows, int shift, int bits, const uint32_t *__restrict__ hist,
+    const uint32_t *__restrict__ totals) {
+  __shared__ uint32_t s_cnt[4][1 << kDigitBits];  // per wave, then the digits' first places
+  __shared__ uint32_t s_wave[4];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, digits = 1u << bits;
+  const uint64_t lt = lane ? (~0ull >> (64 - lane)) : 0ull;
+  const uint64_t base = (uint64_t)blockIdx.x * kTokTile + wave * (kTokTile / 4);
+  uint32_t key[kTokRounds], val[kTokRounds], rank[kTokRounds];
+#pragma unroll
+  for (int r = 0; r < kTokRounds; ++r) {
+    const uint64_t i = base + r * 64 + lane;
+    key[r] = i < count ? token_key(tokens, kin, (uint32_t)i, rows) : 0u;
+    val[r] = i < count ? (kin ? vin[i] : (uint32_t)i) : 0u;
+  }
+  // this thread's digits, 4 tid .. 4 tid + 3: their places in the whole order
+  uint32_t tot[4], first[4];
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    const uint32_t d = 4 * tid + k;
+    tot[k] = d < digits ? totals[d] : 0u;
+    first[k] = d < digits ? hist[(uint64_t)blockIdx.x * digits + d] : 0u;
+  }
+  for (uint32_t d = tid; d < 4 * digits; d += 256) s_cnt[d / digits][d % digits] = 0;
+  uint32_t sum = tot[0] + tot[1] + tot[2] + tot[3];
+  const uint32_t own = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t o = __shfl_up(sum, off, 64);
+    if (lane >= (uint32_t)off) sum += o;
+  }
+  if (lane == 63) s_wave[wave] = sum;
+  __syncthreads();
+  sum -= own;
+  for (uint32_t w = 0; w < wave; ++w) sum += s_wave[w];
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    first[k] += sum;
+    sum += tot[k];
+  }
+#pragma unroll
+  for (int r = 0; r < kTokRounds; ++r) {
+    const bool valid = base + r * 64 + lane < count;
+    const uint32_t d = (key[r] >> shift) & (digits - 1);
+    uint64_t peers = __ballot(valid);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t m = __ballot((d >> b) & 1u);
+      peers &= ((d >> b) & 1u) ? m : ~m;
+    }
+    const uint32_t before = (uint32_t)__popcll(peers & lt);
+    const uint32_t baseq = valid ? s_cnt[wave][d] : 0u;
+    rank[r] = baseq + before;
+    // all lanes read their base before a leader writes (in-order LDS, one wave)
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    if (valid && before == 0) s_cnt[wave][d] = baseq + (uint32_t)__popcll(peers);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    const uint32_t d = 4 * tid + k;
+    if (d >= digits) continue;
+    uint32_t at = first[k];
+#pragma unroll
+    for (uint32_t w = 0; w < 4; ++w) {
+      const uint32_t n = s_cnt[w][d];
+      s_cnt[w][d] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kTokRounds; ++r) {
+    if (base + r * 64 + lane >= count) continue;
+    const uint32_t at = s_cnt[wave][(key[r] >> shift) & (digits - 1)] + rank[r];
+    kout[at] = key[r];
+    vout[at] = val[r];
+  }
 }
 
 // start[v] (v <= rows): sorted positions below it hold tokens below v.
@@ -109,11 +268,11 @@ __global__ __launch_bounds__(256) void k_embed_starts(const uint32_t *__restrict
 }
 
 // acc += the terms pos[from .. to) of one column vector, in order
-template <typename T, int V, typename A>
+template <typename T, int V>
 __device__ __forceinline__ void add_terms(const T *__restrict__ dout, uint64_t stride,
                                           const uint32_t *__restrict__ pos, uint32_t from,
-                                          uint32_t to, A (&acc)[V]) {
-  constexpr uint32_t kAhead = 4;  // loads in flight
+                                          uint32_t to, double (&acc)[V]) {
+  constexpr uint32_t kAhead = 8;  // loads in flight
   uint32_t p = from;
   for (; p + kAhead <= to; p += kAhead) {
     float v[kAhead][V];
@@ -137,39 +296,86 @@ struct LongRow {
   uint32_t row, piece;  // the row, and its first piece in the workspace
 };
 
-// One wave per table row.  Crowded rows are listed: counters[0] counts them,
-// counters[1] their pieces; piece_at[k] = the sorted position piece k starts at.
+// Table rows, `lpr` lanes (a power of two, at most 256) a row.  Most rows have
+// few terms, so what a row costs is a chain of dependent loads (its start, its
+// positions, its terms): a lane group takes kRows rows at a time, kTerms terms
+// of each a round, and issues each link of their chains together.  Crowded
+// rows are listed: counters[0] counts them, counters[1] their pieces;
+// piece_at[k] = the sorted positions of piece k.
 template <typename T, typename G, int V>
 __global__ __launch_bounds__(256) void k_embed_rows(
     const T *__restrict__ dout, uint64_t dout_stride, const uint32_t *__restrict__ pos,
     const uint32_t *__restrict__ start, G *__restrict__ dtable, uint64_t table_stride,
-    uint32_t rows, uint32_t vecs, float scale, uint32_t *__restrict__ counters,
+    uint32_t rows, uint32_t vecs, uint32_t lpr, float scale, uint32_t *__restrict__ counters,
     LongRow *__restrict__ longs, uint2 *__restrict__ piece_at) {
-  const uint32_t lane = threadIdx.x & 63u;
-  for (uint64_t row = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows;
-       row += (uint64_t)gridDim.x * 4) {
-    const uint32_t from = start[row], to = start[row + 1];
-    if (to - from > kLong) {
-      const uint32_t pieces = ceil_div(to - from, kPiece);
-      uint32_t first = 0;
-      if (lane == 0) {
-        first = atomicAdd(&counters[1], pieces);
-        longs[atomicAdd(&counters[0], 1u)] = LongRow{(uint32_t)row, first};
-      }
-      first = __shfl(first, 0, 64);
-      for (uint32_t k = lane; k < pieces; k += 64) {
-        const uint32_t f = from + k * kPiece;
-        piece_at[first + k] = make_uint2(f, f + min(kPiece, to - f));
-      }
-      continue;
-    }
-    G *dst = dtable + row * table_stride;
-    for (uint32_t c = lane; c < vecs; c += 64) {
-      float acc[V] = {};
-      add_terms<T, V>(dout + (uint64_t)c * V, dout_stride, pos, from, to, acc);
+  constexpr uint32_t kRows = 2, kTerms = 4;
+  const uint32_t lane = threadIdx.x & 63u, sub = threadIdx.x / lpr, cl = threadIdx.x % lpr,
+                 per = 256 / lpr, in_wave = min(lpr, 64u);
+  for (uint64_t first = (uint64_t)blockIdx.x * (per * kRows); first < rows;
+       first += (uint64_t)gridDim.x * per * kRows) {
+    uint32_t from[kRows], cnt[kRows];
+    uint64_t row[kRows];
 #pragma unroll
-      for (int k = 0; k < V; ++k) acc[k] *= scale;
-      store_f32<G, V>(dst + (uint64_t)c * V, acc);
+    for (uint32_t k = 0; k < kRows; ++k) {
+      row[k] = first + sub * kRows + k;
+      from[k] = row[k] < rows ? start[row[k]] : 0u;
+      cnt[k] = row[k] < rows ? start[row[k] + 1] : 0u;
+    }
+    uint32_t most = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kRows; ++k) {
+      cnt[k] -= from[k];
+      if (cnt[k] > kLong) {
+        const uint32_t pieces = ceil_div(cnt[k], kPiece);
+        uint32_t at = 0;
+        if (cl == 0) {
+          at = atomicAdd(&counters[1], pieces);
+          longs[atomicAdd(&counters[0], 1u)] = LongRow{(uint32_t)row[k], at};
+        }
+        if (cl < 64) {  // the lanes of the group that share a wave with its first
+          at = __shfl(at, lane - cl % in_wave, 64);
+          for (uint32_t i = cl; i < pieces; i += in_wave) {
+            const uint32_t f = from[k] + i * kPiece;
+            piece_at[at + i] = make_uint2(f, f + min(kPiece, from[k] + cnt[k] - f));
+          }
+        }
+        row[k] = rows;  // not here
+        cnt[k] = 0;
+      }
+      most = max(most, cnt[k]);
+    }
+    for (uint32_t c = cl; c < vecs; c += lpr) {
+      const T *const col = dout + (uint64_t)c * V;
+      float acc[kRows][V] = {};
+      for (uint32_t i = 0; i < most; i += kTerms) {
+        uint32_t p[kRows][kTerms];
+#pragma unroll
+        for (uint32_t k = 0; k < kRows; ++k)
+#pragma unroll
+          for (uint32_t j = 0; j < kTerms; ++j) p[k][j] = i + j < cnt[k] ? pos[from[k] + i + j] : 0u;
+        float v[kRows][kTerms][V];
+#pragma unroll
+        for (uint32_t k = 0; k < kRows; ++k)
+#pragma unroll
+          for (uint32_t j = 0; j < kTerms; ++j) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[k][j][e] = 0.f;
+            if (i + j < cnt[k]) load_f32<T, V>(col + (uint64_t)p[k][j] * dout_stride, v[k][j]);
+          }
+#pragma unroll
+        for (uint32_t k = 0; k < kRows; ++k)
+#pragma unroll
+          for (uint32_t j = 0; j < kTerms; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[k][e] += v[k][j][e];
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < kRows; ++k) {
+        if (row[k] >= rows) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[k][e] *= scale;
+        store_f32<G, V>(dtable + row[k] * table_stride + (uint64_t)c * V, acc[k]);
+      }
     }
   }
 }
@@ -233,9 +439,9 @@ __global__ __launch_bounds__(1024) void k_embed_join(const uint32_t *__restrict_
 // ---- workspace of the gradient
 
 struct GradPlan {
-  uint64_t keys, vals, keys2, vals2, hist, scan, start, counters, longs, pieces, part, total;
-  uint32_t long_max, piece_max;
-  int bits;
+  uint64_t keys, vals, keys2, vals2, hist, totals, start, counters, longs, pieces, part, total;
+  uint32_t long_max, piece_max, tiles;
+  int passes, bits;  // of a pass
 };
 
 GradPlan grad_plan(const nsfps_embed_args &a) {
@@ -246,17 +452,19 @@ GradPlan grad_plan(const nsfps_embed_args &a) {
     off = (off + bytes + 255) & ~255ull;
     return at;
   };
-  p.bits = 1;
-  while (p.bits < 32 && (a.rows >> p.bits)) ++p.bits;  // keys 0 .. rows
+  int bits = 1;
+  while (bits < 32 && (a.rows >> bits)) ++bits;  // keys 0 .. rows
+  p.passes = (bits + kDigitBits - 1) / kDigitBits;
+  p.bits = (bits + p.passes - 1) / p.passes;
+  p.tiles = (uint32_t)host_ceil_div(a.tokens, kTokTile);
   p.long_max = (uint32_t)(a.tokens / (kLong + 1));
   p.piece_max = (uint32_t)(a.tokens / kPiece) + p.long_max;
-  const uint64_t hist = radix_hist_len((uint32_t)a.tokens);
   p.keys = take(4 * a.tokens);
   p.vals = take(4 * a.tokens);
   p.keys2 = take(4 * a.tokens);
   p.vals2 = take(4 * a.tokens);
-  p.hist = take(4 * hist);
-  p.scan = take(4 * (uint64_t)scan_tmp_len((uint32_t)hist));
+  p.hist = take(4ull * p.tiles << p.bits);
+  p.totals = take(4ull << p.bits);
   p.start = take(4 * (a.rows + 1));
   p.counters = take(8);
   p.longs = take(sizeof(LongRow) * (uint64_t)p.long_max);
@@ -272,15 +480,20 @@ hipError_t run_grad(const nsfps_embed_args &a, hipStream_t st) {
   char *const w = (char *)a.workspace;
   uint32_t *const counters = (uint32_t *)(w + p.counters), *const start = (uint32_t *)(w + p.start);
   const uint32_t count = (uint32_t)a.tokens, rows = (uint32_t)a.rows;
-  uint32_t *keys = (uint32_t *)(w + p.keys), *pos = (uint32_t *)(w + p.vals);
-  k_embed_keys<<<(uint32_t)host_ceil_div(std::max(count, 2u), 256), 256, 0, st>>>(
-      a.d_tokens, count, rows, keys, counters);
-  if (count) {
-    const hipError_t e = launch_radix_sort(keys, pos, (uint32_t *)(w + p.keys2),
-                                           (uint32_t *)(w + p.vals2), count, p.bits,
-                                           (uint32_t *)(w + p.hist), (uint32_t *)(w + p.scan), true,
-                                           &keys, &pos, st);
-    if (e != hipSuccess) return e;
+  uint32_t *keys = nullptr, *pos = nullptr;
+  uint32_t *const key_buf[2] = {(uint32_t *)(w + p.keys), (uint32_t *)(w + p.keys2)};
+  uint32_t *const pos_buf[2] = {(uint32_t *)(w + p.vals), (uint32_t *)(w + p.vals2)};
+  uint32_t *const hist = (uint32_t *)(w + p.hist), *const totals = (uint32_t *)(w + p.totals);
+  for (int pass = 0; pass < p.passes && count; ++pass) {
+    const int shift = pass * p.bits;
+    k_token_hist<<<p.tiles, 256, 0, st>>>(a.d_tokens, keys, count, rows, shift, p.bits, hist,
+                                          counters);
+    k_token_scan<<<((1u << p.bits) + 63) / 64, 1024, 0, st>>>(hist, p.tiles, p.bits, totals);
+    k_token_scatter<<<p.tiles, 256, 0, st>>>(a.d_tokens, keys, pos, key_buf[pass & 1],
+                                             pos_buf[pass & 1], count, rows, shift, p.bits, hist,
+                                             totals);
+    keys = key_buf[pass & 1];
+    pos = pos_buf[pass & 1];
   }
   k_embed_starts<<<(uint32_t)host_ceil_div((uint64_t)count + 1, 256), 256, 0, st>>>(keys, count,
                                                                                    rows, start);
@@ -290,9 +503,12 @@ hipError_t run_grad(const nsfps_embed_args &a, hipStream_t st) {
   LongRow *const longs = (LongRow *)(w + p.longs);
   uint2 *const pieces = (uint2 *)(w + p.pieces);
   double *const part = (double *)(w + p.part);
-  k_embed_rows<T, G, V><<<grid_of(host_ceil_div(rows, 4)), 256, 0, st>>>(
-      dout, a.out_stride, pos, start, dtable, a.table_stride, rows, vecs, a.scale, counters, longs,
-      pieces);
+  uint32_t lpr = 1;
+  while (lpr < 256 && lpr < vecs) lpr *= 2;
+  const uint64_t per_group = 2 * (256 / lpr);  // two rows a lane group
+  k_embed_rows<T, G, V><<<grid_of(host_ceil_div(rows, per_group)), 256, 0, st>>>(
+      dout, a.out_stride, pos, start, dtable, a.table_stride, rows, vecs, lpr, a.scale, counters,
+      longs, pieces);
   if (p.long_max) {
     const dim3 gp(std::min(p.piece_max, 4096u), (uint32_t)host_ceil_div(vecs, 64));
     k_embed_pieces<T, V><<<gp, 64, 0, st>>>(dout, a.out_stride, pos, counters, pieces, part, vecs,
@@ -337,19 +553,21 @@ uint64_t embed_grad_bytes(const nsfps_embed_args &a) { return grad_plan(a).total
 hipError_t launch_embed_grad(const nsfps_embed_args &a, hipStream_t st) {
   const bool tf = a.dtype == NSFPS_F32, gf = a.grad_dtype == NSFPS_F32;
   const uint32_t ts = tf ? 4 : 2, gs = gf ? 4 : 2;
-  // 4 elements a lane where both sides' rows allow it (8 to 16 bytes a load)
-  const bool wide = wide_table(a.d_out, a.out_stride, a.width, 4, ts) &&
-                    wide_table(a.d_table, a.table_stride, a.width, 4, gs);
+  // 16 bytes of the wider type a lane, where both sides' rows allow it
+  const auto fits = [&](uint32_t v) {
+    return wide_table(a.d_out, a.out_stride, a.width, v, ts) &&
+           wide_table(a.d_table, a.table_stride, a.width, v, gs);
+  };
   if (tf)
-    return gf ? (wide ? run_grad<float, float, 4>(a, st) : run_grad<float, float, 1>(a, st))
-              : (wide ? run_grad<float, bf16, 4>(a, st) : run_grad<float, bf16, 1>(a, st));
-  return gf ? (wide ? run_grad<bf16, float, 4>(a, st) : run_grad<bf16, float, 1>(a, st))
-            : (wide ? run_grad<bf16, bf16, 4>(a, st) : run_grad<bf16, bf16, 1>(a, st));
+    return gf ? (fits(4) ? run_grad<float, float, 4>(a, st) : run_grad<float, float, 1>(a, st))
+              : (fits(4) ? run_grad<float, bf16, 4>(a, st) : run_grad<float, bf16, 1>(a, st));
+  if (gf) return fits(4) ? run_grad<bf16, float, 4>(a, st) : run_grad<bf16, float, 1>(a, st);
+  return fits(8) ? run_grad<bf16, bf16, 8>(a, st) : run_grad<bf16, bf16, 1>(a, st);
 }
 
 hipError_t preload_embed_kernels() {
   return func_attributes(k_embed<bf16, 8>, k_embed<bf16, 1>, k_embed<float, 4>, k_embed<float, 1>,
-                         k_embed_keys, k_embed_starts, k_embed_rows<bf16, bf16, 4>,
+                         k_token_hist, k_token_scan, k_token_scatter, k_embed_starts, k_embed_rows<bf16, bf16, 8>,
                          k_embed_rows<float, float, 4>);
 }
 
