@@ -102,6 +102,87 @@ def check_no_packed_fp32(asm_dir):
     print(f"  device assembly of {n_files} translation units: no v_pk_add/mul/fma_f32", flush=True)
 
 
+_REG = re.compile(r"\b([va])(?:(\d+)\b|\[(\d+):(\d+)\])")
+
+
+def _registers(text):
+    out = set()
+    for kind, one, lo, hi in _REG.findall(text):
+        out.update((kind, i) for i in ([int(one)] if one else range(int(lo), int(hi) + 1)))
+    return out
+
+
+def _mfma_states(name):
+    """Wait states from a matrix instruction to a reader of its sums."""
+    return 8 if "16x16x32_bf16" in name else 9 if "16x16x4_f32" in name else 20
+
+
+def matrix_hazards(asm):
+    """Vector instructions that read a matrix instruction's sums (or write over
+    them) too few wait states after it, along any path of the control flow
+    graph: [(function, the two instructions, states)]."""
+    found = []
+    for fn in re.split(r"\n(?=_Z\w+:)", asm):
+        if "v_mfma" not in fn:
+            continue
+        code, labels = [], {}
+        for ln in fn.split("\n"):
+            label = re.match(r"(\.LBB\w+):", ln)
+            inst = re.match(r"\t([a-z]\w*)\s*(.*?)(?:;.*)?$", ln)
+            if ln.startswith(".Lfunc_end"):
+                break
+            if label:
+                labels[label.group(1)] = len(code)
+            elif inst:
+                code.append((inst.group(1), inst.group(2)))
+        for n, (name, ops) in enumerate(code):
+            if not name.startswith("v_mfma"):
+                continue
+            need = _mfma_states(name)
+            paths = [(n + 1, 0, frozenset(_registers(ops.split(",")[0])))]
+            seen = set()
+            while paths:
+                k, states, sums = paths.pop()
+                if k >= len(code) or states >= need or not sums or (k, states) in seen:
+                    continue
+                seen.add((k, states))
+                op, args = code[k]
+                if op == "s_endpgm":
+                    continue
+                if op.startswith(("s_branch", "s_cbranch")):
+                    paths.append((labels[args.strip()], states + 1, sums))
+                    if op.startswith("s_branch"):
+                        continue
+                elif op == "s_nop":
+                    states += int(args.strip(), 0)
+                elif op.startswith("v_mfma"):
+                    sums = sums - _registers(args.split(",")[0])
+                elif op.startswith(("v_", "ds_", "global_", "scratch_", "flat_", "buffer_")):
+                    stores = re.match(r"(ds_write|(global|scratch|flat|buffer)_(store|atomic))", op)
+                    dst, _, src = args.partition(",")
+                    reads = _registers(args if stores else src)
+                    writes = _registers(dst) if op.startswith("v_") else set()
+                    if sums & (reads | writes):
+                        found.append((fn.split(":", 1)[0], f"{name} {ops}", f"{op} {args}", states))
+                        continue
+                paths.append((k + 1, states + 1, sums))
+    return found
+
+
+def check_matrix_waits(asm_dir):
+    """Fails when the gfx950 assembly of this build lets a reader of a matrix
+    instruction's sums come too early: the compiler's waits are not complete
+    where a branch leads straight from the one to the other."""
+    found = []
+    for name in sorted(os.listdir(asm_dir)):
+        if name.endswith(".s") and f"amdgcn-amd-amdhsa-{ARCH}" in name:
+            with open(os.path.join(asm_dir, name)) as f:
+                found += [f"{name}: {h}" for h in matrix_hazards(f.read())]
+    if found:
+        raise RuntimeError("readers too close behind matrix instructions:\n" + "\n".join(found[:10]))
+    print("  device assembly: every matrix instruction's sums are waited for", flush=True)
+
+
 def module_path():
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     return os.path.join(MODULE_DIR, "yuezu_fps_module" + suffix)
@@ -133,6 +214,7 @@ def build_lib(out=LIB, extra=()):
             objs = list(pool.map(compile_one, SOURCES))
         _run([HIPCC, f"--offload-arch={ARCH}", "-fPIC", "-shared", *extra, *objs, "-o", tmp], cwd=td)
         check_no_packed_fp32(td)
+        check_matrix_waits(td)
     os.replace(tmp, out)
     return out
 

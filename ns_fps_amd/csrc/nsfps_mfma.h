@@ -50,6 +50,20 @@ __device__ __forceinline__ void mma(f32x4 &sum, bf16x4 a0, bf16x4 a1, bf16x4 b0,
 }
 
 
+// Waits for the sums of products.  At the end of every branch that holds
+// products: the compiler's own waits are not complete across its joins (a
+// product, the branch, and a reader of the sum at the branch's target came out
+// next to each other, and the reader had the old value).
+template <typename T>
+__device__ __forceinline__ void settle() {
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (sizeof(T) == 4)
+    asm volatile("s_nop 7\n\ts_nop 1" ::: "memory");  // 16x16x4 f32: 9 states
+  else
+    asm volatile("s_nop 7" ::: "memory");  // 16x16x32 bf16: 8 states
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 // The same with the products summed apart and added to sum by the vector
 // unit.  The matrix unit aligns its addends and drops what falls below: a
 // bfloat16 product added to a sum already there is off by 0.04 of 2^-24 of it
@@ -66,7 +80,11 @@ __device__ __forceinline__ void mma_apart(f32x4 &sum, bf16x4 a0, bf16x4 a1, bf16
 }
 
 __device__ __forceinline__ f32x4 quad_f32(f32x4 q) { return q; }
-__device__ __forceinline__ f32x4 quad_f32(bf16x4 q) { return __builtin_convertvector(q, f32x4); }
+__device__ __forceinline__ f32x4 quad_f32(bf16x4 q) {
+  const u32x2 w = __builtin_bit_cast(u32x2, q);
+  return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
+               __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u)};
+}
 
 // A float32 value as operand terms whose sum it is: in bfloat16 one term keeps
 // 8 bits, two 16, three all 24; in float32 one term is the value.  (Terms of
@@ -160,36 +178,60 @@ __device__ __forceinline__ Pair<T> pair_col(const T *tile, int ld, int kb, int c
 
 // A tile of 64 rows x COLS columns on its way from global memory to LDS, in
 // the registers of 256 threads: fetched while the tile before it is worked on.
-// Zeros from row `rows` and column `cols` on.  kWideRows: rows start at 16-byte
-// boundaries and cols is a multiple of the elements in 16 bytes.
+// Rows past `rows` and columns past `cols` (both at least 1) are read from the
+// last inside it and become zeros on the way to LDS: a load that is left out
+// would have to be waited for before the next one into its registers.
+// kWideRows: rows start at 16-byte boundaries and cols is a multiple of the
+// elements in 16 bytes.
 template <typename T, int COLS, bool kWideRows>
 struct Tile {
   static constexpr int V = kWide<T>, kVecs = COLS / V, kPer = 64 * kVecs / 256;
   static_assert(kPer >= 1, "tile too small");
   u32x4 v[kPer];
+  uint32_t rows, cols;
 
-  __device__ __forceinline__ void fetch(const T *g, uint64_t row_stride, uint32_t rows,
-                                        uint32_t cols) {
+  __device__ __forceinline__ void fetch(const T *g, uint64_t row_stride, uint32_t nrows,
+                                        uint32_t ncols) {
+    rows = nrows;
+    cols = ncols;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint32_t e = threadIdx.x + 256 * i, r = e / kVecs, c = (e % kVecs) * V;
-      v[i] = u32x4{0, 0, 0, 0};
-      const NSFPS_GLOBAL_SEQ T *at = (const NSFPS_GLOBAL_SEQ T *)(g + r * row_stride + c);
+      const uint32_t e = threadIdx.x + 256 * i, c = (e % kVecs) * V;
+      const NSFPS_GLOBAL_SEQ T *at =
+          (const NSFPS_GLOBAL_SEQ T *)(g + min(e / kVecs, rows - 1) * row_stride);
       if constexpr (kWideRows) {
-        if (r < rows && c < cols) v[i] = *(const NSFPS_GLOBAL_SEQ u32x4 *)at;
-      } else if (r < rows) {
+        v[i] = *(const NSFPS_GLOBAL_SEQ u32x4 *)(at + min(c, cols - V));
+      } else {
+        v[i] = u32x4{0, 0, 0, 0};
 #pragma unroll
         for (uint32_t k = 0; k < V; ++k) {
-          if (c + k >= cols) break;
+          const uint32_t ck = min(c + k, cols - 1);
           if constexpr (sizeof(T) == 4)
-            v[i][k] = *(const NSFPS_GLOBAL_SEQ uint32_t *)(at + k);
+            v[i][k] = *(const NSFPS_GLOBAL_SEQ uint32_t *)(at + ck);
           else
-            v[i][k / 2] |= (uint32_t) * (const NSFPS_GLOBAL_SEQ uint16_t *)(at + k) << (16 * (k % 2));
+            v[i][k / 2] |= (uint32_t) * (const NSFPS_GLOBAL_SEQ uint16_t *)(at + ck) << (16 * (k % 2));
         }
       }
     }
   }
-  __device__ __forceinline__ void put(T *tile) const {
+  __device__ __forceinline__ void put(T *tile) {
+    if (rows < 64 || cols < COLS) {  // the same for all lanes; most tiles are full
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint32_t e = threadIdx.x + 256 * i, c = (e % kVecs) * V;
+        const bool in = e / kVecs < rows;
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+          if constexpr (sizeof(T) == 4) {
+            v[i][k] = in && c + k < cols ? v[i][k] : 0u;
+          } else {
+            const uint32_t keep = (in && c + 2 * k < cols ? 0xffffu : 0u) |
+                                  (in && c + 2 * k + 1 < cols ? 0xffff0000u : 0u);
+            v[i][k] &= keep;
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const uint32_t e = threadIdx.x + 256 * i;

@@ -156,15 +156,13 @@ __global__ __launch_bounds__(256, (kSweepGroups<T, NT, kOut>)) void k_scan_sweep
     if constexpr (kOut) tc.fetch(cb + t0 * s.c.row_stride, s.c.row_stride, rows, sn);
   };
   // the raw step of the chunk this wave finds the steps of, one group ahead
-  float raw = 0.f;
-  const auto fetch_raw = [&](uint32_t k) {
-    raw = 0.f;
-    if (k + wave < mine) {
-      const uint32_t t = chunk_at(k + wave) * kChunk + lane;
-      if (t < len) raw = raw_step<T>(s, b, h, t);
-    }
+  const float a_h = s.a[h], skip = kOut && s.d ? s.d[h] : 0.f, dt_bias = s.dt_bias ? s.dt_bias[h] : 0.f;
+  Raw<T, 1> raw = zero_raw<T, 1>();
+  const auto fetch_raw = [&](uint32_t k) {  // the last token again past the end
+    raw = raw_step<T>(s, b, h, min(chunk_at(min(k + wave, mine - 1)) * kChunk + lane, len - 1));
   };
   float total = 0.f;
+  wait_loads();
   if (mine) {
     fetch(0);
     fetch_raw(0);
@@ -178,7 +176,7 @@ __global__ __launch_bounds__(256, (kSweepGroups<T, NT, kOut>)) void k_scan_sweep
     if constexpr (kOut) tc.put(m.c);
     if (k % kStepAhead == 0) {
       if (k + wave < mine)
-        chunk_steps(m.st[wave], raw, chunk_at(k + wave) * kChunk + lane < len, s.a[h]);
+        chunk_steps(m.st[wave], number(raw) + dt_bias, chunk_at(k + wave) * kChunk + lane < len, a_h);
       fetch_raw(k + kStepAhead);
     }
     __syncthreads();
@@ -201,7 +199,9 @@ __global__ __launch_bounds__(256, (kSweepGroups<T, NT, kOut>)) void k_scan_sweep
         const float hi = sp.hi[i], lo = sp.lo[i];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          q[r] = j0 + r <= i ? q[r] * dj[r] * exp2_fast((hi - hj[r]) + (lo - lj[r])) : 0.f;
+          q[r] *= dj[r] * exp2_fast((hi - hj[r]) + (lo - lj[r]));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) q[r] = j0 + r <= i ? q[r] : 0.f;
         const Terms<T, 2> sc = split<T, 2>(q);
 #pragma unroll
         for (int e = 0; e < kT2; ++e) put_quad(m.m[e], ldm, i, j0, sc.q[e]);
@@ -232,7 +232,6 @@ __global__ __launch_bounds__(256, (kSweepGroups<T, NT, kOut>)) void k_scan_sweep
             for (int e = 0; e < kT2; ++e) mma(carried[it], Pair<T>{h0.q[e], h1.q[e]}, cq);
           }
         }
-        const float skip = s.d ? s.d[h] : 0.f;
         const uint32_t t0 = c * kChunk, out_rows = s.length - t0, rows = len - t0;
         const uint32_t po = 16 * wave + 4 * g;
 #pragma unroll
@@ -242,8 +241,10 @@ __global__ __launch_bounds__(256, (kSweepGroups<T, NT, kOut>)) void k_scan_sweep
           const float e = sp.e[i];
           float o[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            o[r] = i < rows ? fmaf(skip, xv[r], fmaf(e, carried[it][r], own[it][r])) : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            const float v = fmaf(skip, xv[r], fmaf(e, carried[it][r], own[it][r]));
+            o[r] = i < rows ? v : 0.f;
+          }
           T *dst = yb + (t0 + i) * s.y.row_stride + po;
           if (i < out_rows) {
             if constexpr (kWideRows) {
@@ -376,19 +377,25 @@ hipError_t run_sweep(const ScanDev &s, SweepDev d, char *ws, hipStream_t st) {
 
 // ---- one token
 
-constexpr uint32_t kStepRows = 16;  // state rows (head_dim) of a workgroup
-
-// One token of a request and head: 256 threads, kStepRows rows of the state,
-// 16 threads a row.  The workgroup convolves the channels it needs itself (its
-// rows' x; b and c of its group): the ring holds `width` entries, of which the
-// convolution reads the last width - 1 and this token's replaces the oldest,
-// so a workgroup that writes its entry disturbs no other that still reads.
-template <typename T, int W>
+// One token of a request and head: 256 threads, 16 rows of the state at a
+// time, 16 threads a row, kSets times.  The state is all the traffic that
+// counts: its loads go out first and wait while the workgroup convolves the
+// channels it needs itself (its rows' x; b and c of its group).  The ring
+// holds `width` entries, of which the convolution reads the last width - 1 and
+// this token's replaces the oldest, so a workgroup that writes its entry
+// disturbs no other that still reads.
+//
+// kV: 4 state values a load where state_dim and the cache allow it, kCols of
+// those a thread.  kSets: 4 (a head of 64 rows) where that still gives 1,024
+// workgroups, else 1: few requests need the width of the chip more than they
+// need the convolution done once.
+template <typename T, int W, int kV, int kCols, int kSets>
 __global__ __launch_bounds__(256) void k_scan_step(nsfps_step_args a, uint32_t ptiles) {
-  __shared__ float s_bc[2][128], s_x[kStepRows];
+  constexpr uint32_t kRows = 16 * kSets;
+  __shared__ float s_bc[2][128 + 4], s_x[kRows];
   const uint32_t pt = blockIdx.x % ptiles, h = (blockIdx.x / ptiles) % a.heads;
   const uint64_t b = blockIdx.x / ptiles / a.heads;
-  const uint32_t p0 = pt * kStepRows, rows = min(kStepRows, a.head_dim - p0), n = a.state_dim;
+  const uint32_t p0 = pt * kRows, rows = min(kRows, a.head_dim - p0), n = a.state_dim;
   const uint32_t grp = h / (a.heads / a.groups);
   const uint64_t hp = (uint64_t)a.heads * a.head_dim, gn = (uint64_t)a.groups * n,
                  channels = hp + 2 * gn;
@@ -400,57 +407,81 @@ __global__ __launch_bounds__(256) void k_scan_step(nsfps_step_args a, uint32_t p
     return;
   }
   const uint32_t pos = a.d_positions[b] > 0 ? (uint32_t)a.d_positions[b] : 0u;
+  const uint32_t r = threadIdx.x / 16, l = threadIdx.x % 16;
+  float *const state = a.d_state + (((uint64_t)slot * a.heads + h) * a.head_dim + p0) * n;
+  float st[kSets][kCols][kV];
+#pragma unroll
+  for (int q = 0; q < kSets; ++q)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const uint32_t p = 16 * q + r, k = kV * (l + 16 * c);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) st[q][c][i] = 0.f;
+      if (pos && p < rows && k < n) load_f32<float, kV>(state + p * n + k, st[q][c]);
+    }
   const T *xbc = (const T *)a.d_xbc + b * a.xbc_stride, *weight = (const T *)a.d_weight;
   T *const ring = (T *)a.d_cache + (uint64_t)slot * W * channels;
+  float raw[1];
+  load_f32<T, 1>((const T *)a.d_dt + b * a.dt_stride + h, raw);
+  const float a_h = a.d_a[h], skip = a.d_d ? a.d_d[h] : 0.f;
+  if (a.d_dt_bias) raw[0] += a.d_dt_bias[h];
+  uint32_t entry[W];  // the ring's entries, this token's and those before it
+#pragma unroll
+  for (int back = 0; back < W; ++back) entry[back] = (pos + W - back) % W;
   // channels: rows of x, then n of b, then n of c
   for (uint32_t e = threadIdx.x; e < rows + 2 * n; e += 256) {
     const bool is_x = e < rows;
-    const uint32_t k = is_x ? 0 : (e - rows) / n;  // 0: b, 1: c
-    const uint64_t ch = is_x ? (uint64_t)h * a.head_dim + p0 + e
-                             : hp + k * gn + (uint64_t)grp * n + (e - rows) % n;
-    float in[1], w[1], pre[1] = {0.f};
+    const uint32_t o = is_x ? e : e - rows, k = !is_x && o >= n;  // 0: b, 1: c
+    const uint64_t ch = is_x ? (uint64_t)h * a.head_dim + p0 + o
+                             : hp + k * gn + (uint64_t)grp * n + (o - k * n);
+    float in[W][1], w[W][1], pre[1] = {0.f};
     if (a.d_bias) load_f32<T, 1>((const T *)a.d_bias + ch, pre);
-    load_f32<T, 1>(xbc + ch, in);
+    load_f32<T, 1>(xbc + ch, in[0]);
 #pragma unroll
-    for (int back = 1; back < W; ++back) {
-      if (pos < (uint32_t)back) continue;
-      float old[1];
-      load_f32<T, 1>(ring + (uint64_t)((pos - back) % W) * channels + ch, old);
-      load_f32<T, 1>(weight + ch * W + (W - 1 - back), w);
-      pre[0] = fmaf(w[0], old[0], pre[0]);
+    for (int back = 0; back < W; ++back) {
+      load_f32<T, 1>(weight + ch * W + (W - 1 - back), w[back]);
+      if (back) {
+        in[back][0] = 0.f;
+        if (pos >= (uint32_t)back) load_f32<T, 1>(ring + entry[back] * channels + ch, in[back]);
+      }
     }
-    load_f32<T, 1>(weight + ch * W + (W - 1), w);
-    pre[0] = fmaf(w[0], in[0], pre[0]);
+#pragma unroll
+    for (int back = W - 1; back >= 0; --back) pre[0] = fmaf(w[back][0], in[back][0], pre[0]);
     const float v = pre[0] * sigmoid(pre[0]);
     if (is_x)
-      s_x[e] = v;
+      s_x[o] = v;
     else
-      s_bc[k][(e - rows) % n] = v;
+      s_bc[k][o - k * n] = v;
     // one workgroup owns each channel's ring entry
     if (is_x || (pt == 0 && h % (a.heads / a.groups) == 0))
-      store_f32<T, 1>(ring + (uint64_t)(pos % W) * channels + ch, in);
+      store_f32<T, 1>(ring + entry[0] * channels + ch, in[0]);
   }
-  float raw[1];
-  load_f32<T, 1>((const T *)a.d_dt + b * a.dt_stride + h, raw);
-  const float delta = softplus(raw[0] + (a.d_dt_bias ? a.d_dt_bias[h] : 0.f));
-  const float decay = exp2_fast(delta * a.d_a[h] * kLog2e);
+  const float delta = softplus(raw[0]), decay = exp2_fast(delta * a_h * kLog2e);
   __syncthreads();
-  const uint32_t r = threadIdx.x / 16, l = threadIdx.x % 16;
-  float sum = 0.f;
-  if (r < rows) {
-    float *st = a.d_state + (((uint64_t)slot * a.heads + h) * a.head_dim + p0 + r) * n;
-    const float xd = delta * s_x[r];
-    for (uint32_t k = l; k < n; k += 16) {
-      const float v = fmaf(xd, s_bc[0][k], pos ? decay * st[k] : 0.f);
-      st[k] = v;
-      sum = fmaf(v, s_bc[1][k], sum);
-    }
-  }
 #pragma unroll
-  for (int off = 8; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if (r < rows && l == 0) {
-    const float o[1] = {fmaf(a.d_d ? a.d_d[h] : 0.f, s_x[r], sum)};
-    store_f32<T, 1>(y + r, o);
+  for (int q = 0; q < kSets; ++q) {
+    const uint32_t p = 16 * q + r;
+    float sum = 0.f;
+    if (p < rows) {
+      const float xd = delta * s_x[p];
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) {
+        const uint32_t k = kV * (l + 16 * c);
+        if (k >= n) continue;
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          st[q][c][i] = fmaf(xd, s_bc[0][k + i], decay * st[q][c][i]);
+          sum = fmaf(st[q][c][i], s_bc[1][k + i], sum);
+        }
+        store_f32<float, kV>(state + p * n + k, st[q][c]);
+      }
+    }
+#pragma unroll
+    for (int off = 8; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (p < rows && l == 0) {
+      const float o[1] = {fmaf(skip, s_x[p], sum)};
+      store_f32<T, 1>(y + p, o);
+    }
   }
 }
 
@@ -491,22 +522,39 @@ hipError_t launch_states(const nsfps_scan_args &a, const ScanDev &s, const nsfps
 }
 
 hipError_t launch_scan_step(const nsfps_step_args &a, hipStream_t st) {
-  const uint32_t ptiles = (a.head_dim + kStepRows - 1) / kStepRows;
+  const bool many = a.batch * a.heads * host_ceil_div(a.head_dim, 64) >= 1024;
+  const uint32_t rows = many ? 64 : 16, ptiles = (a.head_dim + rows - 1) / rows;
   const uint32_t grid = (uint32_t)(a.batch * a.heads * ptiles);
-  const auto by_width = [&](auto t) {
+  const bool wide = a.state_dim % 4 == 0 && (uintptr_t)a.d_state % 16 == 0;
+  const auto go = [&](auto t, auto w, auto v, auto cols) {
     using T = decltype(t);
-    switch (a.width) {
-      case 2: k_scan_step<T, 2><<<grid, 256, 0, st>>>(a, ptiles); break;
-      case 3: k_scan_step<T, 3><<<grid, 256, 0, st>>>(a, ptiles); break;
-      default: k_scan_step<T, 4><<<grid, 256, 0, st>>>(a, ptiles);
-    }
+    constexpr int W = decltype(w)::value, V = decltype(v)::value, C = decltype(cols)::value;
+    if (many)
+      k_scan_step<T, W, V, C, 4><<<grid, 256, 0, st>>>(a, ptiles);
+    else
+      k_scan_step<T, W, V, C, 1><<<grid, 256, 0, st>>>(a, ptiles);
     return hipGetLastError();
+  };
+  const auto by_state = [&](auto t, auto w) {  // 16 threads a row, so 16 * V * C values
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 4> four;
+    constexpr std::integral_constant<int, 8> eight;
+    if (wide) return a.state_dim <= 64 ? go(t, w, four, one) : go(t, w, four, two);
+    return a.state_dim <= 64 ? go(t, w, one, four) : go(t, w, one, eight);
+  };
+  const auto by_width = [&](auto t) {
+    switch (a.width) {
+      case 2: return by_state(t, std::integral_constant<int, 2>());
+      case 3: return by_state(t, std::integral_constant<int, 3>());
+      default: return by_state(t, std::integral_constant<int, 4>());
+    }
   };
   return a.dtype == NSFPS_F32 ? by_width(float()) : by_width(bf16());
 }
 
 hipError_t preload_scan_kernels() {
-  return func_attributes(k_scan_sweep<bf16, 64, true, false, true>, k_scan_step<bf16, 4>,
+  return func_attributes(k_scan_sweep<bf16, 64, true, false, true>, k_scan_step<bf16, 4, 4, 2, 4>,
                          k_scan_carry<false>);
 }
 

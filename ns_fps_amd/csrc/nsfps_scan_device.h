@@ -37,7 +37,7 @@ __device__ __forceinline__ uint32_t scan_length(const ScanDev &s, uint32_t b) {
 // units as hi + lo, so that the difference of two sums keeps its own relative
 // precision however far the chunk has decayed (a single float32 sum of -500
 // would leave 3e-5 in the exponent of a decay near 1).
-struct Steps {
+struct alignas(16) Steps {  // read four at a time
   float delta[kChunk], hi[kChunk], lo[kChunk];
   float e[kChunk];     // decay from the chunk's start through the token
   float end[kChunk];   // decay from the token to the chunk's end
@@ -52,13 +52,17 @@ __device__ __forceinline__ f32x4 quad_of(const float (&v)[kChunk], int at) {
   return *(const f32x4 *)(v + at);
 }
 
-// The raw step of a token (before softplus), 0 steps past the sequence's end.
+// The raw step of a token (before softplus and its bias).
 template <typename T>
-__device__ __forceinline__ float raw_step(const ScanDev &s, uint32_t b, uint32_t h, uint32_t t) {
+__device__ __forceinline__ Raw<T, 1> raw_step(const ScanDev &s, uint32_t b, uint32_t h, uint32_t t) {
+  return load_raw<T, 1>((const T *)s.dt.p + (uint64_t)b * s.dt.batch_stride +
+                        (uint64_t)t * s.dt.row_stride + h);
+}
+template <typename T>
+__device__ __forceinline__ float number(const Raw<T, 1> &r) {
   float v[1];
-  load_f32<T, 1>((const T *)s.dt.p + (uint64_t)b * s.dt.batch_stride +
-                     (uint64_t)t * s.dt.row_stride + h, v);
-  return v[0] + (s.dt_bias ? s.dt_bias[h] : 0.f);
+  numbers<T, 1>(r, v);
+  return v[0];
 }
 
 // One wave fills the steps of a chunk from its lanes' raw steps; lanes past

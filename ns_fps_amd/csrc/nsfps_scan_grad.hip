@@ -57,7 +57,8 @@ struct GradLds {
   float whole[4];
 };
 
-// 64 x NT values of a state on their way from global memory to LDS.
+// 64 x NT values of a state on their way from global memory to LDS.  Rows and
+// columns past the state's are read from the last inside it and become zeros.
 template <int NT, bool kWideRows>
 struct StateTile {
   static constexpr int kPer = 64 * (NT / 4) / 256;
@@ -65,16 +66,25 @@ struct StateTile {
   __device__ __forceinline__ void fetch(const float *g, uint32_t rows, uint32_t cols) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint32_t e = threadIdx.x + 256 * i, p = e / (NT / 4), n = (e % (NT / 4)) * 4;
-      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const NSFPS_GLOBAL_SEQ float *at = (const NSFPS_GLOBAL_SEQ float *)(g + p * cols + n);
+      const uint32_t e = threadIdx.x + 256 * i, p = min(e / (NT / 4), rows - 1),
+                     n = (e % (NT / 4)) * 4;
+      const NSFPS_GLOBAL_SEQ float *at = (const NSFPS_GLOBAL_SEQ float *)(g + p * cols);
       if constexpr (kWideRows) {
-        if (p < rows && n < cols) v[i] = *(const NSFPS_GLOBAL_SEQ f32x4 *)at;
-      } else if (p < rows) {
+        v[i] = *(const NSFPS_GLOBAL_SEQ f32x4 *)(at + min(n, cols - 4));
+      } else {
 #pragma unroll
-        for (uint32_t k = 0; k < 4; ++k)
-          if (n + k < cols) v[i][k] = at[k];
+        for (uint32_t k = 0; k < 4; ++k) v[i][k] = at[min(n + k, cols - 1)];
       }
+    }
+  }
+  __device__ __forceinline__ void mask(uint32_t rows, uint32_t cols) {
+    if (rows >= 64 && cols >= NT) return;  // the same for all lanes
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + 256 * i, n = (e % (NT / 4)) * 4;
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k)
+        v[i][k] = e / (NT / 4) < rows && n + k < cols ? v[i][k] : 0.f;
     }
   }
   template <typename T>
@@ -149,10 +159,11 @@ __device__ __forceinline__ void store_quad(T *dst, f32x4 v, uint32_t at, uint32_
 }
 
 template <typename T, int NT>
-constexpr int kGradGroups = 1;
+constexpr int kGradGroups = sizeof(GradLds<T, NT>) <= 80 * 1024 ? 2 : 1;  // workgroups a CU
 
 // Work item w: chunk bc = w / groups of all sequences' and group w % groups.
-template <typename T, int NT, bool kWideRows>
+// kOne: head_dim is at most 64, so a head is one tile and its loads run ahead.
+template <typename T, int NT, bool kOne, bool kWideRows>
 __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev s, GradDev gr,
                                                                          uint64_t first_item,
                                                                          uint32_t work) {
@@ -197,7 +208,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
             0.f;
     return;
   }
-  const bool one = s.ptiles == 1;  // the whole head in one tile: its loads run ahead
+  const uint32_t ptiles = kOne ? 1u : s.ptiles;
   const T *const x_at = rows_at(s.x), *const dy_at = rows_at(gr.dy);
   Tile<T, (int)kPTile, kWideRows> tx, tdy;
   StateTile<NT, kWideRows> th, tdh;
@@ -215,59 +226,90 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
   const auto fetch_dh = [&](uint32_t h, uint32_t pt) {
     tdh.fetch(gr.ends + state_at(h, pt), s.head_dim - pt * kPTile, sn);
   };
-  float raw = 0.f;  // of the head this wave finds the steps of
+  // raw steps (and bias and a) of the head this wave finds the steps of; the
+  // last head and token again past the end
+  Raw<T, 1> raw = zero_raw<T, 1>();
+  float raw_bias = 0.f, raw_a = 0.f;
   const auto fetch_raw = [&](uint32_t h) {
-    raw = 0.f;
-    if (h + wave < h1 && lane < rows) raw = raw_step<T>(s, b, h + wave, t0 + lane);
+    const uint32_t hw = min(h + wave, h1 - 1);
+    raw = raw_step<T>(s, b, hw, t0 + min(lane, rows - 1));
+    raw_bias = s.dt_bias ? s.dt_bias[hw] : 0.f;
+    raw_a = s.a[hw];
+  };
+  // the head's own parameters
+  float a_h = 0.f, skip = 0.f;
+  const auto fetch_params = [&](uint32_t h) {
+    a_h = s.a[h];
+    skip = s.d ? s.d[h] : 0.f;
   };
   {
     Tile<T, NT, kWideRows> tb, tc;
+    fetch_params(h0);
     tb.fetch(rows_at(s.b) + grp * sn, s.b.row_stride, rows, sn);
     tc.fetch(rows_at(s.c) + grp * sn, s.c.row_stride, rows, sn);
     fetch_xdy(h0, 0);
-    if (one) fetch_h(h0, 0);
+    if constexpr (kOne) fetch_h(h0, 0);
     fetch_raw(h0);
     tb.put(m.b);
     tc.put(m.c);
   }
   __syncthreads();
 
-  // S with this wave's tokens as columns j (tiles of rows i >= its own) and,
-  // transposed, as columns i (tiles of rows j <= its own)
-  f32x4 s_j[4] = {}, s_i[4] = {};
-  unrolled<kNb>([&](auto kb) __attribute__((always_inline)) {
-    const Pair<T> bo = pair_row(m.b, ldn, own, kb, g), co = pair_row(m.c, ldn, own, kb, g);
-    unrolled<4>([&](auto t) __attribute__((always_inline)) {
-      if (t >= (int)wave) mma_apart(s_j[t], pair_row(m.c, ldn, 16 * t + l, kb, g), bo);
-      if (t <= (int)wave) mma_apart(s_i[t], pair_row(m.b, ldn, 16 * t + l, kb, g), co);
+  // S = c b^T with this wave's tokens as rows i (tiles of columns j <= its
+  // own), transposed, or as columns j (tiles of rows i >= its own).  The same
+  // for every head, and found again for each: it would hold 32 registers.
+  const auto find_s = [&](auto as_i, f32x4(&st)[4]) __attribute__((always_inline)) {
+    constexpr bool kAsI = decltype(as_i)::value;
+    unrolled<kNb>([&](auto kb) __attribute__((always_inline)) {
+      const Pair<T> o = pair_row(kAsI ? m.c : m.b, ldn, own, kb, g);
+      unrolled<4>([&](auto t) __attribute__((always_inline)) {
+        if (kAsI ? t <= (int)wave : t >= (int)wave) {
+          mma_apart(st[t], pair_row(kAsI ? m.b : m.c, ldn, 16 * t + l, kb, g), o);
+          settle<T>();
+        }
+      });
     });
-  });
+  };
 
   f32x4 db[kNt] = {}, dc[kNt] = {};
   for (uint32_t h = h0; h < h1; ++h) {
     const Steps &sp = m.st[(h - h0) % kHeadAhead];
     phase();
-    // ---- W in both orientations, over head_dim
-    f32x4 w_j[4] = {}, w_i[4] = {};
-    for (uint32_t pt = 0; pt < s.ptiles; ++pt) {
-      if (pt || (!one && h > h0)) fetch_xdy(h, pt);
-      __syncthreads();  // all are done with the head (or tile) before
+    const auto put_xdy = [&] {
       tx.put(m.x);
       tdy.put(m.dy);
-      if (one) th.put(m);
+    };
+    // W = dy x^T with this wave's tokens as rows i (kAsI) or columns j, of the
+    // tile in LDS
+    const auto add_w = [&](auto as_i, f32x4(&wt)[4]) __attribute__((always_inline)) {
+      constexpr bool kAsI = decltype(as_i)::value;
+      unrolled<kPb>([&](auto kb) __attribute__((always_inline)) {
+        const Pair<T> o = pair_row(kAsI ? m.dy : m.x, ldx, own, kb, g);
+        unrolled<4>([&](auto t) __attribute__((always_inline)) {
+          if (kAsI ? t <= (int)wave : t >= (int)wave) {
+            mma_apart(wt[t], pair_row(kAsI ? m.x : m.dy, ldx, 16 * t + l, kb, g), o);
+            settle<T>();
+          }
+        });
+      });
+    };
+    f32x4 w_i[4] = {}, w_j[4] = {};
+    for (uint32_t pt = 0; pt < ptiles; ++pt) {
+      if (!kOne && (pt || h > h0)) fetch_xdy(h, pt);
+      __syncthreads();  // all are done with the head (or tile) before
+      put_xdy();
+      if constexpr (kOne) {
+        th.mask(s.head_dim, sn);
+        th.put(m);
+      }
       if (pt == 0 && (h - h0) % kHeadAhead == 0) {
-        if (h + wave < h1) chunk_steps(m.st[wave], raw, lane < rows, s.a[h + wave]);
+        chunk_steps(m.st[wave], number(raw) + raw_bias, lane < rows, raw_a);
         fetch_raw(h + kHeadAhead);
       }
       __syncthreads();
-      if (one) fetch_dh(h, 0);
-      unrolled<kPb>([&](auto kb) __attribute__((always_inline)) {
-        const Pair<T> xo = pair_row(m.x, ldx, own, kb, g), go = pair_row(m.dy, ldx, own, kb, g);
-        unrolled<4>([&](auto t) __attribute__((always_inline)) {
-          if (t >= (int)wave) mma_apart(w_j[t], pair_row(m.dy, ldx, 16 * t + l, kb, g), xo);
-          if (t <= (int)wave) mma_apart(w_i[t], pair_row(m.x, ldx, 16 * t + l, kb, g), go);
-        });
-      });
+      if constexpr (kOne) fetch_dh(h, 0);
+      add_w(std::true_type(), w_i);
+      if constexpr (!kOne) add_w(std::false_type(), w_j);
     }
 
     phase();
@@ -277,6 +319,8 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
     double rt = 0.0;
     {
       Terms<T, 2> g_i[4];
+      f32x4 s_i[4] = {};
+      find_s(std::true_type(), s_i);
       const float hi = sp.hi[own], lo = sp.lo[own];
       unrolled<4>([&](auto t) __attribute__((always_inline)) {
         f32x4 gi = {0.f, 0.f, 0.f, 0.f};
@@ -284,13 +328,12 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
           const int j0 = 16 * t + 4 * g;
           const f32x4 dj = quad_of(sp.delta, j0), hj = quad_of(sp.hi, j0), lj = quad_of(sp.lo, j0);
           unrolled<4>([&](auto r_) __attribute__((always_inline)) {
-              constexpr int r = decltype(r_)::value;
-            if (j0 + r <= own) {
-              const float lw = exp2_fast((hi - hj[r]) + (lo - lj[r]));
-              gi[r] = lw * dj[r] * w_i[t][r];
-              if (j0 + r != own)
-                rt = fma((double)((lw * s_i[t][r]) * w_i[t][r]), (double)dj[r], rt);
-            }
+            constexpr int r = decltype(r_)::value;
+            const float le = exp2_fast((hi - hj[r]) + (lo - lj[r]));
+            const float lw = j0 + r <= own ? le : 0.f;
+            gi[r] = lw * dj[r] * w_i[t][r];
+            const float tv = (lw * s_i[t][r]) * w_i[t][r];
+            rt = fma((double)(j0 + r != own ? tv : 0.f), (double)dj[r], rt);
           });
         }
         g_i[t] = split<T, 2>(gi);
@@ -304,6 +347,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
               mma(dc[nt], a, Pair<T>{g_i[2 * kb].q[k], g_i[2 * kb + 1].q[k]});
             });
           });
+          settle<T>();
         }
       });
     }
@@ -313,8 +357,11 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
     double u_off = 0.0;
     float diag = 0.f, dd = 0.f;
     const float delta = sp.delta[own];
+    if constexpr (kOne) add_w(std::false_type(), w_j);
     {
       Terms<T, 2> g_j[4];
+      f32x4 s_j[4] = {};
+      find_s(std::false_type(), s_j);
       const float hj = sp.hi[own], lj = sp.lo[own];
       unrolled<4>([&](auto t) __attribute__((always_inline)) {
         f32x4 mj = {0.f, 0.f, 0.f, 0.f}, gj = mj;
@@ -322,19 +369,16 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
           const int i0 = 16 * t + 4 * g;
           const f32x4 hi = quad_of(sp.hi, i0), lo = quad_of(sp.lo, i0);
           unrolled<4>([&](auto r_) __attribute__((always_inline)) {
-              constexpr int r = decltype(r_)::value;
-            if (i0 + r >= own) {
-              const float lw = exp2_fast((hi[r] - hj) + (lo[r] - lj));
-              const float ls = lw * s_j[t][r];
-              mj[r] = ls * delta;
-              gj[r] = lw * delta * w_j[t][r];
-              if (i0 + r == own) {
-                dd = w_j[t][r];
-                diag = ls * dd;
-              } else {
-                u_off += (double)(ls * w_j[t][r]);
-              }
-            }
+            constexpr int r = decltype(r_)::value;
+            const float le = exp2_fast((hi[r] - hj) + (lo[r] - lj));
+            const float lw = i0 + r >= own ? le : 0.f, ls = lw * s_j[t][r];
+            const float tv = ls * w_j[t][r];
+            mj[r] = ls * delta;
+            gj[r] = lw * delta * w_j[t][r];
+            const bool on = i0 + r == own;  // the diagonal
+            dd = on ? w_j[t][r] : dd;
+            diag = on ? tv : diag;
+            u_off += (double)(on ? 0.f : tv);
           });
         }
         m_j[t] = split<T, 2>(mj);
@@ -350,6 +394,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
               mma(db[nt], a, Pair<T>{g_j[2 * kb].q[k], g_j[2 * kb + 1].q[k]});
             });
           });
+  settle<T>();
         }
       });
     }
@@ -358,14 +403,14 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
     // ---- what passes through the states, 64 rows of them at a time
     const float e_i = sp.e[own], to_end = sp.end[own], w_end = delta * to_end;
     float thru = 0.f, dot = 0.f, from = 0.f;
-    for (uint32_t pt = 0; pt < s.ptiles; ++pt) {
+    for (uint32_t pt = 0; pt < ptiles; ++pt) {
       const uint32_t p0 = pt * kPTile, pn = s.head_dim - p0;
-      if (!one) {
+      if constexpr (!kOne) {
         fetch_xdy(h, pt);
         fetch_h(h, pt);
         __syncthreads();
-        tx.put(m.x);
-        tdy.put(m.dy);
+        put_xdy();
+        th.mask(pn, sn);
         th.put(m);
         __syncthreads();
         fetch_dh(h, pt);
@@ -388,12 +433,14 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
         dc[nt] += v * e_i;
       });
       __syncthreads();
+      tdh.mask(pn, sn);
       tdh.put(m);
       dot += tdh.dot(th);
       __syncthreads();
-      if (one && h + 1 < h1) {
-        fetch_xdy(h + 1, 0);
-        fetch_h(h + 1, 0);
+      const float skip_h = skip;
+      if constexpr (kOne) {  // the last head again at the end
+        fetch_xdy(min(h + 1, h1 - 1), 0);
+        fetch_h(min(h + 1, h1 - 1), 0);
       }
       // dH^T x_j
       unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
@@ -407,7 +454,6 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
         db[nt] += v * w_end;
       });
       // dx: through the chunk, and dH b_j
-      const float skip = s.d ? s.d[h] : 0.f;
       unrolled<(int)kPTile / 16>([&](auto q) __attribute__((always_inline)) {
         phase();
         f32x4 in = {0.f, 0.f, 0.f, 0.f}, thr = in, low = in;
@@ -417,6 +463,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
             unrolled<kT2>([&](auto k) __attribute__((always_inline)) {
               mma(in, a, Pair<T>{m_j[2 * kb].q[k], m_j[2 * kb + 1].q[k]});
             });
+  settle<T>();
           }
         });
         unrolled<kNb>([&](auto kb) __attribute__((always_inline)) {
@@ -432,7 +479,8 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
         unrolled<4>([&](auto r_) __attribute__((always_inline)) {
               constexpr int r = decltype(r_)::value;
           thru = fmaf(xv[r], thr[r], thru);
-          o[r] = (uint32_t)own < rows ? fmaf(skip, gv[r], fmaf(w_end, thr[r], in[r])) : 0.f;
+          const float v = fmaf(skip_h, gv[r], fmaf(w_end, thr[r], in[r]));
+              o[r] = (uint32_t)own < rows ? v : 0.f;
         });
         if (writes) store_quad<T, kWideRows>(dx_row + h * s.head_dim + p0, o, 16 * q + 4 * g, pn);
       });
@@ -465,7 +513,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
     const float whole =
         exp2_fast(sp.total) * (m.whole[0] + m.whole[1] + m.whole[2] + m.whole[3]);
     const float da = (float)(a_on + f_on + before) + whole;
-    const float ddt = fmaf(s.a[h], da, (float)u_off + diag + thru) * sp.sig[own];
+    const float ddt = fmaf(a_h, da, (float)u_off + diag + thru) * sp.sig[own];
     const float o[1] = {ddt};
     if (writes && g == 0) store_f32<T, 1>(ddt_row + h, o);
     // one quarter each: da, ddt_bias; dd is on the diagonal's lanes
@@ -477,6 +525,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
       if (g == 1) part[2 * s.heads * parts] = sums;
       if (g == 2) part[s.heads * parts] = dd;
     }
+    fetch_params(min(h + 1, h1 - 1));
   }
   if (writes) {
     unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
@@ -546,15 +595,19 @@ hipError_t launch_scan_grad(const nsfps_scan_args &a, const nsfps_scan_grads &g,
       constexpr bool kWideRows = decltype(w)::value;
       constexpr size_t lds = sizeof(GradLds<T, NT>);
       static_assert(lds <= 160 * 1024, "LDS");
-      const hipError_t e2 = hipFuncSetAttribute((const void *)k_scan_grad<T, NT, kWideRows>,
-                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-      if (e2 != hipSuccess) return e2;
-      constexpr uint64_t kLaunch = 1u << 23;  // workgroups of a launch: fewer than 2^32 threads
-      for (uint64_t at = 0; at < work; at += kLaunch) {
-        const uint32_t some = (uint32_t)std::min(kLaunch, work - at);
-        k_scan_grad<T, NT, kWideRows><<<some, 256, lds, st>>>(s, d, at, some);
-      }
-      return hipGetLastError();
+      const auto go = [&](auto kernel) {
+        const hipError_t e2 = hipFuncSetAttribute(
+            (const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e2 != hipSuccess) return e2;
+        constexpr uint64_t kLaunch = 1u << 23;  // workgroups of a launch: fewer than 2^32 threads
+        for (uint64_t at = 0; at < work; at += kLaunch) {
+          const uint32_t some = (uint32_t)std::min(kLaunch, work - at);
+          kernel<<<some, 256, lds, st>>>(s, d, at, some);
+        }
+        return hipGetLastError();
+      };
+      return s.ptiles == 1 ? go(k_scan_grad<T, NT, true, kWideRows>)
+                           : go(k_scan_grad<T, NT, false, kWideRows>);
     });
     if (e != hipSuccess) return e;
   }
@@ -564,7 +617,7 @@ hipError_t launch_scan_grad(const nsfps_scan_args &a, const nsfps_scan_grads &g,
 }
 
 hipError_t preload_scan_grad_kernels() {
-  return func_attributes(k_scan_grad<bf16, 64, true>, k_scan_grad_join);
+  return func_attributes(k_scan_grad<bf16, 64, true, true>, k_scan_grad_join);
 }
 
 }  // namespace nsfps
