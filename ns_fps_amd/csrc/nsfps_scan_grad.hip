@@ -97,12 +97,20 @@ struct StateTile {
       for (int k = 0; k < Terms<T, 3>::kN; ++k) put_quad(m.h[k], kLd<T, NT>, p, n, t.q[k]);
     }
   }
-  __device__ __forceinline__ float dot(const StateTile &o) const {
+  // <this, the state put in LDS by the same threads>: its terms add up to it
+  template <typename T>
+  __device__ __forceinline__ float dot(const GradLds<T, NT> &m) const {
     float d = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + 256 * i, p = e / (NT / 4), n = (e % (NT / 4)) * 4;
+      f32x4 h = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d = fmaf(v[i][k], o.v[i][k], d);
+      for (int k = Terms<T, 3>::kN - 1; k >= 0; --k)
+        h += quad_f32(quad_row(m.h[k], kLd<T, NT>, p, n));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d = fmaf(v[i][k], h[k], d);
+    }
     return d;
   }
 };
@@ -115,16 +123,40 @@ __device__ __forceinline__ void phase() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+// The two 32-lane halves (or, in each half, the two 16-lane quarters) added:
+// the swap leaves one side's values in both places of one result and the other
+// side's in the other.
+__device__ __forceinline__ float add_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_quarters(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <bool kHalves>
+__device__ __forceinline__ double add_sides(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+  uint32_t l[2], h[2];
+  if constexpr (kHalves) {
+    const auto a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+    const auto b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    l[0] = a[0], l[1] = a[1], h[0] = b[0], h[1] = b[1];
+  } else {
+    const auto a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    l[0] = a[0], l[1] = a[1], h[0] = b[0], h[1] = b[1];
+  }
+  return __builtin_bit_cast(double, ((uint64_t)h[0] << 32) | l[0]) +
+         __builtin_bit_cast(double, ((uint64_t)h[1] << 32) | l[1]);
 }
 // over the four quads of a column (lanes l, 16 + l, 32 + l, 48 + l)
-template <typename V>
-__device__ __forceinline__ V column_sum(V v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+__device__ __forceinline__ float column_sum(float v) { return add_halves(add_quarters(v)); }
+__device__ __forceinline__ double column_sum(double v) {
+  return add_sides<true>(add_sides<false>(v));
 }
 
 // v of lane l - K of the same 16 lanes, 0 where there is none (DPP row shift)
@@ -135,13 +167,21 @@ __device__ __forceinline__ double row_shift(double v) {
   const uint32_t hi = __builtin_amdgcn_update_dpp(0u, (uint32_t)(u >> 32), 0x110 + K, 0xf, 0xf, true);
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
+template <int K>
+__device__ __forceinline__ float row_shift(float v) {
+  return __uint_as_float(
+      __builtin_amdgcn_update_dpp(0u, __float_as_uint(v), 0x110 + K, 0xf, 0xf, true));
+}
 // inclusive sum over lanes 0 .. l of each 16
-__device__ __forceinline__ double row_scan(double v) {
+template <typename V>
+__device__ __forceinline__ V row_scan(V v) {
   v += row_shift<1>(v);
   v += row_shift<2>(v);
   v += row_shift<4>(v);
   return v + row_shift<8>(v);
 }
+// over the wave, in lanes 15, 31, 47 and 63
+__device__ __forceinline__ float wave_sum(float v) { return column_sum(row_scan(v)); }
 
 // Four values of a lane's column to a row of global memory.
 template <typename T, bool kWideRows>
@@ -394,7 +434,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
               mma(db[nt], a, Pair<T>{g_j[2 * kb].q[k], g_j[2 * kb + 1].q[k]});
             });
           });
-  settle<T>();
+          settle<T>();
         }
       });
     }
@@ -428,20 +468,18 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
         v += low;
         const f32x4 cv = quad_f32(quad_row(m.c, ldn, own, 16 * nt + 4 * g));
         unrolled<4>([&](auto r_) __attribute__((always_inline)) {
-              constexpr int r = decltype(r_)::value; from = fmaf(cv[r], v[r], from);
+          constexpr int r = decltype(r_)::value;
+          from = fmaf(cv[r], v[r], from);
         });
         dc[nt] += v * e_i;
       });
       __syncthreads();
       tdh.mask(pn, sn);
+      dot += tdh.dot(m);
       tdh.put(m);
-      dot += tdh.dot(th);
       __syncthreads();
       const float skip_h = skip;
-      if constexpr (kOne) {  // the last head again at the end
-        fetch_xdy(min(h + 1, h1 - 1), 0);
-        fetch_h(min(h + 1, h1 - 1), 0);
-      }
+      if constexpr (kOne) fetch_xdy(min(h + 1, h1 - 1), 0);  // the last again at the end
       // dH^T x_j
       unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
         phase();
@@ -463,7 +501,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
             unrolled<kT2>([&](auto k) __attribute__((always_inline)) {
               mma(in, a, Pair<T>{m_j[2 * kb].q[k], m_j[2 * kb + 1].q[k]});
             });
-  settle<T>();
+            settle<T>();
           }
         });
         unrolled<kNb>([&](auto kb) __attribute__((always_inline)) {
@@ -477,33 +515,32 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
         const f32x4 gv = quad_f32(quad_row(m.dy, ldx, own, 16 * q + 4 * g));
         f32x4 o;
         unrolled<4>([&](auto r_) __attribute__((always_inline)) {
-              constexpr int r = decltype(r_)::value;
+          constexpr int r = decltype(r_)::value;
           thru = fmaf(xv[r], thr[r], thru);
           const float v = fmaf(skip_h, gv[r], fmaf(w_end, thr[r], in[r]));
-              o[r] = (uint32_t)own < rows ? v : 0.f;
+          o[r] = (uint32_t)own < rows ? v : 0.f;
         });
         if (writes) store_quad<T, kWideRows>(dx_row + h * s.head_dim + p0, o, 16 * q + 4 * g, pn);
       });
     }
     phase();
+    if constexpr (kOne) fetch_h(min(h + 1, h1 - 1), 0);
     thru = column_sum(thru) * to_end;  // per delta_j
     from = column_sum(from) * e_i;
     dot = wave_sum(dot);
 
     // ---- the exponents: sums over the chunk's tokens from each on, and before
-    // it.  The 16 tokens of a wave are lanes l of each quarter, so the quarters
-    // take one of the sums each.
+    // it.  The 16 tokens of a wave are lanes l of each quarter.
     const double after = rt - (double)delta * u_off;  // cancels over the tokens
     const double mine = (double)delta * thru;
-    const double sum = row_scan(g == 0 ? after : g == 1 ? (double)from : mine);
-    if (l == 15) {
-      if (g == 0) m.after[wave] = sum;
-      if (g == 1) m.from[wave] = sum;
-      if (g == 2) m.before[wave] = sum;
-      if (g == 3) m.whole[wave] = dot;
+    const double sum_after = row_scan(after), sum_from = row_scan((double)from),
+                 sum_before = row_scan(mine);
+    if (lane == 15) {
+      m.after[wave] = sum_after;
+      m.from[wave] = sum_from;
+      m.before[wave] = sum_before;
+      m.whole[wave] = dot;
     }
-    const double sum_after = __shfl(sum, l, 64), sum_from = __shfl(sum, 16 + l, 64),
-                 sum_before = __shfl(sum, 32 + l, 64);
     __syncthreads();
     double a_on = after - sum_after, f_on = (double)from - sum_from, before = sum_before - mine;
     unrolled<4>([&](auto o) __attribute__((always_inline)) {
@@ -536,20 +573,31 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
 }
 
 // One workgroup per head and parameter: the chunks' parts in a fixed order.
-__global__ __launch_bounds__(256) void k_scan_grad_join(const float *__restrict__ part,
-                                                        uint64_t count, uint32_t heads, float *da,
-                                                        float *dd, float *ddt_bias) {
-  __shared__ double s_sum[4];
+__global__ __launch_bounds__(1024) void k_scan_grad_join(const float *__restrict__ part,
+                                                         uint64_t count, uint32_t heads, float *da,
+                                                         float *dd, float *ddt_bias) {
+  constexpr uint32_t kAhead = 8;
+  __shared__ double s_sum[16];
   float *const out[3] = {da, dd, ddt_bias};
   const uint32_t h = blockIdx.x, k = blockIdx.y;
   const float *p = part + ((uint64_t)k * heads + h) * count;
   double sum = 0.0;
-  for (uint64_t i = threadIdx.x; i < count; i += 256) sum += p[i];
+  for (uint64_t i = threadIdx.x; i < count; i += 1024 * kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) v[j] = p[min(i + 1024 * j, count - 1)];
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) sum += i + 1024 * j < count ? (double)v[j] : 0.0;
+  }
 #pragma unroll
   for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
   if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
   __syncthreads();
-  if (threadIdx.x == 0 && out[k]) out[k][h] = (float)(s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3]);
+  if (threadIdx.x == 0 && out[k]) {
+    double all = 0.0;
+    for (int w = 0; w < 16; ++w) all += s_sum[w];
+    out[k][h] = (float)all;
+  }
 }
 
 uint64_t part_bytes(const nsfps_scan_args &a) {
@@ -611,7 +659,7 @@ hipError_t launch_scan_grad(const nsfps_scan_args &a, const nsfps_scan_grads &g,
     });
     if (e != hipSuccess) return e;
   }
-  k_scan_grad_join<<<dim3(a.heads, 3), 256, 0, st>>>(d.part, 4 * parts, a.heads, g.d_da, g.d_dd,
+  k_scan_grad_join<<<dim3(a.heads, 3), 1024, 0, st>>>(d.part, 4 * parts, a.heads, g.d_da, g.d_dd,
                                                      g.d_ddt_bias);
   return hipGetLastError();
 }
