@@ -7,11 +7,10 @@
 // are sorted with their positions (stable, so a row's positions are in
 // order), start[v] is found at the sorted tokens' boundaries, and each table
 // row's terms are added in float32, in that order, by the lanes that hold its
-// columns, and the row is written once: no atomics on values, the same bits every time, and rows
-// without a token cost their zeros.  A crowded row (more than kLong terms:
+// columns, and the row is written once: no atomics on values, the same bits
+// every time, and rows without a token cost their zeros.  A crowded row (more than kLong terms:
 // grid cells near an object) is cut into pieces of kPiece terms, a wave each,
-// whose sums (in float64: the
-// terms may be many) are added in order by a last pass.  Where pieces lie in the
+// whose sums (in float64: the terms may be many) are added in order by a last pass.  Where pieces lie in the
 // workspace is decided by an atomic counter; no sum depends on it.
 #include "nsfps_launch.h"
 #include "nsfps_seq_device.h"
@@ -73,7 +72,7 @@ __global__ __launch_bounds__(256) void k_embed(const T *__restrict__ table,
 // are four waves' runs of 512 in order; a wave ranks 64 at a time by ballots.
 // (The sampling build's 8-bit sort of 4,096-key tiles took 99 us for 524,288
 // tokens of 19 bits, this one 39; for 16,384 tokens of 14 bits one workgroup
-// in LDS took 34 us.)
+// in LDS took 34 us, two passes 28, and one pass over whole keys 13.)
 constexpr int kDigitBits = 10;
 constexpr uint32_t kTokTile = 2048;
 constexpr int kTokRounds = kTokTile / 256;
@@ -87,38 +86,40 @@ __device__ __forceinline__ uint32_t token_key(const int32_t *tokens, const uint3
 }
 
 // keys null: the first pass, from the tokens; it clears the counters too.
-__global__ __launch_bounds__(256) void k_token_hist(const int32_t *__restrict__ tokens,
-                                                    const uint32_t *__restrict__ keys,
-                                                    uint32_t count, uint32_t rows, int shift,
-                                                    int bits, uint32_t *__restrict__ hist,
-                                                    uint32_t *__restrict__ counters) {
-  __shared__ uint32_t s_cnt[1 << kDigitBits];
-  const uint32_t digits = 1u << bits;
+// A key's digit, (key >> shift) & mask, is below digits.
+template <uint32_t kThreads, uint32_t kTile>
+__global__ __launch_bounds__(kThreads) void k_token_hist(
+    const int32_t *__restrict__ tokens, const uint32_t *__restrict__ keys, uint32_t count,
+    uint32_t rows, int shift, uint32_t digits, uint32_t mask, uint32_t *__restrict__ hist,
+    uint32_t *__restrict__ counters) {
+  constexpr uint32_t kRounds = kTile / kThreads;
+  extern __shared__ uint32_t s_cnt[];
   if (!keys && blockIdx.x == 0 && threadIdx.x < 2) counters[threadIdx.x] = 0;
-  for (uint32_t d = threadIdx.x; d < digits; d += 256) s_cnt[d] = 0;
+  for (uint32_t d = threadIdx.x; d < digits; d += kThreads) s_cnt[d] = 0;
   __syncthreads();
-  const uint64_t base = (uint64_t)blockIdx.x * kTokTile;
-  uint32_t key[kTokRounds];
+  const uint64_t base = (uint64_t)blockIdx.x * kTile;
+  uint32_t key[kRounds];
 #pragma unroll
-  for (int r = 0; r < kTokRounds; ++r) {
-    const uint64_t i = base + r * 256 + threadIdx.x;
+  for (uint32_t r = 0; r < kRounds; ++r) {
+    const uint64_t i = base + r * kThreads + threadIdx.x;
     key[r] = i < count ? token_key(tokens, keys, (uint32_t)i, rows) : 0u;
   }
 #pragma unroll
-  for (int r = 0; r < kTokRounds; ++r)
-    if (base + r * 256 + threadIdx.x < count)
-      atomicAdd(&s_cnt[(key[r] >> shift) & (digits - 1)], 1u);
+  for (uint32_t r = 0; r < kRounds; ++r)
+    if (base + r * kThreads + threadIdx.x < count)
+      atomicAdd(&s_cnt[(key[r] >> shift) & mask], 1u);
   __syncthreads();
-  for (uint32_t d = threadIdx.x; d < digits; d += 256)
+  for (uint32_t d = threadIdx.x; d < digits; d += kThreads)
     hist[(uint64_t)blockIdx.x * digits + d] = s_cnt[d];
 }
 
 // hist[tile][digit] becomes the digit's count in the tiles ahead; totals[digit].
 // 64 digits a workgroup, its 16 waves a run of the tiles each.
 __global__ __launch_bounds__(1024) void k_token_scan(uint32_t *__restrict__ hist, uint32_t tiles,
-                                                     int bits, uint32_t *__restrict__ totals) {
+                                                     uint32_t digits,
+                                                     uint32_t *__restrict__ totals) {
   __shared__ uint32_t s_sum[16][64];
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, digits = 1u << bits;
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t d = blockIdx.x * 64 + lane, run = ceil_div(tiles, 16);
   const uint32_t a = min(wave * run, tiles), b = min(a + run, tiles);
   constexpr uint32_t kAhead = 8;
@@ -234,6 +235,102 @@ __global__ __launch_bounds__(256) void k_token_scatter(
     const uint32_t at = s_cnt[wave][(key[r] >> shift) & (digits - 1)] + rank[r];
     kout[at] = key[r];
     vout[at] = val[r];
+  }
+}
+
+// The scatter of a sort in one pass, a digit being a whole key (0 .. rows): the
+// digits' first places are start itself.  Eight waves rank 128 tokens each, so
+// that a wave's count of a key fits a byte.
+constexpr uint32_t kPlaceTile = 1024, kPlaceThreads = 512, kPlaceWaves = 8;
+constexpr uint32_t kPlaceDigits = 12288;  // what 160 KB of LDS hold
+constexpr int kPlaceQuads = kPlaceDigits / 4 / kPlaceThreads;
+constexpr uint32_t place_lds(uint32_t digits) { return ((digits + 3) & ~3u) * (4 + kPlaceWaves); }
+
+__global__ __launch_bounds__(512) void k_token_place(const int32_t *__restrict__ tokens,
+                                                     uint32_t *__restrict__ pos, uint32_t count,
+                                                     uint32_t rows, int bits,
+                                                     const uint32_t *__restrict__ hist,
+                                                     const uint32_t *__restrict__ totals,
+                                                     uint32_t *__restrict__ start) {
+  // first places [d4], then the waves' counts [waves][d4]
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_first[];
+  __shared__ uint32_t s_wave[kPlaceWaves];
+  constexpr int kRounds = kPlaceTile / kPlaceThreads;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, digits = rows + 1,
+                 d4 = (digits + 3) & ~3u, quads = d4 / 4, each = ceil_div(quads, kPlaceThreads);
+  uint8_t *const s_cnt = (uint8_t *)(s_first + d4);
+  const uint64_t lt = lane ? (~0ull >> (64 - lane)) : 0ull;
+  const uint64_t base = (uint64_t)blockIdx.x * kPlaceTile + wave * (kPlaceTile / kPlaceWaves);
+  uint32_t key[kRounds], at[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const uint64_t i = base + r * 64 + lane;
+    key[r] = i < count ? token_key(tokens, nullptr, (uint32_t)i, rows) : 0u;
+  }
+  // this thread's digits: `each` (at most kPlaceQuads) quads of them, one after another.
+  // Past the last digit the arrays' padding is read and written; no sum that
+  // is used has it.
+  uint4 q[kPlaceQuads];
+#pragma unroll
+  for (int k = 0; k < kPlaceQuads; ++k) {
+    const uint32_t v = tid * each + k;
+    q[k] = (uint32_t)k < each && v < quads ? ((const uint4 *)totals)[v] : make_uint4(0, 0, 0, 0);
+  }
+  for (uint32_t v = tid; v < quads * kPlaceWaves / 4; v += kPlaceThreads)
+    ((uint4 *)s_cnt)[v] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) at[r] = hist[(uint64_t)blockIdx.x * digits + key[r]];
+  uint32_t sum = 0;
+#pragma unroll
+  for (int k = 0; k < kPlaceQuads; ++k) sum += q[k].x + q[k].y + q[k].z + q[k].w;
+  const uint32_t own = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t o = __shfl_up(sum, off, 64);
+    if (lane >= (uint32_t)off) sum += o;
+  }
+  if (lane == 63) s_wave[wave] = sum;
+  __syncthreads();
+  sum -= own;
+#pragma unroll
+  for (uint32_t w = 0; w < kPlaceWaves; ++w) sum += w < wave ? s_wave[w] : 0u;
+#pragma unroll
+  for (int k = 0; k < kPlaceQuads; ++k) {
+    const uint32_t v = tid * each + k;
+    if ((uint32_t)k >= each || v >= quads) continue;
+    const uint4 f = make_uint4(sum, sum + q[k].x, sum + q[k].x + q[k].y,
+                               sum + q[k].x + q[k].y + q[k].z);
+    sum = f.w + q[k].w;
+    ((uint4 *)s_first)[v] = f;
+    if (blockIdx.x == 0) ((uint4 *)start)[v] = f;
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const bool valid = base + r * 64 + lane < count;
+    const uint32_t d = key[r];
+    uint64_t peers = __ballot(valid);
+    for (int k = 0; k < bits; ++k) {
+      const uint64_t m = __ballot((d >> k) & 1u);
+      peers &= ((d >> k) & 1u) ? m : ~m;
+    }
+    const uint32_t before = (uint32_t)__popcll(peers & lt);
+    const uint32_t baseq = valid ? s_cnt[wave * d4 + d] : 0u;
+    at[r] += baseq + before;
+    // all lanes read their base before a leader writes (in-order LDS, one wave)
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    if (valid && before == 0)
+      s_cnt[wave * d4 + d] = (uint8_t)(baseq + (uint32_t)__popcll(peers));
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const uint64_t i = base + r * 64 + lane;
+    if (i >= count) continue;
+    uint32_t place = s_first[key[r]] + at[r];
+#pragma unroll
+    for (uint32_t w = 0; w < kPlaceWaves; ++w) place += w < wave ? s_cnt[w * d4 + key[r]] : 0u;
+    pos[place] = (uint32_t)i;
   }
 }
 
@@ -440,9 +537,11 @@ __global__ __launch_bounds__(1024) void k_embed_join(const uint32_t *__restrict_
 
 struct GradPlan {
   uint64_t keys, vals, keys2, vals2, hist, totals, start, counters, longs, pieces, part, total;
-  uint32_t long_max, piece_max, tiles;
+  uint32_t long_max, piece_max, tiles, digits;
   int passes, bits;  // of a pass
+  bool whole;        // one pass, a digit a whole key
 };
+
 
 GradPlan grad_plan(const nsfps_embed_args &a) {
   GradPlan p;
@@ -456,15 +555,22 @@ GradPlan grad_plan(const nsfps_embed_args &a) {
   while (bits < 32 && (a.rows >> bits)) ++bits;  // keys 0 .. rows
   p.passes = (bits + kDigitBits - 1) / kDigitBits;
   p.bits = (bits + p.passes - 1) / p.passes;
-  p.tiles = (uint32_t)host_ceil_div(a.tokens, kTokTile);
+  // One pass over whole keys where their counts fit LDS and the histograms
+  // (one a tile) stay small.  us a gradient of 64 columns, in passes of 10 bits
+  // and in one: 1,000 tokens of 8,192 rows 41, 20; 16,384 of 1,000 46, 37;
+  // 16,384 of 12,000 48, 33; 262,144 of 12,000 220, 208.
+  p.whole = a.rows < kPlaceDigits && a.tokens <= 256 * kPlaceTile;
+  p.tiles = (uint32_t)host_ceil_div(a.tokens, p.whole ? kPlaceTile : kTokTile);
+  if (p.whole) p.passes = 1, p.bits = bits;
+  p.digits = p.whole ? (uint32_t)a.rows + 1 : 1u << p.bits;
   p.long_max = (uint32_t)(a.tokens / (kLong + 1));
   p.piece_max = (uint32_t)(a.tokens / kPiece) + p.long_max;
   p.keys = take(4 * a.tokens);
   p.vals = take(4 * a.tokens);
   p.keys2 = take(4 * a.tokens);
   p.vals2 = take(4 * a.tokens);
-  p.hist = take(4ull * p.tiles << p.bits);
-  p.totals = take(4ull << p.bits);
+  p.hist = take(4ull * p.tiles * p.digits);
+  p.totals = take(4ull * p.digits);
   p.start = take(4 * (a.rows + 1));
   p.counters = take(8);
   p.longs = take(sizeof(LongRow) * (uint64_t)p.long_max);
@@ -486,17 +592,31 @@ hipError_t run_grad(const nsfps_embed_args &a, hipStream_t st) {
   uint32_t *const hist = (uint32_t *)(w + p.hist), *const totals = (uint32_t *)(w + p.totals);
   for (int pass = 0; pass < p.passes && count; ++pass) {
     const int shift = pass * p.bits;
-    k_token_hist<<<p.tiles, 256, 0, st>>>(a.d_tokens, keys, count, rows, shift, p.bits, hist,
-                                          counters);
-    k_token_scan<<<((1u << p.bits) + 63) / 64, 1024, 0, st>>>(hist, p.tiles, p.bits, totals);
+    if (p.whole) {
+      const hipError_t e = hipFuncSetAttribute(
+          (const void *)k_token_place, hipFuncAttributeMaxDynamicSharedMemorySize,
+          (int)place_lds(kPlaceDigits));
+      if (e != hipSuccess) return e;
+      pos = pos_buf[0];
+      k_token_hist<kPlaceTile, kPlaceTile><<<p.tiles, kPlaceTile, 4 * p.digits, st>>>(
+          a.d_tokens, nullptr, count, rows, 0, p.digits, ~0u, hist, counters);
+      k_token_scan<<<(p.digits + 63) / 64, 1024, 0, st>>>(hist, p.tiles, p.digits, totals);
+      k_token_place<<<p.tiles, kPlaceThreads, place_lds(p.digits), st>>>(
+          a.d_tokens, pos, count, rows, p.bits, hist, totals, start);
+      break;
+    }
+    k_token_hist<256, kTokTile><<<p.tiles, 256, 4 * p.digits, st>>>(
+        a.d_tokens, keys, count, rows, shift, p.digits, p.digits - 1, hist, counters);
+    k_token_scan<<<(p.digits + 63) / 64, 1024, 0, st>>>(hist, p.tiles, p.digits, totals);
     k_token_scatter<<<p.tiles, 256, 0, st>>>(a.d_tokens, keys, pos, key_buf[pass & 1],
                                              pos_buf[pass & 1], count, rows, shift, p.bits, hist,
                                              totals);
     keys = key_buf[pass & 1];
     pos = pos_buf[pass & 1];
   }
-  k_embed_starts<<<(uint32_t)host_ceil_div((uint64_t)count + 1, 256), 256, 0, st>>>(keys, count,
-                                                                                   rows, start);
+  if (!p.whole || !count)
+    k_embed_starts<<<(uint32_t)host_ceil_div((uint64_t)count + 1, 256), 256, 0, st>>>(keys, count,
+                                                                                     rows, start);
   const uint32_t vecs = a.width / V;
   const T *dout = (const T *)a.d_out;
   G *dtable = (G *)a.d_table;
@@ -567,7 +687,9 @@ hipError_t launch_embed_grad(const nsfps_embed_args &a, hipStream_t st) {
 
 hipError_t preload_embed_kernels() {
   return func_attributes(k_embed<bf16, 8>, k_embed<bf16, 1>, k_embed<float, 4>, k_embed<float, 1>,
-                         k_token_hist, k_token_scan, k_token_scatter, k_embed_starts, k_embed_rows<bf16, bf16, 8>,
+                         k_token_hist<256, kTokTile>,
+                         k_token_hist<kPlaceTile, kPlaceTile>, k_token_scan, k_token_scatter, k_token_place, k_embed_starts,
+                         k_embed_rows<bf16, bf16, 8>,
                          k_embed_rows<float, float, 4>);
 }
 
