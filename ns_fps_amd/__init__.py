@@ -4,7 +4,10 @@
   reference's import path (SpaceRange, make_range, make_uniform_range, fps,
   fps_with_bbox, constants, plus fps_batched and the grouping step), built
   from csrc/ by ``python -m ns_fps_amd.build``.
-* ``ns_fps_amd.capi`` -- ctypes binding of the C ABI (include/nsfps.h).
+* ``ns_fps_amd.capi`` -- ctypes binding of the C ABI (include/nsfps.h), with
+  the sequence operators over the samples (lookup, causal convolution,
+  selective scan, their gradients, the one-token step); examples/
+  sequence_model.py runs them as one model.
 * ``ns_fps_amd.workloads`` -- seeded synthetic clouds of the benchmark.
 * ``ns_fps_amd.kitti`` -- KITTI scan files: reader, z filter, bounds range
   and the reference drivers' sampling runs.
