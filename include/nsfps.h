@@ -383,9 +383,10 @@ nsfps_status nsfps_conv_grad_device(const nsfps_conv_args *args, const nsfps_con
  * x and y: rows of heads * head_dim; b and c: rows of groups * state_dim
  * (group g serves heads g * heads / groups onwards); dt: rows of heads; all
  * of type dtype; a, d and dt_bias: [heads] float32 (d and dt_bias may be
- * NULL).  a is not positive: exp(step * a) is a decay.  A dt of -infinity is
- * a step of 0: the token leaves the state as it is.  Non-finite inputs
- * elsewhere spoil their sequence, and no other.  d_state (or NULL) is the
+ * NULL).  a is not positive: exp(step * a) is a decay; an a of -infinity
+ * forgets the state at every token, an a of NaN spoils its head.  A dt of
+ * -infinity is a step of 0: the token leaves the state as it is.  Non-finite
+ * inputs elsewhere spoil their sequence, and no other.  d_state (or NULL) is the
  * scan cache.  groups divides heads; head_dim and state_dim at most 128;
  * batch * heads at most 2^20; batch * length at most 2^31 - 1.
  *

@@ -70,13 +70,17 @@ __device__ __forceinline__ float number(const Raw<T, 1> &r) {
 __device__ __forceinline__ void chunk_steps(Steps &o, float raw, bool inside, float a) {
   const uint32_t lane = threadIdx.x & 63u;
   const float delta = inside ? softplus(raw) : 0.f;
-  double sum = (double)delta * (double)a * 1.4426950408889634074;
+  // A decay of 2^-1024 is 0 beside any float32, so no token counts for less:
+  // the chunk's sums stay within 2^16, where the pair resolves 2^-31 however
+  // far a token has gone, and -infinity stays out.  NaN stays in.  Past the end
+  // nothing is added, whatever a is.
+  double sum = inside ? (double)delta * (double)a * 1.4426950408889634074 : 0.0;
+  sum = sum < -1024.0 ? -1024.0 : sum;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const double o2 = __shfl_up(sum, off, 64);
     if (lane >= (uint32_t)off) sum += o2;
   }
-  sum = fmax(sum, -1e30);  // every decay is 0 long before; keeps infinities out
   const double last = __shfl(sum, 63, 64);
   o.delta[lane] = delta;
   o.sig[lane] = inside ? sigmoid(raw) : 0.f;
