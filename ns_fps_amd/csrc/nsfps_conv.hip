@@ -234,8 +234,8 @@ __global__ __launch_bounds__(256) void k_conv_grad(nsfps_rows x, nsfps_rows dy, 
 #pragma unroll
               for (int k = 0; k < W; ++k) pre = fmaf(w[j * W + k], win[k][j], pre);
               const float sig = sigmoid(pre);
-              // past the sequence's end dy was not read: zero
-              const float gt = gv[j] * sig * fmaf(pre, 1.f - sig, 1.f);
+              // past the sequence's end the slope counts for nothing, not even as NaN
+              const float gt = kFull || t < len ? gv[j] * sig * fmaf(pre, 1.f - sig, 1.f) : 0.f;
 #pragma unroll
               for (int k = W - 1; k > 0; --k) g[k][j] = g[k - 1][j];
               g[0][j] = gt;
