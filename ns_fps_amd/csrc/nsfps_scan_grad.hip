@@ -227,7 +227,9 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
   const uint32_t len = scan_length(s, b), t0 = c * kChunk, sn = s.state_dim;
   const uint32_t out_rows = min(kChunk, s.length - t0);
   const uint32_t rows = t0 < len ? min(kChunk, len - t0) : 0u;
-  const bool writes = (uint32_t)own < out_rows;
+  // Rows past the end are zeros even where the sequence is spoiled: sums over
+  // the chunk's tokens bring a NaN to all of them.
+  const bool writes = (uint32_t)own < out_rows, inside = (uint32_t)own < rows;
   const uint64_t parts = (uint64_t)s.batch * s.chunks * 4;
   const auto rows_at = [&](const nsfps_rows &r) {
     return (T *)r.p + (uint64_t)b * r.batch_stride + (uint64_t)t0 * r.row_stride;
@@ -523,7 +525,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
           constexpr int r = decltype(r_)::value;
           thru = fmaf(xv[r], thr[r], thru);
           const float v = fmaf(skip_h, gv[r], fmaf(w_end, thr[r], in[r]));
-          o[r] = (uint32_t)own < rows ? v : 0.f;
+          o[r] = inside ? v : 0.f;
         });
         if (writes) store_quad<T, kWideRows>(dx_row + h * s.head_dim + p0, o, 16 * q + 4 * g, pn);
       });
@@ -556,7 +558,7 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
         exp2_fast(sp.total) * (m.whole[0] + m.whole[1] + m.whole[2] + m.whole[3]);
     const float da = (float)(a_on + f_on + before) + whole;
     const float ddt = fmaf(a_h, da, (float)u_off + diag + thru) * sp.sig[own];
-    const float o[1] = {ddt};
+    const float o[1] = {inside ? ddt : 0.f};
     if (writes && g == 0) store_f32<T, 1>(ddt_row + h, o);
     // one quarter each: da, ddt_bias; dd is on the diagonal's lanes
     const float sums = (float)row_scan(g == 0 ? (double)delta * da : (double)ddt);
@@ -570,9 +572,10 @@ __global__ __launch_bounds__(256, (kGradGroups<T, NT>)) void k_scan_grad(ScanDev
     fetch_params(min(h + 1, h1 - 1));
   }
   if (writes) {
+    const f32x4 z = {0.f, 0.f, 0.f, 0.f};
     unrolled<kNt>([&](auto nt) __attribute__((always_inline)) {
-      store_quad<T, kWideRows>(db_row, db[nt], 16 * nt + 4 * g, sn);
-      store_quad<T, kWideRows>(dc_row, dc[nt], 16 * nt + 4 * g, sn);
+      store_quad<T, kWideRows>(db_row, inside ? db[nt] : z, 16 * nt + 4 * g, sn);
+      store_quad<T, kWideRows>(dc_row, inside ? dc[nt] : z, 16 * nt + 4 * g, sn);
     });
   }
 }

@@ -4,9 +4,16 @@ holds, and nothing of them in the gradients before the end."""
 import pytest
 import torch
 
+import test_sequence as base
 from ns_fps_amd import capi
 from test_sequence import DTYPES, F64, close, lib, ptr, rnd, rows, stream, workspace  # noqa: F401
-from test_sequence_decays import INF, NAN
+from test_sequence_decays import INF, NAN, finite_scan_inputs, run_scan_grad
+
+
+def same(got, want):
+    """The same bits, NaN where NaN is."""
+    return torch.equal(torch.isnan(got), torch.isnan(want)) and \
+        torch.equal(torch.nan_to_num(got, nan=-7.0), torch.nan_to_num(want, nan=-7.0))
 
 
 @pytest.mark.gpu
@@ -74,3 +81,25 @@ def test_convolution_gradient_reads_no_slope_past_the_end(lib, dtype, channels):
     close(dx[0], want, "dx")
     close(dw, torch.stack([(g[1:] * x64[:-1]).sum(0), (g * x64).sum(0)], 1), "dweight")
     close(db, g.sum(0), "dbias")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("what", ["x", "dt", "b", "c", "dy"])
+@pytest.mark.parametrize("case", [(3, 100, 4, 2, 16, 24, "plain"), (2, 100, 5, 1, 100, 64, "plain")])
+def test_scan_gradient_past_the_end_is_zero(lib, case, dtype, what):  # noqa: F811
+    """A sequence spoiled by one NaN has zeros after its end in every output,
+    and the sequences beside it keep their bits."""
+    t, code, gen, x, dt, a, bm, cm, d, bias, _ = finite_scan_inputs(case, dtype)
+    batch, length, heads, groups, p, n, _ = case
+    dy = rnd(gen, batch, length, heads, p, dtype=t)
+    lens = [70] * batch
+    outs = []
+    for spoil in (False, True):
+        if spoil:
+            {"x": x, "dt": dt, "b": bm, "c": cm, "dy": dy}[what][0, 66] = NAN
+        D = base.on_device(case, x, dt, a, bm, cm, d, bias, lens)
+        outs.append(run_scan_grad(lib, case, code, D, dy.flatten(2).cuda())[:4])
+    for clean, got in zip(*outs):
+        assert got[0, 70:].eq(0).all()
+        assert same(got[1:], clean[1:])
