@@ -137,7 +137,8 @@ __global__ __launch_bounds__(256) void k_conv(nsfps_rows x, nsfps_rows y, Seqs s
             float pre = bs[j];
 #pragma unroll
             for (int k = 0; k < W; ++k) pre = fmaf(w[j * W + k], win[k][j], pre);
-            o[j] = kFull || t < len ? pre * sigmoid(pre) : 0.f;
+            const float sig = sizeof(T) == 4 ? sigmoid(pre) : sigmoid_8bit(pre);
+            o[j] = kFull || t < len ? pre * sig : 0.f;
           }
           if (kFull || t < s.length) store_f32<T, V>(yr + (uint64_t)t * y.row_stride, o);
 #pragma unroll
@@ -233,9 +234,9 @@ __global__ __launch_bounds__(256) void k_conv_grad(nsfps_rows x, nsfps_rows dy, 
               float pre = bs[j];
 #pragma unroll
               for (int k = 0; k < W; ++k) pre = fmaf(w[j * W + k], win[k][j], pre);
-              const float sig = sigmoid(pre);
+              const Logistic s1 = logistic(pre);
               // past the sequence's end the slope counts for nothing, not even as NaN
-              const float gt = kFull || t < len ? gv[j] * sig * fmaf(pre, 1.f - sig, 1.f) : 0.f;
+              const float gt = kFull || t < len ? gv[j] * s1.sig * fmaf(pre, s1.rest, 1.f) : 0.f;
 #pragma unroll
               for (int k = W - 1; k > 0; --k) g[k][j] = g[k - 1][j];
               g[0][j] = gt;

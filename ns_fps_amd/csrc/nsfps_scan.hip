@@ -464,7 +464,11 @@ __global__ __launch_bounds__(256) void k_scan_step(nsfps_step_args a, uint32_t p
     if (is_x || (pt == 0 && h % (a.heads / a.groups) == 0))
       store_f32<T, 1>(ring + entry[0] * channels + ch, in[0]);
   }
-  const float delta = softplus(raw[0]), decay = exp2_fast(delta * a_h * kLog2e);
+  float slope;
+  const float delta = softplus(raw[0], slope), log_decay = delta * a_h;
+  // with the bits that the product's rounding took (past -200 it may be infinite)
+  const float decay =
+      exp_f32(log_decay, log_decay < -200.f ? 0.f : fmaf(delta, a_h, -log_decay));
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < kSets; ++q) {

@@ -69,7 +69,8 @@ __device__ __forceinline__ float number(const Raw<T, 1> &r) {
 // the sequence's end have inside = false and a step of 0.
 __device__ __forceinline__ void chunk_steps(Steps &o, float raw, bool inside, float a) {
   const uint32_t lane = threadIdx.x & 63u;
-  const float delta = inside ? softplus(raw) : 0.f;
+  float slope;
+  const float step = softplus(raw, slope), delta = inside ? step : 0.f;
   // A decay of 2^-1024 is 0 beside any float32, so no token counts for less:
   // the chunk's sums stay within 2^16, where the pair resolves 2^-31 however
   // far a token has gone, and -infinity stays out.  NaN stays in.  Past the end
@@ -83,7 +84,7 @@ __device__ __forceinline__ void chunk_steps(Steps &o, float raw, bool inside, fl
   }
   const double last = __shfl(sum, 63, 64);
   o.delta[lane] = delta;
-  o.sig[lane] = inside ? sigmoid(raw) : 0.f;
+  o.sig[lane] = inside ? slope : 0.f;
   o.hi[lane] = (float)sum;
   o.lo[lane] = (float)(sum - (double)(float)sum);
   o.e[lane] = exp2_fast((float)sum);

@@ -142,13 +142,40 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // 2^x (v_exp_f32: within an ulp; results below the normal range become 0)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
-// 1 / (1 + exp(-x)): the exponential's infinity gives 0, its zero gives 1
-__device__ __forceinline__ float sigmoid(float x) {
+constexpr float kLn2 = 0.693147180559945309417f, kLn2Low = -1.90465429995776e-9f;
+// exp(x) is 2^p of the float32 product p = x log2(e) times 1 + (x - p ln 2): what
+// the product's rounding took, which would else put |x| 2^-24 into the result.
+// (float32 ln 2 is off by 2^-28 of itself, kLn2Low is the rest.)
+__device__ __forceinline__ float exp_rest(float x, float p) {
+  return fmaf(-p, kLn2Low, fmaf(-p, kLn2, x));
+}
+// exp(x + low), low a few bits below x, to 2^-22 of itself.  Arguments of -200
+// and less give 0, NaN stays; for x up to 88.
+__device__ __forceinline__ float exp_f32(float x, float low = 0.f) {
+  const float t = x < -200.f ? -200.f : x, p = t * kLog2e, y = exp2_fast(p);
+  return fmaf(y, exp_rest(t, p) + low, y);
+}
+// sig = 1 / (1 + exp(-x)), rest = 1 / (1 + exp(x)), each to a few units of its
+// own last place while sig is not 0; below x = -88 both are 0.  The bounds keep
+// an infinity from meeting a 0.
+struct Logistic {
+  float sig, rest;
+};
+__device__ __forceinline__ Logistic logistic(float x) {
+  const float t = __builtin_amdgcn_fmed3f(-x, -200.f, 200.f), p = t * kLog2e;
+  const float e = exp2_fast(p) * (1.f + exp_rest(t, p)), sig = rcp_fast(1.f + e);
+  return Logistic{sig, fminf(e, 3e38f) * sig};
+}
+__device__ __forceinline__ float sigmoid(float x) { return logistic(x).sig; }
+// The same without the remainder, to |x| 2^-23 of itself (2^-16 at most): for
+// results that are rounded to 8 bits next.
+__device__ __forceinline__ float sigmoid_8bit(float x) {
   return rcp_fast(1.f + exp2_fast(-x * kLog2e));
 }
-// log(1 + exp(x)) without overflow; -infinity gives 0
-__device__ __forceinline__ float softplus(float x) {
-  const float e = exp2_fast(-fabsf(x) * kLog2e);
+// log(1 + exp(x)) without overflow, and its derivative; -infinity gives 0, 0
+__device__ __forceinline__ float softplus(float x, float &slope) {
+  const float e = exp_f32(-fabsf(x)), r = rcp_fast(1.f + e);
+  slope = x < 0.f ? e * r : r;
   return fmaxf(x, 0.f) + log1pf(e);
 }
 
