@@ -113,14 +113,21 @@ def _registers(text):
 
 
 def _mfma_states(name):
-    """Wait states from a matrix instruction to a reader of its sums."""
-    return 8 if "16x16x32_bf16" in name else 9 if "16x16x4_f32" in name else 20
+    """Wait states from a matrix instruction to a reader of its sums, as the
+    compiler places them in straight code."""
+    return 8 if "16x16x32_bf16" in name else 10 if "16x16x4_f32" in name else 20
+
+
+def _operands(args):
+    """An instruction's operands; a register range holds no comma."""
+    return [a.strip() for a in args.split(",")]
 
 
 def matrix_hazards(asm):
-    """Vector instructions that read a matrix instruction's sums (or write over
-    them) too few wait states after it, along any path of the control flow
-    graph: [(function, the two instructions, states)]."""
+    """Instructions that read a matrix instruction's sums, or write over them,
+    too few wait states after it, along any path of the control flow graph:
+    [(function, the two instructions, states)].  Another matrix instruction may
+    add to the sums (its last operand) or replace them: the hardware waits."""
     found = []
     for fn in re.split(r"\n(?=_Z\w+:)", asm):
         if "v_mfma" not in fn:
@@ -139,13 +146,14 @@ def matrix_hazards(asm):
             if not name.startswith("v_mfma"):
                 continue
             need = _mfma_states(name)
-            paths = [(n + 1, 0, frozenset(_registers(ops.split(",")[0])))]
+            paths = [(n + 1, 0, frozenset(_registers(_operands(ops)[0])))]
             seen = set()
             while paths:
-                k, states, sums = paths.pop()
-                if k >= len(code) or states >= need or not sums or (k, states) in seen:
+                at = paths.pop()
+                k, states, sums = at
+                if k >= len(code) or states >= need or not sums or at in seen:
                     continue
-                seen.add((k, states))
+                seen.add(at)
                 op, args = code[k]
                 if op == "s_endpgm":
                     continue
@@ -156,21 +164,20 @@ def matrix_hazards(asm):
                 elif op == "s_nop":
                     states += int(args.strip(), 0)
                 elif op.startswith("v_mfma"):
-                    sums = sums - _registers(args.split(",")[0])
-                elif op.startswith(("v_", "ds_", "global_", "scratch_", "flat_", "buffer_")):
-                    stores = re.match(r"(ds_write|(global|scratch|flat|buffer)_(store|atomic))", op)
-                    dst, _, src = args.partition(",")
-                    reads = _registers(args if stores else src)
-                    writes = _registers(dst) if op.startswith("v_") else set()
-                    if sums & (reads | writes):
+                    dst, a, b = _operands(args)[:3]
+                    if sums & (_registers(a) | _registers(b)):
                         found.append((fn.split(":", 1)[0], f"{name} {ops}", f"{op} {args}", states))
                         continue
+                    sums = sums - _registers(dst)
+                elif not op.startswith("s_") and sums & _registers(args):
+                    found.append((fn.split(":", 1)[0], f"{name} {ops}", f"{op} {args}", states))
+                    continue
                 paths.append((k + 1, states + 1, sums))
     return found
 
 
 def check_matrix_waits(asm_dir):
-    """Fails when the gfx950 assembly of this build lets a reader of a matrix
+    """Fails when the gfx950 assembly of this build lets a user of a matrix
     instruction's sums come too early: the compiler's waits are not complete
     where a branch leads straight from the one to the other."""
     found = []
@@ -179,7 +186,7 @@ def check_matrix_waits(asm_dir):
             with open(os.path.join(asm_dir, name)) as f:
                 found += [f"{name}: {h}" for h in matrix_hazards(f.read())]
     if found:
-        raise RuntimeError("readers too close behind matrix instructions:\n" + "\n".join(found[:10]))
+        raise RuntimeError("users of sums too close behind matrix instructions:\n" + "\n".join(found[:10]))
     print("  device assembly: every matrix instruction's sums are waited for", flush=True)
 
 

@@ -58,7 +58,7 @@ template <typename T>
 __device__ __forceinline__ void settle() {
   __builtin_amdgcn_sched_barrier(0);
   if constexpr (sizeof(T) == 4)
-    asm volatile("s_nop 7\n\ts_nop 1" ::: "memory");  // 16x16x4 f32: 9 states
+    asm volatile("s_nop 7\n\ts_nop 1" ::: "memory");  // 16x16x4 f32: 10 states
   else
     asm volatile("s_nop 7" ::: "memory");  // 16x16x32 bf16: 8 states
   __builtin_amdgcn_sched_barrier(0);
