@@ -133,7 +133,8 @@ int nsfps_device_count(void);
  * counterpart in the reference (a CPU library).  Optional: the first call on
  * a device does the same; calling this first keeps that one-time work (tens
  * of milliseconds, most of it the runtime's own start) out of the first
- * call.  NSFPS_EDEVICE when no device is visible. */
+ * call.  NSFPS_EDEVICE when no device is visible.  The sequence operators'
+ * kernels are loaded by nsfps_init_sequence_device. */
 nsfps_status nsfps_init_device(void);
 
 /* Derived fields and Morton LUTs of a range.  luts receives the x, y and z
@@ -288,7 +289,9 @@ nsfps_status nsfps_ball_query_device(const float *d_xyz, uint64_t n, const float
  * side by side.  Work that the kernels need beside their outputs is the
  * caller's: a call with a _workspace_bytes companion needs that many bytes
  * at workspace (aligned to 256), whose contents need not be kept, and which
- * calls that may overlap must not share.  A workspace that is too small, a
+ * calls that may overlap must not share.  The first call of an operator on a
+ * device loads its kernels (about a millisecond); nsfps_init_sequence_device
+ * does that ahead, as is needed before a capture.  A workspace that is too small, a
  * size or stride that does not fit and a null pointer are NSFPS_EINVAL;
  * sizes beyond the limits named below are NSFPS_EUNSUPPORTED.  Nothing is
  * enqueued by a refused call.
@@ -297,6 +300,9 @@ nsfps_status nsfps_ball_query_device(const float *d_xyz, uint64_t n, const float
  * the gradients of parameters are float32 with both.  Results do not depend
  * on the order in which workgroups run: the same call gives the same bits. */
 typedef enum { NSFPS_F32 = 0, NSFPS_BF16 = 1 } nsfps_dtype;
+
+/* Loads the sequence operators' kernels on the current device.  Optional. */
+nsfps_status nsfps_init_sequence_device(void);
 
 /* A tensor of batch x length rows: row t of sequence b starts at
  * p + (b * batch_stride + t * row_stride) elements.  A row's elements are

@@ -295,6 +295,11 @@ class Lib:
                                                      ctypes.c_uint32(int(nsample)), _vp(d_out),
                                                      _vp(stream)))
 
+    def init_sequence_device(self):
+        """nsfps_init_sequence_device: the sequence operators' kernels, loaded
+        ahead of the first call (and of a capture)."""
+        self._check(self.lib.nsfps_init_sequence_device())
+
     # The sequence operators: args (and grads) are the structs above, filled
     # once and reused with other pointers; everything they point to is device
     # memory, and the calls only enqueue on the stream.

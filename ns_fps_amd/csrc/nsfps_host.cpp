@@ -32,7 +32,6 @@
 
 #include "nsfps_internal.h"
 #include "nsfps_launch.h"
-#include "nsfps_sequence.h"
 #include "nsfps_status.h"
 
 namespace nsfps {
@@ -2181,13 +2180,7 @@ nsfps_status nsfps_init_device(void) {
   return guarded([&]() -> nsfps_status {
     std::lock_guard<std::mutex> lk(g_mu);
     Arena *ap = nullptr;
-    const nsfps_status rc = arena_for_device(&ap);
-    if (rc) return rc;
-    HIP_TRY(preload_embed_kernels());
-    HIP_TRY(preload_conv_kernels());
-    HIP_TRY(preload_scan_kernels());
-    HIP_TRY(preload_scan_grad_kernels());
-    return NSFPS_OK;
+    return arena_for_device(&ap);
   });
 }
 

@@ -216,6 +216,17 @@ using namespace nsfps;
 
 extern "C" {
 
+nsfps_status nsfps_init_sequence_device(void) {
+  return guarded([&]() -> nsfps_status {
+    TRY(need_device());
+    HIP_TRY(preload_embed_kernels());
+    HIP_TRY(preload_conv_kernels());
+    HIP_TRY(preload_scan_kernels());
+    HIP_TRY(preload_scan_grad_kernels());
+    return NSFPS_OK;
+  });
+}
+
 nsfps_status nsfps_embed_device(const nsfps_embed_args *args, void *stream) {
   return guarded([&]() -> nsfps_status {
     TRY(check_embed(args, false));
