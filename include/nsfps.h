@@ -359,7 +359,8 @@ nsfps_status nsfps_embed_grad_device(const nsfps_embed_args *args, void *stream)
  * width 2 to 4, weight [channels][width], bias [channels] (or NULL) of type
  * dtype.  d_cache (or NULL) is read where positions are above 0 and receives
  * the last inputs.  batch * length at most 2^31 - 1, channels at most 2^24.
- * x and y must not overlap.
+ * y must not overlap x, nor dx x or dy (a tile of tokens reads those beside
+ * it); where the strides show it, the call is refused.
  *
  * The gradient starts every sequence anew (d_positions, d_slots, d_cache
  * must be NULL; y is not read): dx of type dtype, d_dweight [channels][width]

@@ -4,7 +4,9 @@
 #include "nsfps_sequence.h"
 #include "nsfps_status.h"
 
+#include <algorithm>
 #include <atomic>
+#include <utility>
 
 namespace nsfps {
 namespace {
@@ -61,6 +63,43 @@ nsfps_status check_rows(const nsfps_rows &r, uint64_t batch, uint64_t length, ui
     return fail(NSFPS_EINVAL, "rows of %s overlap: %llu elements, batch stride %llu, row stride %llu",
                 what, (unsigned long long)width, (unsigned long long)r.batch_stride,
                 (unsigned long long)r.row_stride);
+  return NSFPS_OK;
+}
+
+// Whether two tensors of these sizes share an element, as far as their strides
+// tell: the same first element, or the same strides.  `out` keeps its rows apart
+// (check_rows), so the offsets of two rows of it that can meet are the few
+// nearest to the tensors' distance.
+bool rows_meet(const nsfps_rows &out, const nsfps_rows &in, uint64_t batch, uint64_t length,
+               uint64_t width, uint32_t dtype) {
+  if (out.p == in.p) return true;
+  if ((batch > 1 && out.batch_stride != in.batch_stride) ||
+      (length > 1 && out.row_stride != in.row_stride))
+    return false;
+  struct Step {
+    int64_t stride, most;  // elements; how often it may be taken either way
+  } far{(int64_t)out.batch_stride, (int64_t)batch - 1},
+      near{(int64_t)out.row_stride, (int64_t)length - 1};
+  if (near.most && (!far.most || near.stride > far.stride)) std::swap(far, near);
+  const int64_t d = ((intptr_t)in.p - (intptr_t)out.p) / (int64_t)size_of(dtype),
+                span = far.most * far.stride + near.most * near.stride + (int64_t)width;
+  if (d >= span || -d >= span) return false;
+  const auto nearest = [](const Step &s, int64_t at, int64_t k) {  // at, some steps back
+    const int64_t q = s.most ? std::max(-s.most, std::min(s.most, at / s.stride + k)) : 0;
+    return at - q * s.stride;
+  };
+  for (int64_t k = -1; k <= 1; ++k)
+    for (int64_t j = -1; j <= 1; ++j) {
+      const int64_t left = nearest(near, nearest(far, d, k), j);
+      if (left < (int64_t)width && -left < (int64_t)width) return true;
+    }
+  return false;
+}
+
+nsfps_status check_apart(const nsfps_rows &out, const nsfps_rows &in, const nsfps_conv_args &a,
+                         const char *what) {
+  if (rows_meet(out, in, a.batch, a.length, a.channels, a.dtype))
+    return fail(NSFPS_EINVAL, "%s overlap: tokens beside a row are read after it is written", what);
   return NSFPS_OK;
 }
 
@@ -261,6 +300,7 @@ nsfps_status nsfps_conv_device(const nsfps_conv_args *args, void *stream) {
   return guarded([&]() -> nsfps_status {
     TRY(check_conv(args, false));
     if (!args->batch || !args->length) return NSFPS_OK;
+    TRY(check_apart(args->y, args->x, *args, "x and y"));
     TRY(need_device());
     HIP_TRY(launch_conv(*args, (hipStream_t)stream));
     return NSFPS_OK;
@@ -288,6 +328,10 @@ nsfps_status nsfps_conv_grad_device(const nsfps_conv_args *args, const nsfps_con
     TRY(check_pointer(grads->d_dweight, 4, "d_dweight"));
     TRY(check_optional(grads->d_dbias, 4, "d_dbias"));
     TRY(check_workspace(args->workspace, args->workspace_bytes, conv_grad_bytes(*args)));
+    if (args->batch && args->length) {
+      TRY(check_apart(grads->dx, args->x, *args, "x and dx"));
+      TRY(check_apart(grads->dx, grads->dy, *args, "dy and dx"));
+    }
     TRY(need_device());
     HIP_TRY(launch_conv_grad(*args, *grads, (hipStream_t)stream));
     return NSFPS_OK;
