@@ -341,12 +341,13 @@ __global__ __launch_bounds__(512) void k_token_place(const int32_t *__restrict__
   }
 }
 
-// At most 1,024 tokens: a token's place is the number of tokens before it,
-// those of a smaller key and those of its own that come first.  (A table too
-// large for one pass costs six launches else; us a gradient with them and with this one: 3
-// tokens of 39,481 rows of 58 bf16 33, 15; 395 of 59,072 rows of 57 62, 57.)
-constexpr uint32_t kRankTokens = 1024;
-__global__ __launch_bounds__(1024) void k_token_rank(const int32_t *__restrict__ tokens,
+// At most 512 tokens: a token's place is the number of tokens before it, those
+// of a smaller key and those of its own that come first.  A table too large for
+// one pass costs six launches else (us a gradient with them and with this one,
+// bf16: 3 tokens of 39,481 rows of 58 32, 14; 395 56, 51; 512 55, 54; 576 55.5,
+// 56; 1,024 52, 70; 512 tokens of 262,144 rows of 256 93, 89; 640 90, 90).
+constexpr uint32_t kRankTokens = 512;
+__global__ __launch_bounds__(kRankTokens) void k_token_rank(const int32_t *__restrict__ tokens,
                                                      uint32_t *__restrict__ kout,
                                                      uint32_t *__restrict__ vout, uint32_t count,
                                                      uint32_t rows,

@@ -191,10 +191,11 @@ def lookup_gradient(lib, table_rows, tokens, width):  # noqa: F811
 @pytest.mark.gpu
 @pytest.mark.parametrize("table_rows,tokens", [
     (1, 262144), (3, 262144), (1, 262145), (3, 262145), (1023, 300000), (1 << 20, 3000),
-    ((1 << 20) + 5, 70000), ((1 << 24) + 3, 1025)])
+    ((1 << 20) + 5, 70000), ((1 << 24) + 3, 1025),
+    (40000, 511), (40000, 512), (40000, 513), ((1 << 20) + 5, 512), ((1 << 20) + 5, 513)])
 def test_lookup_gradient_sorts(lib, table_rows, tokens):  # noqa: F811
-    """One pass over whole keys, one, two and three passes over digits; rows
-    of 10^5 terms (added in float64, so the tolerance stays)."""
+    """One pass over whole keys, one, two and three passes over digits, one
+    launch for few tokens, up to its last and beyond; rows of 10^5 terms (added in float64, so the tolerance stays)."""
     outs, td, dd = lookup_gradient(lib, table_rows, tokens, 3)
     hit = (td >= 0) & (td < table_rows)
     want = torch.zeros(table_rows + 1, 3, dtype=F64)
