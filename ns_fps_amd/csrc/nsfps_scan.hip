@@ -394,9 +394,12 @@ hipError_t run_sweep(const ScanDev &s, SweepDev d, char *ws, hipStream_t st) {
 // request of 8 heads: 5 us, one chain of loads.
 //
 // kV: 4 state values a load where state_dim and the cache allow it, kCols of
-// those a thread.  kSets: 4 (a head of 64 rows) where that still gives 1,024
-// workgroups, else 1: few requests need the width of the chip more than they
-// need the convolution done once.
+// those a thread.  kSets: 4 (a head of 64 rows) where that still gives every CU
+// a workgroup, else 1: few requests need the width of the chip more than they
+// need the convolution done once.  us with 1 and with 4, 64 x 128 states,
+// bfloat16: 128 heads of all requests 5.0, 6.2; 256 6.7, 6.8; 512 9.8, 8.3;
+// 1,024 17.7, 13.1; 64 x 64 states: 128 4.1, 4.5; 256 5.3, 4.8; 512 7.7, 5.6;
+// 1,024 12.1, 7.6.
 template <typename T, int W, int kV, int kCols, int kSets>
 __global__ __launch_bounds__(256) void k_scan_step(nsfps_step_args a, uint32_t ptiles) {
   constexpr uint32_t kRows = 16 * kSets;
@@ -534,7 +537,7 @@ hipError_t launch_states(const nsfps_scan_args &a, const ScanDev &s, const nsfps
 }
 
 hipError_t launch_scan_step(const nsfps_step_args &a, hipStream_t st) {
-  const bool many = a.batch * a.heads * host_ceil_div(a.head_dim, 64) >= 1024;
+  const bool many = a.batch * a.heads * host_ceil_div(a.head_dim, 64) >= 256;
   const uint32_t rows = many ? 64 : 16, ptiles = (a.head_dim + rows - 1) / rows;
   const uint32_t grid = (uint32_t)(a.batch * a.heads * ptiles);
   const bool wide = a.state_dim % 4 == 0 && (uintptr_t)a.d_state % 16 == 0;
