@@ -45,9 +45,6 @@ struct alignas(16) Steps {  // read four at a time
   float total;         // log2 of the whole chunk's decay
 };
 
-__device__ __forceinline__ float decay_between(const Steps &s, int i, int j) {  // j <= i
-  return exp2_fast((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]));
-}
 __device__ __forceinline__ f32x4 quad_of(const float (&v)[kChunk], int at) {
   return *(const f32x4 *)(v + at);
 }
@@ -103,8 +100,8 @@ inline uint64_t round256(uint64_t n) { return (n + 255) & ~255ull; }
 // 512 and 1,024 workgroups: 65,536 tokens of 8 heads 223, 159, 173; 64 x 4,096
 // tokens of 8 heads with gradient 1,615, 1,615, 1,919.  Segments of at least
 // 4, 2 and 1 chunks: 1,000 tokens of 8 heads 28.2, 21.1, 18.7; 3 x 1,001 tokens
-// of 6 heads in float32 with gradient 180, 134, 131.  (The gradient of
-// the second case takes 1,444 in all now, by later steps.)
+// of 6 heads in float32 with gradient 180, 134, 131.  (The second case takes
+// 1,450 in all now, by later steps.)
 inline uint32_t segment_chunks(uint64_t sequences, uint64_t chunks) {
   constexpr uint64_t kFill = 512;
   const uint64_t segs = std::max<uint64_t>(1, kFill / std::max<uint64_t>(1, sequences));

@@ -23,7 +23,6 @@ namespace seq {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -50,12 +49,8 @@ __device__ __forceinline__ bf16 from_f32<bf16>(float v) {
   return bf16{bf16_bits(v)};
 }
 
-// V elements at p, p aligned to V elements.
-template <typename T, int V>
-struct Vec {
-  T v[V];
-};
-// As loaded (a load whose values are converted where it stands is waited for there) ...
+// V elements at p, p aligned to V elements, as loaded (a load whose values are
+// converted where it stands is waited for there) ...
 template <typename T, int V>
 struct Raw {
   static constexpr int kBytes = V * (int)sizeof(T), kWords = (kBytes + 3) / 4;
