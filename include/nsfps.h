@@ -290,15 +290,19 @@ nsfps_status nsfps_ball_query_device(const float *d_xyz, uint64_t n, const float
  * caller's: a call with a _workspace_bytes companion needs that many bytes
  * at workspace (aligned to 256), whose contents need not be kept, and which
  * calls that may overlap must not share.  The first call of an operator on a
- * device loads its kernels (about a millisecond); nsfps_init_sequence_device
- * does that ahead, as is needed before a capture.  A workspace that is too small, a
- * size or stride that does not fit and a null pointer are NSFPS_EINVAL;
- * sizes beyond the limits named below are NSFPS_EUNSUPPORTED.  Nothing is
- * enqueued by a refused call.
+ * device loads its kernels (six milliseconds for all of them);
+ * nsfps_init_sequence_device does that ahead, before a capture for instance.
+ * No output may overlap an input or another output.  A workspace that is too
+ * small, a size or stride that does not fit and a null pointer are
+ * NSFPS_EINVAL; sizes beyond the limits named below are NSFPS_EUNSUPPORTED.
+ * Nothing is enqueued by a refused call.
  *
  * Types: NSFPS_F32 and NSFPS_BF16 for inputs and outputs; sums, states and
- * the gradients of parameters are float32 with both.  Results do not depend
- * on the order in which workgroups run: the same call gives the same bits. */
+ * the gradients of parameters are float32 with both.  In bfloat16 calls of the
+ * scan and its gradient, computed factors of a product whose sum becomes a
+ * bfloat16 output (scores, states in y, state gradients in db) hold 16 bits
+ * there, those of other sums 24.  Results do not depend on the order in which
+ * workgroups run: the same call gives the same bits. */
 typedef enum { NSFPS_F32 = 0, NSFPS_BF16 = 1 } nsfps_dtype;
 
 /* Loads the sequence operators' kernels on the current device.  Optional. */
@@ -320,7 +324,8 @@ typedef struct {
  * Its gradient (d_out is then the input and d_table the output): every row v
  * of d_table is written, scale times the sum of the rows of d_out whose
  * token is v, zeros where no token is.  The tokens are sorted, and each
- * row's terms are added in float32 in an order that the tokens alone decide.
+ * row's terms are added in float32 (in float64 where a row has more than 16) in
+ * an order that the tokens alone decide.
  * d_out has type dtype, d_table grad_dtype.  At most 2^31 - 1 tokens and
  * rows (both calls), width at most 65,536. */
 typedef struct {

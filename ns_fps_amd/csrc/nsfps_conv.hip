@@ -14,9 +14,9 @@
 // adds the workgroups' sums in order.
 //
 // Measured, of 4.8 TB/s that a large copy reaches: 16,384 tokens of 323 float32
-// channels 10.6 us (4.0 TB/s); 64 ragged sequences of up to 4,096 tokens, 640
-// bfloat16 channels, 144 us (4.1 TB/s), their gradient 272 us (3.1 TB/s) and
-// the join of its sums 19 us.
+// channels 10.8 us (3.9 TB/s); 64 ragged sequences of up to 4,096 tokens, 640
+// bfloat16 channels, 141 us (4.1 TB/s), their gradient 276 us (3.1 TB/s) and
+// the join of its sums 20 us.
 #include "nsfps_launch.h"
 #include "nsfps_seq_device.h"
 

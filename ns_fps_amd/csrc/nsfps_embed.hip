@@ -8,13 +8,12 @@
 // Gradient: dtable[v] = scale * sum of dout[i] over tok[i] = v.  The tokens
 // are sorted with their positions (stable, so a row's positions are in
 // order), start[v] is found at the sorted tokens' boundaries, and each table
-// row's terms are added in float32, in that order, by the lanes that hold its
-// columns, and the row is written once: no atomics on values, the same bits
-// every time, and rows without a token cost their zeros.  A crowded row (more
-// than kLong terms: grid cells near an object) is cut into pieces of kPiece
-// terms, a wave each,
-// whose sums (in float64: the terms may be many) are added in order by a last
-// pass.  Where pieces lie in the workspace is decided by an atomic counter; no
+// row's terms (at most kLong) are added in float32, in that order, by the lanes
+// that hold its columns, and the row is written once: no atomics on values, the
+// same bits every time, and rows without a token cost their zeros.  A crowded
+// row (more terms: grid cells near an object) is cut into pieces of kPiece
+// terms, a wave each, whose sums (in float64: the terms may be many) are added
+// in order by a last pass.  Where pieces lie in the workspace is decided by an atomic counter; no
 // sum depends on it.  524,288 tokens, 262,144 rows of 512 bytes: the sort 53 us,
 // the starts 5, the rows 142 (2.8 TB/s: scattered rows behind two dependent
 // loads), the crowded rows 23.  16,384 tokens, 8,192 rows of 383 float32: the

@@ -102,7 +102,7 @@ __device__ __forceinline__ void state_io(float *state, f32x4 (&v)[kNt], uint32_t
 // one chunk follow each other, and two workgroups a CU are all that hides them.
 // 65,536 tokens, 8 heads, 64 x 128 states, bfloat16: 49 us for the segments'
 // states and 115 with outputs (1.0 TB/s over both); 64 sequences of up to 4,096 tokens
-// of 8 heads, 64 x 64: 259 us with outputs, 186 without.
+// of 8 heads, 64 x 64: 268 us with outputs, 187 without.
 // Two workgroups a CU where their LDS allows it (160 KB): the compiler may then
 // use 256 registers.
 template <typename T, int NT, bool kOut>
@@ -390,8 +390,8 @@ hipError_t run_sweep(const ScanDev &s, SweepDev d, char *ws, hipStream_t st) {
 // holds `width` entries, of which the convolution reads the last width - 1 and
 // this token's replaces the oldest, so a workgroup that writes its entry
 // disturbs no other that still reads.  512 requests of 16 heads of 64 x 128
-// states: 105 us, 5.2 TB/s of the 546 MB (a large copy reaches 4.8); one
-// request of 8 heads: 5 us, one chain of loads.
+// states: 105 us, 5.2 TB/s of the 546 MB (an update of 4 GiB in place reaches
+// 5.9); one request of 8 heads: 5 us, one chain of loads.
 //
 // kV: 4 state values a load where state_dim and the cache allow it, kCols of
 // those a thread.  kSets: 4 (a head of 64 rows) where that still gives every CU

@@ -13,6 +13,11 @@
 // all terms from inside the chunk, so nothing cancels over the sequence.  Then
 // ddelta_t = a da_t + (what came through delta_t itself), ddt = ddelta sigmoid(raw).
 //
+// In bfloat16 calls, what ends in a bfloat16 output alone (M, G, and dH in db)
+// enters its product as two bfloat16 terms: 2^-17 of a term beside the output's
+// own 2^-9.  H in dc and dH in dx, which da takes along, enter as three (24
+// bits), and every sum is in float32 or more.
+//
 // H and dH come from the forward's sweep over the chunks, and from the same
 // kernel run over dy and c from the sequence's end (nothing is kept from the
 // forward call); then every chunk is done by itself, one workgroup per chunk
@@ -204,7 +209,7 @@ constexpr int kGradGroups = sizeof(GradLds<T, NT>) <= 80 * 1024 ? 2 : 1;  // wor
 // Bound by what surrounds its products: operands are read from LDS for every
 // 16 x 16 tile, states are split into three terms, and the four waves meet at
 // barriers for each head.  64 sequences of up to 4,096 tokens, 8 heads of 64 x
-// 64 in one group, bfloat16: 823 us; 3 of 1,001 tokens, 6 heads of 48 x 33,
+// 64 in one group, bfloat16: 841 us; 3 of 1,001 tokens, 6 heads of 48 x 33,
 // float32: 47 us.
 // Work item w: chunk bc = w / groups of all sequences' and group w % groups.
 // kOne: head_dim is at most 64, so a head is one tile and its loads run ahead.
