@@ -447,6 +447,113 @@ typedef struct {
 } nsfps_step_args;
 nsfps_status nsfps_scan_step_device(const nsfps_step_args *args, void *stream);
 
+/* Norms of queries and keys, head by head, and the rotation by their position,
+ * in one pass; of the scan's c and b say, between convolution and scan.  Per
+ * head, with x its head_dim values:
+ *   n = weight * x / sqrt(mean(x^2) + eps)
+ * and of n's first rotary_dim values the pair (u, v) number i becomes
+ *   u cos(w) - v sin(w), u sin(w) + v cos(w),  w = position * freq[i];
+ * the values behind them stay.  Pairs are (i, i + rotary_dim / 2), with
+ * neighbours != 0 (2i, 2i + 1).  A token's position is the one of its sequence
+ * (d_positions, below 0 as 0; NULL: 0) plus its row's number; angles are exact
+ * to 2^-22 at any position.  Rows past a sequence's length are zeros.
+ *
+ * q and q_out: rows of q_heads * head_dim; k and k_out: rows of k_heads *
+ * head_dim, all of type dtype (one of the two may have no heads).  Weights
+ * [head_dim] of type dtype, or NULL (ones); freq [rotary_dim / 2] float32.
+ * head_dim at most 256, rotary_dim even and at most head_dim (0: no
+ * rotation), eps above 0; (q_heads + k_heads) * head_dim at most 2^24; batch *
+ * length at most 2^31 - 1.  A head whose sum of squares passes float32 (values
+ * near 10^19) becomes zeros.
+ *
+ * The gradient takes those of q_out and k_out and writes all of dq and dk
+ * (type dtype), and d_dq_weight and d_dk_weight ([head_dim] float32, or NULL);
+ * q_out and k_out are not read. */
+typedef struct {
+  uint64_t batch, length;
+  uint32_t q_heads, k_heads, head_dim, rotary_dim, neighbours, dtype;
+  float eps;
+  nsfps_rows q, k, q_out, k_out;
+  const void *d_q_weight, *d_k_weight;
+  const float *d_freq;
+  const int32_t *d_lengths, *d_positions;
+  void *workspace; /* gradient only */
+  uint64_t workspace_bytes;
+} nsfps_norm_args;
+typedef struct {
+  nsfps_rows dq_out, dk_out, dq, dk;
+  float *d_dq_weight, *d_dk_weight;
+} nsfps_norm_grads;
+nsfps_status nsfps_norm_device(const nsfps_norm_args *args, void *stream);
+nsfps_status nsfps_norm_grad_workspace_bytes(const nsfps_norm_args *args, uint64_t *bytes);
+nsfps_status nsfps_norm_grad_device(const nsfps_norm_args *args, const nsfps_norm_grads *grads,
+                                    void *stream);
+
+/* Dropout onto a residual, the mask made where it is used and never stored:
+ *   y = residual + (kept ? x / (1 - p) : 0)
+ * (residual.p NULL: no residual).  Its gradient by x is the same call on dy
+ * without residual, that by residual is dy.  Of a row's channels the eight from
+ * 8 k on take 16 bits each, low half first, of the four words of Philox 4x32-10
+ * (Salmon, Moraes, Dror, Shaw, 2011) at counter (k, row's number b * length +
+ * t, d_seed[1] low, high) and key (d_seed[0] low, high); a value is dropped
+ * where they are below p * 65536, rounded, and the factor is that of the
+ * rounded p.  So the mask hangs on sizes and seed alone, not on types, strides
+ * or lengths.  d_seed: two words in device memory, a key and the number of the
+ * call (a captured graph's caller changes it between replays).  0 <= p <= 1 (1:
+ * all is dropped); channels at most 2^24, batch * length at most 2^31 - 1.  Rows
+ * past a sequence's length are zeros, their inputs are not read. */
+typedef struct {
+  uint64_t batch, length;
+  uint32_t channels, dtype;
+  float p;
+  nsfps_rows x, residual, y;
+  const uint64_t *d_seed;
+  const int32_t *d_lengths;
+} nsfps_dropout_args;
+nsfps_status nsfps_dropout_device(const nsfps_dropout_args *args, void *stream);
+
+/* Softmax cross entropy of tokens over a vocabulary of table rows, the logits
+ * of which are never held at once:
+ *   z[i][v] = scale * x[i] . table[v]   (x: tokens x width, table: rows x width)
+ *   lse[i] = log(sum over v of exp(z[i][v])),  loss[i] = lse[i] - z[i][targets[i]]
+ * A token whose target is outside [0, rows) has a loss of 0 and no gradient,
+ * whatever its row of x holds (its lse is that row's).  d_loss and d_lse: [tokens]
+ * float32, all written.
+ *
+ * The gradient needs d_lse as the call left it (d_loss is not read) and
+ * d_dloss, the gradient of each token's loss: d_dx (type dtype, rows dx_stride
+ * apart) and d_dtable (type grad_dtype, rows dtable_stride apart) are all
+ * written.  exp(z - lse) - (v is the target), times dloss and scale, enters the
+ * products in bfloat16 where the result is bfloat16, with 16 bits for a float32
+ * table gradient of bfloat16 inputs, with 24 in float32 calls.
+ *
+ * At most 2^31 - 1 tokens and rows, width at most 65,536.  The vocabulary is
+ * taken in pieces, whose products live in the workspace; its size goes by
+ * sizes and types alone. */
+typedef struct {
+  uint64_t tokens, rows;
+  uint32_t width, dtype;
+  float scale;
+  uint64_t x_stride, table_stride; /* elements from row to row, >= width */
+  const void *d_x, *d_table;
+  const int32_t *d_targets;
+  float *d_loss, *d_lse;
+  void *workspace;
+  uint64_t workspace_bytes;
+} nsfps_loss_args;
+typedef struct {
+  const float *d_dloss;
+  uint64_t dx_stride, dtable_stride;
+  uint32_t grad_dtype;
+  void *d_dx, *d_dtable;
+} nsfps_loss_grads;
+nsfps_status nsfps_loss_workspace_bytes(const nsfps_loss_args *args, uint64_t *bytes);
+nsfps_status nsfps_loss_device(const nsfps_loss_args *args, void *stream);
+nsfps_status nsfps_loss_grad_workspace_bytes(const nsfps_loss_args *args,
+                                             const nsfps_loss_grads *grads, uint64_t *bytes);
+nsfps_status nsfps_loss_grad_device(const nsfps_loss_args *args, const nsfps_loss_grads *grads,
+                                    void *stream);
+
 /* Measurements of the last compute call made on this thread. */
 nsfps_status nsfps_get_stats(nsfps_stats *stats);
 

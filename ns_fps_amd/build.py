@@ -34,7 +34,8 @@ ARCH = os.environ.get("NSFPS_OFFLOAD_ARCH", "gfx950")
 LIB = os.path.join(HERE, "libnsfps.so")
 SOURCES = ("nsfps_build.hip", "nsfps_sample.hip", "nsfps_runs.hip", "nsfps_small.hip",
            "nsfps_group.hip", "nsfps_embed.hip", "nsfps_conv.hip", "nsfps_scan.hip",
-           "nsfps_scan_grad.hip", "nsfps_host.cpp", "nsfps_sequence.cpp")
+           "nsfps_scan_grad.hip", "nsfps_norm.hip", "nsfps_dropout.hip", "nsfps_loss.hip",
+           "nsfps_host.cpp", "nsfps_sequence.cpp")
 
 # Exact fp32: no contraction, IEEE division/sqrt, denormals kept.
 # "-packed-fp32-ops" turns off the gfx950 packed fp32 instructions

@@ -116,6 +116,46 @@ class StepArgs(ctypes.Structure):
                 ("d_y", ctypes.c_void_p)]
 
 
+class NormArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("length", ctypes.c_uint64),
+                ("q_heads", ctypes.c_uint32), ("k_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("rotary_dim", ctypes.c_uint32),
+                ("neighbours", ctypes.c_uint32), ("dtype", ctypes.c_uint32),
+                ("eps", ctypes.c_float), ("q", Rows), ("k", Rows), ("q_out", Rows),
+                ("k_out", Rows), ("d_q_weight", ctypes.c_void_p), ("d_k_weight", ctypes.c_void_p),
+                ("d_freq", ctypes.c_void_p), ("d_lengths", ctypes.c_void_p),
+                ("d_positions", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class NormGrads(ctypes.Structure):
+    _fields_ = [("dq_out", Rows), ("dk_out", Rows), ("dq", Rows), ("dk", Rows),
+                ("d_dq_weight", ctypes.c_void_p), ("d_dk_weight", ctypes.c_void_p)]
+
+
+class DropoutArgs(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_uint64), ("length", ctypes.c_uint64),
+                ("channels", ctypes.c_uint32), ("dtype", ctypes.c_uint32), ("p", ctypes.c_float),
+                ("x", Rows), ("residual", Rows), ("y", Rows), ("d_seed", ctypes.c_void_p),
+                ("d_lengths", ctypes.c_void_p)]
+
+
+class LossArgs(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_uint64), ("rows", ctypes.c_uint64),
+                ("width", ctypes.c_uint32), ("dtype", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("x_stride", ctypes.c_uint64), ("table_stride", ctypes.c_uint64),
+                ("d_x", ctypes.c_void_p), ("d_table", ctypes.c_void_p),
+                ("d_targets", ctypes.c_void_p), ("d_loss", ctypes.c_void_p),
+                ("d_lse", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_uint64)]
+
+
+class LossGrads(ctypes.Structure):
+    _fields_ = [("d_dloss", ctypes.c_void_p), ("dx_stride", ctypes.c_uint64),
+                ("dtable_stride", ctypes.c_uint64), ("grad_dtype", ctypes.c_uint32),
+                ("d_dx", ctypes.c_void_p), ("d_dtable", ctypes.c_void_p)]
+
+
 class NsfpsError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"nsfps status {status}: {msg}")
@@ -138,12 +178,15 @@ class Lib:
         for name, structs in (("embed", [EmbedArgs]), ("embed_grad", [EmbedArgs]),
                               ("conv", [ConvArgs]), ("conv_grad", [ConvArgs, ConvGrads]),
                               ("scan", [ScanArgs]), ("scan_grad", [ScanArgs, ScanGrads]),
-                              ("scan_step", [StepArgs])):
+                              ("scan_step", [StepArgs]), ("norm", [NormArgs]),
+                              ("norm_grad", [NormArgs, NormGrads]), ("dropout", [DropoutArgs]),
+                              ("loss", [LossArgs]), ("loss_grad", [LossArgs, LossGrads])):
             pointers = [ctypes.POINTER(t) for t in structs]
             getattr(self.lib, f"nsfps_{name}_device").argtypes = pointers + [_vp]
-            if name in ("embed_grad", "conv_grad", "scan", "scan_grad"):
+            if name in ("embed_grad", "conv_grad", "scan", "scan_grad", "norm_grad", "loss",
+                        "loss_grad"):
                 getattr(self.lib, f"nsfps_{name}_workspace_bytes").argtypes = \
-                    pointers[:1] + [ctypes.POINTER(_u64)]
+                    pointers[:2 if name == "loss_grad" else 1] + [ctypes.POINTER(_u64)]
 
     def _check(self, rc):
         if rc != NSFPS_OK:
@@ -304,9 +347,9 @@ class Lib:
     # once and reused with other pointers; everything they point to is device
     # memory, and the calls only enqueue on the stream.
 
-    def _workspace_bytes(self, call, args):
+    def _workspace_bytes(self, call, *args):
         n = _u64()
-        self._check(call(args, n))
+        self._check(call(*args, n))
         return n.value
 
     def embed_device(self, args, stream=None):
@@ -346,6 +389,34 @@ class Lib:
     def scan_step_device(self, args, stream=None):
         """nsfps_scan_step_device: convolution and scan of one token a request."""
         self._check(self.lib.nsfps_scan_step_device(args, stream))
+
+    def norm_device(self, args, stream=None):
+        """nsfps_norm_device: norms of queries and keys by head, and their rotation."""
+        self._check(self.lib.nsfps_norm_device(args, stream))
+
+    def norm_grad_workspace_bytes(self, args):
+        return self._workspace_bytes(self.lib.nsfps_norm_grad_workspace_bytes, args)
+
+    def norm_grad_device(self, args, grads, stream=None):
+        self._check(self.lib.nsfps_norm_grad_device(args, grads, stream))
+
+    def dropout_device(self, args, stream=None):
+        """nsfps_dropout_device: dropout onto a residual (and its gradient by x)."""
+        self._check(self.lib.nsfps_dropout_device(args, stream))
+
+    def loss_workspace_bytes(self, args):
+        return self._workspace_bytes(self.lib.nsfps_loss_workspace_bytes, args)
+
+    def loss_device(self, args, stream=None):
+        """nsfps_loss_device: softmax cross entropy over a table's rows."""
+        self._check(self.lib.nsfps_loss_device(args, stream))
+
+    def loss_grad_workspace_bytes(self, args, grads):
+        return self._workspace_bytes(self.lib.nsfps_loss_grad_workspace_bytes, args, grads)
+
+    def loss_grad_device(self, args, grads, stream=None):
+        """nsfps_loss_grad_device: the loss's gradient by x and by the table."""
+        self._check(self.lib.nsfps_loss_grad_device(args, grads, stream))
 
     def stats(self):
         return self.stats_raw().as_dict()

@@ -1,0 +1,524 @@
+// Norms of queries and keys by head with the rotation by their position, and
+// their gradient.
+//
+//   r = 1 / sqrt(mean(x^2) + eps),  n = r x,  y = R (w n)
+// R turns the pair number i by position * freq[i].  With g = R^T dy:
+//   dw = sum over tokens and heads of g n,  dx = r (g w - n mean(g w n)).
+//
+// A group of lanes holds a head's values as slots of two: a rotated pair, or
+// two values behind the rotation (whose angle is 0), a vector of V slots a
+// lane.  A group takes a token's heads one after another, q's and k's, so the
+// token's cosines and sines are found once; sums over a head go across the
+// group's lanes.  Memory is the bound.
+#include "nsfps_launch.h"
+#include "nsfps_seq_device.h"
+
+#include <algorithm>
+#include <type_traits>
+
+#pragma clang fp contract(fast)
+
+namespace nsfps {
+
+using namespace seq;
+
+namespace {
+
+struct NormDev {
+  uint32_t length, q_heads, k_heads, head_dim, rotary_dim;
+  uint32_t half;             // slots of rotated pairs, then of pairs behind them
+  uint32_t rest;
+  uint32_t lanes;            // of a group
+  uint32_t per, chunks;      // heads of an item, items of a token
+  uint32_t neighbours;
+  float eps;
+  uint64_t items;            // tokens * chunks
+  nsfps_rows q, k, q_out, k_out;  // gradient: x and dx (q_out: dq)
+  nsfps_rows dq_out, dk_out;      // gradient only
+  const void *q_weight, *k_weight;
+  const float *freq;
+  const int32_t *lengths, *positions;
+};
+
+// The place of this lane's slots in a head, and which of them exist.
+template <int V>
+struct Slots {
+  uint32_t first, second;  // elements of the first slot's two values
+  uint32_t step;           // elements from slot to slot (2 where pairs are neighbours)
+  bool one, two;           // whether the slots have a first and a second value
+};
+template <int V>
+__device__ __forceinline__ Slots<V> slots_at(const NormDev &a, uint32_t s) {
+  Slots<V> o;
+  const bool turned = s < a.half;
+  o.one = s < a.half + a.rest;
+  o.step = 1;
+  if (turned && a.neighbours) {
+    o.first = 2 * s;
+    o.second = V == 1 ? 2 * s + 1 : 2 * s + V;  // V slots are 2 V values in a row
+  } else if (turned) {
+    o.first = s;
+    o.second = s + a.half;
+  } else {
+    o.first = a.rotary_dim + (s - a.half);
+    o.second = o.first + a.rest;
+  }
+  o.two = o.one && o.second < a.head_dim;
+  return o;
+}
+
+// Values of the slots: a (first of each pair) and b.
+template <typename T, int V>
+struct RawPair {
+  Raw<T, V> a, b;
+};
+template <typename T, int V>
+__device__ __forceinline__ RawPair<T, V> load_pair(const T *head, const Slots<V> &s) {
+  RawPair<T, V> o{zero_raw<T, V>(), zero_raw<T, V>()};
+  if (s.one) o.a = load_raw<T, V>(head + s.first);
+  if (s.two) o.b = load_raw<T, V>(head + s.second);
+  return o;
+}
+// neighbours: 2 V values in a row are V pairs
+template <int V>
+__device__ __forceinline__ void part(bool neighbours, float (&a)[V], float (&b)[V]) {
+  if constexpr (V > 1) {
+    if (!neighbours) return;
+    float e[2 * V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = a[i], e[V + i] = b[i];
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = e[2 * i], b[i] = e[2 * i + 1];
+  }
+}
+template <int V>
+__device__ __forceinline__ void unpart(bool neighbours, float (&a)[V], float (&b)[V]) {
+  if constexpr (V > 1) {
+    if (!neighbours) return;
+    float e[2 * V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[2 * i] = a[i], e[2 * i + 1] = b[i];
+#pragma unroll
+    for (int i = 0; i < V; ++i) a[i] = e[i], b[i] = e[V + i];
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pair(T *head, const Slots<V> &s, const float (&a)[V],
+                                           const float (&b)[V]) {
+  if (s.one) store_f32<T, V>(head + s.first, a);
+  if (s.two) store_f32<T, V>(head + s.second, b);
+}
+
+// Cosine and sine of position * freq.  The turns are found in float64: 31 bits
+// of a position and 24 of a frequency leave an angle's error at 2^-22 for the
+// farthest position, where float32 would have lost the angle whole.
+__device__ __forceinline__ void turn(double position, float freq, float &c, float &s) {
+  const double t = position * (double)freq * 0.15915494309189533577;  // 1 / (2 pi)
+  sincospif(2.f * (float)(t - rint(t)), &s, &c);
+}
+
+__device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
+  for (uint32_t off = lanes / 2; off; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// A token's place, and its angles for this lane's slots.
+template <int V, int S>
+struct Token {
+  uint32_t b, t;
+  bool inside;
+  float c[S][V], s[S][V];
+};
+template <int V, int S>
+__device__ __forceinline__ void token_at(const NormDev &a, uint32_t token, uint32_t lane,
+                                         Token<V, S> &o) {
+  o.b = token / a.length;
+  o.t = token % a.length;
+  o.inside = true;
+  if (a.lengths) {
+    const int32_t n = a.lengths[o.b];
+    o.inside = n > 0 && o.t < (uint32_t)n;
+  }
+  const int32_t from = a.positions ? max(a.positions[o.b], 0) : 0;
+  const double position = (double)((int64_t)from + o.t);
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    const uint32_t s0 = V * (lane + q * a.lanes);
+    const bool turned = s0 < a.half;  // V slots are all turned or none
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = 0.f;
+    if (turned) load_f32<float, 1>(a.freq + s0, *(float(*)[1])&f[0]);
+#pragma unroll
+    for (int i = 1; i < V; ++i)
+      if (turned) load_f32<float, 1>(a.freq + s0 + i, *(float(*)[1])&f[i]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      o.c[q][i] = 1.f, o.s[q][i] = 0.f;
+      if (turned) turn(position, f[i], o.c[q][i], o.s[q][i]);
+    }
+  }
+}
+
+template <typename T, int V, int S>
+__device__ __forceinline__ void load_head_weights(const NormDev &a, const void *weight,
+                                                  uint32_t lane, float (&wa)[S][V],
+                                                  float (&wb)[S][V]) {
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    const Slots<V> s = slots_at<V>(a, V * (lane + q * a.lanes));
+#pragma unroll
+    for (int i = 0; i < V; ++i) wa[q][i] = wb[q][i] = 1.f;
+    if (weight) {
+      const RawPair<T, V> w = load_pair<T, V>((const T *)weight, s);
+      numbers<T, V>(w.a, wa[q]);
+      numbers<T, V>(w.b, wb[q]);
+    }
+    part<V>(a.neighbours && V * (lane + q * a.lanes) < a.half, wa[q], wb[q]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T *head_at(const NormDev &a, const nsfps_rows &q, const nsfps_rows &k,
+                                      uint32_t b, uint32_t t, uint32_t h) {
+  const bool is_k = h >= a.q_heads;
+  const nsfps_rows &r = is_k ? k : q;
+  return (T *)r.p + (uint64_t)b * r.batch_stride + (uint64_t)t * r.row_stride +
+         (uint64_t)(is_k ? h - a.q_heads : h) * a.head_dim;
+}
+
+template <typename T, int V, int S>
+__global__ __launch_bounds__(256) void k_norm(NormDev a) {
+  const uint32_t lane = threadIdx.x % a.lanes, groups = 256 / a.lanes;
+  Slots<V> at[S];
+  bool mixed[S];  // slots that are pairs of neighbours
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    const uint32_t s0 = V * (lane + q * a.lanes);
+    at[q] = slots_at<V>(a, s0);
+    mixed[q] = a.neighbours && s0 < a.half;
+  }
+  float wqa[S][V], wqb[S][V], wka[S][V], wkb[S][V];
+  load_head_weights<T, V, S>(a, a.q_weight, lane, wqa, wqb);
+  load_head_weights<T, V, S>(a, a.k_weight, lane, wka, wkb);
+  const uint32_t heads = a.q_heads + a.k_heads;
+  const float inv = 1.f / (float)a.head_dim;
+  for (uint64_t item = (uint64_t)blockIdx.x * groups + threadIdx.x / a.lanes; item < a.items;
+       item += (uint64_t)gridDim.x * groups) {
+    const uint32_t h0 = (uint32_t)(item % a.chunks) * a.per, h1 = min(h0 + a.per, heads);
+    Token<V, S> tok;
+    token_at<V, S>(a, (uint32_t)(item / a.chunks), lane, tok);
+    RawPair<T, V> next[S];
+    const auto fetch = [&](uint32_t h) {
+      const T *x = head_at<const T>(a, a.q, a.k, tok.b, tok.t, h);
+#pragma unroll
+      for (int q = 0; q < S; ++q) next[q] = load_pair<T, V>(x, at[q]);
+    };
+    if (tok.inside) fetch(h0);
+    for (uint32_t h = h0; h < h1; ++h) {
+      T *const y = head_at<T>(a, a.q_out, a.k_out, tok.b, tok.t, h);
+      float xa[S][V], xb[S][V];
+      if (!tok.inside) {
+#pragma unroll
+        for (int q = 0; q < S; ++q) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) xa[q][i] = xb[q][i] = 0.f;
+          store_pair<T, V>(y, at[q], xa[q], xb[q]);
+        }
+        continue;
+      }
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < S; ++q) {
+        numbers<T, V>(next[q].a, xa[q]);
+        numbers<T, V>(next[q].b, xb[q]);
+        part<V>(mixed[q], xa[q], xb[q]);
+      }
+      if (h + 1 < h1) fetch(h + 1);
+#pragma unroll
+      for (int q = 0; q < S; ++q)
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          sum = fmaf(xa[q][i], xa[q][i], fmaf(xb[q][i], xb[q][i], sum));
+      const float r = rsqrtf(fmaf(group_sum(sum, a.lanes), inv, a.eps));
+      const bool is_k = h >= a.q_heads;
+#pragma unroll
+      for (int q = 0; q < S; ++q) {
+        float ya[V], yb[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float u = xa[q][i] * r * (is_k ? wka[q][i] : wqa[q][i]),
+                      v = xb[q][i] * r * (is_k ? wkb[q][i] : wqb[q][i]);
+          ya[i] = u * tok.c[q][i] - v * tok.s[q][i];
+          yb[i] = u * tok.s[q][i] + v * tok.c[q][i];
+        }
+        unpart<V>(mixed[q], ya, yb);
+        store_pair<T, V>(y, at[q], ya, yb);
+      }
+    }
+  }
+}
+
+// The weights' sums stay in registers over a group's items, are added in a
+// workgroup through LDS in the groups' order, and k_norm_join adds the
+// workgroups' sums in theirs.  parts: [workgroups][2][head_dim].
+template <typename T, int V, int S>
+__global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict__ parts) {
+  __shared__ float s_sum[256 * 2 * S * V];
+  const uint32_t lane = threadIdx.x % a.lanes, groups = 256 / a.lanes, d = a.head_dim;
+  Slots<V> at[S];
+  bool mixed[S];
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    const uint32_t s0 = V * (lane + q * a.lanes);
+    at[q] = slots_at<V>(a, s0);
+    mixed[q] = a.neighbours && s0 < a.half;
+  }
+  float wqa[S][V], wqb[S][V], wka[S][V], wkb[S][V];
+  load_head_weights<T, V, S>(a, a.q_weight, lane, wqa, wqb);
+  load_head_weights<T, V, S>(a, a.k_weight, lane, wka, wkb);
+  float qa[S][V] = {}, qb[S][V] = {}, ka[S][V] = {}, kb[S][V] = {};
+  const uint32_t heads = a.q_heads + a.k_heads;
+  const float inv = 1.f / (float)d;
+  for (uint64_t item = (uint64_t)blockIdx.x * groups + threadIdx.x / a.lanes; item < a.items;
+       item += (uint64_t)gridDim.x * groups) {
+    const uint32_t h0 = (uint32_t)(item % a.chunks) * a.per, h1 = min(h0 + a.per, heads);
+    Token<V, S> tok;
+    token_at<V, S>(a, (uint32_t)(item / a.chunks), lane, tok);
+    RawPair<T, V> nx[S], ng[S];
+    const auto fetch = [&](uint32_t h) {
+      const T *x = head_at<const T>(a, a.q, a.k, tok.b, tok.t, h);
+      const T *g = head_at<const T>(a, a.dq_out, a.dk_out, tok.b, tok.t, h);
+#pragma unroll
+      for (int q = 0; q < S; ++q) {
+        nx[q] = load_pair<T, V>(x, at[q]);
+        ng[q] = load_pair<T, V>(g, at[q]);
+      }
+    };
+    if (tok.inside) fetch(h0);
+    for (uint32_t h = h0; h < h1; ++h) {
+      T *const dx = head_at<T>(a, a.q_out, a.k_out, tok.b, tok.t, h);
+      float xa[S][V], xb[S][V], ga[S][V], gb[S][V];
+      if (!tok.inside) {
+#pragma unroll
+        for (int q = 0; q < S; ++q) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) xa[q][i] = xb[q][i] = 0.f;
+          store_pair<T, V>(dx, at[q], xa[q], xb[q]);
+        }
+        continue;
+      }
+#pragma unroll
+      for (int q = 0; q < S; ++q) {
+        numbers<T, V>(nx[q].a, xa[q]);
+        numbers<T, V>(nx[q].b, xb[q]);
+        numbers<T, V>(ng[q].a, ga[q]);
+        numbers<T, V>(ng[q].b, gb[q]);
+        part<V>(mixed[q], xa[q], xb[q]);
+        part<V>(mixed[q], ga[q], gb[q]);
+      }
+      if (h + 1 < h1) fetch(h + 1);
+      const bool is_k = h >= a.q_heads;
+      float squares = 0.f, along = 0.f;  // sums of x^2 and of g w x
+#pragma unroll
+      for (int q = 0; q < S; ++q)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float u = ga[q][i] * tok.c[q][i] + gb[q][i] * tok.s[q][i];
+          const float v = gb[q][i] * tok.c[q][i] - ga[q][i] * tok.s[q][i];
+          ga[q][i] = u, gb[q][i] = v;
+          squares = fmaf(xa[q][i], xa[q][i], fmaf(xb[q][i], xb[q][i], squares));
+          along = fmaf(u * (is_k ? wka[q][i] : wqa[q][i]), xa[q][i],
+                       fmaf(v * (is_k ? wkb[q][i] : wqb[q][i]), xb[q][i], along));
+        }
+      const float r = rsqrtf(fmaf(group_sum(squares, a.lanes), inv, a.eps));
+      const float back = group_sum(along, a.lanes) * inv * r * r;
+#pragma unroll
+      for (int q = 0; q < S; ++q) {
+        float da[V], db[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float sa = ga[q][i] * (xa[q][i] * r), sb = gb[q][i] * (xb[q][i] * r);
+          qa[q][i] += is_k ? 0.f : sa, qb[q][i] += is_k ? 0.f : sb;
+          ka[q][i] += is_k ? sa : 0.f, kb[q][i] += is_k ? sb : 0.f;
+          da[i] = r * (ga[q][i] * (is_k ? wka[q][i] : wqa[q][i]) - xa[q][i] * back);
+          db[i] = r * (gb[q][i] * (is_k ? wkb[q][i] : wqb[q][i]) - xb[q][i] * back);
+        }
+        unpart<V>(mixed[q], da, db);
+        store_pair<T, V>(dx, at[q], da, db);
+      }
+    }
+  }
+  for (int side = 0; side < 2; ++side) {
+    __syncthreads();
+    float *const mine = s_sum + threadIdx.x / a.lanes * d;
+#pragma unroll
+    for (int q = 0; q < S; ++q) {
+      float va[V], vb[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        va[i] = side ? ka[q][i] : qa[q][i], vb[i] = side ? kb[q][i] : qb[q][i];
+      unpart<V>(mixed[q], va, vb);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (at[q].one) mine[at[q].first + i] = va[i];
+        if (at[q].two) mine[at[q].second + i] = vb[i];
+      }
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < d; e += 256) {
+      float sum = 0.f;
+      for (uint32_t g = 0; g < groups; ++g) sum += s_sum[g * d + e];
+      parts[((uint64_t)blockIdx.x * 2 + side) * d + e] = sum;
+    }
+  }
+}
+
+// 16 values and 16 runs of workgroups a workgroup.
+__global__ __launch_bounds__(256) void k_norm_join(const float *__restrict__ parts, uint32_t blocks,
+                                                   uint32_t d, float *dq_weight, float *dk_weight) {
+  __shared__ double s_sum[16][17];
+  const uint32_t side = blockIdx.y, e = blockIdx.x * 16 + threadIdx.x % 16, run = threadIdx.x / 16;
+  float *const out = side ? dk_weight : dq_weight;
+  double sum = 0.;
+  if (e < d)
+    for (uint32_t b = run; b < blocks; b += 16) sum += parts[((uint64_t)b * 2 + side) * d + e];
+  s_sum[run][threadIdx.x % 16] = sum;
+  __syncthreads();
+  if (threadIdx.x < 16 && e < d && out) {
+    double all = 0.;
+    for (int k = 0; k < 16; ++k) all += s_sum[k][threadIdx.x];
+    out[e] = (float)all;
+  }
+}
+
+constexpr uint32_t kGradBlocks = 1024;
+
+NormDev norm_dev(const nsfps_norm_args &a) {
+  NormDev d = {};
+  d.length = (uint32_t)a.length;
+  d.q_heads = a.q_heads;
+  d.k_heads = a.k_heads;
+  d.head_dim = a.head_dim;
+  d.rotary_dim = a.rotary_dim;
+  d.half = a.rotary_dim / 2;
+  d.rest = (a.head_dim - a.rotary_dim + 1) / 2;
+  d.neighbours = a.neighbours != 0;
+  d.eps = a.eps;
+  d.q = a.q;
+  d.k = a.k;
+  d.q_out = a.q_out;
+  d.k_out = a.k_out;
+  d.q_weight = a.d_q_weight;
+  d.k_weight = a.d_k_weight;
+  d.freq = a.d_freq;
+  d.lengths = a.d_lengths;
+  d.positions = a.d_positions;
+  return d;
+}
+
+// Slots of a vector: as many as the rotation, the head and every address keep
+// aligned, at most 16 bytes.
+uint32_t norm_vector(const nsfps_norm_args &a, std::initializer_list<const nsfps_rows *> rows) {
+  const uint32_t size = a.dtype == NSFPS_F32 ? 4 : 2;
+  const uint32_t half = a.rotary_dim / 2, behind = a.head_dim - a.rotary_dim;
+  uint32_t v = 16 / size;
+  const auto fits = [&](uint32_t n) {
+    if (half % n || behind % (2 * n) || a.head_dim % n) return false;
+    if (((uintptr_t)a.d_q_weight | (uintptr_t)a.d_k_weight) % (n * size)) return false;
+    for (const nsfps_rows *r : rows)
+      if ((uintptr_t)r->p % (n * size) || (a.batch > 1 && r->batch_stride % n) ||
+          (a.length > 1 && r->row_stride % n))
+        return false;
+    return true;
+  };
+  while (v > 1 && !fits(v)) v /= 2;
+  return v;
+}
+
+void norm_split(NormDev &d, uint64_t tokens, uint32_t v) {
+  const uint32_t slots = d.half + d.rest;
+  uint32_t lanes = 1;
+  while (lanes < 64 && lanes * v < slots) lanes *= 2;
+  d.lanes = lanes;
+  // heads of an item: all, unless tokens are too few to fill the chip
+  constexpr uint64_t kFill = 256 * 1024;  // threads
+  const uint32_t heads = d.q_heads + d.k_heads;
+  const uint64_t want = std::max<uint64_t>(1, kFill / std::max<uint64_t>(1, tokens * lanes));
+  d.chunks = (uint32_t)std::min<uint64_t>(heads, want);
+  d.per = (heads + d.chunks - 1) / d.chunks;
+  d.chunks = (heads + d.per - 1) / d.per;
+  d.items = tokens * d.chunks;
+}
+
+template <typename F>
+hipError_t norm_by(uint32_t dtype, uint32_t v, uint32_t slots, F f) {
+  constexpr std::integral_constant<int, 1> one;
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, 4> four;
+  constexpr std::integral_constant<int, 8> eight;
+  const auto by_vector = [&](auto t) {
+    if constexpr (sizeof(t) == 2)
+      if (v == 8) return f(t, eight, one);
+    if (v == 4) return f(t, four, one);
+    if (v == 2) return f(t, two, one);
+    return slots <= 64 ? f(t, one, one) : f(t, one, two);
+  };
+  return dtype == NSFPS_F32 ? by_vector(float()) : by_vector(bf16());
+}
+
+uint32_t norm_grid(const NormDev &d, uint64_t most) {
+  return (uint32_t)std::min<uint64_t>(most, host_ceil_div(d.items, 256 / d.lanes));
+}
+
+}  // namespace
+
+hipError_t launch_norm(const nsfps_norm_args &a, hipStream_t st) {
+  NormDev d = norm_dev(a);
+  nsfps_rows none = {};
+  const nsfps_rows *q = a.q_heads ? &a.q : &none, *qo = a.q_heads ? &a.q_out : &none,
+                   *k = a.k_heads ? &a.k : &none, *ko = a.k_heads ? &a.k_out : &none;
+  const uint32_t v = norm_vector(a, {q, qo, k, ko});
+  norm_split(d, a.batch * a.length, v);
+  return norm_by(a.dtype, v, d.half + d.rest, [&](auto t, auto vec, auto sets) {
+    k_norm<decltype(t), decltype(vec)::value, decltype(sets)::value>
+        <<<norm_grid(d, 1u << 20), 256, 0, st>>>(d);
+    return hipGetLastError();
+  });
+}
+
+uint64_t norm_grad_bytes(const nsfps_norm_args &a) {
+  return 4ull * kGradBlocks * 2 * a.head_dim;
+}
+
+hipError_t launch_norm_grad(const nsfps_norm_args &a, const nsfps_norm_grads &g, hipStream_t st) {
+  NormDev d = norm_dev(a);
+  d.q_out = g.dq;
+  d.k_out = g.dk;
+  d.dq_out = g.dq_out;
+  d.dk_out = g.dk_out;
+  nsfps_rows none = {};
+  const bool q = a.q_heads != 0, k = a.k_heads != 0;
+  const uint32_t v = norm_vector(a, {q ? &a.q : &none, q ? &g.dq : &none, q ? &g.dq_out : &none,
+                                     k ? &a.k : &none, k ? &g.dk : &none, k ? &g.dk_out : &none});
+  norm_split(d, a.batch * a.length, v);
+  const uint32_t blocks = d.items ? norm_grid(d, kGradBlocks) : 0;
+  float *const parts = (float *)a.workspace;
+  hipError_t e = hipSuccess;
+  if (blocks)
+    e = norm_by(a.dtype, v, d.half + d.rest, [&](auto t, auto vec, auto sets) {
+      k_norm_grad<decltype(t), decltype(vec)::value, decltype(sets)::value>
+          <<<blocks, 256, 0, st>>>(d, parts);
+      return hipGetLastError();
+    });
+  if (e != hipSuccess || (!g.d_dq_weight && !g.d_dk_weight)) return e;
+  k_norm_join<<<dim3((a.head_dim + 15) / 16, 2), 256, 0, st>>>(parts, blocks, a.head_dim,
+                                                              g.d_dq_weight, g.d_dk_weight);
+  return hipGetLastError();
+}
+
+hipError_t preload_norm_kernels() {
+  return func_attributes(k_norm<bf16, 8, 1>, k_norm_grad<bf16, 8, 1>, k_norm_join);
+}
+
+}  // namespace nsfps

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <utility>
 
 namespace nsfps {
@@ -248,6 +249,108 @@ nsfps_status check_step(const nsfps_step_args *a) {
   return NSFPS_OK;
 }
 
+// ------------------------------------------------------------------ norms
+
+nsfps_status check_norm_sizes(const nsfps_norm_args *a) {
+  if (!a) return fail(NSFPS_EINVAL, "null pointer: args");
+  if (!is_dtype(a->dtype)) return fail(NSFPS_EINVAL, "unknown type");
+  if (a->head_dim == 0 || (a->q_heads == 0 && a->k_heads == 0))
+    return fail(NSFPS_EINVAL, "head_dim and one of q_heads and k_heads must be >= 1");
+  if (a->head_dim > 256)
+    return fail(NSFPS_EUNSUPPORTED, "head_dim %u: at most 256 is supported", a->head_dim);
+  if (a->rotary_dim % 2 || a->rotary_dim > a->head_dim)
+    return fail(NSFPS_EINVAL, "rotary_dim %u must be even and at most head_dim %u", a->rotary_dim,
+                a->head_dim);
+  if (!(a->eps > 0.f) || !std::isfinite(a->eps))
+    return fail(NSFPS_EINVAL, "eps must be finite and above 0");
+  if (((uint64_t)a->q_heads + a->k_heads) * a->head_dim > 1u << 24)
+    return fail(NSFPS_EUNSUPPORTED, "more than 2^24 channels");
+  if (a->batch > kMaxCount || a->length > kMaxCount || a->batch * a->length > kMaxCount)
+    return fail(NSFPS_EUNSUPPORTED, "more than 2^31-1 tokens");
+  return NSFPS_OK;
+}
+
+nsfps_status check_norm(const nsfps_norm_args *a, bool grad) {
+  TRY(check_norm_sizes(a));
+  if (a->batch && a->length) {
+    const uint64_t b = a->batch, l = a->length, d = a->head_dim;
+    if (a->q_heads) {
+      TRY(check_rows(a->q, b, l, a->q_heads * d, a->dtype, false, "q"));
+      if (!grad) TRY(check_rows(a->q_out, b, l, a->q_heads * d, a->dtype, true, "q_out"));
+    }
+    if (a->k_heads) {
+      TRY(check_rows(a->k, b, l, a->k_heads * d, a->dtype, false, "k"));
+      if (!grad) TRY(check_rows(a->k_out, b, l, a->k_heads * d, a->dtype, true, "k_out"));
+    }
+  }
+  TRY(check_optional(a->d_q_weight, size_of(a->dtype), "d_q_weight"));
+  TRY(check_optional(a->d_k_weight, size_of(a->dtype), "d_k_weight"));
+  if (a->rotary_dim) TRY(check_pointer(a->d_freq, 4, "d_freq"));
+  TRY(check_optional(a->d_lengths, 4, "d_lengths"));
+  TRY(check_optional(a->d_positions, 4, "d_positions"));
+  return NSFPS_OK;
+}
+
+// ---------------------------------------------------------------- dropout
+
+nsfps_status check_dropout(const nsfps_dropout_args *a) {
+  if (!a) return fail(NSFPS_EINVAL, "null pointer: args");
+  if (!is_dtype(a->dtype)) return fail(NSFPS_EINVAL, "unknown type");
+  if (a->channels == 0) return fail(NSFPS_EINVAL, "channels must be >= 1");
+  if (a->channels > 1u << 24) return fail(NSFPS_EUNSUPPORTED, "more than 2^24 channels");
+  if (!(a->p >= 0.f && a->p <= 1.f)) return fail(NSFPS_EINVAL, "p must be between 0 and 1");
+  if (a->batch > kMaxCount || a->length > kMaxCount || a->batch * a->length > kMaxCount)
+    return fail(NSFPS_EUNSUPPORTED, "more than 2^31-1 tokens");
+  if (a->batch && a->length) {
+    TRY(check_rows(a->x, a->batch, a->length, a->channels, a->dtype, false, "x"));
+    if (a->residual.p)
+      TRY(check_rows(a->residual, a->batch, a->length, a->channels, a->dtype, false, "residual"));
+    TRY(check_rows(a->y, a->batch, a->length, a->channels, a->dtype, true, "y"));
+  }
+  TRY(check_pointer(a->d_seed, 8, "d_seed"));
+  TRY(check_optional(a->d_lengths, 4, "d_lengths"));
+  return NSFPS_OK;
+}
+
+// ------------------------------------------------------- vocabulary loss
+
+nsfps_status check_loss_sizes(const nsfps_loss_args *a) {
+  if (!a) return fail(NSFPS_EINVAL, "null pointer: args");
+  if (!is_dtype(a->dtype)) return fail(NSFPS_EINVAL, "unknown type");
+  if (a->width == 0) return fail(NSFPS_EINVAL, "width must be >= 1");
+  if (a->tokens > kMaxCount || a->rows > kMaxCount)
+    return fail(NSFPS_EUNSUPPORTED, "more than 2^31-1 tokens or rows");
+  if (a->width > 65536) return fail(NSFPS_EUNSUPPORTED, "width above 65536");
+  return NSFPS_OK;
+}
+
+nsfps_status check_row_stride(uint64_t stride, uint64_t rows, uint64_t width, const char *what) {
+  if (rows && stride < width) return fail(NSFPS_EINVAL, "%s must be >= width", what);
+  if (stride > kMaxElems / (rows + 1)) return fail(NSFPS_EINVAL, "%s is too large", what);
+  return NSFPS_OK;
+}
+
+nsfps_status check_loss(const nsfps_loss_args *a, bool grad) {
+  TRY(check_loss_sizes(a));
+  if (!std::isfinite(a->scale)) return fail(NSFPS_EINVAL, "scale must be finite");
+  TRY(check_row_stride(a->x_stride, a->tokens, a->width, "x_stride"));
+  TRY(check_row_stride(a->table_stride, a->rows, a->width, "table_stride"));
+  if (a->rows) TRY(check_pointer(a->d_table, size_of(a->dtype), "d_table"));
+  if (a->tokens) {
+    TRY(check_pointer(a->d_x, size_of(a->dtype), "d_x"));
+    TRY(check_pointer(a->d_targets, 4, "d_targets"));
+    if (!grad) TRY(check_pointer(a->d_loss, 4, "d_loss"));
+    TRY(check_pointer(a->d_lse, 4, "d_lse"));
+  }
+  return NSFPS_OK;
+}
+
+nsfps_status check_loss_grads(const nsfps_loss_grads *g) {
+  if (!g) return fail(NSFPS_EINVAL, "null pointer: grads");
+  if (!is_dtype(g->grad_dtype)) return fail(NSFPS_EINVAL, "unknown type");
+  return NSFPS_OK;
+}
+
 }  // namespace
 }  // namespace nsfps
 
@@ -262,6 +365,9 @@ nsfps_status nsfps_init_sequence_device(void) {
     HIP_TRY(preload_conv_kernels());
     HIP_TRY(preload_scan_kernels());
     HIP_TRY(preload_scan_grad_kernels());
+    HIP_TRY(preload_norm_kernels());
+    HIP_TRY(preload_dropout_kernels());
+    HIP_TRY(preload_loss_kernels());
     return NSFPS_OK;
   });
 }
@@ -399,6 +505,112 @@ nsfps_status nsfps_scan_step_device(const nsfps_step_args *args, void *stream) {
     if (!args->batch) return NSFPS_OK;
     TRY(need_device());
     HIP_TRY(launch_scan_step(*args, (hipStream_t)stream));
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_norm_device(const nsfps_norm_args *args, void *stream) {
+  return guarded([&]() -> nsfps_status {
+    TRY(check_norm(args, false));
+    if (!args->batch || !args->length) return NSFPS_OK;
+    TRY(need_device());
+    HIP_TRY(launch_norm(*args, (hipStream_t)stream));
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_norm_grad_workspace_bytes(const nsfps_norm_args *args, uint64_t *bytes) {
+  return guarded([&]() -> nsfps_status {
+    if (!bytes) return fail(NSFPS_EINVAL, "null pointer: bytes");
+    TRY(check_norm_sizes(args));
+    *bytes = norm_grad_bytes(*args);
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_norm_grad_device(const nsfps_norm_args *args, const nsfps_norm_grads *grads,
+                                    void *stream) {
+  return guarded([&]() -> nsfps_status {
+    TRY(check_norm(args, true));
+    if (!grads) return fail(NSFPS_EINVAL, "null pointer: grads");
+    if (args->batch && args->length) {
+      const uint64_t b = args->batch, l = args->length, d = args->head_dim;
+      const uint32_t t = args->dtype;
+      if (args->q_heads) {
+        TRY(check_rows(grads->dq_out, b, l, args->q_heads * d, t, false, "dq_out"));
+        TRY(check_rows(grads->dq, b, l, args->q_heads * d, t, true, "dq"));
+      }
+      if (args->k_heads) {
+        TRY(check_rows(grads->dk_out, b, l, args->k_heads * d, t, false, "dk_out"));
+        TRY(check_rows(grads->dk, b, l, args->k_heads * d, t, true, "dk"));
+      }
+    }
+    TRY(check_optional(grads->d_dq_weight, 4, "d_dq_weight"));
+    TRY(check_optional(grads->d_dk_weight, 4, "d_dk_weight"));
+    TRY(check_workspace(args->workspace, args->workspace_bytes, norm_grad_bytes(*args)));
+    TRY(need_device());
+    HIP_TRY(launch_norm_grad(*args, *grads, (hipStream_t)stream));
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_dropout_device(const nsfps_dropout_args *args, void *stream) {
+  return guarded([&]() -> nsfps_status {
+    TRY(check_dropout(args));
+    if (!args->batch || !args->length) return NSFPS_OK;
+    TRY(need_device());
+    HIP_TRY(launch_dropout(*args, (hipStream_t)stream));
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_loss_workspace_bytes(const nsfps_loss_args *args, uint64_t *bytes) {
+  return guarded([&]() -> nsfps_status {
+    if (!bytes) return fail(NSFPS_EINVAL, "null pointer: bytes");
+    TRY(check_loss_sizes(args));
+    *bytes = loss_bytes(*args);
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_loss_device(const nsfps_loss_args *args, void *stream) {
+  return guarded([&]() -> nsfps_status {
+    TRY(check_loss(args, false));
+    if (!args->tokens) return NSFPS_OK;
+    TRY(check_workspace(args->workspace, args->workspace_bytes, loss_bytes(*args)));
+    TRY(need_device());
+    HIP_TRY(launch_loss(*args, (hipStream_t)stream));
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_loss_grad_workspace_bytes(const nsfps_loss_args *args,
+                                             const nsfps_loss_grads *grads, uint64_t *bytes) {
+  return guarded([&]() -> nsfps_status {
+    if (!bytes) return fail(NSFPS_EINVAL, "null pointer: bytes");
+    TRY(check_loss_sizes(args));
+    TRY(check_loss_grads(grads));
+    *bytes = loss_grad_bytes(*args, *grads);
+    return NSFPS_OK;
+  });
+}
+
+nsfps_status nsfps_loss_grad_device(const nsfps_loss_args *args, const nsfps_loss_grads *grads,
+                                    void *stream) {
+  return guarded([&]() -> nsfps_status {
+    TRY(check_loss(args, true));
+    TRY(check_loss_grads(grads));
+    TRY(check_row_stride(grads->dx_stride, args->tokens, args->width, "dx_stride"));
+    TRY(check_row_stride(grads->dtable_stride, args->rows, args->width, "dtable_stride"));
+    if (args->tokens) {
+      TRY(check_pointer(grads->d_dloss, 4, "d_dloss"));
+      TRY(check_pointer(grads->d_dx, size_of(args->dtype), "d_dx"));
+    }
+    if (args->rows) TRY(check_pointer(grads->d_dtable, size_of(grads->grad_dtype), "d_dtable"));
+    if (!args->tokens && !args->rows) return NSFPS_OK;
+    TRY(check_workspace(args->workspace, args->workspace_bytes, loss_grad_bytes(*args, *grads)));
+    TRY(need_device());
+    HIP_TRY(launch_loss_grad(*args, *grads, (hipStream_t)stream));
     return NSFPS_OK;
   });
 }
