@@ -527,8 +527,9 @@ nsfps_status nsfps_dropout_device(const nsfps_dropout_args *args, void *stream);
  * products in bfloat16 where the result is bfloat16, with 16 bits for a float32
  * table gradient of bfloat16 inputs, with 24 in float32 calls.
  *
- * At most 2^31 - 1 tokens and rows, width at most 65,536.  The vocabulary is
- * taken in pieces, whose products live in the workspace; its size goes by
+ * A row of the table that is not finite spoils every token.  At most 2^30
+ * tokens, 2^31 - 1 rows, width at most 65,536.  The gradient takes the
+ * vocabulary in pieces, whose products live in the workspace; its size goes by
  * sizes and types alone. */
 typedef struct {
   uint64_t tokens, rows;

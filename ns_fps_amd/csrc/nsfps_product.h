@@ -1,19 +1,23 @@
-// Products of bfloat16 matrices on the matrix cores, fed straight from global
-// memory to LDS: a workgroup's tile of sums C[m][n] = sum over k of M[m][k] N[n][k].
+// Products of matrices on the matrix cores from tiles in LDS: a workgroup's tile
+// of sums C[m][n] = sum over k of M[m][k] N[n][k], from operands whose terms lie
+// along the row (Row: element (m, k) at m * ld + k) or down the column (Col: at
+// k * ld + m) of memory.
 //
-// An operand lies in memory with its terms k along the row (Row: element (m, k)
-// at m * ld + k) or down the column (Col: at k * ld + m).  Stages of 64 terms go
-// to LDS in 16-byte pieces, 64 of them an instruction in the order of the lanes,
-// so a tile's rows have no padding; the pieces of a row are exchanged instead,
-// by a number that the row gives, so that the 16 rows which lanes read at once
-// lie in different banks.  Reads of a Col tile transpose on the way.
+// Operands in LDS are bfloat16; a float32 value is there as up to three terms
+// whose sum it is, in planes, and its products are those of the planes that
+// matter (kPasses).  Rows of a tile have no padding; the 16-byte pieces of a row
+// are exchanged instead, by a number that the row gives (the turn), so that rows
+// which lanes read at once lie in different banks.  Reads of a Col tile transpose
+// on the way.
+//
+// Tiles come to LDS in one of two ways: straight from memory where rows allow
+// 16-byte pieces (Feed), or through registers from any rows of either type,
+// which are split into planes and masked on the way (Stage).
 //
 // Lane layout, with g = lane / 16, l = lane % 16: an operand of 32 terms holds
 // row l, terms 8g .. 8g + 7; a tile of sums holds row m = l, columns n = 4g .. 4g
 // + 3.  kPerm (four column tiles): column 4g + r of tile nt stands for column 16g
 // + 4nt + r of the wave's 64, so that a lane's 16 sums of a row are neighbours.
-//
-// Sizes are whole: tiles inside the operands, terms a multiple of 64.
 #pragma once
 
 #include "nsfps_mfma.h"
@@ -23,59 +27,39 @@
 namespace nsfps {
 namespace seq {
 
-constexpr uint32_t kStage = 64;  // terms of a stage
-
-// The number that exchanges a row's pieces.  Row: 128 bytes a row, 8 pieces; the
-// rows 0 .. 15 and the rows 16a + 4c + b (a, b < 4) get all 8 at both parities.
+// The number that exchanges the pieces of a row of kTerms terms (Row): the rows
+// 0 .. 15, and the rows 16a + 4c + b (a, b < 4), meet no bank twice, taken 8 or
+// 16 at a time.
+template <int kTerms>
 __device__ __forceinline__ uint32_t row_turn(uint32_t r) {
-  return ((r >> 1) & 1) | ((((r >> 2) + (r >> 4)) & 3) << 1);
+  static_assert(kTerms == 64 || kTerms == 32, "terms of a stage");
+  if constexpr (kTerms == 64)
+    return ((2 * ((r >> 2) + (r >> 4)) + ((r >> 1) & 1)) ^ ((r & 1) << 2)) & 7;
+  else
+    return ((r >> 2) + (r >> 4) + (r & 2)) & 3;
 }
-// Col: pairs of pieces (16 columns); rows 8g + i (g, i < 4).
+// Col, T columns a row: pairs of pieces (16 columns); rows 8g + i (g, i < 4).
 template <int T>
 __device__ __forceinline__ uint32_t col_turn(uint32_t k) {
   if constexpr (T == 64) return (((k >> 1) & 1) | ((k >> 2) & 2)) << 1;
   return ((k & 3) | ((k >> 1) & 4)) << 1;
 }
 
-// The pieces of an operand's stage that this thread brings.
-template <int T, bool kCol, int kThreads>
-struct Feed {
-  static constexpr int kPer = T * (int)kStage / 8 / kThreads;
-  static_assert(kPer >= 1, "tile too small");
-  const bf16 *p[kPer];
-
-  // at: the tile's first row (Row) or column (Col) at term 0
-  __device__ __forceinline__ void start(const bf16 *at, uint64_t ld) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t e = threadIdx.x + kThreads * i;
-      if constexpr (kCol) {
-        const uint32_t k = e / (T / 8), c = (e % (T / 8)) ^ col_turn<T>(k);
-        p[i] = at + k * ld + 8 * c;
-      } else {
-        const uint32_t r = e / 8, c = (e % 8) ^ row_turn(r);
-        p[i] = at + r * ld + 8 * c;
-      }
-    }
-  }
-  __device__ __forceinline__ void issue(bf16 *stage, uint64_t offset) const {
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void *)(p[i] + offset),
-          (__attribute__((address_space(3))) void *)(stage + 8 * (64 * wave + kThreads * i)), 16, 0,
-          0);
-  }
-};
+// Where the 8 values from column c (a multiple of 8) of memory row r go.
+template <int T, int kTerms, bool kCol>
+__device__ __forceinline__ uint32_t piece_at(uint32_t r, uint32_t c) {
+  if constexpr (kCol) return r * T + 8 * ((c / 8) ^ col_turn<T>(r));
+  return r * kTerms + 8 * ((c / 8) ^ row_turn<kTerms>(r));
+}
 
 // A lane's operand of terms 32 kb .. 32 kb + 31; r: this lane's row.
-__device__ __forceinline__ bf16x8 read_row(const bf16 *stage, uint32_t r, uint32_t kb, uint32_t g) {
-  return *(const bf16x8 *)(stage + 8 * (8 * r + ((4 * kb + g) ^ row_turn(r))));
+template <int kTerms>
+__device__ __forceinline__ bf16x8 read_row(const bf16 *tile, uint32_t r, uint32_t kb, uint32_t g) {
+  return *(const bf16x8 *)(tile + r * kTerms + 8 * ((4 * kb + g) ^ row_turn<kTerms>(r)));
 }
-// c: the tile's first column
+// c: the first of the 16 columns
 template <int T>
-__device__ __forceinline__ bf16x8 read_col(const bf16 *stage, uint32_t c, uint32_t kb, uint32_t g,
+__device__ __forceinline__ bf16x8 read_col(const bf16 *tile, uint32_t c, uint32_t kb, uint32_t g,
                                            uint32_t l) {
   typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
   const uint32_t k = 32 * kb + 8 * g + l / 4, at = c + 4 * (l % 4);
@@ -85,57 +69,226 @@ __device__ __forceinline__ bf16x8 read_col(const bf16 *stage, uint32_t c, uint32
     const uint32_t row = k + 4 * i;
     q[i] = __builtin_bit_cast(
         bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s16x4 *)(stage + row * T + 8 * ((at / 8) ^ col_turn<T>(row)) + at % 8)));
+                    (lds_s16x4 *)(tile + row * T + 8 * ((at / 8) ^ col_turn<T>(row)) + at % 8)));
   }
   return __builtin_shufflevector(q[0], q[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// WM x WN waves of MT x NT tiles of 16 x 16 sums.
-template <int WM, int WN, int MT, int NT, bool kMCol, bool kNCol, bool kPerm>
+// A tile straight from memory to LDS, 64 pieces of 16 bytes an instruction in
+// the order of the lanes: the pieces' exchange is in the addresses.  Pieces are
+// whole; memory rows past the last are the last one again.
+template <int T, int kTerms, bool kCol, int kThreads>
+struct Feed {
+  static constexpr int kPer = T * kTerms / 8 / kThreads;
+  static_assert(kPer >= 1, "tile too small");
+  const bf16 *p[kPer];
+
+  // at: the tile's first value; rows: how many of memory there are (at least 1)
+  __device__ __forceinline__ void start(const bf16 *at, uint64_t ld, uint32_t rows) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + kThreads * i;
+      if constexpr (kCol) {
+        const uint32_t k = e / (T / 8);
+        p[i] = at + min(k, rows - 1) * ld + 8 * ((e % (T / 8)) ^ col_turn<T>(k));
+      } else {
+        const uint32_t r = e / (kTerms / 8);
+        p[i] = at + min(r, rows - 1) * ld + 8 * ((e % (kTerms / 8)) ^ row_turn<kTerms>(r));
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(bf16 *tile, uint64_t offset) const {
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void *)(p[i] + offset),
+          (__attribute__((address_space(3))) void *)(tile + 8 * (64 * wave + kThreads * i)), 16, 0,
+          0);
+  }
+};
+
+// Eight values of a row, at any address that holds such values.
+template <typename T>
+struct Eight {
+  static constexpr int kWords = 8 * (int)sizeof(T) / 4;
+  uint32_t w[kWords];
+};
+struct __attribute__((packed, aligned(2))) Packed16 {
+  uint32_t w[4];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load_eight(const T *p) {
+  Eight<T> o;
+#pragma unroll
+  for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
+    const Packed16 v = ((const NSFPS_GLOBAL_SEQ Packed16 *)p)[i];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o.w[4 * i + k] = v.w[k];
+  }
+  return o;
+}
+// its first n
+template <typename T>
+__device__ __forceinline__ Eight<T> load_some(const T *p, uint32_t n) {
+  Eight<T> o = {};
+#pragma unroll
+  for (uint32_t k = 0; k < 8; ++k)
+    if (k < n) {
+      const Raw<T, 1> v = load_raw<T, 1>(p + k);
+      if constexpr (sizeof(T) == 4)
+        o.w[k] = v.w[0];
+      else
+        o.w[k / 2] |= v.w[0] << (16 * (k % 2));
+    }
+  return o;
+}
+
+// A tile through registers: ROWS x COLS of memory, fetched while the tile before
+// it is worked on, split into P planes and put.  What lies outside is zeros.
+template <typename T, int ROWS, int COLS, int kThreads>
+struct Stage {
+  static constexpr int kPer = ROWS * COLS / 8 / kThreads, kVecs = COLS / 8;
+  static_assert(kPer >= 1, "tile too small");
+  Eight<T> v[kPer];
+
+  // at: the tile's first value; rows, cols: how many of it are inside.
+  // counts(row): whether a row inside is wanted.
+  template <typename F>
+  __device__ __forceinline__ void fetch(const T *at, uint64_t ld, uint32_t rows, uint32_t cols,
+                                        F counts) {
+    const bool whole = rows >= (uint32_t)ROWS && cols >= (uint32_t)COLS;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + kThreads * i, r = e / kVecs, c = e % kVecs * 8;
+      const T *p = at + r * ld + c;
+      if (whole) {
+        v[i] = load_eight<T>(p);
+      } else {
+        v[i] = Eight<T>{};
+        if (r < rows && c + 8 <= cols)
+          v[i] = load_eight<T>(p);
+        else if (r < rows && c < cols)
+          v[i] = load_some<T>(p, cols - c);
+      }
+      if (!counts(r)) v[i] = Eight<T>{};
+    }
+  }
+  // kT: columns of a Col tile; plane: values of a plane in LDS
+  template <int kT, int kTerms, bool kCol, int P>
+  __device__ __forceinline__ void put(bf16 *tile, uint32_t plane) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t e = threadIdx.x + kThreads * i, r = e / kVecs, c = e % kVecs * 8;
+      bf16 *const to = tile + piece_at<kT, kTerms, kCol>(r, c);
+      if constexpr (sizeof(T) == 2) {
+        static_assert(P == 1, "a bfloat16 value is one term");
+        *(u32x4 *)to = u32x4{v[i].w[0], v[i].w[1], v[i].w[2], v[i].w[3]};
+      } else {
+        f32x4 a, b;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          a[k] = __uint_as_float(v[i].w[k]), b[k] = __uint_as_float(v[i].w[4 + k]);
+        const Terms<bf16, P> ta = split<bf16, P>(a), tb = split<bf16, P>(b);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          *(bf16x8 *)(to + p * plane) =
+              __builtin_shufflevector(ta.q[p], tb.q[p], 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    }
+  }
+};
+
+// The products of planes that make one product to the bits of the planes, the
+// smallest first: plane of m, plane of n.
+template <int PM, int PN>
+struct Passes;
+template <>
+struct Passes<1, 1> {
+  static constexpr int kN = 1, m[kN] = {0}, n[kN] = {0};
+};
+template <>
+struct Passes<2, 1> {
+  static constexpr int kN = 2, m[kN] = {1, 0}, n[kN] = {0, 0};
+};
+template <>
+struct Passes<3, 3> {  // to 24 bits: what is left out is below 2^-24 of the product
+  static constexpr int kN = 6, m[kN] = {2, 0, 1, 1, 0, 0}, n[kN] = {0, 2, 1, 0, 1, 0};
+};
+
+// WM x WN waves of MT x NT tiles of 16 x 16 sums; stages of kTerms terms, PM and
+// PN planes.
+template <int WM, int WN, int MT, int NT, int kTerms, int PM, int PN, bool kMCol, bool kNCol,
+          bool kPerm>
 struct Product {
   static constexpr int kM = 16 * WM * MT, kN = 16 * WN * NT, kThreads = 64 * WM * WN;
   static_assert(!kPerm || (NT == 4 && !kNCol), "layout");
+  static constexpr int kMPlane = kM * kTerms, kNPlane = kN * kTerms;
   struct alignas(16) Lds {
-    bf16 m[2][kM * kStage], n[2][kN * kStage];
+    bf16 m[PM * kMPlane], n[PN * kNPlane];
   };
-  Feed<kM, kMCol, kThreads> fm;
-  Feed<kN, kNCol, kThreads> fn;
+  typedef f32x4 Sum[MT][NT];
 
-  __device__ __forceinline__ void issue(Lds &lds, uint32_t buf, uint64_t m, uint64_t n) const {
-    fm.issue(lds.m[buf], m);
-    fn.issue(lds.n[buf], n);
+  static __device__ __forceinline__ uint32_t wave_id() {
+    return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   }
-  // Waits for the stage issued last, adds its products; next() issues the one
-  // after it, once this one's operands are in registers: the other half of LDS
-  // was read before the barrier.
-  template <typename F>
-  __device__ __forceinline__ void add(f32x4 (&sum)[MT][NT], const Lds &lds, uint32_t buf, F next) {
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t m0 = wave / WN * (16 * MT), n0 = wave % WN * (16 * NT);
-    wait_loads();
-    __syncthreads();
-    bf16x8 m[2][MT], n[2][NT];
+  static __device__ __forceinline__ uint32_t first_m() { return wave_id() / WN * (16 * MT); }
+  static __device__ __forceinline__ uint32_t first_n() { return wave_id() % WN * (16 * NT); }
+
+  static __device__ __forceinline__ bf16x8 read_m(const Lds &lds, int p, int t, uint32_t kb) {
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u, m0 = first_m() + 16 * t;
+    const bf16 *tile = lds.m + p * kMPlane;
+    return kMCol ? read_col<kM>(tile, m0, kb, g, l) : read_row<kTerms>(tile, m0 + l, kb, g);
+  }
+  static __device__ __forceinline__ bf16x8 read_n(const Lds &lds, int p, int t, uint32_t kb) {
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u, n0 = first_n();
+    const bf16 *tile = lds.n + p * kNPlane;
+    return kNCol   ? read_col<kN>(tile, n0 + 16 * t, kb, g, l)
+           : kPerm ? read_row<kTerms>(tile, n0 + 16 * (l / 4) + 4 * t + l % 4, kb, g)
+                   : read_row<kTerms>(tile, n0 + 16 * t + l, kb, g);
+  }
+  static __device__ __forceinline__ void add_block(Sum &sum, const bf16x8 (&m)[PM][MT],
+                                                   const bf16x8 (&n)[PN][NT]) {
+    typedef Passes<PM, PN> P;
 #pragma unroll
-    for (uint32_t kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-        m[kb][t] = kMCol ? read_col<kM>(lds.m[buf], m0 + 16 * t, kb, g, l)
-                         : read_row(lds.m[buf], m0 + 16 * t + l, kb, g);
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-        n[kb][t] = kNCol ? read_col<kN>(lds.n[buf], n0 + 16 * t, kb, g, l)
-                   : kPerm ? read_row(lds.n[buf], n0 + 16 * (l / 4) + 4 * t + l % 4, kb, g)
-                           : read_row(lds.n[buf], n0 + 16 * t + l, kb, g);
-    }
-    next();
-#pragma unroll
-    for (uint32_t kb = 0; kb < 2; ++kb)
+    for (int p = 0; p < P::kN; ++p)
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-          sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(n[kb][j], m[kb][i], sum[i][j], 0, 0, 0);
+          sum[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(n[P::n[p]][j], m[P::m[p]][i],
+                                                              sum[i][j], 0, 0, 0);
+  }
+  static __device__ __forceinline__ void read_block(const Lds &lds, uint32_t kb,
+                                                    bf16x8 (&m)[PM][MT], bf16x8 (&n)[PN][NT]) {
+#pragma unroll
+    for (int p = 0; p < PM; ++p)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) m[p][t] = read_m(lds, p, t, kb);
+#pragma unroll
+    for (int p = 0; p < PN; ++p)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) n[p][t] = read_n(lds, p, t, kb);
+  }
+  // Adds a stage that is in LDS.
+  static __device__ __forceinline__ void add(Sum &sum, const Lds &lds) {
+#pragma unroll
+    for (uint32_t kb = 0; kb < kTerms / 32; ++kb) {
+      bf16x8 m[PM][MT], n[PN][NT];
+      read_block(lds, kb, m, n);
+      add_block(sum, m, n);
+    }
+  }
+  // The same; next() runs once all of the stage's operands are in registers (a
+  // copy straight to LDS, after which reads of LDS would wait for it).
+  template <typename F>
+  static __device__ __forceinline__ void add_then(Sum &sum, const Lds &lds, F next) {
+    bf16x8 m[kTerms / 32][PM][MT], n[kTerms / 32][PN][NT];
+#pragma unroll
+    for (uint32_t kb = 0; kb < kTerms / 32; ++kb) read_block(lds, kb, m[kb], n[kb]);
+    next();
+#pragma unroll
+    for (uint32_t kb = 0; kb < kTerms / 32; ++kb) add_block(sum, m[kb], n[kb]);
   }
 };
 

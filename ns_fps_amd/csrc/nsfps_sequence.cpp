@@ -318,8 +318,8 @@ nsfps_status check_loss_sizes(const nsfps_loss_args *a) {
   if (!a) return fail(NSFPS_EINVAL, "null pointer: args");
   if (!is_dtype(a->dtype)) return fail(NSFPS_EINVAL, "unknown type");
   if (a->width == 0) return fail(NSFPS_EINVAL, "width must be >= 1");
-  if (a->tokens > kMaxCount || a->rows > kMaxCount)
-    return fail(NSFPS_EUNSUPPORTED, "more than 2^31-1 tokens or rows");
+  if (a->tokens > 1u << 30 || a->rows > kMaxCount)
+    return fail(NSFPS_EUNSUPPORTED, "more than 2^30 tokens or 2^31-1 rows");
   if (a->width > 65536) return fail(NSFPS_EUNSUPPORTED, "width above 65536");
   return NSFPS_OK;
 }
