@@ -41,6 +41,7 @@ struct Matrix {
 
 struct LogitDev {
   Matrix x, e;                // e: the piece
+  uint32_t tokens;            // (x may be padded)
   uint32_t ttiles, vtiles;    // tiles of tokens, of the piece's vocabulary
   uint32_t sweep, sweeps;     // vocabulary tiles a workgroup takes one after another
   float scale2;               // scale * log2(e)
@@ -56,10 +57,12 @@ struct LogitDev {
   uint64_t d_ld;
 };
 
-// Workgroup w's tile of tokens and sweep: tokens change fastest, within groups
+// Workgroup w's tile of tokens and sweep, the latter as vocabulary tiles of N rows:
+// tokens change fastest, within groups
 // that share sweeps, so that workgroups of one XCD read the same rows.
-__device__ __forceinline__ bool logit_item(const LogitDev &a, uint32_t &ttile, uint32_t &first,
-                                           uint32_t &last) {
+template <uint32_t N>
+__device__ __forceinline__ bool logit_item(const LogitDev &a, uint32_t &ttile, uint32_t &sweep,
+                                           uint32_t &first, uint32_t &last) {
   const uint32_t work = a.ttiles * a.sweeps, per = (work + 7) / 8;
   const uint32_t w = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (blockIdx.x / 8 >= per || w >= work) return false;
@@ -67,48 +70,51 @@ __device__ __forceinline__ bool logit_item(const LogitDev &a, uint32_t &ttile, u
   const uint32_t whole = kGroup * a.sweeps, group = w / whole, t0 = group * kGroup;
   const uint32_t size = min(kGroup, a.ttiles - t0), in = w - group * whole;
   ttile = t0 + in % size;
-  first = in / size * a.sweep;
-  last = min(first + a.sweep, a.vtiles);
+  sweep = in / size;
+  first = kTile / N * (sweep * a.sweep);
+  last = kTile / N * min(sweep * a.sweep + a.sweep, a.vtiles);
   return true;
 }
 
-// The tiles of z that a workgroup walks, one after another; epilogue(sum, tile)
-// has each.  Operands through registers: any rows, either type.
-template <typename T, int P>
-struct StagedLogits {
+// The tiles of z that a workgroup walks, one after another; epilogue.whole(sum,
+// tile) has each.  Operands through registers: any rows, either type.
+template <typename T, int P, bool kPerm>
+struct StagedLogits {  // (every row is wanted)
   static constexpr int kTerms = P == 1 ? 64 : 32;
-  typedef Product<2, 2, 4, 4, kTerms, P, P, false, false, true> Prod;
+  typedef Product<2, 2, 4, 4, kTerms, P, P, false, false, kPerm> Prod;
   typedef typename Prod::Lds Lds;
   static constexpr bool kDirect = false;
 
   template <typename F>
   static __device__ __forceinline__ void walk(const LogitDev &a, Lds &lds, uint32_t ttile,
-                                              uint32_t first, uint32_t last, F epilogue) {
+                                              uint32_t first, uint32_t last, F &epilogue) {
     Stage<T, kTile, kTerms, 256> sx, se;
     const uint32_t width = a.x.cols, steps = ceil_div(width, kTerms);
     const uint32_t t0 = ttile * kTile;
     const T *const x = (const T *)a.x.p + (uint64_t)t0 * a.x.ld;
+    const auto none = [](uint32_t) { return 0u; };
     const auto all = [](uint32_t) { return true; };
     uint32_t tile = first, k = 0;  // of the stage fetched next
     const auto fetch = [&] {
       const uint32_t v0 = tile * kTile;
-      sx.fetch(x + k * kTerms, a.x.ld, a.x.rows - t0, width - k * kTerms, all);
+      sx.fetch(x + k * kTerms, a.x.ld, a.x.rows - t0, width - k * kTerms, none);
       se.fetch((const T *)a.e.p + (uint64_t)v0 * a.e.ld + k * kTerms, a.e.ld, a.e.rows - v0,
-               width - k * kTerms, all);
+               width - k * kTerms, none);
       if (++k == steps) k = 0, ++tile;
     };
+    wait_loads();
     fetch();
     for (uint32_t t = first; t < last; ++t) {
       typename Prod::Sum sum = {};
       for (uint32_t s = 0; s < steps; ++s) {
         __syncthreads();
-        sx.template put<Prod::kM, kTerms, false, P>(lds.m, Prod::kMPlane);
-        se.template put<Prod::kN, kTerms, false, P>(lds.n, Prod::kNPlane);
+        sx.template put<Prod::kM, kTerms, false, P>(lds.m, Prod::kMPlane, all);
+        se.template put<Prod::kN, kTerms, false, P>(lds.n, Prod::kNPlane, all);
         __syncthreads();
         if (tile < last) fetch();
         Prod::add(sum, lds);
       }
-      epilogue(sum, t);
+      epilogue.whole(sum, t);
     }
   }
 };
@@ -124,33 +130,96 @@ struct DirectLogits {
 
   template <typename F>
   static __device__ __forceinline__ void walk(const LogitDev &a, Lds &lds, uint32_t ttile,
-                                              uint32_t first, uint32_t last, F epilogue) {
+                                              uint32_t first, uint32_t last, F &epilogue) {
     Feed<kTile, 64, false, 256> fx, fe;
     const uint32_t steps = a.x.cols / 64;
-    fx.start((const bf16 *)a.x.p + (uint64_t)ttile * kTile * a.x.ld, a.x.ld,
-             a.x.rows - ttile * kTile);
+    const bf16 *const x = (const bf16 *)a.x.p + (uint64_t)ttile * kTile * a.x.ld;
+    fx.start(a.x.ld, a.x.rows - ttile * kTile);
+    fe.start(a.e.ld, ~0u);
     uint32_t tile = first, k = 0, buf = 0;  // of the stage issued next
     const auto issue = [&](uint32_t b) {
-      if (k == 0)
-        fe.start((const bf16 *)a.e.p + (uint64_t)tile * kTile * a.e.ld, a.e.ld,
-                 a.e.rows - tile * kTile);
-      fx.issue(lds.buf[b].m, 64 * k);
-      fe.issue(lds.buf[b].n, 64 * k);
+      const uint32_t v0 = min(tile * kTile, a.e.rows - 1);
+      if (k == 0 && v0 + kTile > a.e.rows) fe.start(a.e.ld, a.e.rows - v0);
+      fx.issue(lds.buf[b].m, x + 64 * k);
+      fe.issue(lds.buf[b].n, (const bf16 *)a.e.p + (uint64_t)v0 * a.e.ld + 64 * k);
       if (++k == steps) k = 0, ++tile;
     };
+    wait_loads();
     issue(0);
     for (uint32_t t = first; t < last; ++t) {
       typename Prod::Sum sum = {};
       for (uint32_t s = 0; s < steps; ++s) {
-        wait_loads();
+        landed<0>();
         __syncthreads();
-        Prod::add_then(sum, lds.buf[buf], [&] {
-          if (tile < last) issue(buf ^ 1);
-        });
+        if (tile < last) issue(buf ^ 1);
+        Prod::add(sum, lds.buf[buf]);
         buf ^= 1;
       }
-      epilogue(sum, t);
+      epilogue.whole(sum, t);
     }
+  }
+};
+
+// The same for widths of up to 256: a workgroup's tokens stay in registers, so
+// that LDS, which gives 128 bytes a cycle, is read for the vocabulary alone (with
+// both from LDS those reads and the copies took half as long again as the
+// products).  Three stages are under way while a fourth is worked on.
+template <int kTerms, int kSteps>
+struct ResidentLogits {
+  typedef Product<2, 2, 4, 2, kTerms, 1, 1, false, false, true> Prod;
+  struct alignas(16) Lds {
+    bf16 buf[4][Prod::kN * kTerms];
+  };
+  static constexpr bool kDirect = true;
+
+  template <typename F>
+  static __device__ __forceinline__ void walk(const LogitDev &a, Lds &lds, uint32_t ttile,
+                                              uint32_t first, uint32_t last, F &epilogue) {
+    constexpr int kBlocks = kTerms / 32;
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
+    bf16x8 x[kSteps][kBlocks][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = min(ttile * kTile + Prod::first_m() + 16 * i + l, a.x.rows - 1);
+      const bf16 *row = (const bf16 *)a.x.p + r * a.x.ld + 8 * g;
+#pragma unroll
+      for (int k = 0; k < kBlocks * kSteps; ++k)
+        x[k / kBlocks][k % kBlocks][i] = *(const NSFPS_GLOBAL_SEQ bf16x8 *)(row + 32 * k);
+    }
+    Feed<Prod::kN, kTerms, false, 256> fe;
+    constexpr int kCopies = fe.kPer;
+    fe.start(a.e.ld, ~0u);
+    uint32_t tile = first, k = 0, to = 0, buf = 0;
+    const auto issue = [&] {  // past the end the last tile again: counts stay the same
+      const uint32_t v0 = min(min(tile, last - 1) * Prod::kN, a.e.rows - 1);
+      if (v0 + Prod::kN > a.e.rows) fe.start(a.e.ld, a.e.rows - v0);
+      fe.issue(lds.buf[to], (const bf16 *)a.e.p + (uint64_t)v0 * a.e.ld + kTerms * k);
+      if (++k == kSteps) k = 0, ++tile;
+      to = (to + 1) % 4;
+    };
+    wait_loads();
+    issue();
+    issue();
+    issue();
+    for (uint32_t t = first; t < last; ++t) {
+      typename Prod::Sum sum = {};
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        landed<2 * kCopies>();
+        __syncthreads();
+        issue();
+#pragma unroll
+        for (uint32_t kb = 0; kb < kBlocks; ++kb) {
+          const bf16x8 n[1][2] = {
+              {Prod::read_n(lds.buf[buf], 0, kb), Prod::read_n(lds.buf[buf], 1, kb)}};
+          const bf16x8 m[1][4] = {{x[s][kb][0], x[s][kb][1], x[s][kb][2], x[s][kb][3]}};
+          Prod::add_block(sum, m, n);
+        }
+        buf = (buf + 1) % 4;
+      }
+      epilogue.whole(sum, t);
+    }
+    landed<0>();
   }
 };
 
@@ -160,167 +229,225 @@ __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s
   m = top;
 }
 
+// Running maximum and sum of a lane's columns, for its four tokens.
+template <typename Prod>
+struct Stats {
+  const LogitDev &a;
+  const float by;  // (-infinity times 0 would be NaN)
+  float top[4], sum[4];
+
+  __device__ __forceinline__ explicit Stats(const LogitDev &args)
+      : a(args), by(fmaxf(fabsf(args.scale2), 1e-38f)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = -INFINITY, sum[i] = 0.f;
+  }
+  // nothing to do but part(): no column past the end, no sign to turn
+  __device__ __forceinline__ bool plain(uint32_t tile) const {
+    return (tile + 1) * Prod::kN <= a.e.rows && a.scale2 >= 0.f;
+  }
+  __device__ __forceinline__ void part(const typename Prod::Sum &z, uint32_t, int i) {
+    float m = z[i][0][0];
+#pragma unroll
+    for (int j = 0; j < Prod::kNT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, z[i][j][r]);
+    m = fmaxf(top[i], m * by);
+    const float at = m == -INFINITY ? 0.f : m;
+    float s = sum[i] * exp2_fast(top[i] - at);
+#pragma unroll
+    for (int j = 0; j < Prod::kNT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s += exp2_fast(fmaf(z[i][j][r], by, -at));
+    top[i] = m;
+    sum[i] = s;
+  }
+  __device__ __forceinline__ void whole(typename Prod::Sum &z, uint32_t tile) {
+    if (!plain(tile)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < Prod::kNT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (a.scale2 < 0.f) z[i][j][r] = -z[i][j][r];
+            if (tile * Prod::kN + Prod::column(j) + r >= a.e.rows) z[i][j][r] = -INFINITY;
+          }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) part(z, tile, i);
+  }
+};
+
 template <typename Logits>
 __global__ __launch_bounds__(256, 2) void k_loss_stats(LogitDev a) {
+  typedef typename Logits::Prod Prod;
   __shared__ typename Logits::Lds lds;
   __shared__ float2 s_part[2][kTile];
-  uint32_t ttile, first, last;
-  if (!logit_item(a, ttile, first, last)) return;
+  uint32_t ttile, sweep, first, last;
+  if (!logit_item<Prod::kN>(a, ttile, sweep, first, last)) return;
   const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
-  float top[4], sum[4];  // of this lane's columns, for its four tokens
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top[i] = -INFINITY, sum[i] = 0.f;
-  Logits::walk(a, lds, ttile, first, last, [&](f32x4(&z)[4][4], uint32_t tile) {
-    const uint32_t v0 = tile * kTile + 64 * wn + 16 * g;
-    const bool ragged = (tile + 1) * kTile > a.e.rows;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float m = top[i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v = z[i][j][r] * a.scale2;
-          if (ragged && v0 + 4 * j + r >= a.e.rows) v = -INFINITY;
-          z[i][j][r] = v;
-          m = fmaxf(m, v);
-        }
-      const float at = m == -INFINITY ? 0.f : m;
-      float s = sum[i] * exp2_fast(top[i] - at);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s += exp2_fast(z[i][j][r] - at);
-      top[i] = m;
-      sum[i] = s;
-    }
-  });
+  Stats<Prod> o(a);
+  Logits::walk(a, lds, ttile, first, last, o);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int off = 16; off < 64; off <<= 1)
-      join_stats(top[i], sum[i], __shfl_xor(top[i], off, 64), __shfl_xor(sum[i], off, 64));
-    if (g == 0) s_part[wn][64 * wm + 16 * i + l] = make_float2(top[i], sum[i]);
+      join_stats(o.top[i], o.sum[i], __shfl_xor(o.top[i], off, 64), __shfl_xor(o.sum[i], off, 64));
+    if (g == 0) s_part[wn][64 * wm + 16 * i + l] = make_float2(o.top[i], o.sum[i]);
   }
   __syncthreads();
   const uint32_t token = ttile * kTile + threadIdx.x;
   if (threadIdx.x < kTile && token < a.x.rows) {
     float2 v = s_part[0][threadIdx.x];
     join_stats(v.x, v.y, s_part[1][threadIdx.x].x, s_part[1][threadIdx.x].y);
-    a.parts[first / a.sweep * a.part_stride + token] = v;
+    a.parts[sweep * a.part_stride + token] = v;
   }
 }
 
-// lse and loss of 16 tokens: 16 runs of parts each, then a wave finds the
-// logits of four tokens' targets.
+// lse and loss: a workgroup has `group` tokens (a power of two, at most 16), 256 /
+// group runs of parts for each; then its waves find the logits of the tokens'
+// targets.
 template <typename T>
 __global__ __launch_bounds__(256) void k_loss_join(const float2 *__restrict__ parts, uint32_t nparts,
-                                                   uint64_t part_stride, Matrix x, Matrix table,
-                                                   float scale, const int32_t *__restrict__ targets,
+                                                   uint64_t part_stride, uint32_t group, Matrix x,
+                                                   Matrix table, float scale,
+                                                   const int32_t *__restrict__ targets,
                                                    float *__restrict__ loss,
                                                    float *__restrict__ lse) {
   __shared__ float2 s_part[4][16];
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, tokens = x.rows;
-  for (uint32_t t0 = blockIdx.x * 16; t0 < tokens; t0 += gridDim.x * 16) {
-    const uint32_t mine = min(t0 + lane % 16, tokens - 1);
+  for (uint32_t t0 = blockIdx.x * group; t0 < tokens; t0 += gridDim.x * group) {
+    const uint32_t mine = min(t0 + lane % group, tokens - 1), runs = 256 / group;
     float m = -INFINITY, s = 0.f;
-    for (uint32_t p = threadIdx.x / 16; p < nparts; p += 16) {
+    for (uint32_t p = threadIdx.x / group; p < nparts; p += runs) {
       const float2 v = parts[p * part_stride + mine];
       join_stats(m, s, v.x, v.y);
     }
-#pragma unroll
-    for (int off = 16; off < 64; off <<= 1)
+    for (uint32_t off = group; off < 64; off <<= 1)
       join_stats(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
-    if (lane < 16) s_part[wave][lane] = make_float2(m, s);
-    float dot[4];
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      const uint32_t token = t0 + 4 * wave + i;
-      dot[i] = 0.f;
-      if (token < tokens && (uint32_t)targets[token] < table.rows) {
-        const T *xr = (const T *)x.p + token * x.ld,
-                *er = (const T *)table.p + (uint64_t)(uint32_t)targets[token] * table.ld;
+    if (lane < group) s_part[wave][lane] = make_float2(m, s);
+    __syncthreads();
+    for (uint32_t i = wave; i < group; i += 4) {
+      const uint32_t token = t0 + i;
+      if (token >= tokens) break;
+      const uint32_t target = (uint32_t)targets[token];
+      float dot = 0.f;
+      if (target < table.rows) {
+        const T *xr = (const T *)x.p + token * x.ld, *er = (const T *)table.p + target * table.ld;
         for (uint32_t c = lane; c < x.cols; c += 64) {
           float u[1], v[1];
           load_f32<T, 1>(xr + c, u);
           load_f32<T, 1>(er + c, v);
-          dot[i] = fmaf(u[0], v[0], dot[i]);
+          dot = fmaf(u[0], v[0], dot);
         }
       }
-    }
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1)
+      for (int off = 1; off < 64; off <<= 1) dot += __shfl_xor(dot, off, 64);
+      float2 v = s_part[0][i];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) dot[i] += __shfl_xor(dot[i], off, 64);
-    __syncthreads();
-    const uint32_t token = t0 + 4 * wave + lane;
-    if (lane < 4 && token < tokens) {
-      float2 v = s_part[0][4 * wave + lane];
-#pragma unroll
-      for (int k = 1; k < 4; ++k)
-        join_stats(v.x, v.y, s_part[k][4 * wave + lane].x, s_part[k][4 * wave + lane].y);
-      const float z = scale * (lane == 0 ? dot[0] : lane == 1 ? dot[1] : lane == 2 ? dot[2] : dot[3]);
+      for (int k = 1; k < 4; ++k) join_stats(v.x, v.y, s_part[k][i].x, s_part[k][i].y);
       const float all = (v.x + log2f(v.y)) * kLn2;
-      lse[token] = all;
-      loss[token] = (uint32_t)targets[token] < table.rows ? all - z : 0.f;
+      if (lane == 0) {
+        lse[token] = all;
+        loss[token] = target < table.rows ? all - scale * dot : 0.f;
+      }
     }
     __syncthreads();
   }
 }
 
-// A piece's d, as D.
+// A piece's d, as D, for a lane's four tokens.
 template <typename Logits, typename D>
-__global__ __launch_bounds__(256, 2) void k_loss_d(LogitDev a) {
-  __shared__ typename Logits::Lds lds;
-  uint32_t ttile, first, last;
-  if (!logit_item(a, ttile, first, last)) return;
-  const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
-  const uint32_t token0 = ttile * kTile + 64 * wm + l;
+struct Derivatives {
+  typedef typename Logits::Prod Prod;
+  const LogitDev &a;
+  const uint32_t token0;
   float lse2[4], weight[4];
   uint32_t target[4];  // in the piece
   bool counts[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t token = token0 + 16 * i;
-    lse2[i] = weight[i] = 0.f;
-    target[i] = ~0u;
-    counts[i] = token < a.x.rows && (uint32_t)a.targets[token] < a.vocabulary;
-    if (counts[i]) {
-      lse2[i] = a.lse[token] * kLog2e;
-      weight[i] = a.dloss[token] * a.scale;
-      target[i] = (uint32_t)a.targets[token] - a.row0;
-    }
-  }
-  Logits::walk(a, lds, ttile, first, last, [&](f32x4(&z)[4][4], uint32_t tile) {
-    const uint32_t v0 = tile * kTile + 64 * wn + 16 * g;
-    const bool ragged = (tile + 1) * kTile > a.e.rows;
+
+  __device__ __forceinline__ Derivatives(const LogitDev &args, uint32_t ttile)
+      : a(args), token0(ttile * kTile + Prod::first_m() + (threadIdx.x & 15u)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t hit = target[i] - v0;
-      float d[16];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float p = exp2_fast(fmaf(z[i][j][r], a.scale2, -lse2[i]));
-          if (hit == 4 * j + r) p -= 1.f;
-          const bool in = counts[i] && (!ragged || v0 + 4 * j + r < a.e.rows);
-          d[4 * j + r] = in ? p * weight[i] : 0.f;
-        }
-      if (!Logits::kDirect && token0 + 16 * i >= a.x.rows) continue;
-      D *const out = (D *)a.d + (uint64_t)(token0 + 16 * i) * a.d_ld + v0;
-      constexpr int V = kWide<D>;
-#pragma unroll
-      for (int k = 0; k < 16; k += V) {
-        float o[V];
-#pragma unroll
-        for (int q = 0; q < V; ++q) o[q] = d[k + q];
-        store_f32<D, V>(out + k, o);
+      const uint32_t token = token0 + 16 * i;
+      lse2[i] = weight[i] = 0.f;
+      target[i] = ~0u;
+      counts[i] = token < a.tokens && (uint32_t)a.targets[token] < a.vocabulary;
+      if (counts[i]) {
+        lse2[i] = a.lse[token] * kLog2e;
+        weight[i] = a.dloss[token] * a.scale;
+        target[i] = (uint32_t)a.targets[token] - a.row0;
       }
     }
-  });
+  }
+  // no column past the end, no token's target, and no token that does not count
+  // (whose row is zeros where tiles go straight to LDS, and so is its d)
+  __device__ __forceinline__ bool plain(uint32_t tile) const {
+    bool special = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      special |= target[i] - tile * Prod::kN < Prod::kN || (!Logits::kDirect && !counts[i]);
+    return (tile + 1) * Prod::kN <= a.e.rows && !__any(special);
+  }
+  __device__ __forceinline__ void values(const typename Prod::Sum &z, int i,
+                                         float (&d)[4 * Prod::kNT]) const {
+#pragma unroll
+    for (int j = 0; j < Prod::kNT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        d[4 * j + r] = exp2_fast(fmaf(z[i][j][r], a.scale2, -lse2[i])) * weight[i];
+  }
+  // 16 bytes a lane, the four lanes of a row beside each other
+  __device__ __forceinline__ void store(uint32_t tile, int i, const float (&d)[4 * Prod::kNT]) const {
+    if (!Logits::kDirect && token0 + 16 * i >= a.x.rows) return;
+    D *const out = (D *)a.d + (uint64_t)(token0 + 16 * i) * a.d_ld + tile * Prod::kN;
+    constexpr int V = kWide<D>;
+#pragma unroll
+    for (int k = 0; k < 4 * Prod::kNT; k += V) {
+      float o[V];
+#pragma unroll
+      for (int q = 0; q < V; ++q) o[q] = d[k + q];
+      store_f32<D, V>(out + Prod::column(k / 4), o);
+    }
+  }
+  __device__ __forceinline__ void part(const typename Prod::Sum &z, uint32_t tile, int i) const {
+    float d[4 * Prod::kNT];
+    values(z, i, d);
+    store(tile, i, d);
+  }
+  __device__ __forceinline__ void whole(const typename Prod::Sum &z, uint32_t tile) const {
+    const bool simple = plain(tile);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float d[4 * Prod::kNT];
+      values(z, i, d);
+      if (!simple) {
+#pragma unroll
+        for (int j = 0; j < Prod::kNT; ++j) {
+          const uint32_t v = tile * Prod::kN + Prod::column(j);
+#pragma unroll
+          for (uint32_t r = 0; r < 4; ++r) {
+            if (target[i] == v + r)
+              d[4 * j + r] =
+                  (exp2_fast(fmaf(z[i][j][r], a.scale2, -lse2[i])) - 1.f) * weight[i];
+            if (!counts[i] || v + r >= a.e.rows) d[4 * j + r] = 0.f;
+          }
+        }
+      }
+      store(tile, i, d);
+    }
+  }
+};
+
+template <typename Logits, typename D>
+__global__ __launch_bounds__(256, 2) void k_loss_d(LogitDev a) {
+  __shared__ typename Logits::Lds lds;
+  uint32_t ttile, sweep, first, last;
+  if (!logit_item<Logits::Prod::kN>(a, ttile, sweep, first, last)) return;
+  Derivatives<Logits, D> o(a, ttile);
+  Logits::walk(a, lds, ttile, first, last, o);
 }
 
 // ---- the products of d
@@ -337,7 +464,7 @@ struct ProductDev {
   float *sums;           // [splits][rows][sums_ld], null: out is written
   uint64_t sums_split, sums_ld;
   uint32_t add;          // to what sums holds
-  const int32_t *targets;  // of n's rows, null: all count
+  const int32_t *targets;  // dE through registers: of n's rows
   uint32_t vocabulary;
 };
 
@@ -411,10 +538,10 @@ struct StagedProduct {
       const uint32_t mr = kMCol ? k : m0, mc = kMCol ? m0 : k;
       sm.fetch((const TM *)a.m.p + (uint64_t)mr * a.m.ld + mc, a.m.ld,
                (kMCol ? a.terms : a.m.rows) - mr, (kMCol ? a.m.cols : a.terms) - mc,
-               [](uint32_t) { return true; });
+               [](uint32_t) { return 0u; });
       sn.fetch((const TN *)a.n.p + (uint64_t)k * a.n.ld + n0, a.n.ld, a.terms - k, a.n.cols - n0,
                [&](uint32_t r) {
-                 return !a.targets || (uint32_t)a.targets[min(k + r, a.terms - 1)] < a.vocabulary;
+                 return kMCol ? (uint32_t)a.targets[min(k + r, a.terms - 1)] : 0u;
                });
       k += kTerms;
     };
@@ -422,8 +549,10 @@ struct StagedProduct {
     if (it.k0 < it.k1) fetch();
     for (uint32_t s = it.k0; s < it.k1; s += kTerms) {
       __syncthreads();
-      sm.template put<Prod::kM, kTerms, kMCol, PM>(lds.m, Prod::kMPlane);
-      sn.template put<Prod::kN, kTerms, true, PN>(lds.n, Prod::kNPlane);
+      sm.template put<Prod::kM, kTerms, kMCol, PM>(lds.m, Prod::kMPlane,
+                                                     [](uint32_t) { return true; });
+      sn.template put<Prod::kN, kTerms, true, PN>(
+          lds.n, Prod::kNPlane, [&](uint32_t target) { return !kMCol || target < a.vocabulary; });
       __syncthreads();
       if (k < it.k1) fetch();
       Prod::add(sum, lds);
@@ -433,43 +562,47 @@ struct StagedProduct {
 };
 
 // Straight to LDS: bfloat16, M and N whole tiles (rows of N past its end are its
-// last again, and meet zeros of M).
-template <int NT, bool kMCol>
+// last again, and meet zeros of M).  Of three places in LDS one is read and two are
+// under way, for d comes from beyond the L2 caches.
+template <int WM, int WN, int MT, bool kMCol>
 struct DirectProduct {
-  typedef Product<2, 2, 4, NT, 64, 1, 1, kMCol, true, false> Prod;
+  static constexpr uint32_t kTerms = 64, kPlaces = 3;
+  typedef Product<WM, WN, MT, 4, kTerms, 1, 1, kMCol, true, false> Prod;
   struct Lds {
-    typename Prod::Lds buf[2];
+    typename Prod::Lds buf[kPlaces];
   };
 
   static __device__ __forceinline__ void run(const ProductDev &a, Lds &lds, uint32_t w) {
     const ProductItem it = product_item(a, w);
     const uint32_t m0 = it.mt * Prod::kM, n0 = it.nt * Prod::kN;
-    Feed<Prod::kM, 64, kMCol, 256> fm;
-    Feed<Prod::kN, 64, true, 256> fn;
+    Feed<Prod::kM, kTerms, kMCol, Prod::kThreads> fm;
+    Feed<Prod::kN, kTerms, true, Prod::kThreads> fn;
+    constexpr int kCopies = fm.kPer + fn.kPer;
     const bf16 *const m = (const bf16 *)a.m.p + (kMCol ? m0 : (uint64_t)m0 * a.m.ld);
     const bf16 *const n = (const bf16 *)a.n.p + n0;
-    fm.start(m, a.m.ld, ~0u);
-    fn.start(n, a.n.ld, ~0u);
-    uint32_t k = it.k0, buf = 0;
-    const auto issue = [&](uint32_t b) {
-      fm.issue(lds.buf[b].m, kMCol ? (uint64_t)k * a.m.ld : k);
-      if (k + 64 > a.n.rows) {
-        fn.start(n + (uint64_t)k * a.n.ld, a.n.ld, a.n.rows - k);
-        fn.issue(lds.buf[b].n, 0);
-      } else {
-        fn.issue(lds.buf[b].n, (uint64_t)k * a.n.ld);
-      }
-      k += 64;
+    fm.start(a.m.ld, ~0u);
+    fn.start(a.n.ld, ~0u);
+    uint32_t k = it.k0, to = 0, buf = 0;
+    const auto issue = [&] {  // past the end the last stage again: counts stay the same
+      const uint32_t at = min(k, (it.k1 - 1) & ~(kTerms - 1));
+      if (at + kTerms > a.n.rows) fn.start(a.n.ld, a.n.rows - at);
+      fm.issue(lds.buf[to].m, m + (kMCol ? (uint64_t)at * a.m.ld : at));
+      fn.issue(lds.buf[to].n, n + (uint64_t)at * a.n.ld);
+      k += kTerms;
+      to = to + 1 < kPlaces ? to + 1 : 0;
     };
     typename Prod::Sum sum = {};
-    if (it.k0 < it.k1) issue(0);
-    for (uint32_t s = it.k0; s < it.k1; s += 64) {
-      wait_loads();
-      __syncthreads();
-      Prod::add_then(sum, lds.buf[buf], [&] {
-        if (k < it.k1) issue(buf ^ 1);
-      });
-      buf ^= 1;
+    if (it.k0 < it.k1) {
+      issue();
+      issue();
+      for (uint32_t s = it.k0; s < it.k1; s += kTerms) {
+        landed<kCopies>();
+        __syncthreads();  // the stage before is done with: its place takes the next
+        issue();
+        Prod::add(sum, lds.buf[buf]);
+        buf = buf + 1 < kPlaces ? buf + 1 : 0;
+      }
+      landed<0>();
     }
     put_result<Prod>(a, sum, m0, n0, it.split);
   }
@@ -503,21 +636,18 @@ __global__ __launch_bounds__(256, 2) void k_loss_products(ProductDev dx, Product
   else
     E::run(de, lds.e, w);
 }
-template <int NT>
-__global__ __launch_bounds__(256, 2) void k_loss_products_direct(ProductDev dx, ProductDev de) {
-  typedef DirectProduct<NT, false> X;
-  typedef DirectProduct<NT, true> E;
-  __shared__ union {
-    typename X::Lds x;
-    typename E::Lds e;
-  } lds;
+template <int WM, int WN, int MT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_loss_products_direct(ProductDev dx, ProductDev de) {
+  typedef DirectProduct<WM, WN, MT, false> X;
+  typedef DirectProduct<WM, WN, MT, true> E;
+  extern __shared__ __attribute__((aligned(16))) char s_raw[];
   uint32_t w;
   bool is_dx;
   if (!product_work(dx, de, w, is_dx)) return;
   if (is_dx)
-    X::run(dx, lds.x, w);
+    X::run(dx, *(typename X::Lds *)s_raw, w);
   else
-    E::run(de, lds.e, w);
+    E::run(de, *(typename E::Lds *)s_raw, w);
 }
 
 // x as whole tiles of rows for the copies straight to LDS: zeros past the end
@@ -574,12 +704,20 @@ uint32_t grid_of(uint64_t threads) {
 }
 uint32_t xcd_grid(uint64_t work) { return (uint32_t)((work + 7) / 8 * 8); }
 
-// Vocabulary tiles a workgroup takes one after another, and such sweeps: enough
-// workgroups to fill the chip several times, few parts for each token.
+// Vocabulary tiles a workgroup takes one after another, and such sweeps: the
+// least time for rounds of 512 workgroups, which need about as long to begin as
+// for XX tiles.  us with sweeps of 2 and of 8 tiles (16,384 tokens x 4,096 rows,
+// width 256): YY.
 void plan_sweeps(uint32_t ttiles, uint32_t vtiles, uint32_t &sweep, uint32_t &sweeps) {
-  const uint64_t tiles = (uint64_t)ttiles * vtiles, most = 1u << 23;  // workgroups of a launch
-  sweep = (uint32_t)std::max(std::min<uint64_t>({vtiles, 16, std::max<uint64_t>(1, tiles / 2048)}),
-                             std::min<uint64_t>(vtiles, host_ceil_div(tiles, most)));
+  uint64_t best = ~0ull;
+  const uint64_t most = 1u << 23;  // workgroups of a launch
+  for (uint64_t s = 1; s <= vtiles; s = s < 64 ? s + 1 : 2 * s) {
+    const uint64_t work = ttiles * host_ceil_div(vtiles, s),
+                   cost = host_ceil_div(work, 512) * (2 * s + 3);
+    if (s > 1 && (cost >= best || s > 64) && ttiles * host_ceil_div(vtiles, sweep) <= most) continue;
+    best = cost;
+    sweep = (uint32_t)s;
+  }
   sweeps = (vtiles + sweep - 1) / sweep;
 }
 
@@ -596,42 +734,67 @@ LossPlan loss_plan(const nsfps_loss_args &a) {
   return p;
 }
 
-// kDirect of a call hangs on its addresses, the workspace does not: it has room
-// for either.
+constexpr uint32_t kPad = 256;  // of tokens and pieces: whole tiles of any kind
+
+// Whether a call's tiles go straight to LDS hangs on its addresses, the workspace
+// does not: it has room for either.
 struct GradPlan {
   uint64_t tokens;             // padded
-  uint64_t piece, pieces;      // vocabulary rows of a piece, a multiple of kTile
-  uint32_t nt;                 // columns of a product's tile
+  uint64_t piece, pieces;      // vocabulary rows of a piece, a multiple of kPad
+  uint32_t mt, nt;             // rows and columns of a product's tile
   uint32_t per, dx_splits, de_splits;
-  uint64_t d_size;
-  bool dx_sums, de_sums;
+  uint64_t d_size, d_ld;       // (rows a whole number of 4 KB apart meet in one memory channel)
+  bool direct, dx_sums, de_sums;
   uint64_t x, d, dx, de, bytes;  // workspace offsets
 };
-GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype) {
+// k of a split, of both products alike.  at_once workgroups run at once and take 1
+// us for 64 terms of a pass; splits' sums go to memory and come back, 4 TB/s.  The
+// split with the least of both: 16,384 tokens and pieces of 4,096 rows, width 384
+// in float32, XX with it and YY with as many splits as just fill the chip.
+void plan_splits(GradPlan &p, uint64_t dx_tiles, uint64_t dx_terms, uint64_t de_tiles,
+                 uint64_t de_terms, uint32_t passes, uint64_t at_once, uint64_t dx_bytes,
+                 uint64_t de_bytes) {
+  double best = 0.;
+  for (uint64_t n = 1; n <= 512; ++n) {
+    const uint64_t per = up(host_ceil_div(std::max(dx_terms, de_terms), n), 64);
+    if (n > 1 && per < 256) break;
+    const uint64_t dx = host_ceil_div(dx_terms, per), de = host_ceil_div(de_terms, per);
+    const double rounds = (double)host_ceil_div(dx_tiles * dx + de_tiles * de, at_once);
+    const double longest = (double)std::min(per, std::max(dx_terms, de_terms));
+    const double sums = (dx > 1 || p.pieces > 1 ? 2. * dx * dx_bytes : 0.) +
+                        (de > 1 ? 2. * de * de_bytes : 0.);
+    const double us = rounds * longest / 64. * passes + sums / 4e6;
+    if (n == 1 || us < best) {
+      best = us;
+      p.per = (uint32_t)per;
+      p.dx_splits = (uint32_t)dx;
+      p.de_splits = (uint32_t)de;
+    }
+  }
+}
+
+GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype, bool direct) {
   GradPlan p = {};
-  p.tokens = up(a.tokens, kTile);
-  const uint64_t whole = up(a.rows, kTile);
+  p.tokens = up(a.tokens, kPad);
+  const uint64_t whole = up(a.rows, kPad);
   p.bytes = 256;
   if (!p.tokens || !whole) return p;
   const bool one = a.dtype == NSFPS_BF16 && grad_dtype == NSFPS_BF16;
   p.d_size = one ? 2 : 4;
   // a piece of d: 64 million values, and 1,024 rows at least
   constexpr uint64_t kValues = 1ull << 26;
-  p.piece = std::min(whole, std::max<uint64_t>(1024, kValues / p.tokens / kTile * kTile));
+  p.piece = std::min(whole, std::max<uint64_t>(1024, kValues / p.tokens / kPad * kPad));
   p.pieces = host_ceil_div(whole, p.piece);
-  p.nt = a.width <= 64 ? 64 : 128;
-  // k of a split: enough splits of both products to fill the chip
-  const uint64_t ntiles = host_ceil_div(a.width, p.nt), dx_tiles = p.tokens / kTile * ntiles,
-                 de_tiles = p.piece / kTile * ntiles,
-                 dx_terms = std::min(p.piece, a.rows);
-  constexpr uint64_t kFill = 512, kLeast = 256;
-  p.per = (uint32_t)std::max(
-      kLeast, up(host_ceil_div(dx_tiles * dx_terms + de_tiles * a.tokens, kFill), 64));
-  p.dx_splits = (uint32_t)host_ceil_div(dx_terms, p.per);
-  p.de_splits = (uint32_t)host_ceil_div(a.tokens, p.per);
+  p.direct = direct;
+  p.nt = direct ? (a.width % 256 == 0 ? 256 : a.width % 128 == 0 ? 128 : 64)
+                : a.width <= 64 ? 64 : 128;
+  p.mt = direct && p.nt < 256 ? 256 : kTile;
+  const uint64_t ntiles = host_ceil_div(a.width, p.nt), ld = ntiles * p.nt;
+  plan_splits(p, p.tokens / p.mt * ntiles, std::min(p.piece, a.rows), p.piece / p.mt * ntiles,
+              a.tokens, a.dtype == NSFPS_F32 ? 6 : one ? 1 : 2, direct ? 256 : 512,
+              4 * a.tokens * ld, 4 * p.piece * ld);
   p.dx_sums = p.dx_splits > 1 || p.pieces > 1;
   p.de_sums = p.de_splits > 1;
-  const uint64_t ld = ntiles * p.nt;
   uint64_t at = 0;
   const auto take = [&](uint64_t n) {
     const uint64_t was = at;
@@ -639,7 +802,8 @@ GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype) {
     return was;
   };
   p.x = take(one ? 2 * p.tokens * a.width : 0);
-  p.d = take(p.d_size * p.tokens * p.piece);
+  p.d_ld = p.piece + 256 / p.d_size;
+  p.d = take(p.d_size * p.tokens * p.d_ld);
   p.dx = take(p.dx_sums ? 4 * p.dx_splits * a.tokens * ld : 0);
   p.de = take(p.de_sums ? 4 * p.de_splits * p.piece * ld : 0);
   p.bytes = at;
@@ -650,7 +814,20 @@ GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype) {
 // boundaries.
 bool direct_rows(const nsfps_loss_args &a) {
   return a.dtype == NSFPS_BF16 && a.width % 64 == 0 && a.x_stride % 8 == 0 &&
-         a.table_stride % 8 == 0 && ((uintptr_t)a.d_x | (uintptr_t)a.d_table) % 16 == 0;
+         a.table_stride % 8 == 0 && ((uintptr_t)a.d_x | (uintptr_t)a.d_table) % 16 == 0 &&
+         std::max(a.x_stride, a.table_stride) < 1u << 23;  // (a Feed's offsets)
+}
+
+// f(the walk of tiles straight to LDS)
+template <typename F>
+void by_steps(uint32_t width, F f) {
+  switch (width) {
+    case 64: return f(ResidentLogits<64, 1>());
+    case 128: return f(ResidentLogits<128, 1>());
+    case 192: return f(ResidentLogits<64, 3>());
+    case 256: return f(ResidentLogits<128, 2>());
+    default: return f(DirectLogits());
+  }
 }
 
 LogitDev logits(const nsfps_loss_args &a, uint64_t row0, uint64_t rows) {
@@ -659,6 +836,7 @@ LogitDev logits(const nsfps_loss_args &a, uint64_t row0, uint64_t rows) {
   d.x = {a.d_x, a.x_stride, (uint32_t)a.tokens, a.width};
   d.e = {(const char *)a.d_table + row0 * a.table_stride * size, a.table_stride, (uint32_t)rows,
          a.width};
+  d.tokens = (uint32_t)a.tokens;
   d.ttiles = (uint32_t)host_ceil_div(a.tokens, kTile);
   d.vtiles = (uint32_t)host_ceil_div(rows, kTile);
   plan_sweeps(d.ttiles, d.vtiles, d.sweep, d.sweeps);
@@ -669,6 +847,18 @@ LogitDev logits(const nsfps_loss_args &a, uint64_t row0, uint64_t rows) {
   d.targets = a.d_targets;
   d.lse = a.d_lse;
   return d;
+}
+
+template <int WM, int WN, int MT>
+hipError_t run_direct(const ProductDev &dx, const ProductDev &de, uint32_t grid, hipStream_t st) {
+  typedef DirectProduct<WM, WN, MT, false> X;
+  constexpr size_t lds = sizeof(typename X::Lds);
+  static_assert(lds == sizeof(typename DirectProduct<WM, WN, MT, true>::Lds) && lds <= 160 * 1024, "LDS");
+  const hipError_t e = hipFuncSetAttribute((const void *)k_loss_products_direct<WM, WN, MT>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (e != hipSuccess) return e;
+  k_loss_products_direct<WM, WN, MT><<<grid, X::Prod::kThreads, lds, st>>>(dx, de);
+  return hipGetLastError();
 }
 
 template <typename T>
@@ -723,16 +913,19 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
     d.part_stride = stride;
     const uint32_t grid = xcd_grid((uint64_t)d.ttiles * d.sweeps);
     if (direct_rows(a))
-      k_loss_stats<DirectLogits><<<grid, 256, 0, st>>>(d);
+      by_steps(a.width, [&](auto z) { k_loss_stats<decltype(z)><<<grid, 256, 0, st>>>(d); });
     else if (a.dtype == NSFPS_F32)
-      k_loss_stats<StagedLogits<float, 3>><<<grid, 256, 0, st>>>(d);
+      k_loss_stats<StagedLogits<float, 3, false>><<<grid, 256, 0, st>>>(d);
     else
-      k_loss_stats<StagedLogits<bf16, 1>><<<grid, 256, 0, st>>>(d);
+      k_loss_stats<StagedLogits<bf16, 1, true>><<<grid, 256, 0, st>>>(d);
     LAUNCH(hipGetLastError());
   }
   const auto join = [&](auto t) {
-    k_loss_join<decltype(t)><<<grid_of(a.tokens * 16), 256, 0, st>>>(
-        parts, p.sweeps, stride, Matrix{a.d_x, a.x_stride, (uint32_t)a.tokens, a.width},
+    uint32_t group = 16;  // as many workgroups as fill the chip
+    while (group > 1 && a.tokens / group < 256) group /= 2;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(1u << 16, host_ceil_div(a.tokens, group));
+    k_loss_join<decltype(t)><<<grid, 256, 0, st>>>(
+        parts, p.sweeps, stride, group, Matrix{a.d_x, a.x_stride, (uint32_t)a.tokens, a.width},
         Matrix{a.d_table, a.table_stride, (uint32_t)a.rows, a.width}, a.scale, a.d_targets, a.d_loss,
         a.d_lse);
     return hipGetLastError();
@@ -741,17 +934,19 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
 }
 
 uint64_t loss_grad_bytes(const nsfps_loss_args &a, const nsfps_loss_grads &g) {
-  return grad_plan(a, g.grad_dtype).bytes;
+  return std::max(grad_plan(a, g.grad_dtype, false).bytes, grad_plan(a, g.grad_dtype, true).bytes);
 }
 
 hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g, hipStream_t st) {
-  const GradPlan p = grad_plan(a, g.grad_dtype);
+  // (tokens are padded to whole tiles there, which few would pay for)
+  const bool direct = g.grad_dtype == NSFPS_BF16 && a.tokens >= kPad && direct_rows(a);
+  const GradPlan p = grad_plan(a, g.grad_dtype, direct);
   if (!p.pieces) {
     LAUNCH(write_zeros(a.dtype, g.d_dx, g.dx_stride, a.tokens, a.width, st));
     return write_zeros(g.grad_dtype, g.d_dtable, g.dtable_stride, a.rows, a.width, st);
   }
   char *const ws = (char *)a.workspace;
-  const bool one = p.d_size == 2, direct = one && direct_rows(a);
+  const bool one = p.d_size == 2;
   const uint32_t ntiles = (uint32_t)host_ceil_div(a.width, p.nt);
   const uint64_t z = g.grad_dtype == NSFPS_F32 ? 4 : 2;
   const Matrix x = {a.d_x, a.x_stride, (uint32_t)a.tokens, a.width};
@@ -761,7 +956,7 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     LAUNCH(hipGetLastError());
   }
   ProductDev dx = {};
-  dx.mtiles = (uint32_t)(p.tokens / kTile);
+  dx.mtiles = (uint32_t)host_ceil_div(a.tokens, p.mt);
   dx.ntiles = ntiles;
   dx.per = p.per;
   dx.out = g.d_dx;
@@ -778,19 +973,25 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     LogitDev l = logits(a, row0, rows);
     l.dloss = g.d_dloss;
     l.d = ws + p.d;
-    l.d_ld = p.piece;
+    l.d_ld = p.d_ld;
+    if (direct) {  // whole tiles of every product
+      l.x = {ws + p.x, a.width, (uint32_t)p.tokens, a.width};
+      l.ttiles = (uint32_t)(p.tokens / kTile);
+      l.vtiles = (uint32_t)(up(rows, kPad) / kTile);
+      plan_sweeps(l.ttiles, l.vtiles, l.sweep, l.sweeps);
+    }
     const uint32_t grid = xcd_grid((uint64_t)l.ttiles * l.sweeps);
     if (direct)
-      k_loss_d<DirectLogits, bf16><<<grid, 256, 0, st>>>(l);
+      by_steps(a.width, [&](auto z) { k_loss_d<decltype(z), bf16><<<grid, 256, 0, st>>>(l); });
     else if (a.dtype == NSFPS_F32)
-      k_loss_d<StagedLogits<float, 3>, float><<<grid, 256, 0, st>>>(l);
+      k_loss_d<StagedLogits<float, 3, false>, float><<<grid, 256, 0, st>>>(l);
     else if (one)
-      k_loss_d<StagedLogits<bf16, 1>, bf16><<<grid, 256, 0, st>>>(l);
+      k_loss_d<StagedLogits<bf16, 1, true>, bf16><<<grid, 256, 0, st>>>(l);
     else
-      k_loss_d<StagedLogits<bf16, 1>, float><<<grid, 256, 0, st>>>(l);
+      k_loss_d<StagedLogits<bf16, 1, false>, float><<<grid, 256, 0, st>>>(l);
     LAUNCH(hipGetLastError());
 
-    const Matrix d = {ws + p.d, p.piece, (uint32_t)(direct ? p.tokens : a.tokens), (uint32_t)rows};
+    const Matrix d = {ws + p.d, p.d_ld, (uint32_t)(direct ? p.tokens : a.tokens), (uint32_t)rows};
     dx.m = d;
     dx.n = l.e;
     dx.terms = (uint32_t)rows;
@@ -798,9 +999,9 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     dx.add = k > 0;
     ProductDev de = dx;
     de.n = direct ? Matrix{ws + p.x, a.width, (uint32_t)p.tokens, a.width} : x;
-    de.targets = direct ? nullptr : a.d_targets;
+    de.targets = a.d_targets;
     de.vocabulary = (uint32_t)a.rows;
-    de.mtiles = (uint32_t)host_ceil_div(rows, kTile);
+    de.mtiles = (uint32_t)host_ceil_div(rows, p.mt);
     de.terms = (uint32_t)a.tokens;
     de.splits = p.de_splits;
     de.out = (char *)g.d_dtable + row0 * g.dtable_stride * z;
@@ -813,11 +1014,9 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     de.add = 0;
     const uint32_t work = xcd_grid((uint64_t)dx.mtiles * ntiles * dx.splits +
                                    (uint64_t)de.mtiles * ntiles * de.splits);
-    const auto products = [&](auto nt) {
+    const auto staged = [&](auto nt) {
       constexpr int NT = decltype(nt)::value;
-      if (direct)
-        k_loss_products_direct<NT><<<work, 256, 0, st>>>(dx, de);
-      else if (a.dtype == NSFPS_F32)
+      if (a.dtype == NSFPS_F32)
         k_loss_products<float, 3, 3, float, 3, NT><<<work, 256, 0, st>>>(dx, de);
       else if (one)
         k_loss_products<bf16, 1, 1, bf16, 1, NT><<<work, 256, 0, st>>>(dx, de);
@@ -825,8 +1024,12 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
         k_loss_products<float, 1, 2, bf16, 1, NT><<<work, 256, 0, st>>>(dx, de);
       return hipGetLastError();
     };
-    LAUNCH(p.nt == 64 ? products(std::integral_constant<int, 2>())
-                      : products(std::integral_constant<int, 4>()));
+    const hipError_t e = p.nt == 256             ? run_direct<2, 4, 4>(dx, de, work, st)
+                         : direct && p.nt == 128 ? run_direct<4, 2, 4>(dx, de, work, st)
+                         : direct                ? run_direct<4, 1, 4>(dx, de, work, st)
+                         : p.nt == 64            ? staged(std::integral_constant<int, 2>())
+                                                 : staged(std::integral_constant<int, 4>());
+    LAUNCH(e);
     if (de.sums) LAUNCH(write_out(de, st));
   }
   return dx.sums ? write_out(dx, st) : hipSuccess;
@@ -834,7 +1037,7 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
 
 hipError_t preload_loss_kernels() {
   return func_attributes(k_loss_stats<DirectLogits>, k_loss_join<bf16>, k_loss_d<DirectLogits, bf16>,
-                         k_loss_products_direct<4>, k_loss_out<bf16, 8>, k_loss_rows);
+                         k_loss_products_direct<2, 4, 4>, k_loss_out<bf16, 8>, k_loss_rows);
 }
 
 }  // namespace nsfps

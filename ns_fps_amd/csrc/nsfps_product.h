@@ -16,8 +16,8 @@
 //
 // Lane layout, with g = lane / 16, l = lane % 16: an operand of 32 terms holds
 // row l, terms 8g .. 8g + 7; a tile of sums holds row m = l, columns n = 4g .. 4g
-// + 3.  kPerm (four column tiles): column 4g + r of tile nt stands for column 16g
-// + 4nt + r of the wave's 64, so that a lane's 16 sums of a row are neighbours.
+// + 3.  kPerm: column 4g + r of the tiles 2t and 2t + 1 stands for columns 32t + 8g
+// + r and + 4 + r, so that a lane has eight neighbours: 16 bytes of bfloat16.
 #pragma once
 
 #include "nsfps_mfma.h"
@@ -27,16 +27,17 @@
 namespace nsfps {
 namespace seq {
 
-// The number that exchanges the pieces of a row of kTerms terms (Row): the rows
-// 0 .. 15, and the rows 16a + 4c + b (a, b < 4), meet no bank twice, taken 8 or
-// 16 at a time.
+// The number that exchanges the pieces of a row of kTerms terms (Row).  A 16-byte
+// read takes 16 lanes at a time, rows 0 .. 3 and 12 .. 15 of one piece and rows 4
+// .. 11 of the next one (then the other way round), over 256 bytes of banks.  One,
+// two or four rows lie in those, so the others' bits have to give the piece, and
+// with the pieces' own difference: counted, no read meets a bank twice, be its rows 0 ..
+// 15 or (kPerm) 8a + 4c + b (a, b < 4).
 template <int kTerms>
 __device__ __forceinline__ uint32_t row_turn(uint32_t r) {
-  static_assert(kTerms == 64 || kTerms == 32, "terms of a stage");
-  if constexpr (kTerms == 64)
-    return ((2 * ((r >> 2) + (r >> 4)) + ((r >> 1) & 1)) ^ ((r & 1) << 2)) & 7;
-  else
-    return ((r >> 2) + (r >> 4) + (r & 2)) & 3;
+  static_assert(kTerms == 128 || kTerms == 64 || kTerms == 32, "terms of a stage");
+  const uint32_t b3 = (r >> 3) & 1;
+  return kTerms == 128 ? 9 * b3 | (r & 2) | (r & 1) << 2 : kTerms == 64 ? 5 * b3 | (r & 2) : 2 * b3;
 }
 // Col, T columns a row: pairs of pieces (16 columns); rows 8g + i (g, i < 4).
 template <int T>
@@ -76,37 +77,51 @@ __device__ __forceinline__ bf16x8 read_col(const bf16 *tile, uint32_t c, uint32_
 
 // A tile straight from memory to LDS, 64 pieces of 16 bytes an instruction in
 // the order of the lanes: the pieces' exchange is in the addresses.  Pieces are
-// whole; memory rows past the last are the last one again.
+// whole; memory rows past the last are the last one again.  Rows lie less than
+// 2^23 values apart, so that a lane's place is a 32-bit offset from a base that
+// all lanes share.
+//
+// The copies are written as instructions: the compiler, which takes every read of
+// LDS behind such a copy for a read of what it brings, would wait for all of them
+// there, and a tile could only be asked for once the one before it is in
+// registers.  Nothing comes back to registers.  Whoever reads the tile waits
+// himself: landed<n>() and a barrier.
 template <int T, int kTerms, bool kCol, int kThreads>
 struct Feed {
-  static constexpr int kPer = T * kTerms / 8 / kThreads;
-  static_assert(kPer >= 1, "tile too small");
-  const bf16 *p[kPer];
+  static constexpr int kPer = T * kTerms / 8 / kThreads;  // copies a thread
+  static_assert(kPer >= 1 && T * kTerms / 8 % kThreads == 0, "tile and threads");
+  uint32_t at[kPer];  // bytes
 
-  // at: the tile's first value; rows: how many of memory there are (at least 1)
-  __device__ __forceinline__ void start(const bf16 *at, uint64_t ld, uint32_t rows) {
+  // rows: how many there are of memory from the tile's first on (at least 1)
+  __device__ __forceinline__ void start(uint64_t ld, uint32_t rows) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const uint32_t e = threadIdx.x + kThreads * i;
-      if constexpr (kCol) {
-        const uint32_t k = e / (T / 8);
-        p[i] = at + min(k, rows - 1) * ld + 8 * ((e % (T / 8)) ^ col_turn<T>(k));
-      } else {
-        const uint32_t r = e / (kTerms / 8);
-        p[i] = at + min(r, rows - 1) * ld + 8 * ((e % (kTerms / 8)) ^ row_turn<kTerms>(r));
-      }
+      constexpr uint32_t kVecs = kCol ? T / 8 : kTerms / 8;
+      const uint32_t r = e / kVecs, turn = kCol ? col_turn<T>(r) : row_turn<kTerms>(r);
+      at[i] = 2 * (min(r, rows - 1) * (uint32_t)ld + 8 * (e % kVecs ^ turn));
     }
   }
-  __device__ __forceinline__ void issue(bf16 *tile, uint64_t offset) const {
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // from: the tile's first value
+  __device__ __forceinline__ void issue(bf16 *tile, const bf16 *from) const {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) bf16 *)tile +
+        16 * (threadIdx.x & ~63u));
+    const uint64_t base = (uint64_t)from;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void *)(p[i] + offset),
-          (__attribute__((address_space(3))) void *)(tile + 8 * (64 * wave + kThreads * i)), 16, 0,
-          0);
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                   :
+                   : "v"(at[i]), "s"(base), "s"(to + 16 * kThreads * i)
+                   : "memory");
   }
 };
+// Waits until at most n of this wave's copies are under way.
+template <int n>
+__device__ __forceinline__ void landed() {
+  static_assert(n < 64, "counter");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
+}
 
 // Eight values of a row, at any address that holds such values.
 template <typename T>
@@ -151,12 +166,14 @@ struct Stage {
   static constexpr int kPer = ROWS * COLS / 8 / kThreads, kVecs = COLS / 8;
   static_assert(kPer >= 1, "tile too small");
   Eight<T> v[kPer];
+  uint32_t tag[kPer];  // of the pieces' rows
 
   // at: the tile's first value; rows, cols: how many of it are inside.
-  // counts(row): whether a row inside is wanted.
+  // tag_of(row): what put() decides by whether the row is wanted.  (Not here: a
+  // value that is used is waited for.)
   template <typename F>
   __device__ __forceinline__ void fetch(const T *at, uint64_t ld, uint32_t rows, uint32_t cols,
-                                        F counts) {
+                                        F tag_of) {
     const bool whole = rows >= (uint32_t)ROWS && cols >= (uint32_t)COLS;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -171,14 +188,15 @@ struct Stage {
         else if (r < rows && c < cols)
           v[i] = load_some<T>(p, cols - c);
       }
-      if (!counts(r)) v[i] = Eight<T>{};
+      tag[i] = tag_of(r);
     }
   }
   // kT: columns of a Col tile; plane: values of a plane in LDS
-  template <int kT, int kTerms, bool kCol, int P>
-  __device__ __forceinline__ void put(bf16 *tile, uint32_t plane) const {
+  template <int kT, int kTerms, bool kCol, int P, typename F>
+  __device__ __forceinline__ void put(bf16 *tile, uint32_t plane, F wanted) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
+      if (!wanted(tag[i])) v[i] = Eight<T>{};
       const uint32_t e = threadIdx.x + kThreads * i, r = e / kVecs, c = e % kVecs * 8;
       bf16 *const to = tile + piece_at<kT, kTerms, kCol>(r, c);
       if constexpr (sizeof(T) == 2) {
@@ -221,8 +239,9 @@ struct Passes<3, 3> {  // to 24 bits: what is left out is below 2^-24 of the pro
 template <int WM, int WN, int MT, int NT, int kTerms, int PM, int PN, bool kMCol, bool kNCol,
           bool kPerm>
 struct Product {
+  static constexpr int kMT = MT, kNT = NT;
   static constexpr int kM = 16 * WM * MT, kN = 16 * WN * NT, kThreads = 64 * WM * WN;
-  static_assert(!kPerm || (NT == 4 && !kNCol), "layout");
+  static_assert(!kPerm || (NT % 2 == 0 && !kNCol), "layout");
   static constexpr int kMPlane = kM * kTerms, kNPlane = kN * kTerms;
   struct alignas(16) Lds {
     bf16 m[PM * kMPlane], n[PN * kNPlane];
@@ -235,16 +254,20 @@ struct Product {
   static __device__ __forceinline__ uint32_t first_m() { return wave_id() / WN * (16 * MT); }
   static __device__ __forceinline__ uint32_t first_n() { return wave_id() % WN * (16 * NT); }
 
+  // the first of this lane's four columns of tile t
+  static __device__ __forceinline__ uint32_t column(int t) {
+    const uint32_t g = (threadIdx.x & 63u) >> 4;
+    return first_n() + (kPerm ? 32 * (t / 2) + 8 * g + 4 * (t % 2) : 16 * t + 4 * g);
+  }
   static __device__ __forceinline__ bf16x8 read_m(const Lds &lds, int p, int t, uint32_t kb) {
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u, m0 = first_m() + 16 * t;
     const bf16 *tile = lds.m + p * kMPlane;
     return kMCol ? read_col<kM>(tile, m0, kb, g, l) : read_row<kTerms>(tile, m0 + l, kb, g);
   }
-  static __device__ __forceinline__ bf16x8 read_n(const Lds &lds, int p, int t, uint32_t kb) {
+  static __device__ __forceinline__ bf16x8 read_n(const bf16 *tile, int t, uint32_t kb) {
     const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u, n0 = first_n();
-    const bf16 *tile = lds.n + p * kNPlane;
     return kNCol   ? read_col<kN>(tile, n0 + 16 * t, kb, g, l)
-           : kPerm ? read_row<kTerms>(tile, n0 + 16 * (l / 4) + 4 * t + l % 4, kb, g)
+           : kPerm ? read_row<kTerms>(tile, n0 + 32 * (t / 2) + 8 * (l / 4) + 4 * (t % 2) + l % 4, kb, g)
                    : read_row<kTerms>(tile, n0 + 16 * t + l, kb, g);
   }
   static __device__ __forceinline__ void add_block(Sum &sum, const bf16x8 (&m)[PM][MT],
@@ -268,7 +291,7 @@ struct Product {
 #pragma unroll
     for (int p = 0; p < PN; ++p)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) n[p][t] = read_n(lds, p, t, kb);
+      for (int t = 0; t < NT; ++t) n[p][t] = read_n(lds.n + p * kNPlane, t, kb);
   }
   // Adds a stage that is in LDS.
   static __device__ __forceinline__ void add(Sum &sum, const Lds &lds) {
@@ -278,17 +301,6 @@ struct Product {
       read_block(lds, kb, m, n);
       add_block(sum, m, n);
     }
-  }
-  // The same; next() runs once all of the stage's operands are in registers (a
-  // copy straight to LDS, after which reads of LDS would wait for it).
-  template <typename F>
-  static __device__ __forceinline__ void add_then(Sum &sum, const Lds &lds, F next) {
-    bf16x8 m[kTerms / 32][PM][MT], n[kTerms / 32][PN][NT];
-#pragma unroll
-    for (uint32_t kb = 0; kb < kTerms / 32; ++kb) read_block(lds, kb, m[kb], n[kb]);
-    next();
-#pragma unroll
-    for (uint32_t kb = 0; kb < kTerms / 32; ++kb) add_block(sum, m[kb], n[kb]);
   }
 };
 
