@@ -37,11 +37,35 @@ struct Matrix {
   uint32_t rows, cols;
 };
 
+// The tokens' weights, dloss * scale.  d is held relative to one of them, which the
+// products' results get back: where all weights are alike, as for a mean, a
+// token's own term is then -(1 - p), which 8 bits hold to 2^-9 and mostly better,
+// and not a value whose rounding, the same for every token, would show in all
+// results (error against 64 bits up to 0.0032, where the results' own rounding
+// leaves 0.0017).
+struct Weights {
+  const float *dloss;
+  const int32_t *targets;
+  uint32_t tokens, vocabulary;
+  float scale;
+
+  __device__ __forceinline__ bool counts(uint32_t token) const {
+    return token < tokens && (uint32_t)targets[token] < vocabulary;
+  }
+  // That of the first of 64 tokens that counts, if it is of an ordinary size.
+  __device__ __forceinline__ float reference() const {
+    const uint32_t lane = threadIdx.x & 63u;
+    const float w = counts(lane) ? dloss[lane] * scale : 0.f;
+    const uint64_t fit = __ballot(fabsf(w) >= 0x1p-30f && fabsf(w) <= 0x1p30f);
+    return fit ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), __builtin_ctzll(fit)))
+               : 1.f;
+  }
+};
+
 // ---- tiles of z
 
 struct LogitDev {
-  Matrix x, e;                // e: the piece
-  uint32_t tokens;            // (x may be padded)
+  Matrix x, e;                // e: the piece (x may be padded)
   uint32_t ttiles, vtiles;    // tiles of tokens, of the piece's vocabulary
   uint32_t sweep, sweeps;     // vocabulary tiles a workgroup takes one after another
   float scale2;               // scale * log2(e)
@@ -49,10 +73,9 @@ struct LogitDev {
   float2 *parts;              // [sweeps][part_stride]: maximum and sum, in powers of two
   uint64_t part_stride;
   // gradient
-  const float *lse, *dloss;
-  const int32_t *targets;
-  uint32_t row0, vocabulary;  // the piece's first row, rows of the whole table
-  float scale;
+  const float *lse;
+  Weights weights;
+  uint32_t row0;              // the piece's first
   void *d;                    // [tokens][d_ld] (kDirect: whole tiles of tokens)
   uint64_t d_ld;
 };
@@ -369,16 +392,17 @@ struct Derivatives {
 
   __device__ __forceinline__ Derivatives(const LogitDev &args, uint32_t ttile)
       : a(args), token0(ttile * kTile + Prod::first_m() + (threadIdx.x & 15u)) {
+    const float reference = a.weights.reference();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t token = token0 + 16 * i;
       lse2[i] = weight[i] = 0.f;
       target[i] = ~0u;
-      counts[i] = token < a.tokens && (uint32_t)a.targets[token] < a.vocabulary;
+      counts[i] = a.weights.counts(token);
       if (counts[i]) {
         lse2[i] = a.lse[token] * kLog2e;
-        weight[i] = a.dloss[token] * a.scale;
-        target[i] = (uint32_t)a.targets[token] - a.row0;
+        weight[i] = a.weights.dloss[token] * a.weights.scale / reference;
+        target[i] = (uint32_t)a.weights.targets[token] - a.row0;
       }
     }
   }
@@ -464,14 +488,14 @@ struct ProductDev {
   float *sums;           // [splits][rows][sums_ld], null: out is written
   uint64_t sums_split, sums_ld;
   uint32_t add;          // to what sums holds
-  const int32_t *targets;  // dE through registers: of n's rows
-  uint32_t vocabulary;
+  Weights weights;
 };
 
 template <typename Prod>
 __device__ __forceinline__ void put_result(const ProductDev &a, const typename Prod::Sum &sum,
                                            uint32_t m0, uint32_t n0, uint32_t split) {
-  constexpr int MT = sizeof(sum) / sizeof(sum[0]), NT = sizeof(sum[0]) / sizeof(sum[0][0]);
+  constexpr int MT = Prod::kMT, NT = Prod::kNT;
+  const float by = a.sums ? 1.f : a.weights.reference();
   const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
   const uint32_t m = m0 + Prod::first_m() + l, n = n0 + Prod::first_n() + 4 * g;
 #pragma unroll
@@ -486,7 +510,7 @@ __device__ __forceinline__ void put_result(const ProductDev &a, const typename P
         *at = a.add ? *at + sum[i][j] : sum[i][j];
         continue;
       }
-      const float v[4] = {sum[i][j][0], sum[i][j][1], sum[i][j][2], sum[i][j][3]};
+      const float v[4] = {sum[i][j][0] * by, sum[i][j][1] * by, sum[i][j][2] * by, sum[i][j][3] * by};
       const auto store = [&](auto t) {
         using T = decltype(t);
         T *const out = (T *)a.out + row * a.out_ld + col;
@@ -541,7 +565,7 @@ struct StagedProduct {
                [](uint32_t) { return 0u; });
       sn.fetch((const TN *)a.n.p + (uint64_t)k * a.n.ld + n0, a.n.ld, a.terms - k, a.n.cols - n0,
                [&](uint32_t r) {
-                 return kMCol ? (uint32_t)a.targets[min(k + r, a.terms - 1)] : 0u;
+                 return kMCol ? (uint32_t)a.weights.targets[min(k + r, a.terms - 1)] : 0u;
                });
       k += kTerms;
     };
@@ -552,7 +576,7 @@ struct StagedProduct {
       sm.template put<Prod::kM, kTerms, kMCol, PM>(lds.m, Prod::kMPlane,
                                                      [](uint32_t) { return true; });
       sn.template put<Prod::kN, kTerms, true, PN>(
-          lds.n, Prod::kNPlane, [&](uint32_t target) { return !kMCol || target < a.vocabulary; });
+          lds.n, Prod::kNPlane, [&](uint32_t target) { return !kMCol || target < a.weights.vocabulary; });
       __syncthreads();
       if (k < it.k1) fetch();
       Prod::add(sum, lds);
@@ -670,6 +694,7 @@ __global__ __launch_bounds__(256) void k_loss_rows(Matrix x, const int32_t *__re
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_loss_out(ProductDev a) {
   const uint32_t vecs = (a.out_cols + V - 1) / V;
+  const float by = a.weights.reference();
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)a.out_rows * vecs;
        i += (uint64_t)gridDim.x * 256) {
     const uint64_t r = i / vecs, c = i % vecs * V, at = r * a.sums_ld + c;
@@ -683,6 +708,8 @@ __global__ __launch_bounds__(256) void k_loss_out(ProductDev a) {
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] += t[k];
     }
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] *= by;
     store_f32<T, V>((T *)a.out + r * a.out_ld + c, v);
   }
 }
@@ -836,15 +863,11 @@ LogitDev logits(const nsfps_loss_args &a, uint64_t row0, uint64_t rows) {
   d.x = {a.d_x, a.x_stride, (uint32_t)a.tokens, a.width};
   d.e = {(const char *)a.d_table + row0 * a.table_stride * size, a.table_stride, (uint32_t)rows,
          a.width};
-  d.tokens = (uint32_t)a.tokens;
   d.ttiles = (uint32_t)host_ceil_div(a.tokens, kTile);
   d.vtiles = (uint32_t)host_ceil_div(rows, kTile);
   plan_sweeps(d.ttiles, d.vtiles, d.sweep, d.sweeps);
-  d.scale = a.scale;
   d.scale2 = a.scale * kLog2e;
   d.row0 = (uint32_t)row0;
-  d.vocabulary = (uint32_t)a.rows;
-  d.targets = a.d_targets;
   d.lse = a.d_lse;
   return d;
 }
@@ -956,6 +979,7 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     LAUNCH(hipGetLastError());
   }
   ProductDev dx = {};
+  dx.weights = {g.d_dloss, a.d_targets, (uint32_t)a.tokens, (uint32_t)a.rows, a.scale};
   dx.mtiles = (uint32_t)host_ceil_div(a.tokens, p.mt);
   dx.ntiles = ntiles;
   dx.per = p.per;
@@ -971,7 +995,7 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
   for (uint64_t k = 0; k < p.pieces; ++k) {
     const uint64_t row0 = k * p.piece, rows = std::min(p.piece, a.rows - row0);
     LogitDev l = logits(a, row0, rows);
-    l.dloss = g.d_dloss;
+    l.weights = dx.weights;
     l.d = ws + p.d;
     l.d_ld = p.d_ld;
     if (direct) {  // whole tiles of every product
@@ -999,8 +1023,6 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     dx.add = k > 0;
     ProductDev de = dx;
     de.n = direct ? Matrix{ws + p.x, a.width, (uint32_t)p.tokens, a.width} : x;
-    de.targets = a.d_targets;
-    de.vocabulary = (uint32_t)a.rows;
     de.mtiles = (uint32_t)host_ceil_div(rows, p.mt);
     de.terms = (uint32_t)a.tokens;
     de.splits = p.de_splits;
