@@ -64,10 +64,15 @@ struct Weights {
 
 // ---- tiles of z
 
+// Tiles of tokens and of a piece's vocabulary; how many of the latter a workgroup
+// takes one after another, and such sweeps.
+struct Tiling {
+  uint32_t ttiles, vtiles, sweep, sweeps;
+};
+
 struct LogitDev {
   Matrix x, e;                // e: the piece (x may be padded)
-  uint32_t ttiles, vtiles;    // tiles of tokens, of the piece's vocabulary
-  uint32_t sweep, sweeps;     // vocabulary tiles a workgroup takes one after another
+  Tiling tiles;
   float scale2;               // scale * log2(e)
   // statistics
   float2 *parts;              // [sweeps][part_stride]: maximum and sum, in powers of two
@@ -83,61 +88,76 @@ struct LogitDev {
 // Workgroup w's tile of tokens and sweep, the latter as vocabulary tiles of N rows:
 // tokens change fastest, within groups
 // that share sweeps, so that workgroups of one XCD read the same rows.
-template <uint32_t N>
+template <uint32_t N, uint32_t kUnit>
 __device__ __forceinline__ bool logit_item(const LogitDev &a, uint32_t &ttile, uint32_t &sweep,
                                            uint32_t &first, uint32_t &last) {
-  const uint32_t work = a.ttiles * a.sweeps, per = (work + 7) / 8;
+  const uint32_t work = a.tiles.ttiles * a.tiles.sweeps, per = (work + 7) / 8;
   const uint32_t w = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (blockIdx.x / 8 >= per || w >= work) return false;
   constexpr uint32_t kGroup = 8;
-  const uint32_t whole = kGroup * a.sweeps, group = w / whole, t0 = group * kGroup;
-  const uint32_t size = min(kGroup, a.ttiles - t0), in = w - group * whole;
+  const uint32_t whole = kGroup * a.tiles.sweeps, group = w / whole, t0 = group * kGroup;
+  const uint32_t size = min(kGroup, a.tiles.ttiles - t0), in = w - group * whole;
   ttile = t0 + in % size;
   sweep = in / size;
-  first = kTile / N * (sweep * a.sweep);
-  last = kTile / N * min(sweep * a.sweep + a.sweep, a.vtiles);
+  first = kUnit / N * (sweep * a.tiles.sweep);
+  last = kUnit / N * min(sweep * a.tiles.sweep + a.tiles.sweep, a.tiles.vtiles);
   return true;
 }
 
 // The tiles of z that a workgroup walks, one after another; epilogue.whole(sum,
 // tile) has each.  Operands through registers: any rows, either type.
-template <typename T, int P, bool kPerm>
+// kTiles: 16 x 16 tiles of a wave either way.
+template <typename T, int P, bool kPerm, Ends kEnds, int kTiles>
 struct StagedLogits {  // (every row is wanted)
   static constexpr int kTerms = P == 1 ? 64 : 32;
-  typedef Product<2, 2, 4, 4, kTerms, P, P, false, false, kPerm> Prod;
+  static constexpr int kAhead = 2;  // stages under way
+  typedef Product<2, 2, kTiles, kTiles, kTerms, P, P, false, false, kPerm> Prod;
+  static constexpr uint32_t kUnit = Prod::kN;
   typedef typename Prod::Lds Lds;
   static constexpr bool kDirect = false;
 
   template <typename F>
   static __device__ __forceinline__ void walk(const LogitDev &a, Lds &lds, uint32_t ttile,
                                               uint32_t first, uint32_t last, F &epilogue) {
-    Stage<T, kTile, kTerms, 256> sx, se;
+    Stage<T, Prod::kM, kTerms, 256, kEnds> sx[kAhead], se[kAhead];
     const uint32_t width = a.x.cols, steps = ceil_div(width, kTerms);
-    const uint32_t t0 = ttile * kTile;
+    const uint32_t t0 = ttile * Prod::kM;
     const T *const x = (const T *)a.x.p + (uint64_t)t0 * a.x.ld;
     const auto none = [](uint32_t) { return 0u; };
     const auto all = [](uint32_t) { return true; };
     uint32_t tile = first, k = 0;  // of the stage fetched next
-    const auto fetch = [&] {
-      const uint32_t v0 = tile * kTile;
-      sx.fetch(x + k * kTerms, a.x.ld, a.x.rows - t0, width - k * kTerms, none);
-      se.fetch((const T *)a.e.p + (uint64_t)v0 * a.e.ld + k * kTerms, a.e.ld, a.e.rows - v0,
-               width - k * kTerms, none);
+    const auto fetch = [&](int to) {  // past the end the last tile again
+      const uint32_t v0 = min(min(tile, last - 1) * Prod::kN, a.e.rows - 1);
+      sx[to].fetch(x + k * kTerms, a.x.ld, a.x.rows - t0, width - k * kTerms, none);
+      se[to].fetch((const T *)a.e.p + (uint64_t)v0 * a.e.ld + k * kTerms, a.e.ld, a.e.rows - v0,
+                   width - k * kTerms, none);
       if (++k == steps) k = 0, ++tile;
     };
     wait_loads();
-    fetch();
-    for (uint32_t t = first; t < last; ++t) {
-      typename Prod::Sum sum = {};
-      for (uint32_t s = 0; s < steps; ++s) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch(i);
+    typename Prod::Sum sum = {};
+    uint32_t s = 0;
+    for (uint32_t t = first; t < last;) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (t >= last) break;
         __syncthreads();
-        sx.template put<Prod::kM, kTerms, false, P>(lds.m, Prod::kMPlane, all);
-        se.template put<Prod::kN, kTerms, false, P>(lds.n, Prod::kNPlane, all);
+        sx[i].template put<Prod::kM, kTerms, false, P>(lds.m, Prod::kMPlane, all);
+        se[i].template put<Prod::kN, kTerms, false, P>(lds.n, Prod::kNPlane, all);
         __syncthreads();
-        if (tile < last) fetch();
+        fetch(i);
         Prod::add(sum, lds);
+        if (++s == steps) {
+          epilogue.whole(sum, t);
+#pragma unroll
+          for (int q = 0; q < Prod::kMT; ++q)
+#pragma unroll
+            for (int j = 0; j < Prod::kNT; ++j) sum[q][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          s = 0;
+          ++t;
+        }
       }
-      epilogue.whole(sum, t);
     }
   }
 };
@@ -150,6 +170,7 @@ struct DirectLogits {
     typename Prod::Lds buf[2];
   };
   static constexpr bool kDirect = true;
+  static constexpr uint32_t kUnit = kTile;
 
   template <typename F>
   static __device__ __forceinline__ void walk(const LogitDev &a, Lds &lds, uint32_t ttile,
@@ -194,6 +215,7 @@ struct ResidentLogits {
     bf16 buf[4][Prod::kN * kTerms];
   };
   static constexpr bool kDirect = true;
+  static constexpr uint32_t kUnit = kTile;
 
   template <typename F>
   static __device__ __forceinline__ void walk(const LogitDev &a, Lds &lds, uint32_t ttile,
@@ -252,17 +274,17 @@ __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s
   m = top;
 }
 
-// Running maximum and sum of a lane's columns, for its four tokens.
+// Running maximum and sum of a lane's columns, for its tokens.
 template <typename Prod>
 struct Stats {
   const LogitDev &a;
   const float by;  // (-infinity times 0 would be NaN)
-  float top[4], sum[4];
+  float top[Prod::kMT], sum[Prod::kMT];
 
   __device__ __forceinline__ explicit Stats(const LogitDev &args)
       : a(args), by(fmaxf(fabsf(args.scale2), 1e-38f)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top[i] = -INFINITY, sum[i] = 0.f;
+    for (int i = 0; i < Prod::kMT; ++i) top[i] = -INFINITY, sum[i] = 0.f;
   }
   // nothing to do but part(): no column past the end, no sign to turn
   __device__ __forceinline__ bool plain(uint32_t tile) const {
@@ -287,7 +309,7 @@ struct Stats {
   __device__ __forceinline__ void whole(typename Prod::Sum &z, uint32_t tile) {
     if (!plain(tile)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < Prod::kMT; ++i)
 #pragma unroll
         for (int j = 0; j < Prod::kNT; ++j)
 #pragma unroll
@@ -297,7 +319,7 @@ struct Stats {
           }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part(z, tile, i);
+    for (int i = 0; i < Prod::kMT; ++i) part(z, tile, i);
   }
 };
 
@@ -305,23 +327,23 @@ template <typename Logits>
 __global__ __launch_bounds__(256, 2) void k_loss_stats(LogitDev a) {
   typedef typename Logits::Prod Prod;
   __shared__ typename Logits::Lds lds;
-  __shared__ float2 s_part[2][kTile];
+  __shared__ float2 s_part[2][Prod::kM];
   uint32_t ttile, sweep, first, last;
-  if (!logit_item<Prod::kN>(a, ttile, sweep, first, last)) return;
+  if (!logit_item<Prod::kN, Logits::kUnit>(a, ttile, sweep, first, last)) return;
   const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / 2, wn = wave % 2;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % 2;
   Stats<Prod> o(a);
   Logits::walk(a, lds, ttile, first, last, o);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < Prod::kMT; ++i) {
 #pragma unroll
     for (int off = 16; off < 64; off <<= 1)
       join_stats(o.top[i], o.sum[i], __shfl_xor(o.top[i], off, 64), __shfl_xor(o.sum[i], off, 64));
-    if (g == 0) s_part[wn][64 * wm + 16 * i + l] = make_float2(o.top[i], o.sum[i]);
+    if (g == 0) s_part[wn][Prod::first_m() + 16 * i + l] = make_float2(o.top[i], o.sum[i]);
   }
   __syncthreads();
-  const uint32_t token = ttile * kTile + threadIdx.x;
-  if (threadIdx.x < kTile && token < a.x.rows) {
+  const uint32_t token = ttile * Prod::kM + threadIdx.x;
+  if (threadIdx.x < Prod::kM && token < a.x.rows) {
     float2 v = s_part[0][threadIdx.x];
     join_stats(v.x, v.y, s_part[1][threadIdx.x].x, s_part[1][threadIdx.x].y);
     a.parts[sweep * a.part_stride + token] = v;
@@ -380,21 +402,21 @@ __global__ __launch_bounds__(256) void k_loss_join(const float2 *__restrict__ pa
   }
 }
 
-// A piece's d, as D, for a lane's four tokens.
+// A piece's d, as D, for a lane's tokens.
 template <typename Logits, typename D>
 struct Derivatives {
   typedef typename Logits::Prod Prod;
   const LogitDev &a;
   const uint32_t token0;
-  float lse2[4], weight[4];
-  uint32_t target[4];  // in the piece
-  bool counts[4];
+  float lse2[Prod::kMT], weight[Prod::kMT];
+  uint32_t target[Prod::kMT];  // in the piece
+  bool counts[Prod::kMT];
 
   __device__ __forceinline__ Derivatives(const LogitDev &args, uint32_t ttile)
-      : a(args), token0(ttile * kTile + Prod::first_m() + (threadIdx.x & 15u)) {
+      : a(args), token0(ttile * Prod::kM + Prod::first_m() + (threadIdx.x & 15u)) {
     const float reference = a.weights.reference();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < Prod::kMT; ++i) {
       const uint32_t token = token0 + 16 * i;
       lse2[i] = weight[i] = 0.f;
       target[i] = ~0u;
@@ -411,7 +433,7 @@ struct Derivatives {
   __device__ __forceinline__ bool plain(uint32_t tile) const {
     bool special = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < Prod::kMT; ++i)
       special |= target[i] - tile * Prod::kN < Prod::kN || (!Logits::kDirect && !counts[i]);
     return (tile + 1) * Prod::kN <= a.e.rows && !__any(special);
   }
@@ -444,7 +466,7 @@ struct Derivatives {
   __device__ __forceinline__ void whole(const typename Prod::Sum &z, uint32_t tile) const {
     const bool simple = plain(tile);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < Prod::kMT; ++i) {
       float d[4 * Prod::kNT];
       values(z, i, d);
       if (!simple) {
@@ -469,7 +491,7 @@ template <typename Logits, typename D>
 __global__ __launch_bounds__(256, 2) void k_loss_d(LogitDev a) {
   __shared__ typename Logits::Lds lds;
   uint32_t ttile, sweep, first, last;
-  if (!logit_item<Logits::Prod::kN>(a, ttile, sweep, first, last)) return;
+  if (!logit_item<Logits::Prod::kN, Logits::kUnit>(a, ttile, sweep, first, last)) return;
   Derivatives<Logits, D> o(a, ttile);
   Logits::walk(a, lds, ttile, first, last, o);
 }
@@ -484,12 +506,23 @@ struct ProductDev {
   // the result: either rows of it, or the splits' sums
   void *out;
   uint64_t out_ld;
-  uint32_t out_rows, out_cols, out_dtype, out_wide;  // wide: four values a store
+  uint32_t out_rows, out_cols, out_dtype;
   float *sums;           // [splits][rows][sums_ld], null: out is written
   uint64_t sums_split, sums_ld;
   uint32_t add;          // to what sums holds
   Weights weights;
 };
+
+// at any address of such values
+__device__ __forceinline__ void store_four(float *p, const float (&v)[4]) {
+  *(NSFPS_GLOBAL_SEQ Packed16 *)p = Packed16{{__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                              __float_as_uint(v[2]), __float_as_uint(v[3])}};
+}
+__device__ __forceinline__ void store_four(bf16 *p, const float (&v)[4]) {
+  *(NSFPS_GLOBAL_SEQ Packed8 *)p =
+      Packed8{{(uint32_t)bf16_bits(v[0]) | (uint32_t)bf16_bits(v[1]) << 16,
+               (uint32_t)bf16_bits(v[2]) | (uint32_t)bf16_bits(v[3]) << 16}};
+}
 
 template <typename Prod>
 __device__ __forceinline__ void put_result(const ProductDev &a, const typename Prod::Sum &sum,
@@ -514,8 +547,8 @@ __device__ __forceinline__ void put_result(const ProductDev &a, const typename P
       const auto store = [&](auto t) {
         using T = decltype(t);
         T *const out = (T *)a.out + row * a.out_ld + col;
-        if (a.out_wide) {
-          store_f32<T, 4>(out, v);
+        if (col + 4 <= a.out_cols) {
+          store_four(out, v);
         } else {
 #pragma unroll
           for (uint32_t k = 0; k < 4; ++k) {
@@ -545,9 +578,9 @@ __device__ __forceinline__ ProductItem product_item(const ProductDev &a, uint32_
 }
 
 // M's terms along its rows (dx) or down its columns (dE), N's down its columns.
-template <typename TM, int PM, typename TN, int PN, int NT, bool kMCol>
+template <typename TM, int PM, typename TN, int PN, int NT, bool kMCol, Ends kEnds>
 struct StagedProduct {
-  static constexpr int kTerms = PM * PN == 1 ? 64 : 32;
+  static constexpr int kTerms = PM * PN == 1 ? 64 : 32, kAhead = 2;
   typedef Product<2, 2, 4, NT, kTerms, PM, PN, kMCol, true, false> Prod;
   static constexpr int kMRows = kMCol ? kTerms : Prod::kM, kMCols = kMCol ? Prod::kM : kTerms;
 
@@ -555,31 +588,41 @@ struct StagedProduct {
                                              uint32_t w) {
     const ProductItem it = product_item(a, w);
     const uint32_t m0 = it.mt * Prod::kM, n0 = it.nt * Prod::kN;
-    Stage<TM, kMRows, kMCols, 256> sm;
-    Stage<TN, kTerms, Prod::kN, 256> sn;
+    Stage<TM, kMRows, kMCols, 256, Ends::kPadded> sm[kAhead];
+    Stage<TN, kTerms, Prod::kN, 256, kEnds> sn[kAhead];
     uint32_t k = it.k0;
-    const auto fetch = [&] {
-      const uint32_t mr = kMCol ? k : m0, mc = kMCol ? m0 : k;
-      sm.fetch((const TM *)a.m.p + (uint64_t)mr * a.m.ld + mc, a.m.ld,
-               (kMCol ? a.terms : a.m.rows) - mr, (kMCol ? a.m.cols : a.terms) - mc,
-               [](uint32_t) { return 0u; });
-      sn.fetch((const TN *)a.n.p + (uint64_t)k * a.n.ld + n0, a.n.ld, a.terms - k, a.n.cols - n0,
-               [&](uint32_t r) {
-                 return kMCol ? (uint32_t)a.weights.targets[min(k + r, a.terms - 1)] : 0u;
-               });
+    const auto fetch = [&](int to) {  // past the end the last stage again
+      const uint32_t at = min(k, (it.k1 - 1) / kTerms * kTerms);
+      const uint32_t mr = kMCol ? at : m0, mc = kMCol ? m0 : at;
+      sm[to].fetch((const TM *)a.m.p + (uint64_t)mr * a.m.ld + mc, a.m.ld,
+                   (kMCol ? a.terms : a.m.rows) - mr, (kMCol ? a.m.cols : a.terms) - mc,
+                   [](uint32_t) { return 0u; });
+      sn[to].fetch((const TN *)a.n.p + (uint64_t)at * a.n.ld + n0, a.n.ld, a.terms - at,
+                   a.n.cols - n0, [&](uint32_t r) {
+                     return kMCol ? (uint32_t)a.weights.targets[min(at + r, a.terms - 1)] : 0u;
+                   });
       k += kTerms;
     };
     typename Prod::Sum sum = {};
-    if (it.k0 < it.k1) fetch();
-    for (uint32_t s = it.k0; s < it.k1; s += kTerms) {
-      __syncthreads();
-      sm.template put<Prod::kM, kTerms, kMCol, PM>(lds.m, Prod::kMPlane,
-                                                     [](uint32_t) { return true; });
-      sn.template put<Prod::kN, kTerms, true, PN>(
-          lds.n, Prod::kNPlane, [&](uint32_t target) { return !kMCol || target < a.weights.vocabulary; });
-      __syncthreads();
-      if (k < it.k1) fetch();
-      Prod::add(sum, lds);
+    if (it.k0 < it.k1) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) fetch(i);
+      for (uint32_t s = it.k0; s < it.k1;) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (s >= it.k1) break;
+          __syncthreads();
+          sm[i].template put<Prod::kM, kTerms, kMCol, PM>(lds.m, Prod::kMPlane,
+                                                          [](uint32_t) { return true; });
+          sn[i].template put<Prod::kN, kTerms, true, PN>(
+              lds.n, Prod::kNPlane,
+              [&](uint32_t target) { return !kMCol || target < a.weights.vocabulary; });
+          __syncthreads();
+          fetch(i);
+          Prod::add(sum, lds);
+          s += kTerms;
+        }
+      }
     }
     put_result<Prod>(a, sum, m0, n0, it.split);
   }
@@ -644,10 +687,10 @@ __device__ __forceinline__ bool product_work(const ProductDev &dx, const Product
   return true;
 }
 
-template <typename TD, int PDX, int PDE, typename T, int P, int NT>
+template <typename TD, int PDX, int PDE, typename T, int P, int NT, Ends kEnds>
 __global__ __launch_bounds__(256, 2) void k_loss_products(ProductDev dx, ProductDev de) {
-  typedef StagedProduct<TD, PDX, T, P, NT, false> X;
-  typedef StagedProduct<TD, PDE, T, P, NT, true> E;
+  typedef StagedProduct<TD, PDX, T, P, NT, false, kEnds> X;
+  typedef StagedProduct<TD, PDE, T, P, NT, true, kEnds> E;
   __shared__ union {
     typename X::Prod::Lds x;
     typename E::Prod::Lds e;
@@ -690,27 +733,37 @@ __global__ __launch_bounds__(256) void k_loss_rows(Matrix x, const int32_t *__re
   }
 }
 
-// The splits' sums, added in order, as rows of the result.
-template <typename T, int V>
+// The splits' sums, added in order, as rows of the result: four values a thread,
+// eight splits loaded together.
+template <typename T>
 __global__ __launch_bounds__(256) void k_loss_out(ProductDev a) {
-  const uint32_t vecs = (a.out_cols + V - 1) / V;
+  const uint32_t vecs = (a.out_cols + 3) / 4;
   const float by = a.weights.reference();
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)a.out_rows * vecs;
        i += (uint64_t)gridDim.x * 256) {
-    const uint64_t r = i / vecs, c = i % vecs * V, at = r * a.sums_ld + c;
-    float v[V] = {};
-    for (uint32_t s = 0; s < a.splits; ++s) {
-      float t[V];
-      constexpr int W = V < 4 ? V : 4;
+    const uint64_t r = i / vecs, c = i % vecs * 4;
+    const NSFPS_GLOBAL_SEQ float *from = (const NSFPS_GLOBAL_SEQ float *)(a.sums + r * a.sums_ld + c);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s0 = 0; s0 < a.splits; s0 += 8) {
+      f32x4 v[8];
 #pragma unroll
-      for (int k = 0; k < V; k += W)
-        load_f32<float, W>(a.sums + s * a.sums_split + at + k, *(float(*)[W])&t[k]);
+      for (uint32_t s = 0; s < 8; ++s)
+        v[s] = *(const NSFPS_GLOBAL_SEQ f32x4 *)(from + min(s0 + s, a.splits - 1) * a.sums_split);
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] += t[k];
+      for (uint32_t s = 0; s < 8; ++s)
+        if (s0 + s < a.splits) sum += v[s];
     }
+    const float o[4] = {sum[0] * by, sum[1] * by, sum[2] * by, sum[3] * by};
+    T *const out = (T *)a.out + r * a.out_ld + c;
+    if (c + 4 <= a.out_cols) {
+      store_four(out, o);
+    } else {
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] *= by;
-    store_f32<T, V>((T *)a.out + r * a.out_ld + c, v);
+      for (uint32_t k = 0; k < 4; ++k) {
+        const float one[1] = {o[k]};
+        if (c + k < a.out_cols) store_f32<T, 1>(out + k, one);
+      }
+    }
   }
 }
 
@@ -748,23 +801,24 @@ void plan_sweeps(uint32_t ttiles, uint32_t vtiles, uint32_t &sweep, uint32_t &sw
   sweeps = (vtiles + sweep - 1) / sweep;
 }
 
-struct LossPlan {
-  uint32_t ttiles, vtiles, sweep, sweeps;
-  uint64_t bytes;
-};
-LossPlan loss_plan(const nsfps_loss_args &a) {
-  LossPlan p = {};
-  p.ttiles = (uint32_t)host_ceil_div(a.tokens, kTile);
-  p.vtiles = (uint32_t)host_ceil_div(a.rows, kTile);
-  if (p.vtiles) plan_sweeps(p.ttiles, p.vtiles, p.sweep, p.sweeps);
-  p.bytes = std::max<uint64_t>(256, bytes256(8 * p.sweeps * up(a.tokens, 16)));
-  return p;
+// Tiles of a call through registers: of 64 where those of 128 leave CUs without
+// one.  us (130 tokens x 901 x 847 bfloat16 with gradient): XX.
+uint32_t staged_tile(uint64_t tokens, uint64_t rows) {
+  return host_ceil_div(tokens, 128) * host_ceil_div(rows, 128) <= 128 ? 64 : 128;
 }
 
-constexpr uint32_t kPad = 256;  // of tokens and pieces: whole tiles of any kind
+Tiling tiling(uint64_t tokens, uint64_t rows, uint32_t tile) {
+  Tiling t = {};
+  t.ttiles = (uint32_t)host_ceil_div(tokens, tile);
+  t.vtiles = (uint32_t)host_ceil_div(rows, tile);
+  if (t.vtiles) plan_sweeps(t.ttiles, t.vtiles, t.sweep, t.sweeps);
+  return t;
+}
 
 // Whether a call's tiles go straight to LDS hangs on its addresses, the workspace
 // does not: it has room for either.
+constexpr uint32_t kPad = 256;  // of tokens and pieces: whole tiles of any kind
+
 struct GradPlan {
   uint64_t tokens;             // padded
   uint64_t piece, pieces;      // vocabulary rows of a piece, a multiple of kPad
@@ -857,15 +911,26 @@ void by_steps(uint32_t width, F f) {
   }
 }
 
-LogitDev logits(const nsfps_loss_args &a, uint64_t row0, uint64_t rows) {
+template <Ends kEnds>
+using EndsOf = std::integral_constant<Ends, kEnds>;
+template <typename F>
+void by_ends(uint32_t width, uint32_t tile, F f) {
+  constexpr std::integral_constant<int, 2> two;
+  constexpr std::integral_constant<int, 4> four;
+  if (width < 8)
+    tile == 64 ? f(EndsOf<Ends::kNarrow>(), two) : f(EndsOf<Ends::kNarrow>(), four);
+  else
+    tile == 64 ? f(EndsOf<Ends::kWide>(), two) : f(EndsOf<Ends::kWide>(), four);
+}
+
+LogitDev logits(const nsfps_loss_args &a, uint64_t row0, uint64_t rows, uint64_t x_rows,
+                uint64_t e_rows, uint32_t tile) {
   LogitDev d = {};
   const uint64_t size = a.dtype == NSFPS_F32 ? 4 : 2;
   d.x = {a.d_x, a.x_stride, (uint32_t)a.tokens, a.width};
   d.e = {(const char *)a.d_table + row0 * a.table_stride * size, a.table_stride, (uint32_t)rows,
          a.width};
-  d.ttiles = (uint32_t)host_ceil_div(a.tokens, kTile);
-  d.vtiles = (uint32_t)host_ceil_div(rows, kTile);
-  plan_sweeps(d.ttiles, d.vtiles, d.sweep, d.sweeps);
+  d.tiles = tiling(x_rows, e_rows, tile);
   d.scale2 = a.scale * kLog2e;
   d.row0 = (uint32_t)row0;
   d.lse = a.d_lse;
@@ -884,26 +949,13 @@ hipError_t run_direct(const ProductDev &dx, const ProductDev &de, uint32_t grid,
   return hipGetLastError();
 }
 
-template <typename T>
-bool wide_rows(const void *out, uint64_t ld, uint32_t width, uint32_t v) {
-  return width % v == 0 && ld % v == 0 && (uintptr_t)out % (v * sizeof(T)) == 0;
-}
-bool wide_any(uint32_t dtype, const void *out, uint64_t ld, uint32_t width, uint32_t v) {
-  return dtype == NSFPS_F32 ? wide_rows<float>(out, ld, width, v)
-                            : wide_rows<bf16>(out, ld, width, v);
-}
-
 hipError_t write_out(const ProductDev &d, hipStream_t st) {
-  const auto go = [&](auto t) {
-    using T = decltype(t);
-    constexpr int V = kWide<T>;
-    if (wide_rows<T>(d.out, d.out_ld, d.out_cols, V))
-      k_loss_out<T, V><<<grid_of((uint64_t)d.out_rows * (d.out_cols / V)), 256, 0, st>>>(d);
-    else
-      k_loss_out<T, 1><<<grid_of((uint64_t)d.out_rows * d.out_cols), 256, 0, st>>>(d);
-    return hipGetLastError();
-  };
-  return d.out_dtype == NSFPS_F32 ? go(float()) : go(bf16());
+  const uint32_t grid = grid_of((uint64_t)d.out_rows * ((d.out_cols + 3) / 4));
+  if (d.out_dtype == NSFPS_F32)
+    k_loss_out<float><<<grid, 256, 0, st>>>(d);
+  else
+    k_loss_out<bf16><<<grid, 256, 0, st>>>(d);
+  return hipGetLastError();
 }
 
 hipError_t write_zeros(uint32_t dtype, void *out, uint64_t stride, uint64_t rows, uint32_t width,
@@ -924,23 +976,32 @@ hipError_t write_zeros(uint32_t dtype, void *out, uint64_t stride, uint64_t rows
 
 }  // namespace
 
-uint64_t loss_bytes(const nsfps_loss_args &a) { return loss_plan(a).bytes; }
+uint64_t loss_bytes(const nsfps_loss_args &a) {
+  const uint32_t sweeps = std::max(tiling(a.tokens, a.rows, kTile).sweeps,
+                                   tiling(a.tokens, a.rows, staged_tile(a.tokens, a.rows)).sweeps);
+  return std::max<uint64_t>(256, bytes256(8 * sweeps * up(a.tokens, 16)));
+}
 
 hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
-  const LossPlan p = loss_plan(a);
+  const bool direct = direct_rows(a);
+  const uint32_t tile = direct ? kTile : staged_tile(a.tokens, a.rows);
   const uint64_t stride = up(a.tokens, 16);
   float2 *const parts = (float2 *)a.workspace;
-  if (p.vtiles) {
-    LogitDev d = logits(a, 0, a.rows);
+  LogitDev d = logits(a, 0, a.rows, a.tokens, a.rows, tile);
+  if (a.rows) {
     d.parts = parts;
     d.part_stride = stride;
-    const uint32_t grid = xcd_grid((uint64_t)d.ttiles * d.sweeps);
-    if (direct_rows(a))
-      by_steps(a.width, [&](auto z) { k_loss_stats<decltype(z)><<<grid, 256, 0, st>>>(d); });
-    else if (a.dtype == NSFPS_F32)
-      k_loss_stats<StagedLogits<float, 3, false>><<<grid, 256, 0, st>>>(d);
+    const uint32_t grid = xcd_grid((uint64_t)d.tiles.ttiles * d.tiles.sweeps);
+    const auto go = [&](auto z) { k_loss_stats<decltype(z)><<<grid, 256, 0, st>>>(d); };
+    if (direct)
+      by_steps(a.width, go);
     else
-      k_loss_stats<StagedLogits<bf16, 1, true>><<<grid, 256, 0, st>>>(d);
+      by_ends(a.width, tile, [&](auto ends, auto tiles) {
+        constexpr Ends kEnds = decltype(ends)::value;
+        constexpr int kTiles = decltype(tiles)::value;
+        a.dtype == NSFPS_F32 ? go(StagedLogits<float, 3, false, kEnds, kTiles>())
+                             : go(StagedLogits<bf16, 1, true, kEnds, kTiles>());
+      });
     LAUNCH(hipGetLastError());
   }
   const auto join = [&](auto t) {
@@ -948,7 +1009,8 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
     while (group > 1 && a.tokens / group < 256) group /= 2;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(1u << 16, host_ceil_div(a.tokens, group));
     k_loss_join<decltype(t)><<<grid, 256, 0, st>>>(
-        parts, p.sweeps, stride, group, Matrix{a.d_x, a.x_stride, (uint32_t)a.tokens, a.width},
+        parts, d.tiles.sweeps, stride, group,
+        Matrix{a.d_x, a.x_stride, (uint32_t)a.tokens, a.width},
         Matrix{a.d_table, a.table_stride, (uint32_t)a.rows, a.width}, a.scale, a.d_targets, a.d_loss,
         a.d_lse);
     return hipGetLastError();
@@ -988,31 +1050,32 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
   dx.out_rows = (uint32_t)a.tokens;
   dx.out_cols = a.width;
   dx.out_dtype = a.dtype;
-  dx.out_wide = wide_any(a.dtype, g.d_dx, g.dx_stride, a.width, 4);
   dx.sums = p.dx_sums ? (float *)(ws + p.dx) : nullptr;
   dx.sums_ld = (uint64_t)ntiles * p.nt;
   dx.sums_split = a.tokens * dx.sums_ld;
   for (uint64_t k = 0; k < p.pieces; ++k) {
     const uint64_t row0 = k * p.piece, rows = std::min(p.piece, a.rows - row0);
-    LogitDev l = logits(a, row0, rows);
+    // straight to LDS, whole tiles of every product
+    LogitDev l = direct ? logits(a, row0, rows, p.tokens, up(rows, kPad), kTile)
+                        : logits(a, row0, rows, a.tokens, rows, staged_tile(a.tokens, rows));
+    if (direct) l.x = {ws + p.x, a.width, (uint32_t)p.tokens, a.width};
     l.weights = dx.weights;
     l.d = ws + p.d;
     l.d_ld = p.d_ld;
-    if (direct) {  // whole tiles of every product
-      l.x = {ws + p.x, a.width, (uint32_t)p.tokens, a.width};
-      l.ttiles = (uint32_t)(p.tokens / kTile);
-      l.vtiles = (uint32_t)(up(rows, kPad) / kTile);
-      plan_sweeps(l.ttiles, l.vtiles, l.sweep, l.sweeps);
-    }
-    const uint32_t grid = xcd_grid((uint64_t)l.ttiles * l.sweeps);
+    const uint32_t grid = xcd_grid((uint64_t)l.tiles.ttiles * l.tiles.sweeps);
     if (direct)
       by_steps(a.width, [&](auto z) { k_loss_d<decltype(z), bf16><<<grid, 256, 0, st>>>(l); });
-    else if (a.dtype == NSFPS_F32)
-      k_loss_d<StagedLogits<float, 3, false>, float><<<grid, 256, 0, st>>>(l);
-    else if (one)
-      k_loss_d<StagedLogits<bf16, 1, true>, bf16><<<grid, 256, 0, st>>>(l);
     else
-      k_loss_d<StagedLogits<bf16, 1, false>, float><<<grid, 256, 0, st>>>(l);
+      by_ends(a.width, staged_tile(a.tokens, rows), [&](auto ends, auto tiles) {
+        constexpr Ends kEnds = decltype(ends)::value;
+        constexpr int kTiles = decltype(tiles)::value;
+        if (a.dtype == NSFPS_F32)
+          k_loss_d<StagedLogits<float, 3, false, kEnds, kTiles>, float><<<grid, 256, 0, st>>>(l);
+        else if (one)
+          k_loss_d<StagedLogits<bf16, 1, true, kEnds, kTiles>, bf16><<<grid, 256, 0, st>>>(l);
+        else
+          k_loss_d<StagedLogits<bf16, 1, false, kEnds, kTiles>, float><<<grid, 256, 0, st>>>(l);
+      });
     LAUNCH(hipGetLastError());
 
     const Matrix d = {ws + p.d, p.d_ld, (uint32_t)(direct ? p.tokens : a.tokens), (uint32_t)rows};
@@ -1030,27 +1093,30 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     de.out_ld = g.dtable_stride;
     de.out_rows = (uint32_t)rows;
     de.out_dtype = g.grad_dtype;
-    de.out_wide = wide_any(g.grad_dtype, de.out, de.out_ld, a.width, 4);
     de.sums = p.de_sums ? (float *)(ws + p.de) : nullptr;
     de.sums_split = p.piece * de.sums_ld;
     de.add = 0;
     const uint32_t work = xcd_grid((uint64_t)dx.mtiles * ntiles * dx.splits +
                                    (uint64_t)de.mtiles * ntiles * de.splits);
-    const auto staged = [&](auto nt) {
+    const auto staged = [&](auto nt, auto ends) {
       constexpr int NT = decltype(nt)::value;
+      constexpr Ends kEnds = decltype(ends)::value;
       if (a.dtype == NSFPS_F32)
-        k_loss_products<float, 3, 3, float, 3, NT><<<work, 256, 0, st>>>(dx, de);
+        k_loss_products<float, 3, 3, float, 3, NT, kEnds><<<work, 256, 0, st>>>(dx, de);
       else if (one)
-        k_loss_products<bf16, 1, 1, bf16, 1, NT><<<work, 256, 0, st>>>(dx, de);
+        k_loss_products<bf16, 1, 1, bf16, 1, NT, kEnds><<<work, 256, 0, st>>>(dx, de);
       else
-        k_loss_products<float, 1, 2, bf16, 1, NT><<<work, 256, 0, st>>>(dx, de);
+        k_loss_products<float, 1, 2, bf16, 1, NT, kEnds><<<work, 256, 0, st>>>(dx, de);
       return hipGetLastError();
     };
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::integral_constant<int, 4> four;
     const hipError_t e = p.nt == 256             ? run_direct<2, 4, 4>(dx, de, work, st)
                          : direct && p.nt == 128 ? run_direct<4, 2, 4>(dx, de, work, st)
                          : direct                ? run_direct<4, 1, 4>(dx, de, work, st)
-                         : p.nt == 64            ? staged(std::integral_constant<int, 2>())
-                                                 : staged(std::integral_constant<int, 4>());
+                         : a.width < 8           ? staged(two, EndsOf<Ends::kNarrow>())
+                         : p.nt == 64            ? staged(two, EndsOf<Ends::kWide>())
+                                                 : staged(four, EndsOf<Ends::kWide>());
     LAUNCH(e);
     if (de.sums) LAUNCH(write_out(de, st));
   }
@@ -1059,7 +1125,7 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
 
 hipError_t preload_loss_kernels() {
   return func_attributes(k_loss_stats<DirectLogits>, k_loss_join<bf16>, k_loss_d<DirectLogits, bf16>,
-                         k_loss_products_direct<2, 4, 4>, k_loss_out<bf16, 8>, k_loss_rows);
+                         k_loss_products_direct<2, 4, 4>, k_loss_out<bf16>, k_loss_rows);
 }
 
 }  // namespace nsfps

@@ -123,7 +123,8 @@ __device__ __forceinline__ void landed() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory");
 }
 
-// Eight values of a row, at any address that holds such values.
+// Eight values of a row, at any address that holds such values (16-byte accesses
+// need no alignment here).
 template <typename T>
 struct Eight {
   static constexpr int kWords = 8 * (int)sizeof(T) / 4;
@@ -131,6 +132,9 @@ struct Eight {
 };
 struct __attribute__((packed, aligned(2))) Packed16 {
   uint32_t w[4];
+};
+struct __attribute__((packed, aligned(2))) Packed8 {
+  uint32_t w[2];
 };
 template <typename T>
 __device__ __forceinline__ Eight<T> load_eight(const T *p) {
@@ -143,7 +147,7 @@ __device__ __forceinline__ Eight<T> load_eight(const T *p) {
   }
   return o;
 }
-// its first n
+// its first n, n below 8, one after another
 template <typename T>
 __device__ __forceinline__ Eight<T> load_some(const T *p, uint32_t n) {
   Eight<T> o = {};
@@ -158,46 +162,99 @@ __device__ __forceinline__ Eight<T> load_some(const T *p, uint32_t n) {
     }
   return o;
 }
+// The values from number n on, zeros behind them; all zeros from 8 on.
+template <typename T>
+__device__ __forceinline__ void drop(Eight<T> &v, uint32_t n) {
+  constexpr int N = Eight<T>::kWords;
+  constexpr uint32_t kWordsOf4 = sizeof(T);  // words of four values
+#pragma unroll
+  for (uint32_t step = 4; step >= (sizeof(T) == 4 ? 1 : 2); step /= 2) {
+    const int words = step * kWordsOf4 / 4;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t from = i + words < N ? v.w[i + words] : 0u;
+      v.w[i] = n & step ? from : v.w[i];
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t next = i + 1 < N ? v.w[i + 1] : 0u;
+      v.w[i] = n & 1 ? v.w[i] >> 16 | next << 16 : v.w[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v.w[i] = n < 8 ? v.w[i] : 0u;
+}
 
-// A tile through registers: ROWS x COLS of memory, fetched while the tile before
-// it is worked on, split into P planes and put.  What lies outside is zeros.
-template <typename T, int ROWS, int COLS, int kThreads>
+// The first n values, zeros behind them.
+template <typename T>
+__device__ __forceinline__ void keep(Eight<T> &v, uint32_t n) {
+#pragma unroll
+  for (uint32_t i = 0; i < Eight<T>::kWords; ++i) {
+    if constexpr (sizeof(T) == 4)
+      v.w[i] = i < n ? v.w[i] : 0u;
+    else
+      v.w[i] &= (2 * i < n ? 0xffffu : 0u) | (2 * i + 1 < n ? 0xffff0000u : 0u);
+  }
+}
+
+// What may be read of a tile's rows beside the values inside.
+enum class Ends {
+  kWide,    // nothing; rows have 8 values or more: a row's last 8 are fetched for its end
+  kNarrow,  // nothing; rows have fewer than 8 values, which come one after another
+  kPadded,  // as many values as the tile is wide, of whatever they are
+};
+
+// A tile through registers: ROWS x COLS of memory, fetched while the tiles before
+// it are worked on, split into P planes and put.  What lies outside is zeros: the
+// last row, or other values, are fetched in its place and put() mends that.  (A
+// load that waits for a condition, or whose value is used where it stands, would
+// hold up those behind it: so it is with kNarrow.)
+template <typename T, int ROWS, int COLS, int kThreads, Ends kEnds>
 struct Stage {
   static constexpr int kPer = ROWS * COLS / 8 / kThreads, kVecs = COLS / 8;
   static_assert(kPer >= 1, "tile too small");
   Eight<T> v[kPer];
-  uint32_t tag[kPer];  // of the pieces' rows
+  uint32_t tag[kPer];   // of the pieces' rows
+  uint32_t rows, cols;  // inside
 
-  // at: the tile's first value; rows, cols: how many of it are inside.
-  // tag_of(row): what put() decides by whether the row is wanted.  (Not here: a
-  // value that is used is waited for.)
+  // at: the tile's first value; nrows, ncols: how many of it are inside, at least 1.
+  // tag_of(row): what put() decides by whether the row is wanted.
   template <typename F>
-  __device__ __forceinline__ void fetch(const T *at, uint64_t ld, uint32_t rows, uint32_t cols,
+  __device__ __forceinline__ void fetch(const T *at, uint64_t ld, uint32_t nrows, uint32_t ncols,
                                         F tag_of) {
-    const bool whole = rows >= (uint32_t)ROWS && cols >= (uint32_t)COLS;
+    rows = nrows;
+    cols = min(ncols, (uint32_t)COLS);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint32_t e = threadIdx.x + kThreads * i, r = e / kVecs, c = e % kVecs * 8;
-      const T *p = at + r * ld + c;
-      if (whole) {
-        v[i] = load_eight<T>(p);
-      } else {
-        v[i] = Eight<T>{};
-        if (r < rows && c + 8 <= cols)
-          v[i] = load_eight<T>(p);
-        else if (r < rows && c < cols)
-          v[i] = load_some<T>(p, cols - c);
-      }
+      const uint32_t e = threadIdx.x + kThreads * i, r = min(e / kVecs, rows - 1), c = e % kVecs * 8;
+      const T *row = at + r * ld;
+      if constexpr (kEnds == Ends::kWide)
+        v[i] = load_eight<T>(row + min((int32_t)c, (int32_t)cols - 8));
+      else if constexpr (kEnds == Ends::kNarrow)
+        v[i] = load_some<T>(row, c ? 0u : cols);
+      else
+        v[i] = load_eight<T>(row + c);
       tag[i] = tag_of(r);
     }
+    __builtin_amdgcn_sched_barrier(0);  // asked for now, and in order: put() counts on both
   }
   // kT: columns of a Col tile; plane: values of a plane in LDS
   template <int kT, int kTerms, bool kCol, int P, typename F>
   __device__ __forceinline__ void put(bf16 *tile, uint32_t plane, F wanted) {
+    const bool whole = rows >= (uint32_t)ROWS && cols >= (uint32_t)COLS;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (!wanted(tag[i])) v[i] = Eight<T>{};
       const uint32_t e = threadIdx.x + kThreads * i, r = e / kVecs, c = e % kVecs * 8;
+      if (!whole) {  // the same for all lanes; most tiles are
+        if constexpr (kEnds == Ends::kWide)
+          drop<T>(v[i], c + 8 > cols ? c + 8 - cols : 0u);
+        else if constexpr (kEnds == Ends::kPadded)
+          keep<T>(v[i], cols > c ? cols - c : 0u);
+        if (r >= rows) v[i] = Eight<T>{};
+      }
+      if (!wanted(tag[i])) v[i] = Eight<T>{};
       bf16 *const to = tile + piece_at<kT, kTerms, kCol>(r, c);
       if constexpr (sizeof(T) == 2) {
         static_assert(P == 1, "a bfloat16 value is one term");
