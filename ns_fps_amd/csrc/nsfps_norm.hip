@@ -374,20 +374,28 @@ __global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict_
   }
 }
 
-// 16 values and 16 runs of workgroups a workgroup.
+// 8 values and 32 runs of workgroups a workgroup, eight loads of a run together.
 __global__ __launch_bounds__(256) void k_norm_join(const float *__restrict__ parts, uint32_t blocks,
                                                    uint32_t d, float *dq_weight, float *dk_weight) {
-  __shared__ double s_sum[16][17];
-  const uint32_t side = blockIdx.y, e = blockIdx.x * 16 + threadIdx.x % 16, run = threadIdx.x / 16;
+  constexpr uint32_t kRuns = 32, kAhead = 8;
+  __shared__ double s_sum[kRuns][8];
+  const uint32_t side = blockIdx.y, e = blockIdx.x * 8 + threadIdx.x % 8, run = threadIdx.x / 8;
   float *const out = side ? dk_weight : dq_weight;
   double sum = 0.;
   if (e < d)
-    for (uint32_t b = run; b < blocks; b += 16) sum += parts[((uint64_t)b * 2 + side) * d + e];
-  s_sum[run][threadIdx.x % 16] = sum;
+    for (uint32_t b = run; b < blocks; b += kRuns * kAhead) {
+      float v[kAhead];
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; ++k)
+        v[k] = parts[((uint64_t)min(b + kRuns * k, blocks - 1) * 2 + side) * d + e];
+#pragma unroll
+      for (uint32_t k = 0; k < kAhead; ++k) sum += b + kRuns * k < blocks ? v[k] : 0.f;
+    }
+  s_sum[run][threadIdx.x % 8] = sum;
   __syncthreads();
-  if (threadIdx.x < 16 && e < d && out) {
+  if (threadIdx.x < 8 && e < d && out) {
     double all = 0.;
-    for (int k = 0; k < 16; ++k) all += s_sum[k][threadIdx.x];
+    for (uint32_t k = 0; k < kRuns; ++k) all += s_sum[k][threadIdx.x];
     out[e] = (float)all;
   }
 }
@@ -512,7 +520,7 @@ hipError_t launch_norm_grad(const nsfps_norm_args &a, const nsfps_norm_grads &g,
       return hipGetLastError();
     });
   if (e != hipSuccess || (!g.d_dq_weight && !g.d_dk_weight)) return e;
-  k_norm_join<<<dim3((a.head_dim + 15) / 16, 2), 256, 0, st>>>(parts, blocks, a.head_dim,
+  k_norm_join<<<dim3((a.head_dim + 7) / 8, 2), 256, 0, st>>>(parts, blocks, a.head_dim,
                                                               g.d_dq_weight, g.d_dk_weight);
   return hipGetLastError();
 }
