@@ -133,9 +133,9 @@ struct StagedLogits {  // (every row is wanted)
                    width - k * kTerms, none);
       if (++k == steps) k = 0, ++tile;
     };
-    wait_loads();
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) fetch(i);
+    wait_loads();
     typename Prod::Sum sum = {};
     uint32_t s = 0;
     for (uint32_t t = first; t < last;) {
@@ -188,8 +188,8 @@ struct DirectLogits {
       fe.issue(lds.buf[b].n, (const bf16 *)a.e.p + (uint64_t)v0 * a.e.ld + 64 * k);
       if (++k == steps) k = 0, ++tile;
     };
-    wait_loads();
     issue(0);
+    wait_loads();
     for (uint32_t t = first; t < last; ++t) {
       typename Prod::Sum sum = {};
       for (uint32_t s = 0; s < steps; ++s) {
@@ -221,16 +221,6 @@ struct ResidentLogits {
   static __device__ __forceinline__ void walk(const LogitDev &a, Lds &lds, uint32_t ttile,
                                               uint32_t first, uint32_t last, F &epilogue) {
     constexpr int kBlocks = kTerms / 32;
-    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
-    bf16x8 x[kSteps][kBlocks][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t r = min(ttile * kTile + Prod::first_m() + 16 * i + l, a.x.rows - 1);
-      const bf16 *row = (const bf16 *)a.x.p + r * a.x.ld + 8 * g;
-#pragma unroll
-      for (int k = 0; k < kBlocks * kSteps; ++k)
-        x[k / kBlocks][k % kBlocks][i] = *(const NSFPS_GLOBAL_SEQ bf16x8 *)(row + 32 * k);
-    }
     Feed<Prod::kN, kTerms, false, 256> fe;
     constexpr int kCopies = fe.kPer;
     fe.start(a.e.ld, ~0u);
@@ -242,10 +232,20 @@ struct ResidentLogits {
       if (++k == kSteps) k = 0, ++tile;
       to = (to + 1) % 4;
     };
+    issue();
+    issue();
+    issue();
+    const uint32_t lane = threadIdx.x & 63u, g = lane >> 4, l = lane & 15u;
+    bf16x8 x[kSteps][kBlocks][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r = min(ttile * kTile + Prod::first_m() + 16 * i + l, a.x.rows - 1);
+      const bf16 *row = (const bf16 *)a.x.p + r * a.x.ld + 8 * g;
+#pragma unroll
+      for (int k = 0; k < kBlocks * kSteps; ++k)
+        x[k / kBlocks][k % kBlocks][i] = *(const NSFPS_GLOBAL_SEQ bf16x8 *)(row + 32 * k);
+    }
     wait_loads();
-    issue();
-    issue();
-    issue();
     for (uint32_t t = first; t < last; ++t) {
       typename Prod::Sum sum = {};
 #pragma unroll
@@ -736,7 +736,7 @@ __global__ __launch_bounds__(256) void k_loss_rows(Matrix x, const int32_t *__re
 // The splits' sums, added in order, as rows of the result: four values a thread,
 // eight splits loaded together.
 template <typename T>
-__global__ __launch_bounds__(256) void k_loss_out(ProductDev a) {
+__device__ __forceinline__ void write_result(const ProductDev &a) {
   const uint32_t vecs = (a.out_cols + 3) / 4;
   const float by = a.weights.reference();
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)a.out_rows * vecs;
@@ -765,6 +765,15 @@ __global__ __launch_bounds__(256) void k_loss_out(ProductDev a) {
       }
     }
   }
+}
+
+// first's result, second's with blockIdx.y = 1
+__global__ __launch_bounds__(256) void k_loss_out(ProductDev first, ProductDev second) {
+  const ProductDev &a = blockIdx.y ? second : first;
+  if (a.out_dtype == NSFPS_F32)
+    write_result<float>(a);
+  else
+    write_result<bf16>(a);
 }
 
 template <typename T>
@@ -949,12 +958,11 @@ hipError_t run_direct(const ProductDev &dx, const ProductDev &de, uint32_t grid,
   return hipGetLastError();
 }
 
-hipError_t write_out(const ProductDev &d, hipStream_t st) {
-  const uint32_t grid = grid_of((uint64_t)d.out_rows * ((d.out_cols + 3) / 4));
-  if (d.out_dtype == NSFPS_F32)
-    k_loss_out<float><<<grid, 256, 0, st>>>(d);
-  else
-    k_loss_out<bf16><<<grid, 256, 0, st>>>(d);
+// The sums of one product, or of two, as rows of their results.
+hipError_t write_out(const ProductDev &first, const ProductDev *second, hipStream_t st) {
+  const auto threads = [](const ProductDev &d) { return (uint64_t)d.out_rows * ((d.out_cols + 3) / 4); };
+  const uint32_t grid = grid_of(std::max(threads(first), second ? threads(*second) : 0));
+  k_loss_out<<<dim3(grid, second ? 2 : 1), 256, 0, st>>>(first, second ? *second : first);
   return hipGetLastError();
 }
 
@@ -1118,14 +1126,16 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
                          : p.nt == 64            ? staged(two, EndsOf<Ends::kWide>())
                                                  : staged(four, EndsOf<Ends::kWide>());
     LAUNCH(e);
-    if (de.sums) LAUNCH(write_out(de, st));
+    const bool last = k + 1 == p.pieces;
+    if (de.sums) LAUNCH(write_out(de, last && dx.sums ? &dx : nullptr, st));
+    if (!de.sums && last && dx.sums) LAUNCH(write_out(dx, nullptr, st));
   }
-  return dx.sums ? write_out(dx, st) : hipSuccess;
+  return hipSuccess;
 }
 
 hipError_t preload_loss_kernels() {
   return func_attributes(k_loss_stats<DirectLogits>, k_loss_join<bf16>, k_loss_d<DirectLogits, bf16>,
-                         k_loss_products_direct<2, 4, 4>, k_loss_out<bf16>, k_loss_rows);
+                         k_loss_products_direct<2, 4, 4>, k_loss_out, k_loss_rows);
 }
 
 }  // namespace nsfps

@@ -110,7 +110,9 @@ struct Feed {
     const uint64_t base = (uint64_t)from;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+      // (m0 is set where it is used, here and by the compiler; a scalar register that
+      // the vector unit wrote may be read five states later)
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                    :
                    : "v"(at[i]), "s"(base), "s"(to + 16 * kThreads * i)
                    : "memory");
