@@ -717,19 +717,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_loss_products_direct(Produc
     E::run(de, *(typename E::Lds *)s_raw, w);
 }
 
-// x as whole tiles of rows for the copies straight to LDS: zeros past the end
-// and where a row counts for nothing, which may hold anything.
-__global__ __launch_bounds__(256) void k_loss_rows(Matrix x, const int32_t *__restrict__ targets,
+// Rows for the copies straight to LDS: out_rows x out_cols, zeros past the ends and
+// (targets not null) where a row counts for nothing, which may hold anything.
+__global__ __launch_bounds__(256) void k_loss_pack(Matrix in, const int32_t *__restrict__ targets,
                                                    uint32_t vocabulary, bf16 *__restrict__ out,
-                                                   uint64_t out_rows) {
-  const uint32_t vecs = x.cols / 8;
+                                                   uint64_t out_rows, uint32_t out_cols) {
+  const uint32_t vecs = out_cols / 8;
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < out_rows * vecs;
        i += (uint64_t)gridDim.x * 256) {
-    const uint64_t r = i / vecs, c = i % vecs * 8;
-    u32x4 v = {0, 0, 0, 0};
-    if (r < x.rows && (uint32_t)targets[r] < vocabulary)
-      v = *(const NSFPS_GLOBAL_SEQ u32x4 *)((const bf16 *)x.p + r * x.ld + c);
-    *(NSFPS_GLOBAL_SEQ u32x4 *)(out + r * x.cols + c) = v;
+    const uint64_t r = i / vecs;
+    const uint32_t c = (uint32_t)(i % vecs) * 8;
+    Eight<bf16> v = {};
+    if (r < in.rows && c < in.cols && (!targets || (uint32_t)targets[r] < vocabulary)) {
+      const bf16 *const row = (const bf16 *)in.p + r * in.ld + c;
+      v = c + 8 <= in.cols ? load_eight<bf16>(row) : load_some<bf16>(row, in.cols - c);
+    }
+    *(NSFPS_GLOBAL_SEQ u32x4 *)(out + r * out_cols + c) = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
   }
 }
 
@@ -795,8 +798,8 @@ uint32_t xcd_grid(uint64_t work) { return (uint32_t)((work + 7) / 8 * 8); }
 
 // Vocabulary tiles a workgroup takes one after another, and such sweeps: the
 // least time for rounds of 512 workgroups, which need about as long to begin as
-// for XX tiles.  us with sweeps of 2 and of 8 tiles (16,384 tokens x 4,096 rows,
-// width 256): YY.
+// for 1.5 tiles.  us of the derivatives with sweeps of 2 and of 8 tiles (16,384
+// tokens x 4,096 rows, width 256): 77 and 61.
 void plan_sweeps(uint32_t ttiles, uint32_t vtiles, uint32_t &sweep, uint32_t &sweeps) {
   uint64_t best = ~0ull;
   const uint64_t most = 1u << 23;  // workgroups of a launch
@@ -811,7 +814,8 @@ void plan_sweeps(uint32_t ttiles, uint32_t vtiles, uint32_t &sweep, uint32_t &sw
 }
 
 // Tiles of a call through registers: of 64 where those of 128 leave CUs without
-// one.  us (130 tokens x 901 x 847 bfloat16 with gradient): XX.
+// one.  us (130 tokens x 901 x 847 bfloat16): statistics 15, 32 with tiles of 128;
+// derivatives 15 and 33.
 uint32_t staged_tile(uint64_t tokens, uint64_t rows) {
   return host_ceil_div(tokens, 128) * host_ceil_div(rows, 128) <= 128 ? 64 : 128;
 }
@@ -824,88 +828,56 @@ Tiling tiling(uint64_t tokens, uint64_t rows, uint32_t tile) {
   return t;
 }
 
-// Whether a call's tiles go straight to LDS hangs on its addresses, the workspace
-// does not: it has room for either.
+// (How tiles come to LDS hangs on a call's addresses too; the workspace has room for
+// either way.)
 constexpr uint32_t kPad = 256;  // of tokens and pieces: whole tiles of any kind
 
-struct GradPlan {
-  uint64_t tokens;             // padded
-  uint64_t piece, pieces;      // vocabulary rows of a piece, a multiple of kPad
-  uint32_t mt, nt;             // rows and columns of a product's tile
-  uint32_t per, dx_splits, de_splits;
-  uint64_t d_size, d_ld;       // (rows a whole number of 4 KB apart meet in one memory channel)
-  bool direct, dx_sums, de_sums;
-  uint64_t x, d, dx, de, bytes;  // workspace offsets
-};
-// k of a split, of both products alike.  at_once workgroups run at once and take 1
-// us for 64 terms of a pass; splits' sums go to memory and come back, 4 TB/s.  The
-// split with the least of both: 16,384 tokens and pieces of 4,096 rows, width 384
-// in float32, XX with it and YY with as many splits as just fill the chip.
-void plan_splits(GradPlan &p, uint64_t dx_tiles, uint64_t dx_terms, uint64_t de_tiles,
-                 uint64_t de_terms, uint32_t passes, uint64_t at_once, uint64_t dx_bytes,
-                 uint64_t de_bytes) {
-  double best = 0.;
-  for (uint64_t n = 1; n <= 512; ++n) {
-    const uint64_t per = up(host_ceil_div(std::max(dx_terms, de_terms), n), 64);
-    if (n > 1 && per < 256) break;
-    const uint64_t dx = host_ceil_div(dx_terms, per), de = host_ceil_div(de_terms, per);
-    const double rounds = (double)host_ceil_div(dx_tiles * dx + de_tiles * de, at_once);
-    const double longest = (double)std::min(per, std::max(dx_terms, de_terms));
-    const double sums = (dx > 1 || p.pieces > 1 ? 2. * dx * dx_bytes : 0.) +
-                        (de > 1 ? 2. * de * de_bytes : 0.);
-    const double us = rounds * longest / 64. * passes + sums / 4e6;
-    if (n == 1 || us < best) {
-      best = us;
-      p.per = (uint32_t)per;
-      p.dx_splits = (uint32_t)dx;
-      p.de_splits = (uint32_t)de;
-    }
-  }
-}
+// How a call's tiles come to LDS: through registers; straight from its inputs,
+// bfloat16 rows of whole 64s at 16-byte boundaries; or straight from copies of
+// them in the workspace, bfloat16 rows padded with zeros, a piece of the vocabulary
+// at a time.
+enum class Way { kStaged, kDirect, kPacked };
 
-GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype, bool direct) {
-  GradPlan p = {};
-  p.tokens = up(a.tokens, kPad);
-  const uint64_t whole = up(a.rows, kPad);
-  p.bytes = 256;
-  if (!p.tokens || !whole) return p;
-  const bool one = a.dtype == NSFPS_BF16 && grad_dtype == NSFPS_BF16;
-  p.d_size = one ? 2 : 4;
-  // a piece of d: 64 million values, and 1,024 rows at least
-  constexpr uint64_t kValues = 1ull << 26;
-  p.piece = std::min(whole, std::max<uint64_t>(1024, kValues / p.tokens / kPad * kPad));
-  p.pieces = host_ceil_div(whole, p.piece);
-  p.direct = direct;
-  p.nt = direct ? (a.width % 256 == 0 ? 256 : a.width % 128 == 0 ? 128 : 64)
-                : a.width <= 64 ? 64 : 128;
-  p.mt = direct && p.nt < 256 ? 256 : kTile;
-  const uint64_t ntiles = host_ceil_div(a.width, p.nt), ld = ntiles * p.nt;
-  plan_splits(p, p.tokens / p.mt * ntiles, std::min(p.piece, a.rows), p.piece / p.mt * ntiles,
-              a.tokens, a.dtype == NSFPS_F32 ? 6 : one ? 1 : 2, direct ? 256 : 512,
-              4 * a.tokens * ld, 4 * p.piece * ld);
-  p.dx_sums = p.dx_splits > 1 || p.pieces > 1;
-  p.de_sums = p.de_splits > 1;
-  uint64_t at = 0;
-  const auto take = [&](uint64_t n) {
-    const uint64_t was = at;
-    at += bytes256(n);
-    return was;
-  };
-  p.x = take(one ? 2 * p.tokens * a.width : 0);
-  p.d_ld = p.piece + 256 / p.d_size;
-  p.d = take(p.d_size * p.tokens * p.d_ld);
-  p.dx = take(p.dx_sums ? 4 * p.dx_splits * a.tokens * ld : 0);
-  p.de = take(p.de_sums ? 4 * p.de_splits * p.piece * ld : 0);
-  p.bytes = at;
-  return p;
+// Whether copies of the inputs pay.  us with and without, 5,003 rows, loss: 512
+// tokens of width 847 29 and 34, 1,024 of 257 21 and 19, 8,192 of 65 31 and 35;
+// loss and gradient: 512 tokens of width 257 50 and 53, 1,024 of 65 54 and 49,
+// 2,048 of 65 66 and 68, 8,192 of 847 420 and 532, 200 of 847 72 and 65.  (Three
+// planes of a float32 call's terms lost by up to a quarter: the products of the
+// terms bound it, not the loads.)
+bool loss_packs(const nsfps_loss_args &a) {
+  return a.dtype == NSFPS_BF16 && a.tokens >= 512 && a.rows >= kPad &&
+         a.tokens * a.width >= 400000;
 }
-
-// Whether tiles can go straight to LDS: bfloat16 rows of whole 64s at 16-byte
-// boundaries.
-bool direct_rows(const nsfps_loss_args &a) {
+bool grad_packs(const nsfps_loss_args &a, bool one) {
+  return one && a.tokens >= 512 && a.rows >= kPad && a.tokens * a.width >= 1u << 17;
+}
+bool direct_sizes(const nsfps_loss_args &a) {
   return a.dtype == NSFPS_BF16 && a.width % 64 == 0 && a.x_stride % 8 == 0 &&
-         a.table_stride % 8 == 0 && ((uintptr_t)a.d_x | (uintptr_t)a.d_table) % 16 == 0 &&
+         a.table_stride % 8 == 0 &&
          std::max(a.x_stride, a.table_stride) < 1u << 23;  // (a Feed's offsets)
+}
+bool direct_places(const nsfps_loss_args &a) {
+  return ((uintptr_t)a.d_x | (uintptr_t)a.d_table) % 16 == 0;
+}
+
+LogitDev logits(const nsfps_loss_args &a, const Matrix &x, const Matrix &e, uint64_t row0,
+                uint64_t x_rows, uint64_t e_rows, uint32_t tile) {
+  LogitDev d = {};
+  d.x = x;
+  d.e = e;
+  d.tiles = tiling(x_rows, e_rows, tile);
+  d.scale2 = a.scale * kLog2e;
+  d.row0 = (uint32_t)row0;
+  d.lse = a.d_lse;
+  return d;
+}
+// x and rows of the table as they are
+Matrix x_of(const nsfps_loss_args &a) {
+  return {a.d_x, a.x_stride, (uint32_t)a.tokens, a.width};
+}
+Matrix table_of(const nsfps_loss_args &a, uint64_t row0, uint64_t rows) {
+  return {(const char *)a.d_table + row0 * a.table_stride * (a.dtype == NSFPS_F32 ? 4 : 2),
+          a.table_stride, (uint32_t)rows, a.width};
 }
 
 // f(the walk of tiles straight to LDS)
@@ -932,29 +904,34 @@ void by_ends(uint32_t width, uint32_t tile, F f) {
     tile == 64 ? f(EndsOf<Ends::kWide>(), two) : f(EndsOf<Ends::kWide>(), four);
 }
 
-LogitDev logits(const nsfps_loss_args &a, uint64_t row0, uint64_t rows, uint64_t x_rows,
-                uint64_t e_rows, uint32_t tile) {
-  LogitDev d = {};
-  const uint64_t size = a.dtype == NSFPS_F32 ? 4 : 2;
-  d.x = {a.d_x, a.x_stride, (uint32_t)a.tokens, a.width};
-  d.e = {(const char *)a.d_table + row0 * a.table_stride * size, a.table_stride, (uint32_t)rows,
-         a.width};
-  d.tiles = tiling(x_rows, e_rows, tile);
-  d.scale2 = a.scale * kLog2e;
-  d.row0 = (uint32_t)row0;
-  d.lse = a.d_lse;
-  return d;
+template <typename Logits>
+hipError_t run_stats(const LogitDev &d, hipStream_t st) {
+  k_loss_stats<Logits><<<xcd_grid((uint64_t)d.tiles.ttiles * d.tiles.sweeps), 256, 0, st>>>(d);
+  return hipGetLastError();
 }
-
+template <typename Logits, typename D>
+hipError_t run_d(const LogitDev &d, hipStream_t st) {
+  k_loss_d<Logits, D><<<xcd_grid((uint64_t)d.tiles.ttiles * d.tiles.sweeps), 256, 0, st>>>(d);
+  return hipGetLastError();
+}
 template <int WM, int WN, int MT>
 hipError_t run_direct(const ProductDev &dx, const ProductDev &de, uint32_t grid, hipStream_t st) {
   typedef DirectProduct<WM, WN, MT, false> X;
-  constexpr size_t lds = sizeof(typename X::Lds);
-  static_assert(lds == sizeof(typename DirectProduct<WM, WN, MT, true>::Lds) && lds <= 160 * 1024, "LDS");
-  const hipError_t e = hipFuncSetAttribute((const void *)k_loss_products_direct<WM, WN, MT>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-  if (e != hipSuccess) return e;
-  k_loss_products_direct<WM, WN, MT><<<grid, X::Prod::kThreads, lds, st>>>(dx, de);
+  const size_t lds = sizeof(typename X::Lds);
+  static_assert(sizeof(typename X::Lds) == sizeof(typename DirectProduct<WM, WN, MT, true>::Lds), "LDS");
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void *)k_loss_products_direct<WM, WN, MT>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  k_loss_products_direct<WM, WN, MT><<<grid, 64 * WM * WN, lds, st>>>(dx, de);
+  return hipGetLastError();
+}
+
+hipError_t run_pack(const Matrix &in, const int32_t *targets, uint32_t vocabulary, void *out,
+                    uint64_t out_rows, uint32_t out_cols, hipStream_t st) {
+  k_loss_pack<<<grid_of(out_rows * (out_cols / 8)), 256, 0, st>>>(in, targets, vocabulary,
+                                                                   (bf16 *)out, out_rows, out_cols);
   return hipGetLastError();
 }
 
@@ -982,71 +959,207 @@ hipError_t write_zeros(uint32_t dtype, void *out, uint64_t stride, uint64_t rows
     if (e_ != hipSuccess) return e_;      \
   } while (0)
 
+// Places in a workspace.
+struct Places {
+  uint64_t at = 0;
+  uint64_t take(uint64_t n) {
+    const uint64_t was = at;
+    at += bytes256(n);
+    return was;
+  }
+};
+
+struct LossPlan {
+  Way way;
+  uint32_t tile, width;  // of packed rows
+  uint64_t piece, pieces, nparts;  // rows of a piece; parts of all pieces
+  uint64_t parts, x, e, bytes;
+};
+LossPlan loss_plan(const nsfps_loss_args &a, Way way) {
+  LossPlan p = {};
+  p.way = way;
+  p.tile = way == Way::kStaged ? staged_tile(a.tokens, a.rows) : kTile;
+  p.width = (uint32_t)up(a.width, 64);
+  p.piece = way == Way::kPacked ? std::min<uint64_t>(a.rows, 1u << 16) : a.rows;
+  p.pieces = a.rows ? host_ceil_div(a.rows, p.piece) : 0;
+  for (uint64_t k = 0; k < std::min<uint64_t>(p.pieces, 2); ++k) {  // whole pieces, and the last
+    const uint64_t rows = k ? a.rows - (p.pieces - 1) * p.piece : p.piece,
+                   sweeps = tiling(a.tokens, rows, p.tile).sweeps;
+    p.nparts += k ? sweeps : p.pieces > 1 ? (p.pieces - 1) * sweeps : sweeps;
+  }
+  Places w;
+  p.parts = w.take(8 * p.nparts * up(a.tokens, 16));
+  if (way == Way::kPacked) {
+    p.x = w.take(2ull * a.tokens * p.width);
+    p.e = w.take(2ull * p.piece * p.width);
+  }
+  p.bytes = std::max<uint64_t>(256, w.at);
+  return p;
+}
+Way loss_fallback(const nsfps_loss_args &a) {
+  return loss_packs(a) ? Way::kPacked : Way::kStaged;
+}
+
+struct GradPlan {
+  Way way;
+  uint64_t tokens;             // padded
+  uint64_t piece, pieces;      // vocabulary rows of a piece, a multiple of kPad
+  uint32_t mt, nt;             // rows and columns of a product's tile
+  uint32_t width;              // of packed rows
+  uint32_t per, dx_splits, de_splits;
+  uint64_t d_size, d_ld;       // (rows a whole number of 4 KB apart meet in one memory channel)
+  bool dx_sums, de_sums;
+  uint64_t x, e, d, dx, de, bytes;  // workspace offsets
+};
+
+// k of a split, of both products alike.  at_once workgroups run at once and take 1
+// us for 64 terms of a pass; splits' sums go to memory and come back, 4 TB/s.  The
+// split with the least of both.  us of the products of 16,384 tokens and pieces of
+// 4,096 rows, width 383 in float32: 620 so, 888 with as many splits as just fill
+// the chip.
+void plan_splits(GradPlan &p, uint64_t dx_tiles, uint64_t dx_terms, uint64_t de_tiles,
+                 uint64_t de_terms, uint32_t passes, uint64_t at_once, uint64_t dx_bytes,
+                 uint64_t de_bytes) {
+  double best = 0.;
+  for (uint64_t n = 1; n <= 512; ++n) {
+    const uint64_t per = up(host_ceil_div(std::max(dx_terms, de_terms), n), 64);
+    if (n > 1 && per < 256) break;
+    const uint64_t dx = host_ceil_div(dx_terms, per), de = host_ceil_div(de_terms, per);
+    const double rounds = (double)host_ceil_div(dx_tiles * dx + de_tiles * de, at_once);
+    const double longest = (double)std::min(per, std::max(dx_terms, de_terms));
+    const double sums = (dx > 1 || p.pieces > 1 ? 2. * dx * dx_bytes : 0.) +
+                        (de > 1 ? 2. * de * de_bytes : 0.);
+    const double us = rounds * longest / 64. * passes + sums / 4e6;
+    if (n == 1 || us < best) {
+      best = us;
+      p.per = (uint32_t)per;
+      p.dx_splits = (uint32_t)dx;
+      p.de_splits = (uint32_t)de;
+    }
+  }
+}
+
+GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype, Way way) {
+  GradPlan p = {};
+  p.way = way;
+  p.tokens = up(a.tokens, kPad);
+  const uint64_t whole = up(a.rows, kPad);
+  p.bytes = 256;
+  if (!p.tokens || !whole) return p;
+  const bool one = a.dtype == NSFPS_BF16 && grad_dtype == NSFPS_BF16, direct = way != Way::kStaged;
+  p.width = (uint32_t)up(a.width, 64);
+  p.d_size = one ? 2 : 4;
+  // a piece of d: 64 million values, and 1,024 rows at least
+  constexpr uint64_t kValues = 1ull << 26;
+  p.piece = std::min(whole, std::max<uint64_t>(1024, kValues / p.tokens / kPad * kPad));
+  p.pieces = host_ceil_div(whole, p.piece);
+  if (direct) {
+    p.nt = p.width % 256 == 0 ? 256 : p.width % 128 == 0 ? 128 : 64;
+    p.mt = p.nt < 256 ? 256 : kTile;
+  } else {
+    p.nt = a.width <= 64 ? 64 : 128;
+    p.mt = kTile;
+  }
+  const uint64_t ntiles = host_ceil_div(a.width, p.nt), ld = ntiles * p.nt;
+  plan_splits(p, p.tokens / p.mt * ntiles, std::min(p.piece, a.rows), p.piece / p.mt * ntiles,
+              a.tokens, a.dtype == NSFPS_F32 ? 6 : one ? 1 : 2, direct ? 256 : 512,
+              4 * a.tokens * ld, 4 * p.piece * ld);
+  p.dx_sums = p.dx_splits > 1 || p.pieces > 1;
+  p.de_sums = p.de_splits > 1;
+  Places w;
+  if (direct) p.x = w.take(2ull * p.tokens * p.width);
+  if (way == Way::kPacked) p.e = w.take(2ull * p.piece * p.width);
+  p.d_ld = p.piece + 256 / p.d_size;
+  p.d = w.take(p.d_size * p.tokens * p.d_ld);
+  p.dx = w.take(p.dx_sums ? 4 * p.dx_splits * a.tokens * ld : 0);
+  p.de = w.take(p.de_sums ? 4 * p.de_splits * p.piece * ld : 0);
+  p.bytes = w.at;
+  return p;
+}
+// (tokens are padded to whole tiles there, which few would pay for)
+bool grad_direct(const nsfps_loss_args &a, bool one) {
+  return one && a.tokens >= kPad && direct_sizes(a);
+}
+Way grad_fallback(const nsfps_loss_args &a, bool one) {
+  return grad_packs(a, one) ? Way::kPacked : Way::kStaged;
+}
+
 }  // namespace
 
 uint64_t loss_bytes(const nsfps_loss_args &a) {
-  const uint32_t sweeps = std::max(tiling(a.tokens, a.rows, kTile).sweeps,
-                                   tiling(a.tokens, a.rows, staged_tile(a.tokens, a.rows)).sweeps);
-  return std::max<uint64_t>(256, bytes256(8 * sweeps * up(a.tokens, 16)));
+  const uint64_t other = loss_plan(a, loss_fallback(a)).bytes;
+  return direct_sizes(a) ? std::max(other, loss_plan(a, Way::kDirect).bytes) : other;
 }
 
 hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
-  const bool direct = direct_rows(a);
-  const uint32_t tile = direct ? kTile : staged_tile(a.tokens, a.rows);
+  const Way way = direct_sizes(a) && direct_places(a) ? Way::kDirect : loss_fallback(a);
+  const LossPlan p = loss_plan(a, way);
+  char *const ws = (char *)a.workspace;
   const uint64_t stride = up(a.tokens, 16);
-  float2 *const parts = (float2 *)a.workspace;
-  LogitDev d = logits(a, 0, a.rows, a.tokens, a.rows, tile);
-  if (a.rows) {
+  Matrix x = x_of(a);
+  if (way == Way::kPacked) {
+    x = {ws + p.x, p.width, (uint32_t)a.tokens, p.width};
+    LAUNCH(run_pack(x_of(a), nullptr, 0, ws + p.x, a.tokens, p.width, st));
+  }
+  float2 *parts = (float2 *)(ws + p.parts);
+  for (uint64_t k = 0; k < p.pieces; ++k) {
+    const uint64_t row0 = k * p.piece, rows = std::min(p.piece, a.rows - row0);
+    Matrix e = table_of(a, row0, rows);
+    if (way == Way::kPacked) {
+      LAUNCH(run_pack(e, nullptr, 0, ws + p.e, rows, p.width, st));
+      e = {ws + p.e, p.width, (uint32_t)rows, p.width};
+    }
+    LogitDev d = logits(a, x, e, row0, a.tokens, rows, p.tile);
     d.parts = parts;
     d.part_stride = stride;
-    const uint32_t grid = xcd_grid((uint64_t)d.tiles.ttiles * d.tiles.sweeps);
-    const auto go = [&](auto z) { k_loss_stats<decltype(z)><<<grid, 256, 0, st>>>(d); };
-    if (direct)
-      by_steps(a.width, go);
+    parts += d.tiles.sweeps * stride;
+    hipError_t rc = hipSuccess;
+    const auto go = [&](auto z) { rc = run_stats<decltype(z)>(d, st); };
+    if (way != Way::kStaged)
+      by_steps(p.width, go);
     else
-      by_ends(a.width, tile, [&](auto ends, auto tiles) {
+      by_ends(a.width, p.tile, [&](auto ends, auto tiles) {
         constexpr Ends kEnds = decltype(ends)::value;
         constexpr int kTiles = decltype(tiles)::value;
         a.dtype == NSFPS_F32 ? go(StagedLogits<float, 3, false, kEnds, kTiles>())
                              : go(StagedLogits<bf16, 1, true, kEnds, kTiles>());
       });
-    LAUNCH(hipGetLastError());
+    LAUNCH(rc);
   }
   const auto join = [&](auto t) {
     uint32_t group = 16;  // as many workgroups as fill the chip
     while (group > 1 && a.tokens / group < 256) group /= 2;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(1u << 16, host_ceil_div(a.tokens, group));
     k_loss_join<decltype(t)><<<grid, 256, 0, st>>>(
-        parts, d.tiles.sweeps, stride, group,
-        Matrix{a.d_x, a.x_stride, (uint32_t)a.tokens, a.width},
-        Matrix{a.d_table, a.table_stride, (uint32_t)a.rows, a.width}, a.scale, a.d_targets, a.d_loss,
-        a.d_lse);
+        (const float2 *)(ws + p.parts), (uint32_t)p.nparts, stride, group, x_of(a),
+        table_of(a, 0, a.rows), a.scale, a.d_targets, a.d_loss, a.d_lse);
     return hipGetLastError();
   };
   return a.dtype == NSFPS_F32 ? join(float()) : join(bf16());
 }
 
 uint64_t loss_grad_bytes(const nsfps_loss_args &a, const nsfps_loss_grads &g) {
-  return std::max(grad_plan(a, g.grad_dtype, false).bytes, grad_plan(a, g.grad_dtype, true).bytes);
+  const bool one = a.dtype == NSFPS_BF16 && g.grad_dtype == NSFPS_BF16;
+  const uint64_t other = grad_plan(a, g.grad_dtype, grad_fallback(a, one)).bytes;
+  return grad_direct(a, one) ? std::max(other, grad_plan(a, g.grad_dtype, Way::kDirect).bytes) : other;
 }
 
 hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g, hipStream_t st) {
-  // (tokens are padded to whole tiles there, which few would pay for)
-  const bool direct = g.grad_dtype == NSFPS_BF16 && a.tokens >= kPad && direct_rows(a);
-  const GradPlan p = grad_plan(a, g.grad_dtype, direct);
+  const bool one = a.dtype == NSFPS_BF16 && g.grad_dtype == NSFPS_BF16;
+  const Way way = grad_direct(a, one) && direct_places(a) ? Way::kDirect : grad_fallback(a, one);
+  const bool direct = way != Way::kStaged;
+  const GradPlan p = grad_plan(a, g.grad_dtype, way);
   if (!p.pieces) {
     LAUNCH(write_zeros(a.dtype, g.d_dx, g.dx_stride, a.tokens, a.width, st));
     return write_zeros(g.grad_dtype, g.d_dtable, g.dtable_stride, a.rows, a.width, st);
   }
   char *const ws = (char *)a.workspace;
-  const bool one = p.d_size == 2;
   const uint32_t ntiles = (uint32_t)host_ceil_div(a.width, p.nt);
   const uint64_t z = g.grad_dtype == NSFPS_F32 ? 4 : 2;
-  const Matrix x = {a.d_x, a.x_stride, (uint32_t)a.tokens, a.width};
-  if (direct) {
-    k_loss_rows<<<grid_of(p.tokens * a.width / 8), 256, 0, st>>>(
-        x, a.d_targets, (uint32_t)a.rows, (bf16 *)(ws + p.x), p.tokens);
-    LAUNCH(hipGetLastError());
+  Matrix x = x_of(a);
+  if (direct) {  // whole tiles, and zeros for rows that count for nothing
+    LAUNCH(run_pack(x, a.d_targets, (uint32_t)a.rows, ws + p.x, p.tokens, p.width, st));
+    x = {ws + p.x, p.width, (uint32_t)p.tokens, p.width};
   }
   ProductDev dx = {};
   dx.weights = {g.d_dloss, a.d_targets, (uint32_t)a.tokens, (uint32_t)a.rows, a.scale};
@@ -1063,37 +1176,37 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
   dx.sums_split = a.tokens * dx.sums_ld;
   for (uint64_t k = 0; k < p.pieces; ++k) {
     const uint64_t row0 = k * p.piece, rows = std::min(p.piece, a.rows - row0);
-    // straight to LDS, whole tiles of every product
-    LogitDev l = direct ? logits(a, row0, rows, p.tokens, up(rows, kPad), kTile)
-                        : logits(a, row0, rows, a.tokens, rows, staged_tile(a.tokens, rows));
-    if (direct) l.x = {ws + p.x, a.width, (uint32_t)p.tokens, a.width};
+    Matrix e = table_of(a, row0, rows);
+    if (way == Way::kPacked) {
+      LAUNCH(run_pack(e, nullptr, 0, ws + p.e, rows, p.width, st));
+      e = {ws + p.e, p.width, (uint32_t)rows, p.width};
+    }
+    const uint32_t tile = direct ? kTile : staged_tile(a.tokens, rows);
+    LogitDev l = direct ? logits(a, x, e, row0, p.tokens, up(rows, kPad), tile)
+                        : logits(a, x, e, row0, a.tokens, rows, tile);
     l.weights = dx.weights;
     l.d = ws + p.d;
     l.d_ld = p.d_ld;
-    const uint32_t grid = xcd_grid((uint64_t)l.tiles.ttiles * l.tiles.sweeps);
+    hipError_t rc = hipSuccess;
     if (direct)
-      by_steps(a.width, [&](auto z) { k_loss_d<decltype(z), bf16><<<grid, 256, 0, st>>>(l); });
+      by_steps(p.width, [&](auto w) { rc = run_d<decltype(w), bf16>(l, st); });
     else
-      by_ends(a.width, staged_tile(a.tokens, rows), [&](auto ends, auto tiles) {
+      by_ends(a.width, tile, [&](auto ends, auto tiles) {
         constexpr Ends kEnds = decltype(ends)::value;
         constexpr int kTiles = decltype(tiles)::value;
-        if (a.dtype == NSFPS_F32)
-          k_loss_d<StagedLogits<float, 3, false, kEnds, kTiles>, float><<<grid, 256, 0, st>>>(l);
-        else if (one)
-          k_loss_d<StagedLogits<bf16, 1, true, kEnds, kTiles>, bf16><<<grid, 256, 0, st>>>(l);
-        else
-          k_loss_d<StagedLogits<bf16, 1, false, kEnds, kTiles>, float><<<grid, 256, 0, st>>>(l);
+        rc = a.dtype == NSFPS_F32 ? run_d<StagedLogits<float, 3, false, kEnds, kTiles>, float>(l, st)
+             : one ? run_d<StagedLogits<bf16, 1, true, kEnds, kTiles>, bf16>(l, st)
+                   : run_d<StagedLogits<bf16, 1, false, kEnds, kTiles>, float>(l, st);
       });
-    LAUNCH(hipGetLastError());
+    LAUNCH(rc);
 
-    const Matrix d = {ws + p.d, p.d_ld, (uint32_t)(direct ? p.tokens : a.tokens), (uint32_t)rows};
-    dx.m = d;
-    dx.n = l.e;
+    dx.m = {ws + p.d, p.d_ld, (uint32_t)(direct ? p.tokens : a.tokens), (uint32_t)rows};
+    dx.n = e;
     dx.terms = (uint32_t)rows;
     dx.splits = p.dx_splits;  // those of a short last piece may be empty: they add nothing
     dx.add = k > 0;
     ProductDev de = dx;
-    de.n = direct ? Matrix{ws + p.x, a.width, (uint32_t)p.tokens, a.width} : x;
+    de.n = x;
     de.mtiles = (uint32_t)host_ceil_div(rows, p.mt);
     de.terms = (uint32_t)a.tokens;
     de.splits = p.de_splits;
@@ -1119,13 +1232,15 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     };
     constexpr std::integral_constant<int, 2> two;
     constexpr std::integral_constant<int, 4> four;
-    const hipError_t e = p.nt == 256             ? run_direct<2, 4, 4>(dx, de, work, st)
-                         : direct && p.nt == 128 ? run_direct<4, 2, 4>(dx, de, work, st)
-                         : direct                ? run_direct<4, 1, 4>(dx, de, work, st)
-                         : a.width < 8           ? staged(two, EndsOf<Ends::kNarrow>())
-                         : p.nt == 64            ? staged(two, EndsOf<Ends::kWide>())
-                                                 : staged(four, EndsOf<Ends::kWide>());
-    LAUNCH(e);
+    if (direct)
+      rc = p.nt == 256   ? run_direct<2, 4, 4>(dx, de, work, st)
+           : p.nt == 128 ? run_direct<4, 2, 4>(dx, de, work, st)
+                         : run_direct<4, 1, 4>(dx, de, work, st);
+    else
+      rc = a.width < 8   ? staged(two, EndsOf<Ends::kNarrow>())
+           : p.nt == 64 ? staged(two, EndsOf<Ends::kWide>())
+                        : staged(four, EndsOf<Ends::kWide>());
+    LAUNCH(rc);
     const bool last = k + 1 == p.pieces;
     if (de.sums) LAUNCH(write_out(de, last && dx.sums ? &dx : nullptr, st));
     if (!de.sums && last && dx.sums) LAUNCH(write_out(dx, nullptr, st));
@@ -1134,8 +1249,9 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
 }
 
 hipError_t preload_loss_kernels() {
-  return func_attributes(k_loss_stats<DirectLogits>, k_loss_join<bf16>, k_loss_d<DirectLogits, bf16>,
-                         k_loss_products_direct<2, 4, 4>, k_loss_out, k_loss_rows);
+  return func_attributes(k_loss_stats<ResidentLogits<128, 2>>, k_loss_join<bf16>,
+                         k_loss_d<ResidentLogits<128, 2>, bf16>, k_loss_products_direct<2, 4, 4>,
+                         k_loss_out, k_loss_pack);
 }
 
 }  // namespace nsfps

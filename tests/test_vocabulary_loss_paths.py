@@ -74,6 +74,50 @@ def test_pieces_straight_to_lds(lib, width):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # rows copied for the gradient; for the loss too; several pieces of the table in
+    # the loss, the last one short; several in the gradient
+    (3000, 257, 72, 3), (6000, 700, 83, 5), (513, 256, 840, 0), (600, 66000, 700, 1),
+    (66000, 2300, 33, 0)])
+def test_rows_copied_first(lib, case):  # noqa: F811
+    """Many tokens with rows that cannot go straight to LDS; NaN beside the rows."""
+    got, want = both(lib, case, "bf16", "bf16")
+    check(got, want, "bf16", "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [128, 320])
+def test_addresses_do_not_matter(lib, width):  # noqa: F811
+    """Rows of whole 64s at odd addresses give the bits of aligned ones, in a
+    workspace of the same size; rows that count for nothing hold NaN."""
+    n, rows = 4000, 777
+    case = (n, rows, width, 0)
+    t, code, gen, x, table, target, scale = inputs(case, "bf16")
+    dloss = rnd(gen, n).cuda()
+    x[(target < 0) | (target >= rows)] = float("nan")
+    results = []
+    for shift in (0, 1):
+        xd, td = (torch.empty(v.numel() + 8, dtype=t, device="cuda")[shift:shift + v.numel()]
+                  .view(v.shape).copy_(v) for v in (x, table))
+        tg = target.cuda()
+        loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+        args = args_of(case, code, xd, td, tg, scale, loss, lse)
+        dx, dtable = torch.empty_like(xd), torch.empty_like(td)
+        grads = capi.LossGrads(d_dloss=ptr(dloss), dx_stride=width, dtable_stride=width,
+                               grad_dtype=code, d_dx=ptr(dx), d_dtable=ptr(dtable))
+        sizes = lib.loss_workspace_bytes(args), lib.loss_grad_workspace_bytes(args, grads)
+        ws = give(args, max(sizes))
+        lib.loss_device(args, stream())
+        lib.loss_grad_device(args, grads, stream())
+        torch.cuda.synchronize()
+        results.append((sizes, loss, dx, dtable))
+        del ws
+    assert results[0][0] == results[1][0]
+    for a, b in zip(results[0][1:], results[1][1:]):
+        assert torch.equal(a, b) and not a.isnan().any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale", [-0.7, 0.0, 3.0])
 @pytest.mark.parametrize("case,dtype", [((300, 700, 64, 0), "bf16"), ((300, 333, 320, 0), "bf16"),
                                         ((90, 200, 50, 0), "f32"), ((90, 200, 50, 0), "bf16")])
