@@ -49,13 +49,16 @@ struct Weights {
   uint32_t tokens, vocabulary;
   float scale;
 
+  // (loads that wait for no other: all of them are asked for at once)
+  __device__ __forceinline__ uint32_t in(uint32_t token) const { return min(token, tokens - 1); }
   __device__ __forceinline__ bool counts(uint32_t token) const {
-    return token < tokens && (uint32_t)targets[token] < vocabulary;
+    const uint32_t target = (uint32_t)targets[in(token)];
+    return token < tokens && target < vocabulary;
   }
   // That of the first of 64 tokens that counts, if it is of an ordinary size.
   __device__ __forceinline__ float reference() const {
     const uint32_t lane = threadIdx.x & 63u;
-    const float w = counts(lane) ? dloss[lane] * scale : 0.f;
+    const float own = dloss[in(lane)] * scale, w = counts(lane) ? own : 0.f;
     const uint64_t fit = __ballot(fabsf(w) >= 0x1p-30f && fabsf(w) <= 0x1p30f);
     return fit ? __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), __builtin_ctzll(fit)))
                : 1.f;
@@ -86,8 +89,8 @@ struct LogitDev {
 };
 
 // Workgroup w's tile of tokens and sweep, the latter as vocabulary tiles of N rows:
-// tokens change fastest, within groups
-// that share sweeps, so that workgroups of one XCD read the same rows.
+// tokens change fastest, within groups that share sweeps, so that workgroups of one
+// XCD read the same rows.
 template <uint32_t N, uint32_t kUnit>
 __device__ __forceinline__ bool logit_item(const LogitDev &a, uint32_t &ttile, uint32_t &sweep,
                                            uint32_t &first, uint32_t &last) {
@@ -417,15 +420,13 @@ struct Derivatives {
     const float reference = a.weights.reference();
 #pragma unroll
     for (int i = 0; i < Prod::kMT; ++i) {
-      const uint32_t token = token0 + 16 * i;
-      lse2[i] = weight[i] = 0.f;
-      target[i] = ~0u;
+      const uint32_t token = token0 + 16 * i, at = a.weights.in(token);
+      const float lse = a.lse[at] * kLog2e,
+                  own = a.weights.dloss[at] * a.weights.scale / reference;
       counts[i] = a.weights.counts(token);
-      if (counts[i]) {
-        lse2[i] = a.lse[token] * kLog2e;
-        weight[i] = a.weights.dloss[token] * a.weights.scale / reference;
-        target[i] = (uint32_t)a.weights.targets[token] - a.row0;
-      }
+      lse2[i] = counts[i] ? lse : 0.f;
+      weight[i] = counts[i] ? own : 0.f;
+      target[i] = counts[i] ? (uint32_t)a.weights.targets[at] - a.row0 : ~0u;
     }
   }
   // no column past the end, no token's target, and no token that does not count
@@ -703,6 +704,7 @@ __global__ __launch_bounds__(256, 2) void k_loss_products(ProductDev dx, Product
   else
     E::run(de, lds.e, w);
 }
+
 template <int WM, int WN, int MT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_loss_products_direct(ProductDev dx, ProductDev de) {
   typedef DirectProduct<WM, WN, MT, false> X;
