@@ -290,7 +290,7 @@ nsfps_status nsfps_ball_query_device(const float *d_xyz, uint64_t n, const float
  * caller's: a call with a _workspace_bytes companion needs that many bytes
  * at workspace (aligned to 256), whose contents need not be kept, and which
  * calls that may overlap must not share.  The first call of an operator on a
- * device loads its kernels (six milliseconds for all of them);
+ * device loads its kernels (seven and a half milliseconds for all of them);
  * nsfps_init_sequence_device does that ahead, before a capture for instance.
  * No output may overlap an input or another output.  A workspace that is too
  * small, a size or stride that does not fit and a null pointer are
@@ -529,8 +529,10 @@ nsfps_status nsfps_dropout_device(const nsfps_dropout_args *args, void *stream);
  *
  * A row of the table that is not finite spoils every token.  At most 2^30
  * tokens, 2^31 - 1 rows, width at most 65,536.  The gradient takes the
- * vocabulary in pieces, whose products live in the workspace; its size goes by
- * sizes and types alone. */
+ * vocabulary in pieces, whose products live in the workspace, beside copies of
+ * rows that the kernels cannot take as they are; its size goes by sizes and types
+ * alone.  bfloat16 rows of a multiple of 64 values at 16-byte boundaries are the
+ * fastest. */
 typedef struct {
   uint64_t tokens, rows;
   uint32_t width, dtype;

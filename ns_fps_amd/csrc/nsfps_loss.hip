@@ -14,6 +14,17 @@
 // terms that reach 24 bits.  d is rounded to one term (8 bits) where the
 // products' results are bfloat16, to two for a float32 table gradient of
 // bfloat16 inputs, to three in float32 calls.  Sums are float32 everywhere.
+//
+// The matrix cores bound large calls: the statistics of 16,384 tokens, 262,144
+// rows of 256 bfloat16 take 1.96 ms, 1.12 PFLOP/s, as fast as a plain product of
+// 8,192^3 (1.13).  Their gradient takes 64 pieces of 4,096 rows: d 62 us (30 of
+// them the product, 18 the 134 MB that it writes, the rest the start of its
+// workgroups), the two products that read it 70 us (0.98 PFLOP/s), the sums' rows
+// 5.6 us.  64 million values of d a piece: 32, 128 and 256 million were no faster,
+// and more than 128 million would not stay in the memory-side cache.  A float32
+// call's six products a product: 16,384 tokens, 8,192 rows, width 383 in 2.3 ms,
+// where float32 matrix instructions would need 2.7.  A table's one reading bounds
+// calls of few tokens: 7 tokens, 262,144 rows of 256 bfloat16 26 us, 5.1 TB/s.
 #include "nsfps_launch.h"
 #include "nsfps_product.h"
 
@@ -207,7 +218,7 @@ struct DirectLogits {
   }
 };
 
-// The same for widths of up to 256: a workgroup's tokens stay in registers, so
+// The same for widths of up to 256 and long sweeps: a workgroup's tokens stay in registers, so
 // that LDS, which gives 128 bytes a cycle, is read for the vocabulary alone (with
 // both from LDS those reads and the copies took half as long again as the
 // products).  Three stages are under way while a fourth is worked on.
@@ -721,6 +732,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_loss_products_direct(Produc
 
 // Rows for the copies straight to LDS: out_rows x out_cols, zeros past the ends and
 // (targets not null) where a row counts for nothing, which may hold anything.
+// Memory bound: 16,384 rows of 256 5.8 us.
 __global__ __launch_bounds__(256) void k_loss_pack(Matrix in, const int32_t *__restrict__ targets,
                                                    uint32_t vocabulary, bf16 *__restrict__ out,
                                                    uint64_t out_rows, uint32_t out_cols) {
@@ -817,7 +829,7 @@ void plan_sweeps(uint32_t ttiles, uint32_t vtiles, uint32_t &sweep, uint32_t &sw
 
 // Tiles of a call through registers: of 64 where those of 128 leave CUs without
 // one.  us (130 tokens x 901 x 847 bfloat16): statistics 15, 32 with tiles of 128;
-// derivatives 15 and 33.
+// derivatives 15 and 33; all of 64 tokens x 5,003 x 256 30 and 36.
 uint32_t staged_tile(uint64_t tokens, uint64_t rows) {
   return host_ceil_div(tokens, 128) * host_ceil_div(rows, 128) <= 128 ? 64 : 128;
 }
@@ -840,18 +852,27 @@ constexpr uint32_t kPad = 256;  // of tokens and pieces: whole tiles of any kind
 // at a time.
 enum class Way { kStaged, kDirect, kPacked };
 
-// Whether copies of the inputs pay.  us with and without, 5,003 rows, loss: 512
-// tokens of width 847 29 and 34, 1,024 of 257 21 and 19, 8,192 of 65 31 and 35;
-// loss and gradient: 512 tokens of width 257 50 and 53, 1,024 of 65 54 and 49,
-// 2,048 of 65 66 and 68, 8,192 of 847 420 and 532, 200 of 847 72 and 65.  (Three
-// planes of a float32 call's terms lost by up to a quarter: the products of the
-// terms bound it, not the loads.)
+// Tiles of z of a call.
+uint64_t whole_tiles(const nsfps_loss_args &a) {
+  return host_ceil_div(a.tokens, kTile) * host_ceil_div(a.rows, kTile);
+}
+// Whether copies of the inputs pay for the loss.  us with and without, 5,003 rows:
+// 512 tokens of width 847 29 and 34, 1,024 of 257 21 and 19, 8,192 of 65 31 and 35.
 bool loss_packs(const nsfps_loss_args &a) {
   return a.dtype == NSFPS_BF16 && a.tokens >= 512 && a.rows >= kPad &&
-         a.tokens * a.width >= 400000;
+         whole_tiles(a) * a.width >= 1u << 17;
 }
-bool grad_packs(const nsfps_loss_args &a, bool one) {
-  return one && a.tokens >= 512 && a.rows >= kPad && a.tokens * a.width >= 1u << 17;
+// Whether the gradient's tiles go straight to LDS, from the inputs or their copies
+// (tokens are padded to whole tiles there, and all tiles are of 128).  us of loss
+// and gradient so and through registers, aligned: 256 tokens x 5,003 rows x width
+// 256 39 and 33, 512 x 5,003 x 256 41 and 41, 1,024 x 5,003 x 256 48 and 51, 2,048
+// x 1,024 x 1,024 74 and 70, 2,048 x 5,003 x 1,024 164 and 197; copied: 512 x 5,003
+// x 257 49 and 53, 1,024 x 5,003 x 65 54 and 49, 8,192 x 5,003 x 847 420 and 532.
+// (Three planes of a float32 call's terms, copied, lost by up to a quarter: the
+// products of the terms bound it, not the loads.)
+bool grad_straight(const nsfps_loss_args &a, bool one) {
+  return one && a.tokens >= kPad && a.rows >= kPad && whole_tiles(a) > 128 &&
+         whole_tiles(a) * a.width >= 40000;
 }
 bool direct_sizes(const nsfps_loss_args &a) {
   return a.dtype == NSFPS_BF16 && a.width % 64 == 0 && a.x_stride % 8 == 0 &&
@@ -882,9 +903,14 @@ Matrix table_of(const nsfps_loss_args &a, uint64_t row0, uint64_t rows) {
           a.table_stride, (uint32_t)rows, a.width};
 }
 
-// f(the walk of tiles straight to LDS)
+// f(the walk of tiles straight to LDS).  Tokens in registers, which take their time
+// to come there, pay in long sweeps.  us of the loss with and without, width 256:
+// 16,384 tokens x 16,384 rows (sweeps of 32 tiles) 141 and 164, x 4,096 (8) 50 and
+// 51, x 2,048 (4) 35 and 32, 4,096 x 2,048 (1) 20 and 14; width 128, 16,384 tokens
+// x 4,096 rows 32 and 34, x 2,048 22 and 22, x 1,024 (2) 18 and 15.
 template <typename F>
-void by_steps(uint32_t width, F f) {
+void by_steps(uint32_t width, uint32_t sweep, F f) {
+  if (sweep < 8) return f(DirectLogits());
   switch (width) {
     case 64: return f(ResidentLogits<64, 1>());
     case 128: return f(ResidentLogits<128, 1>());
@@ -1055,6 +1081,8 @@ GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype, Way way) {
   constexpr uint64_t kValues = 1ull << 26;
   p.piece = std::min(whole, std::max<uint64_t>(1024, kValues / p.tokens / kPad * kPad));
   p.pieces = host_ceil_div(whole, p.piece);
+  // columns: us of 8,192 x 5,003 x 256 bfloat16 140, 142 with 128; of 16,384 x 8,192
+  // x 64 float32 521, 632 with 128
   if (direct) {
     p.nt = p.width % 256 == 0 ? 256 : p.width % 128 == 0 ? 128 : 64;
     p.mt = p.nt < 256 ? 256 : kTile;
@@ -1078,12 +1106,8 @@ GradPlan grad_plan(const nsfps_loss_args &a, uint32_t grad_dtype, Way way) {
   p.bytes = w.at;
   return p;
 }
-// (tokens are padded to whole tiles there, which few would pay for)
-bool grad_direct(const nsfps_loss_args &a, bool one) {
-  return one && a.tokens >= kPad && direct_sizes(a);
-}
-Way grad_fallback(const nsfps_loss_args &a, bool one) {
-  return grad_packs(a, one) ? Way::kPacked : Way::kStaged;
+Way grad_way(const nsfps_loss_args &a, bool one, bool direct) {
+  return !grad_straight(a, one) ? Way::kStaged : direct ? Way::kDirect : Way::kPacked;
 }
 
 }  // namespace
@@ -1118,7 +1142,7 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
     hipError_t rc = hipSuccess;
     const auto go = [&](auto z) { rc = run_stats<decltype(z)>(d, st); };
     if (way != Way::kStaged)
-      by_steps(p.width, go);
+      by_steps(p.width, d.tiles.sweep, go);
     else
       by_ends(a.width, p.tile, [&](auto ends, auto tiles) {
         constexpr Ends kEnds = decltype(ends)::value;
@@ -1129,7 +1153,9 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
     LAUNCH(rc);
   }
   const auto join = [&](auto t) {
-    uint32_t group = 16;  // as many workgroups as fill the chip
+    // as many workgroups as fill the chip (us of 7 tokens x 262,144 rows 30, 46 with
+    // 16 tokens a workgroup; with gradient 16,384 x 8,192 x 64 220, 235 with one)
+    uint32_t group = 16;
     while (group > 1 && a.tokens / group < 256) group /= 2;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(1u << 16, host_ceil_div(a.tokens, group));
     k_loss_join<decltype(t)><<<grid, 256, 0, st>>>(
@@ -1142,13 +1168,12 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
 
 uint64_t loss_grad_bytes(const nsfps_loss_args &a, const nsfps_loss_grads &g) {
   const bool one = a.dtype == NSFPS_BF16 && g.grad_dtype == NSFPS_BF16;
-  const uint64_t other = grad_plan(a, g.grad_dtype, grad_fallback(a, one)).bytes;
-  return grad_direct(a, one) ? std::max(other, grad_plan(a, g.grad_dtype, Way::kDirect).bytes) : other;
+  return grad_plan(a, g.grad_dtype, grad_way(a, one, false)).bytes;  // (the copies' is the larger)
 }
 
 hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g, hipStream_t st) {
   const bool one = a.dtype == NSFPS_BF16 && g.grad_dtype == NSFPS_BF16;
-  const Way way = grad_direct(a, one) && direct_places(a) ? Way::kDirect : grad_fallback(a, one);
+  const Way way = grad_way(a, one, direct_sizes(a) && direct_places(a));
   const bool direct = way != Way::kStaged;
   const GradPlan p = grad_plan(a, g.grad_dtype, way);
   if (!p.pieces) {
@@ -1191,7 +1216,7 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     l.d_ld = p.d_ld;
     hipError_t rc = hipSuccess;
     if (direct)
-      by_steps(p.width, [&](auto w) { rc = run_d<decltype(w), bf16>(l, st); });
+      by_steps(p.width, l.tiles.sweep, [&](auto w) { rc = run_d<decltype(w), bf16>(l, st); });
     else
       by_ends(a.width, tile, [&](auto ends, auto tiles) {
         constexpr Ends kEnds = decltype(ends)::value;

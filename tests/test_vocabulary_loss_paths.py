@@ -57,6 +57,9 @@ def check(got, want, dtype, grad):
     # through registers: large tiles, narrow rows, widths around a stage's ends
     (2000, 3000, 40, 0), (3000, 2000, 72, 3), (300, 500, 1, 0), (129, 300, 3, 0), (1500, 2500, 7, 1),
     (200, 300, 8, 0), (200, 300, 9, 0), (64, 65, 65, 0), (70, 70, 127, 0), (2100, 1200, 95, 0),
+    # the gradient straight to LDS too: every width of a product's tiles
+    (2000, 1100, 320, 0), (1000, 2300, 512, 8), (900, 3100, 256, 0), (4100, 2500, 64, 0),
+    (2100, 2500, 128, 0), (257, 6000, 384, 0),
     # few rows, few tokens
     (1000, 1, 64, 0), (1000, 5, 33, 0), (1, 3000, 100, 0), (2, 2, 2, 0)])
 def test_every_path(lib, case, dtype, grad):  # noqa: F811
@@ -74,10 +77,19 @@ def test_pieces_straight_to_lds(lib, width):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [64, 128, 192, 256])
+def test_long_sweeps(lib, width):  # noqa: F811
+    """Tokens and rows of 129 and 33 tiles, the last ones short: a workgroup's tokens stay in
+    registers over eight tiles and more."""
+    got, want = both(lib, (16500, 4100, width, 0), "bf16", "bf16")
+    check(got, want, "bf16", "bf16")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("case", [
     # rows copied for the gradient; for the loss too; several pieces of the table in
     # the loss, the last one short; several in the gradient
-    (3000, 257, 72, 3), (6000, 700, 83, 5), (513, 256, 840, 0), (600, 66000, 700, 1),
+    (3000, 3000, 72, 3), (6000, 4300, 83, 5), (513, 4300, 840, 0), (600, 66000, 700, 1),
     (66000, 2300, 33, 0)])
 def test_rows_copied_first(lib, case):  # noqa: F811
     """Many tokens with rows that cannot go straight to LDS; NaN beside the rows."""
@@ -90,7 +102,7 @@ def test_rows_copied_first(lib, case):  # noqa: F811
 def test_addresses_do_not_matter(lib, width):  # noqa: F811
     """Rows of whole 64s at odd addresses give the bits of aligned ones, in a
     workspace of the same size; rows that count for nothing hold NaN."""
-    n, rows = 4000, 777
+    n, rows = 4000, 4100
     case = (n, rows, width, 0)
     t, code, gen, x, table, target, scale = inputs(case, "bf16")
     dloss = rnd(gen, n).cuda()
@@ -120,6 +132,7 @@ def test_addresses_do_not_matter(lib, width):  # noqa: F811
 @pytest.mark.gpu
 @pytest.mark.parametrize("scale", [-0.7, 0.0, 3.0])
 @pytest.mark.parametrize("case,dtype", [((300, 700, 64, 0), "bf16"), ((300, 333, 320, 0), "bf16"),
+                                        ((2100, 2500, 128, 0), "bf16"),
                                         ((90, 200, 50, 0), "f32"), ((90, 200, 50, 0), "bf16")])
 def test_scales(lib, case, dtype, scale):  # noqa: F811
     got, want = both(lib, case, dtype, dtype, scale=scale)
@@ -127,10 +140,11 @@ def test_scales(lib, case, dtype, scale):  # noqa: F811
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("case", [(300, 700, 64, 0), (2100, 2500, 128, 0)])
 @pytest.mark.parametrize("weights", ["alike", "first is zero", "tiny", "huge", "none"])
-def test_weights_of_the_tokens(lib, weights):  # noqa: F811
+def test_weights_of_the_tokens(lib, case, weights):  # noqa: F811
     """d is held relative to one token's weight, whichever that is."""
-    n = 300
+    n = case[0]
     dloss = torch.full((n,), 1.0 / 300)
     if weights == "first is zero":
         dloss[:100] = 0
@@ -141,7 +155,7 @@ def test_weights_of_the_tokens(lib, weights):  # noqa: F811
         dloss[1::2] *= 1e12
     elif weights == "none":
         dloss[:] = 0
-    got, want = both(lib, (n, 700, 64, 0), "bf16", "bf16", dloss=dloss)
+    got, want = both(lib, case, "bf16", "bf16", dloss=dloss)
     check(got, want, "bf16", "bf16")
     if weights == "alike":
         # a rounding of 8 bits each of the results, with d's own below it: the norm of
@@ -212,7 +226,8 @@ def calls(lib, gen, cases):  # noqa: F811
     return call, outs
 
 
-MANY = [((300, 700, 256, 0), "bf16"), ((300, 500, 50, 0), "bf16"), ((150, 400, 33, 0), "f32"),
+MANY = [((300, 700, 256, 0), "bf16"), ((2000, 2200, 256, 0), "bf16"), ((2000, 2200, 65, 0), "bf16"),
+        ((300, 500, 50, 0), "bf16"), ((150, 400, 33, 0), "f32"),
         ((66000, 1100, 64, 0), "bf16")]
 
 
