@@ -522,6 +522,7 @@ struct ProductDev {
   float *sums;           // [splits][rows][sums_ld], null: out is written
   uint64_t sums_split, sums_ld;
   uint32_t add;          // to what sums holds
+  uint32_t out_lanes;    // for a value of the result, a power of two of at most 64
   Weights weights;
 };
 
@@ -750,26 +751,32 @@ __global__ __launch_bounds__(256) void k_loss_pack(Matrix in, const int32_t *__r
   }
 }
 
-// The splits' sums, added in order, as rows of the result: four values a thread,
-// eight splits loaded together.
+// The splits' sums as rows of the result: four values a group of lanes, each of which
+// adds every lanes-th split in order, eight loaded together, and then pairs of lanes.
 template <typename T>
 __device__ __forceinline__ void write_result(const ProductDev &a) {
   const uint32_t vecs = (a.out_cols + 3) / 4;
   const float by = a.weights.reference();
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)a.out_rows * vecs;
-       i += (uint64_t)gridDim.x * 256) {
+  const uint32_t lanes = a.out_lanes, lane = threadIdx.x % lanes;
+  for (uint64_t i = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+       i < (uint64_t)a.out_rows * vecs; i += (uint64_t)gridDim.x * 256 / lanes) {
     const uint64_t r = i / vecs, c = i % vecs * 4;
     const NSFPS_GLOBAL_SEQ float *from = (const NSFPS_GLOBAL_SEQ float *)(a.sums + r * a.sums_ld + c);
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t s0 = 0; s0 < a.splits; s0 += 8) {
+    for (uint32_t s0 = lane; s0 < a.splits; s0 += 8 * lanes) {
       f32x4 v[8];
 #pragma unroll
       for (uint32_t s = 0; s < 8; ++s)
-        v[s] = *(const NSFPS_GLOBAL_SEQ f32x4 *)(from + min(s0 + s, a.splits - 1) * a.sums_split);
+        v[s] = *(const NSFPS_GLOBAL_SEQ f32x4 *)(from +
+                                                 min(s0 + s * lanes, a.splits - 1) * a.sums_split);
 #pragma unroll
       for (uint32_t s = 0; s < 8; ++s)
-        if (s0 + s < a.splits) sum += v[s];
+        if (s0 + s * lanes < a.splits) sum += v[s];
     }
+    for (uint32_t off = 1; off < lanes; off <<= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] += __shfl_xor(sum[k], off, 64);
+    if (lane) continue;
     const float o[4] = {sum[0] * by, sum[1] * by, sum[2] * by, sum[3] * by};
     T *const out = (T *)a.out + r * a.out_ld + c;
     if (c + 4 <= a.out_cols) {
@@ -827,11 +834,13 @@ void plan_sweeps(uint32_t ttiles, uint32_t vtiles, uint32_t &sweep, uint32_t &sw
   sweeps = (vtiles + sweep - 1) / sweep;
 }
 
-// Tiles of a call through registers: of 64 where those of 128 leave CUs without
-// one.  us (130 tokens x 901 x 847 bfloat16): statistics 15, 32 with tiles of 128;
-// derivatives 15 and 33; all of 64 tokens x 5,003 x 256 30 and 36.
+// Tiles of a call through registers: of 64 where those of 128 leave CUs without one
+// or would be half empty.  us with tiles of 64 and of 128: loss of 30 tokens x 19,106
+// rows x width 719 bfloat16 22 and 35; loss and gradient of 130 x 901 x 847 bfloat16
+// 30 and 65, 1,000 x 4,096 x 64 float32 41 and 44, 46 x 241,327 x 79 bfloat16 154 and
+// 169, 200 x 30,000 x 500 float32 254 and 207.
 uint32_t staged_tile(uint64_t tokens, uint64_t rows) {
-  return host_ceil_div(tokens, 128) * host_ceil_div(rows, 128) <= 128 ? 64 : 128;
+  return tokens <= 64 || host_ceil_div(tokens, 128) * host_ceil_div(rows, 128) <= 256 ? 64 : 128;
 }
 
 Tiling tiling(uint64_t tokens, uint64_t rows, uint32_t tile) {
@@ -963,11 +972,20 @@ hipError_t run_pack(const Matrix &in, const int32_t *targets, uint32_t vocabular
   return hipGetLastError();
 }
 
-// The sums of one product, or of two, as rows of their results.
-hipError_t write_out(const ProductDev &first, const ProductDev *second, hipStream_t st) {
-  const auto threads = [](const ProductDev &d) { return (uint64_t)d.out_rows * ((d.out_cols + 3) / 4); };
-  const uint32_t grid = grid_of(std::max(threads(first), second ? threads(*second) : 0));
-  k_loss_out<<<dim3(grid, second ? 2 : 1), 256, 0, st>>>(first, second ? *second : first);
+// The sums of one product, or of two, as rows of their results.  A group of lanes
+// takes a value where results are too few to fill the chip (46 tokens x 241,327 rows
+// x width 79, 512 splits: 6 us, 30 with a lane a value).
+hipError_t write_out(ProductDev first, const ProductDev *other, hipStream_t st) {
+  ProductDev second = other ? *other : first;
+  const auto threads = [](ProductDev &d) {
+    const uint64_t values = (uint64_t)d.out_rows * ((d.out_cols + 3) / 4);
+    d.out_lanes = 1;
+    while (d.out_lanes < 64 && 8 * d.out_lanes < d.splits && values * d.out_lanes < 1u << 17)
+      d.out_lanes *= 2;
+    return values * d.out_lanes;
+  };
+  const uint32_t grid = grid_of(std::max(threads(first), threads(second)));
+  k_loss_out<<<dim3(grid, other ? 2 : 1), 256, 0, st>>>(first, second);
   return hipGetLastError();
 }
 
