@@ -6,8 +6,9 @@
   from csrc/ by ``python -m ns_fps_amd.build``.
 * ``ns_fps_amd.capi`` -- ctypes binding of the C ABI (include/nsfps.h), with
   the sequence operators over the samples (lookup, causal convolution,
-  selective scan, their gradients, the one-token step); examples/
-  sequence_model.py runs them as one model.
+  selective scan, their gradients, the one-token step, norms with rotation,
+  dropout, the loss over a vocabulary); examples/sequence_model.py runs the
+  first of them as one model.
 * ``ns_fps_amd.workloads`` -- seeded synthetic clouds of the benchmark.
 * ``ns_fps_amd.kitti`` -- KITTI scan files: reader, z filter, bounds range
   and the reference drivers' sampling runs.
