@@ -127,7 +127,8 @@ __device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
   return v;
 }
 
-// A token's place, and its angles for this lane's slots.
+// A token's place, and its angles for this lane's slots (found while its first
+// head's values are on their way).
 template <int V, int S>
 struct Token {
   uint32_t b, t;
@@ -135,8 +136,7 @@ struct Token {
   float c[S][V], s[S][V];
 };
 template <int V, int S>
-__device__ __forceinline__ void token_at(const NormDev &a, uint32_t token, uint32_t lane,
-                                         Token<V, S> &o) {
+__device__ __forceinline__ void token_at(const NormDev &a, uint32_t token, Token<V, S> &o) {
   o.b = token / a.length;
   o.t = token % a.length;
   o.inside = true;
@@ -144,25 +144,37 @@ __device__ __forceinline__ void token_at(const NormDev &a, uint32_t token, uint3
     const int32_t n = a.lengths[o.b];
     o.inside = n > 0 && o.t < (uint32_t)n;
   }
+}
+// This lane's frequencies, 0 behind the rotation: cosine 1 and sine 0.
+template <int V, int S>
+__device__ __forceinline__ void load_freq(const NormDev &a, uint32_t lane, float (&f)[S][V]) {
+  struct __attribute__((packed, aligned(4))) Some {
+    float v[V];
+  };
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    const uint32_t s0 = V * (lane + q * a.lanes);  // V slots are all turned or none
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[q][i] = 0.f;
+    if (s0 < a.half) {
+      const Some o = *(const NSFPS_GLOBAL_SEQ Some *)(a.freq + s0);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[q][i] = o.v[i];
+    }
+  }
+}
+template <int V, int S>
+__device__ __forceinline__ void find_angles(const NormDev &a, const float (&f)[S][V],
+                                            Token<V, S> &o) {
   const int32_t from = a.positions ? max(a.positions[o.b], 0) : 0;
   const double position = (double)((int64_t)from + o.t);
 #pragma unroll
-  for (int q = 0; q < S; ++q) {
-    const uint32_t s0 = V * (lane + q * a.lanes);
-    const bool turned = s0 < a.half;  // V slots are all turned or none
-    float f[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = 0.f;
-    if (turned) load_f32<float, 1>(a.freq + s0, *(float(*)[1])&f[0]);
-#pragma unroll
-    for (int i = 1; i < V; ++i)
-      if (turned) load_f32<float, 1>(a.freq + s0 + i, *(float(*)[1])&f[i]);
+  for (int q = 0; q < S; ++q)
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       o.c[q][i] = 1.f, o.s[q][i] = 0.f;
-      if (turned) turn(position, f[i], o.c[q][i], o.s[q][i]);
+      if (a.half) turn(position, f[q][i], o.c[q][i], o.s[q][i]);
     }
-  }
 }
 
 template <typename T, int V, int S>
@@ -203,7 +215,8 @@ __global__ __launch_bounds__(256) void k_norm(NormDev a) {
     at[q] = slots_at<V>(a, s0);
     mixed[q] = a.neighbours && s0 < a.half;
   }
-  float wqa[S][V], wqb[S][V], wka[S][V], wkb[S][V];
+  float freq[S][V], wqa[S][V], wqb[S][V], wka[S][V], wkb[S][V];
+  load_freq<V, S>(a, lane, freq);
   load_head_weights<T, V, S>(a, a.q_weight, lane, wqa, wqb);
   load_head_weights<T, V, S>(a, a.k_weight, lane, wka, wkb);
   const uint32_t heads = a.q_heads + a.k_heads;
@@ -212,14 +225,17 @@ __global__ __launch_bounds__(256) void k_norm(NormDev a) {
        item += (uint64_t)gridDim.x * groups) {
     const uint32_t h0 = (uint32_t)(item % a.chunks) * a.per, h1 = min(h0 + a.per, heads);
     Token<V, S> tok;
-    token_at<V, S>(a, (uint32_t)(item / a.chunks), lane, tok);
+    token_at<V, S>(a, (uint32_t)(item / a.chunks), tok);
     RawPair<T, V> next[S];
     const auto fetch = [&](uint32_t h) {
       const T *x = head_at<const T>(a, a.q, a.k, tok.b, tok.t, h);
 #pragma unroll
       for (int q = 0; q < S; ++q) next[q] = load_pair<T, V>(x, at[q]);
     };
-    if (tok.inside) fetch(h0);
+    if (tok.inside) {
+      fetch(h0);
+      find_angles<V, S>(a, freq, tok);
+    }
     for (uint32_t h = h0; h < h1; ++h) {
       T *const y = head_at<T>(a, a.q_out, a.k_out, tok.b, tok.t, h);
       float xa[S][V], xb[S][V];
@@ -279,7 +295,8 @@ __global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict_
     at[q] = slots_at<V>(a, s0);
     mixed[q] = a.neighbours && s0 < a.half;
   }
-  float wqa[S][V], wqb[S][V], wka[S][V], wkb[S][V];
+  float freq[S][V], wqa[S][V], wqb[S][V], wka[S][V], wkb[S][V];
+  load_freq<V, S>(a, lane, freq);
   load_head_weights<T, V, S>(a, a.q_weight, lane, wqa, wqb);
   load_head_weights<T, V, S>(a, a.k_weight, lane, wka, wkb);
   float qa[S][V] = {}, qb[S][V] = {}, ka[S][V] = {}, kb[S][V] = {};
@@ -289,7 +306,7 @@ __global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict_
        item += (uint64_t)gridDim.x * groups) {
     const uint32_t h0 = (uint32_t)(item % a.chunks) * a.per, h1 = min(h0 + a.per, heads);
     Token<V, S> tok;
-    token_at<V, S>(a, (uint32_t)(item / a.chunks), lane, tok);
+    token_at<V, S>(a, (uint32_t)(item / a.chunks), tok);
     RawPair<T, V> nx[S], ng[S];
     const auto fetch = [&](uint32_t h) {
       const T *x = head_at<const T>(a, a.q, a.k, tok.b, tok.t, h);
@@ -300,7 +317,10 @@ __global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict_
         ng[q] = load_pair<T, V>(g, at[q]);
       }
     };
-    if (tok.inside) fetch(h0);
+    if (tok.inside) {
+      fetch(h0);
+      find_angles<V, S>(a, freq, tok);
+    }
     for (uint32_t h = h0; h < h1; ++h) {
       T *const dx = head_at<T>(a, a.q_out, a.k_out, tok.b, tok.t, h);
       float xa[S][V], xb[S][V], ga[S][V], gb[S][V];
