@@ -232,6 +232,29 @@ MANY = [((300, 700, 256, 0), "bf16"), ((2000, 2200, 256, 0), "bf16"), ((2000, 22
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("stride", [(1 << 23) - 8, 1 << 23])
+def test_rows_far_apart(lib, stride):  # noqa: F811
+    """Rows of x and of the table as far apart as tiles straight to LDS take them, and
+    one step farther: a tile's rows span 2 GB and more."""
+    case = (130, 150, 128, 0)
+    n, rows, width, _ = case
+    _, code, gen, x, table, target, scale = inputs(case, "bf16")
+    wide = torch.empty(rows, stride, dtype=torch.bfloat16, device="cuda")
+    far = torch.empty(n, stride, dtype=torch.bfloat16, device="cuda")
+    wide[:, :width], far[:, :width] = table.cuda(), x.cuda()
+    loss, lse = torch.empty(n, device="cuda"), torch.empty(n, device="cuda")
+    tg = target.cuda()
+    args = args_of(case, code, far, wide, tg, scale, loss, lse)
+    ws = give(args, lib.loss_workspace_bytes(args))
+    lib.loss_device(args, stream())
+    torch.cuda.synchronize()
+    want = Want(x, table, target, scale)
+    within(lse, want.lse, want.E, "lse")
+    within(loss, want.loss, 2 * want.E, "loss")
+    del ws
+
+
+@pytest.mark.gpu
 def test_graph_replays_equal_eager_calls(lib):  # noqa: F811
     call, outs = calls(lib, torch.Generator().manual_seed(2), MANY)
     call()
