@@ -734,20 +734,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_loss_products_direct(Produc
 // Rows for the copies straight to LDS: out_rows x out_cols, zeros past the ends and
 // (targets not null) where a row counts for nothing, which may hold anything.
 // Memory bound: 16,384 rows of 256 5.8 us.
-__global__ __launch_bounds__(256) void k_loss_pack(Matrix in, const int32_t *__restrict__ targets,
-                                                   uint32_t vocabulary, bf16 *__restrict__ out,
-                                                   uint64_t out_rows, uint32_t out_cols) {
-  const uint32_t vecs = out_cols / 8;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < out_rows * vecs;
+struct PackDev {
+  Matrix in;
+  const int32_t *targets;
+  uint32_t vocabulary, out_cols;
+  bf16 *out;
+  uint64_t out_rows;
+};
+// first's rows, second's with blockIdx.y = 1
+__global__ __launch_bounds__(256) void k_loss_pack(PackDev first, PackDev second) {
+  const PackDev &a = blockIdx.y ? second : first;
+  const uint32_t vecs = a.out_cols / 8;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < a.out_rows * vecs;
        i += (uint64_t)gridDim.x * 256) {
     const uint64_t r = i / vecs;
     const uint32_t c = (uint32_t)(i % vecs) * 8;
     Eight<bf16> v = {};
-    if (r < in.rows && c < in.cols && (!targets || (uint32_t)targets[r] < vocabulary)) {
-      const bf16 *const row = (const bf16 *)in.p + r * in.ld + c;
-      v = c + 8 <= in.cols ? load_eight<bf16>(row) : load_some<bf16>(row, in.cols - c);
+    if (r < a.in.rows && c < a.in.cols &&
+        (!a.targets || (uint32_t)a.targets[r] < a.vocabulary)) {
+      const bf16 *const row = (const bf16 *)a.in.p + r * a.in.ld + c;
+      v = c + 8 <= a.in.cols ? load_eight<bf16>(row) : load_some<bf16>(row, a.in.cols - c);
     }
-    *(NSFPS_GLOBAL_SEQ u32x4 *)(out + r * out_cols + c) = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+    *(NSFPS_GLOBAL_SEQ u32x4 *)(a.out + r * a.out_cols + c) = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
   }
 }
 
@@ -965,10 +973,14 @@ hipError_t run_direct(const ProductDev &dx, const ProductDev &de, uint32_t grid,
   return hipGetLastError();
 }
 
-hipError_t run_pack(const Matrix &in, const int32_t *targets, uint32_t vocabulary, void *out,
-                    uint64_t out_rows, uint32_t out_cols, hipStream_t st) {
-  k_loss_pack<<<grid_of(out_rows * (out_cols / 8)), 256, 0, st>>>(in, targets, vocabulary,
-                                                                   (bf16 *)out, out_rows, out_cols);
+// The copy that a PackDev makes; and one or two of them in a launch.
+Matrix packed(const PackDev &p) {
+  return {p.out, p.out_cols, (uint32_t)p.out_rows, p.out_cols};
+}
+hipError_t run_pack(const PackDev &first, const PackDev *second, hipStream_t st) {
+  const auto threads = [](const PackDev &p) { return p.out_rows * (p.out_cols / 8); };
+  const uint32_t grid = grid_of(std::max(threads(first), second ? threads(*second) : 0));
+  k_loss_pack<<<dim3(grid, second ? 2 : 1), 256, 0, st>>>(first, second ? *second : first);
   return hipGetLastError();
 }
 
@@ -1142,17 +1154,16 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
   char *const ws = (char *)a.workspace;
   const uint64_t stride = up(a.tokens, 16);
   Matrix x = x_of(a);
-  if (way == Way::kPacked) {
-    x = {ws + p.x, p.width, (uint32_t)a.tokens, p.width};
-    LAUNCH(run_pack(x_of(a), nullptr, 0, ws + p.x, a.tokens, p.width, st));
-  }
+  const PackDev px = {x, nullptr, 0, p.width, (bf16 *)(ws + p.x), a.tokens};
+  if (way == Way::kPacked) x = packed(px);
   float2 *parts = (float2 *)(ws + p.parts);
   for (uint64_t k = 0; k < p.pieces; ++k) {
     const uint64_t row0 = k * p.piece, rows = std::min(p.piece, a.rows - row0);
     Matrix e = table_of(a, row0, rows);
     if (way == Way::kPacked) {
-      LAUNCH(run_pack(e, nullptr, 0, ws + p.e, rows, p.width, st));
-      e = {ws + p.e, p.width, (uint32_t)rows, p.width};
+      const PackDev pe = {e, nullptr, 0, p.width, (bf16 *)(ws + p.e), rows};
+      LAUNCH(run_pack(pe, k ? nullptr : &px, st));
+      e = packed(pe);
     }
     LogitDev d = logits(a, x, e, row0, a.tokens, rows, p.tile);
     d.parts = parts;
@@ -1203,10 +1214,10 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
   const uint32_t ntiles = (uint32_t)host_ceil_div(a.width, p.nt);
   const uint64_t z = g.grad_dtype == NSFPS_F32 ? 4 : 2;
   Matrix x = x_of(a);
-  if (direct) {  // whole tiles, and zeros for rows that count for nothing
-    LAUNCH(run_pack(x, a.d_targets, (uint32_t)a.rows, ws + p.x, p.tokens, p.width, st));
-    x = {ws + p.x, p.width, (uint32_t)p.tokens, p.width};
-  }
+  // whole tiles, and zeros for rows that count for nothing
+  const PackDev px = {x, a.d_targets, (uint32_t)a.rows, p.width, (bf16 *)(ws + p.x), p.tokens};
+  if (way == Way::kDirect) LAUNCH(run_pack(px, nullptr, st));
+  if (direct) x = packed(px);
   ProductDev dx = {};
   dx.weights = {g.d_dloss, a.d_targets, (uint32_t)a.tokens, (uint32_t)a.rows, a.scale};
   dx.mtiles = (uint32_t)host_ceil_div(a.tokens, p.mt);
@@ -1224,8 +1235,9 @@ hipError_t launch_loss_grad(const nsfps_loss_args &a, const nsfps_loss_grads &g,
     const uint64_t row0 = k * p.piece, rows = std::min(p.piece, a.rows - row0);
     Matrix e = table_of(a, row0, rows);
     if (way == Way::kPacked) {
-      LAUNCH(run_pack(e, nullptr, 0, ws + p.e, rows, p.width, st));
-      e = {ws + p.e, p.width, (uint32_t)rows, p.width};
+      const PackDev pe = {e, nullptr, 0, p.width, (bf16 *)(ws + p.e), rows};
+      LAUNCH(run_pack(pe, k ? nullptr : &px, st));
+      e = packed(pe);
     }
     const uint32_t tile = direct ? kTile : staged_tile(a.tokens, rows);
     LogitDev l = direct ? logits(a, x, e, row0, p.tokens, up(rows, kPad), tile)

@@ -294,3 +294,16 @@ def test_calls_on_other_streams(lib):  # noqa: F811
     torch.cuda.synchronize()
     for (_, outs), want in zip(sets, wants):
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("case,copied", [((6000, 4300, 83, 5), True), ((513, 4300, 840, 0), True),
+                                         ((600, 66000, 700, 1), True), ((500, 4300, 840, 0), False),
+                                         ((3000, 3000, 72, 3), False)])
+def test_sizes_reach_the_copies(case, copied):
+    """What test_rows_copied_first is for: the loss's workspace holds the tokens' copy
+    and a piece's of the table, or does not."""
+    n, rows, width, pad = case
+    args = capi.LossArgs(tokens=n, rows=rows, width=width, dtype=capi.BF16, x_stride=width + pad,
+                         table_stride=width + pad)
+    copies = 2 * (n + min(rows, 65536)) * ((width + 63) // 64 * 64)
+    assert (capi.Lib().loss_workspace_bytes(args) >= copies) == copied
