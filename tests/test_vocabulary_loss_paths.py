@@ -100,8 +100,8 @@ def test_rows_copied_first(lib, case):  # noqa: F811
 @pytest.mark.gpu
 @pytest.mark.parametrize("width", [128, 320])
 def test_addresses_do_not_matter(lib, width):  # noqa: F811
-    """Rows of whole 64s at odd addresses give the bits of aligned ones, in a
-    workspace of the same size; rows that count for nothing hold NaN."""
+    """Rows of whole 64s at odd addresses, copied first, give the bits of aligned ones,
+    in a workspace of the same size; rows that count for nothing hold NaN."""
     n, rows = 4000, 4100
     case = (n, rows, width, 0)
     t, code, gen, x, table, target, scale = inputs(case, "bf16")
