@@ -364,9 +364,16 @@ __global__ __launch_bounds__(256, 2) void k_loss_stats(LogitDev a) {
   }
 }
 
+template <typename T>
+__device__ __forceinline__ float value(const Eight<T> &v, int k) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(v.w[k]);
+  return __uint_as_float(k % 2 ? v.w[k / 2] & 0xffff0000u : v.w[k / 2] << 16);
+}
+
 // lse and loss: a workgroup has `group` tokens (a power of two, at most 16), 256 /
-// group runs of parts for each; then its waves find the logits of the tokens'
-// targets.
+// group runs of parts for each; then as many lanes, a wave at most, find the logit of
+// a token's target.  Its bytes bound it in large calls (14,990 tokens x 147 rows x
+// width 954 float32: 14 us), else its three loads one after another (4 us).
 template <typename T>
 __global__ __launch_bounds__(256) void k_loss_join(const float2 *__restrict__ parts, uint32_t nparts,
                                                    uint64_t part_stride, uint32_t group, Matrix x,
@@ -387,27 +394,32 @@ __global__ __launch_bounds__(256) void k_loss_join(const float2 *__restrict__ pa
       join_stats(m, s, __shfl_xor(m, off, 64), __shfl_xor(s, off, 64));
     if (lane < group) s_part[wave][lane] = make_float2(m, s);
     __syncthreads();
-    for (uint32_t i = wave; i < group; i += 4) {
-      const uint32_t token = t0 + i;
-      if (token >= tokens) break;
-      const uint32_t target = (uint32_t)targets[token];
+    const uint32_t per = min(256 / group, 64u), i = threadIdx.x / per, token = t0 + i;
+    if (i < group && token < tokens) {
+      const uint32_t target = (uint32_t)targets[token], own = threadIdx.x % per;
       float dot = 0.f;
       if (target < table.rows) {
         const T *xr = (const T *)x.p + token * x.ld, *er = (const T *)table.p + target * table.ld;
-        for (uint32_t c = lane; c < x.cols; c += 64) {
+        const uint32_t whole = x.cols / 8, c = 8 * whole + own;
+#pragma unroll 2
+        for (uint32_t q = own; q < whole; q += per) {
+          const Eight<T> u = load_eight<T>(xr + 8 * q), v = load_eight<T>(er + 8 * q);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dot = fmaf(value(u, k), value(v, k), dot);
+        }
+        if (c < x.cols) {
           float u[1], v[1];
           load_f32<T, 1>(xr + c, u);
           load_f32<T, 1>(er + c, v);
           dot = fmaf(u[0], v[0], dot);
         }
       }
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) dot += __shfl_xor(dot, off, 64);
+      for (uint32_t off = 1; off < per; off <<= 1) dot += __shfl_xor(dot, off, 64);
       float2 v = s_part[0][i];
 #pragma unroll
       for (int k = 1; k < 4; ++k) join_stats(v.x, v.y, s_part[k][i].x, s_part[k][i].y);
       const float all = (v.x + log2f(v.y)) * kLn2;
-      if (lane == 0) {
+      if (own == 0) {
         lse[token] = all;
         loss[token] = target < table.rows ? all - scale * dot : 0.f;
       }
