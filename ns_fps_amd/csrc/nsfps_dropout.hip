@@ -69,10 +69,10 @@ __device__ __forceinline__ float dropped(float x, float r, bool keep, float fact
   return fmaf(keep ? x : 0.f, factor, r);
 }
 
-// kWideRows: a lane has a block of eight values, in 16-byte accesses (the case
-// above 287 us, 684 the other way).  Else a wave makes the masks of 64 blocks, a lane each, and takes their 512 values 64
-// neighbours at a time, each lane asking for the mask of its value's block (16,384
-// rows of 323 float32: 10.8 us, 3.9 TB/s).
+// kWideRows: a lane has a block of eight values, in 16-byte accesses (the case above
+// 287 us, 684 the other way).  Else a wave makes the masks of 64 blocks, a lane each,
+// and takes their 512 values 64 neighbours at a time, each lane asking for the mask of
+// its value's block (16,384 rows of 323 float32: 10.8 us, 3.9 TB/s).
 template <typename T, bool kWideRows>
 __global__ __launch_bounds__(256) void k_dropout(DropDev a) {
   const uint64_t seed = a.seed[0], call = a.seed[1];

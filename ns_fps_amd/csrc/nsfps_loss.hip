@@ -218,10 +218,10 @@ struct DirectLogits {
   }
 };
 
-// The same for widths of up to 256 and long sweeps: a workgroup's tokens stay in registers, so
-// that LDS, which gives 128 bytes a cycle, is read for the vocabulary alone (with
-// both from LDS those reads and the copies took half as long again as the
-// products).  Three stages are under way while a fourth is worked on.
+// The same for widths of up to 256 and long sweeps: a workgroup's tokens stay in
+// registers, so that LDS, which gives 128 bytes a cycle, is read for the vocabulary
+// alone (with both from LDS those reads and the copies took half as long again as
+// the products).  Three stages are under way while a fourth is worked on.
 template <int kTerms, int kSteps>
 struct ResidentLogits {
   typedef Product<2, 2, 4, 2, kTerms, 1, 1, false, false, true> Prod;
@@ -871,14 +871,12 @@ Tiling tiling(uint64_t tokens, uint64_t rows, uint32_t tile) {
   return t;
 }
 
-// (How tiles come to LDS hangs on a call's addresses too; the workspace has room for
-// either way.)
 constexpr uint32_t kPad = 256;  // of tokens and pieces: whole tiles of any kind
 
 // How a call's tiles come to LDS: through registers; straight from its inputs,
 // bfloat16 rows of whole 64s at 16-byte boundaries; or straight from copies of
 // them in the workspace, bfloat16 rows padded with zeros, a piece of the vocabulary
-// at a time.
+// at a time.  Hangs on addresses too; the workspace has room for either way.
 enum class Way { kStaged, kDirect, kPacked };
 
 // Tiles of z of a call.
