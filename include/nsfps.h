@@ -292,9 +292,11 @@ nsfps_status nsfps_ball_query_device(const float *d_xyz, uint64_t n, const float
  * calls that may overlap must not share.  The first call of an operator on a
  * device loads its kernels (seven and a half milliseconds for all of them);
  * nsfps_init_sequence_device does that ahead, before a capture for instance.
- * No output may overlap an input or another output.  A workspace that is too
- * small, a size or stride that does not fit and a null pointer are
- * NSFPS_EINVAL; sizes beyond the limits named below are NSFPS_EUNSUPPORTED.
+ * No output may overlap an input or another output, but those of norms and
+ * dropout may be their own inputs' very rows (below).  Convolution, norms,
+ * dropout and loss refuse other overlaps where the strides show them.  A
+ * workspace that is too small, a size or stride that does not fit and a null
+ * pointer are NSFPS_EINVAL; sizes beyond the limits named below are NSFPS_EUNSUPPORTED.
  * Nothing is enqueued by a refused call.
  *
  * Types: NSFPS_F32 and NSFPS_BF16 for inputs and outputs; sums, states and
@@ -464,7 +466,8 @@ nsfps_status nsfps_scan_step_device(const nsfps_step_args *args, void *stream);
  * head_dim at most 256, rotary_dim even and at most head_dim (0: no
  * rotation), eps above 0; (q_heads + k_heads) * head_dim at most 2^24; batch *
  * length at most 2^31 - 1.  A head whose sum of squares passes float32 (values
- * near 10^19) becomes zeros.
+ * near 10^19) becomes zeros.  In place: q_out may be q's rows and k_out k's, and
+ * of the gradient dq those of q or dq_out, dk those of k or dk_out.
  *
  * The gradient takes those of q_out and k_out and writes all of dq and dk
  * (type dtype), and d_dq_weight and d_dk_weight ([head_dim] float32, or NULL);
@@ -501,7 +504,8 @@ nsfps_status nsfps_norm_grad_device(const nsfps_norm_args *args, const nsfps_nor
  * or lengths.  d_seed: two words in device memory, a key and the number of the
  * call (a captured graph's caller changes it between replays).  0 <= p <= 1 (1:
  * all is dropped); channels at most 2^24, batch * length at most 2^31 - 1.  Rows
- * past a sequence's length are zeros, their inputs are not read. */
+ * past a sequence's length are zeros, their inputs are not read.  In place: y may
+ * be the rows of x or of residual. */
 typedef struct {
   uint64_t batch, length;
   uint32_t channels, dtype;

@@ -69,6 +69,7 @@ __device__ __forceinline__ float dropped(float x, float r, bool keep, float fact
   return fmaf(keep ? x : 0.f, factor, r);
 }
 
+// A lane writes the places that it has read: y may be the rows of x or residual.
 // kWideRows: a lane has a block of eight values, in 16-byte accesses (the case above
 // 287 us, 684 the other way).  Else a wave makes the masks of 64 blocks, a lane each,
 // and takes their 512 values 64 neighbours at a time, each lane asking for the mask of

@@ -9,7 +9,8 @@
 // two values behind the rotation (whose angle is 0), a vector of V slots a
 // lane.  A group takes a token's heads one after another, q's and k's, so the
 // token's cosines and sines are found once; sums over a head go across the
-// group's lanes.
+// group's lanes.  A lane writes the places of the values that it has read, and no
+// others: outputs may be the inputs' own rows.
 //
 // Memory is the bound: 64 x 4,096 rows of 2 x 8 heads of 64, bfloat16, three
 // quarters of them inside their sequences: norms 208 us (4.5 TB/s read and

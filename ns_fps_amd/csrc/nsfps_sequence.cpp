@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 #include <utility>
 
 namespace nsfps {
@@ -71,8 +72,8 @@ nsfps_status check_rows(const nsfps_rows &r, uint64_t batch, uint64_t length, ui
 // tell: the same first element, or the same strides.  `out` keeps its rows apart
 // (check_rows), so the offsets of two rows of it that can meet are the few
 // nearest to the tensors' distance.
-bool rows_meet(const nsfps_rows &out, const nsfps_rows &in, uint64_t batch, uint64_t length,
-               uint64_t width, uint32_t dtype) {
+bool rows_meet(const nsfps_rows &out, uint64_t out_width, const nsfps_rows &in, uint64_t in_width,
+               uint64_t batch, uint64_t length, uint32_t dtype) {
   if (out.p == in.p) return true;
   if ((batch > 1 && out.batch_stride != in.batch_stride) ||
       (length > 1 && out.row_stride != in.row_stride))
@@ -83,8 +84,8 @@ bool rows_meet(const nsfps_rows &out, const nsfps_rows &in, uint64_t batch, uint
       near{(int64_t)out.row_stride, (int64_t)length - 1};
   if (near.most && (!far.most || near.stride > far.stride)) std::swap(far, near);
   const int64_t d = ((intptr_t)in.p - (intptr_t)out.p) / (int64_t)size_of(dtype),
-                span = far.most * far.stride + near.most * near.stride + (int64_t)width;
-  if (d >= span || -d >= span) return false;
+                span = far.most * far.stride + near.most * near.stride;
+  if (d >= span + (int64_t)out_width || -d >= span + (int64_t)in_width) return false;
   const auto nearest = [](const Step &s, int64_t at, int64_t k) {  // at, some steps back
     const int64_t q = s.most ? std::max(-s.most, std::min(s.most, at / s.stride + k)) : 0;
     return at - q * s.stride;
@@ -92,15 +93,88 @@ bool rows_meet(const nsfps_rows &out, const nsfps_rows &in, uint64_t batch, uint
   for (int64_t k = -1; k <= 1; ++k)
     for (int64_t j = -1; j <= 1; ++j) {
       const int64_t left = nearest(near, nearest(far, d, k), j);
-      if (left < (int64_t)width && -left < (int64_t)width) return true;
+      if (left < (int64_t)out_width && -left < (int64_t)in_width) return true;
     }
   return false;
 }
 
 nsfps_status check_apart(const nsfps_rows &out, const nsfps_rows &in, const nsfps_conv_args &a,
                          const char *what) {
-  if (rows_meet(out, in, a.batch, a.length, a.channels, a.dtype))
+  if (rows_meet(out, a.channels, in, a.channels, a.batch, a.length, a.dtype))
     return fail(NSFPS_EINVAL, "%s overlap: tokens beside a row are read after it is written", what);
+  return NSFPS_OK;
+}
+
+// Rows of one tensor of an operator whose lanes take their values before they write
+// the same places: an output may be its own input's very rows (check_own), and must
+// share nothing with another tensor's (check_other).
+struct Tensor {
+  nsfps_rows rows;
+  uint64_t width;
+  const char *what;
+};
+struct Sizes {
+  uint64_t batch, length;
+  uint32_t dtype;
+};
+nsfps_status check_other(const Tensor &out, const Tensor &in, const Sizes &n) {
+  if (!out.width || !in.width) return NSFPS_OK;  // no heads
+  const auto whole = [&](const Tensor &t) {  // one piece of memory
+    return (n.length == 1 || t.rows.row_stride == t.width) &&
+           (n.batch == 1 || t.rows.batch_stride == n.length * t.width);
+  };
+  const uint64_t bytes = n.batch * n.length * size_of(n.dtype), o = (uintptr_t)out.rows.p,
+                 i = (uintptr_t)in.rows.p;
+  const bool meet = whole(out) && whole(in)
+                        ? o < i + bytes * in.width && i < o + bytes * out.width
+                        : rows_meet(out.rows, out.width, in.rows, in.width, n.batch, n.length, n.dtype);
+  if (meet)
+    return fail(NSFPS_EINVAL, "%s and %s overlap", out.what, in.what);
+  return NSFPS_OK;
+}
+nsfps_status check_own(const Tensor &out, const Tensor &in, const Sizes &n) {
+  const bool same = out.rows.p == in.rows.p &&
+                    (n.batch <= 1 || out.rows.batch_stride == in.rows.batch_stride) &&
+                    (n.length <= 1 || out.rows.row_stride == in.rows.row_stride);
+  return same ? NSFPS_OK : check_other(out, in, n);
+}
+
+// Rows of a matrix, in bytes.
+struct Span {
+  const void *p;
+  uint64_t rows, stride, width;
+  const char *what;
+};
+// Whether they share a byte, as far as their strides tell: exactly where one of the two
+// has no gaps, or where both have the same stride.
+bool spans_meet(const Span &a, const Span &b) {
+  if (!a.rows || !b.rows) return false;
+  if (a.p == b.p) return true;
+  const bool a_whole = a.rows == 1 || a.stride == a.width, b_whole = b.rows == 1 || b.stride == b.width;
+  const auto last = [](const Span &s) { return (int64_t)((s.rows - 1) * s.stride + s.width); };
+  const int64_t d = (intptr_t)b.p - (intptr_t)a.p;  // from a's first to b's first
+  if (d >= last(a) || -d >= last(b)) return false;
+  // a whole one, from `from` to `to` in the other's bytes, meets the first row that ends
+  // behind `from`
+  const auto meets = [](const Span &s, int64_t from, int64_t to) {
+    const int64_t w = (int64_t)s.width, st = (int64_t)std::max<uint64_t>(s.stride, 1);
+    const int64_t row = from < w ? 0 : (from - w) / st + 1;
+    return row < (int64_t)s.rows && row * (int64_t)s.stride < to;
+  };
+  if (a_whole) return meets(b, -d, last(a) - d);
+  if (b_whole) return meets(a, d, d + last(b));
+  if (a.stride != b.stride) return false;
+  const int64_t st = (int64_t)a.stride, in = (d % st + st) % st;  // b's row in a's period
+  return in < (int64_t)a.width || in + (int64_t)b.width > st;
+}
+nsfps_status check_spans(std::initializer_list<Span> outs, std::initializer_list<Span> ins) {
+  for (auto out = outs.begin(); out != outs.end(); ++out) {
+    for (auto other = outs.begin(); other != out; ++other)
+      if (spans_meet(*out, *other))
+        return fail(NSFPS_EINVAL, "%s and %s overlap", other->what, out->what);
+    for (const Span &in : ins)
+      if (spans_meet(*out, in)) return fail(NSFPS_EINVAL, "%s and %s overlap", out->what, in.what);
+  }
   return NSFPS_OK;
 }
 
@@ -270,6 +344,26 @@ nsfps_status check_norm_sizes(const nsfps_norm_args *a) {
   return NSFPS_OK;
 }
 
+// Outputs (y, or dx) of queries and keys: over their own inputs or gradients, or apart.
+nsfps_status check_norm_places(const nsfps_norm_args &a, const nsfps_rows &q_out,
+                               const nsfps_rows &k_out, const nsfps_norm_grads *g) {
+  const uint64_t d = a.head_dim, qw = a.q_heads * d, kw = a.k_heads * d;
+  const Sizes n = {a.batch, a.length, a.dtype};
+  const Tensor q = {a.q, qw, "q"}, k = {a.k, kw, "k"}, qo = {q_out, qw, g ? "dq" : "q_out"},
+               ko = {k_out, kw, g ? "dk" : "k_out"};
+  TRY(check_other(qo, ko, n));
+  TRY(check_own(qo, q, n));
+  TRY(check_own(ko, k, n));
+  TRY(check_other(qo, k, n));
+  TRY(check_other(ko, q, n));
+  if (!g) return NSFPS_OK;
+  const Tensor dq = {g->dq_out, qw, "dq_out"}, dk = {g->dk_out, kw, "dk_out"};
+  TRY(check_own(qo, dq, n));
+  TRY(check_own(ko, dk, n));
+  TRY(check_other(qo, dk, n));
+  return check_other(ko, dq, n);
+}
+
 nsfps_status check_norm(const nsfps_norm_args *a, bool grad) {
   TRY(check_norm_sizes(a));
   if (a->batch && a->length) {
@@ -306,6 +400,10 @@ nsfps_status check_dropout(const nsfps_dropout_args *a) {
     if (a->residual.p)
       TRY(check_rows(a->residual, a->batch, a->length, a->channels, a->dtype, false, "residual"));
     TRY(check_rows(a->y, a->batch, a->length, a->channels, a->dtype, true, "y"));
+    const Sizes n = {a->batch, a->length, a->dtype};
+    const Tensor y = {a->y, a->channels, "y"};
+    TRY(check_own(y, {a->x, a->channels, "x"}, n));
+    if (a->residual.p) TRY(check_own(y, {a->residual, a->channels, "residual"}, n));
   }
   TRY(check_pointer(a->d_seed, 8, "d_seed"));
   TRY(check_optional(a->d_lengths, 4, "d_lengths"));
@@ -343,6 +441,18 @@ nsfps_status check_loss(const nsfps_loss_args *a, bool grad) {
     TRY(check_pointer(a->d_lse, 4, "d_lse"));
   }
   return NSFPS_OK;
+}
+
+// The loss writes rows while others are still to be read: nothing may overlap.
+struct LossSpans {
+  Span x, table, targets, lse;
+};
+LossSpans loss_spans(const nsfps_loss_args &a) {
+  const uint64_t z = size_of(a.dtype), n = a.tokens;
+  return {{a.d_x, n, a.x_stride * z, a.width * z, "d_x"},
+          {a.d_table, a.rows, a.table_stride * z, a.width * z, "d_table"},
+          {a.d_targets, n, 4, 4, "d_targets"},
+          {a.d_lse, n, 4, 4, "d_lse"}};
 }
 
 nsfps_status check_loss_grads(const nsfps_loss_grads *g) {
@@ -513,6 +623,7 @@ nsfps_status nsfps_norm_device(const nsfps_norm_args *args, void *stream) {
   return guarded([&]() -> nsfps_status {
     TRY(check_norm(args, false));
     if (!args->batch || !args->length) return NSFPS_OK;
+    TRY(check_norm_places(*args, args->q_out, args->k_out, nullptr));
     TRY(need_device());
     HIP_TRY(launch_norm(*args, (hipStream_t)stream));
     return NSFPS_OK;
@@ -544,6 +655,7 @@ nsfps_status nsfps_norm_grad_device(const nsfps_norm_args *args, const nsfps_nor
         TRY(check_rows(grads->dk_out, b, l, args->k_heads * d, t, false, "dk_out"));
         TRY(check_rows(grads->dk, b, l, args->k_heads * d, t, true, "dk"));
       }
+      TRY(check_norm_places(*args, grads->dq, grads->dk, grads));
     }
     TRY(check_optional(grads->d_dq_weight, 4, "d_dq_weight"));
     TRY(check_optional(grads->d_dk_weight, 4, "d_dk_weight"));
@@ -577,6 +689,8 @@ nsfps_status nsfps_loss_device(const nsfps_loss_args *args, void *stream) {
   return guarded([&]() -> nsfps_status {
     TRY(check_loss(args, false));
     if (!args->tokens) return NSFPS_OK;
+    const LossSpans s = loss_spans(*args);
+    TRY(check_spans({s.lse, {args->d_loss, args->tokens, 4, 4, "d_loss"}}, {s.x, s.table, s.targets}));
     TRY(check_workspace(args->workspace, args->workspace_bytes, loss_bytes(*args)));
     TRY(need_device());
     HIP_TRY(launch_loss(*args, (hipStream_t)stream));
@@ -608,6 +722,11 @@ nsfps_status nsfps_loss_grad_device(const nsfps_loss_args *args, const nsfps_los
     }
     if (args->rows) TRY(check_pointer(grads->d_dtable, size_of(grads->grad_dtype), "d_dtable"));
     if (!args->tokens && !args->rows) return NSFPS_OK;
+    const LossSpans s = loss_spans(*args);
+    const uint64_t z = size_of(args->dtype), gz = size_of(grads->grad_dtype), w = args->width;
+    TRY(check_spans({{grads->d_dx, args->tokens, grads->dx_stride * z, w * z, "d_dx"},
+                     {grads->d_dtable, args->rows, grads->dtable_stride * gz, w * gz, "d_dtable"}},
+                    {s.x, s.table, s.targets, s.lse, {grads->d_dloss, args->tokens, 4, 4, "d_dloss"}}));
     TRY(check_workspace(args->workspace, args->workspace_bytes, loss_grad_bytes(*args, *grads)));
     TRY(need_device());
     HIP_TRY(launch_loss_grad(*args, *grads, (hipStream_t)stream));
