@@ -495,7 +495,8 @@ nsfps_status nsfps_norm_grad_device(const nsfps_norm_args *args, const nsfps_nor
 /* Dropout onto a residual, the mask made where it is used and never stored:
  *   y = residual + (kept ? x / (1 - p) : 0)
  * (residual.p NULL: no residual).  Its gradient by x is the same call on dy
- * without residual, that by residual is dy.  Of a row's channels the eight from
+ * without residual; that by residual is dy inside the sequences and 0 past their
+ * ends, which the same call with p = 0 makes.  Of a row's channels the eight from
  * 8 k on take 16 bits each, low half first, of the four words of Philox 4x32-10
  * (Salmon, Moraes, Dror, Shaw, 2011) at counter (k, row's number b * length +
  * t, d_seed[1] low, high) and key (d_seed[0] low, high); a value is dropped
