@@ -458,7 +458,7 @@ nsfps_status nsfps_scan_step_device(const nsfps_step_args *args, void *stream);
  * the values behind them stay.  Pairs are (i, i + rotary_dim / 2), with
  * neighbours != 0 (2i, 2i + 1).  A token's position is the one of its sequence
  * (d_positions, below 0 as 0; NULL: 0) plus its row's number; angles are exact
- * to 2^-22 at any position.  Rows past a sequence's length are zeros.
+ * to 2^-22 at any position, for frequencies of up to 2^40.  Rows past a sequence's length are zeros.
  *
  * q and q_out: rows of q_heads * head_dim; k and k_out: rows of k_heads *
  * head_dim, all of type dtype (one of the two may have no heads).  Weights

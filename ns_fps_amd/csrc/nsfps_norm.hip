@@ -115,12 +115,20 @@ __device__ __forceinline__ void store_pair(T *head, const Slots<V> &s, const flo
   if (s.two) store_f32<T, V>(head + s.second, b);
 }
 
-// Cosine and sine of position * freq.  The turns are found in float64: 31 bits
-// of a position and 24 of a frequency leave an angle's error at 2^-22 for the
-// farthest position, where float32 would have lost the angle whole.
+// Cosine and sine of position * freq.  Whole turns drop out, so what counts is the
+// angle's error in radians: with products in float64 alone it was 2^-20 at the farthest
+// position and freq 1, 2^-10 at freq 1,000.  Therefore angle and 1 / (2 pi) are two
+// float64 each, and the turns the sum of their products' parts: off by 2^-32 radians at
+// freq 2^40, less below, beside the 2^-23 that float32 leaves of half a turn.  (The
+// norms of the case above take as long with either.)
 __device__ __forceinline__ void turn(double position, float freq, float &c, float &s) {
-  const double t = position * (double)freq * 0.15915494309189533577;  // 1 / (2 pi)
-  sincospif(2.f * (float)(t - rint(t)), &s, &c);
+#pragma clang fp contract(off)
+  constexpr double kTurn = 0x1.45f306dc9c883p-3, kLow = -0x1.6b01ec5417056p-57;  // 1 / (2 pi)
+  const double f = (double)freq, angle = position * f, rest = fma(position, f, -angle);
+  const double turns = angle * kTurn;
+  double t = (turns - rint(turns)) + (fma(angle, kTurn, -turns) + fma(angle, kLow, rest * kTurn));
+  t -= rint(t);
+  sincospif(2.f * (float)t, &s, &c);
 }
 
 __device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
