@@ -466,8 +466,9 @@ nsfps_status nsfps_scan_step_device(const nsfps_step_args *args, void *stream);
  * head_dim at most 256, rotary_dim even and at most head_dim (0: no
  * rotation), eps above 0; (q_heads + k_heads) * head_dim at most 2^24; batch *
  * length at most 2^31 - 1.  A head whose sum of squares passes float32 (values
- * near 10^19) becomes zeros.  In place: q_out may be q's rows and k_out k's, and
- * of the gradient dq those of q or dq_out, dk those of k or dk_out.
+ * near 10^19) becomes zeros, and so does its gradient.  In place: q_out may be
+ * q's rows and k_out k's, and of the gradient dq those of q or dq_out, dk those
+ * of k or dk_out.
  *
  * The gradient takes those of q_out and k_out and writes all of dq and dk
  * (type dtype), and d_dq_weight and d_dk_weight ([head_dim] float32, or NULL);

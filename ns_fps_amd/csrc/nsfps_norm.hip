@@ -366,7 +366,9 @@ __global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict_
                        fmaf(v * (is_k ? wkb[q][i] : wqb[q][i]), xb[q][i], along));
         }
       const float r = rsqrtf(fmaf(group_sum(squares, a.lanes), inv, a.eps));
-      const float back = group_sum(along, a.lanes) * inv * r * r;
+      // (a head whose squares pass float32 has a root of 0, and all of it is 0, though
+      // the other sum may have passed float32 too)
+      const float dot = group_sum(along, a.lanes), back = r > 0.f ? dot * inv * r * r : 0.f;
 #pragma unroll
       for (int q = 0; q < S; ++q) {
         float da[V], db[V];
