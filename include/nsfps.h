@@ -471,7 +471,8 @@ nsfps_status nsfps_scan_step_device(const nsfps_step_args *args, void *stream);
  * of k or dk_out.
  *
  * The gradient takes those of q_out and k_out and writes all of dq and dk
- * (type dtype), and d_dq_weight and d_dk_weight ([head_dim] float32, or NULL);
+ * (type dtype), and d_dq_weight and d_dk_weight ([head_dim] float32, or NULL),
+ * whose sums are off by 2^-16 of the terms' sizes at most, however many tokens;
  * q_out and k_out are not read. */
 typedef struct {
   uint64_t batch, length;

@@ -289,9 +289,11 @@ __global__ __launch_bounds__(256) void k_norm(NormDev a) {
   }
 }
 
-// The weights' sums stay in registers over a group's items, are added in a
-// workgroup through LDS in the groups' order, and k_norm_join adds the
-// workgroups' sums in theirs.  parts: [workgroups][2][head_dim].
+// The weights' sums stay in registers over a group's items, of kTerms heads at most
+// (norm_blocks), so that a sum is off by kTerms 2^-24 of its terms' sizes whatever the
+// tokens; they are added in a workgroup through LDS in the groups' order, and
+// k_norm_join adds the workgroups' sums in theirs, both in float64.  parts:
+// [workgroups][2][head_dim].
 template <typename T, int V, int S>
 __global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict__ parts) {
   __shared__ float s_sum[256 * 2 * S * V];
@@ -403,9 +405,9 @@ __global__ __launch_bounds__(256) void k_norm_grad(NormDev a, float *__restrict_
     }
     __syncthreads();
     for (uint32_t e = threadIdx.x; e < d; e += 256) {
-      float sum = 0.f;
+      double sum = 0.;
       for (uint32_t g = 0; g < groups; ++g) sum += s_sum[g * d + e];
-      parts[((uint64_t)blockIdx.x * 2 + side) * d + e] = sum;
+      parts[((uint64_t)blockIdx.x * 2 + side) * d + e] = (float)sum;
     }
   }
 }
@@ -438,6 +440,7 @@ __global__ __launch_bounds__(256) void k_norm_join(const float *__restrict__ par
 }
 
 constexpr uint32_t kGradBlocks = 1024;
+constexpr uint32_t kTerms = 256;  // heads that a lane adds one after another
 
 NormDev norm_dev(const nsfps_norm_args &a) {
   NormDev d = {};
@@ -482,7 +485,7 @@ uint32_t norm_vector(const nsfps_norm_args &a, std::initializer_list<const nsfps
   return v;
 }
 
-void norm_split(NormDev &d, uint64_t tokens, uint32_t v) {
+void norm_split(NormDev &d, uint64_t tokens, uint32_t v, uint32_t most = ~0u) {
   const uint32_t slots = d.half + d.rest;
   uint32_t lanes = 1;
   while (lanes < 64 && lanes * v < slots) lanes *= 2;
@@ -493,7 +496,8 @@ void norm_split(NormDev &d, uint64_t tokens, uint32_t v) {
   // 125 with all heads an item)
   constexpr uint64_t kFill = 256 * 1024;  // threads
   const uint32_t heads = d.q_heads + d.k_heads;
-  const uint64_t want = std::max<uint64_t>(1, kFill / std::max<uint64_t>(1, tokens * lanes));
+  const uint64_t want = std::max<uint64_t>(host_ceil_div(heads, most),
+                                           kFill / std::max<uint64_t>(1, tokens * lanes));
   d.chunks = (uint32_t)std::min<uint64_t>(heads, want);
   d.per = (heads + d.chunks - 1) / d.chunks;
   d.chunks = (heads + d.per - 1) / d.per;
@@ -520,6 +524,16 @@ uint32_t norm_grid(const NormDev &d, uint64_t most) {
   return (uint32_t)std::min<uint64_t>(most, host_ceil_div(d.items, 256 / d.lanes));
 }
 
+// Workgroups of the gradient: kGradBlocks at most, or as many as leave a group kTerms
+// heads (an item has no more of them, by norm_split).  us of norms and gradient of
+// 16 x 65,536 rows of 8 + 8 heads of 64 bfloat16, single values: 4,739 so, 5,623 with
+// kGradBlocks alone; of 64 x 16,384 in vectors, where kGradBlocks are enough, 2,092.
+uint64_t norm_blocks(const NormDev &d) {
+  const uint64_t groups = 256 / d.lanes, items = std::max<uint64_t>(1, kTerms / d.per);
+  return std::max(std::min<uint64_t>(kGradBlocks, host_ceil_div(d.items, groups)),
+                  host_ceil_div(d.items, groups * items));
+}
+
 }  // namespace
 
 hipError_t launch_norm(const nsfps_norm_args &a, hipStream_t st) {
@@ -536,8 +550,15 @@ hipError_t launch_norm(const nsfps_norm_args &a, hipStream_t st) {
   });
 }
 
+// Of whichever vector the rows' addresses allow.
 uint64_t norm_grad_bytes(const nsfps_norm_args &a) {
-  return 4ull * kGradBlocks * 2 * a.head_dim;
+  uint64_t blocks = kGradBlocks;
+  for (uint32_t v = 1; v <= 8; v *= 2) {
+    NormDev d = norm_dev(a);
+    norm_split(d, a.batch * a.length, v, kTerms);
+    blocks = std::max(blocks, norm_blocks(d));
+  }
+  return 4 * blocks * 2 * a.head_dim;
 }
 
 hipError_t launch_norm_grad(const nsfps_norm_args &a, const nsfps_norm_grads &g, hipStream_t st) {
@@ -550,8 +571,8 @@ hipError_t launch_norm_grad(const nsfps_norm_args &a, const nsfps_norm_grads &g,
   const bool q = a.q_heads != 0, k = a.k_heads != 0;
   const uint32_t v = norm_vector(a, {q ? &a.q : &none, q ? &g.dq : &none, q ? &g.dq_out : &none,
                                      k ? &a.k : &none, k ? &g.dk : &none, k ? &g.dk_out : &none});
-  norm_split(d, a.batch * a.length, v);
-  const uint32_t blocks = d.items ? norm_grid(d, kGradBlocks) : 0;
+  norm_split(d, a.batch * a.length, v, kTerms);
+  const uint32_t blocks = (uint32_t)norm_blocks(d);
   float *const parts = (float *)a.workspace;
   hipError_t e = hipSuccess;
   if (blocks)
