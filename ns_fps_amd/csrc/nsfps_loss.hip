@@ -29,6 +29,7 @@
 #include "nsfps_product.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #pragma clang fp contract(fast)
@@ -88,6 +89,7 @@ struct LogitDev {
   Matrix x, e;                // e: the piece (x may be padded)
   Tiling tiles;
   float scale2;               // scale * log2(e)
+  double to_2;                // exponents of an lse: scale2 / scale
   // statistics
   float2 *parts;              // [sweeps][part_stride]: maximum and sum, in powers of two
   uint64_t part_stride;
@@ -288,15 +290,21 @@ __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s
   m = top;
 }
 
+// What exponents are, in powers of two, of a logit without its scale (not 0: -infinity
+// times 0 would be NaN).
+__host__ __device__ __forceinline__ float exponent_by(float scale2) {
+  return fmaxf(fabsf(scale2), 1e-38f);
+}
+
 // Running maximum and sum of a lane's columns, for its tokens.
 template <typename Prod>
 struct Stats {
   const LogitDev &a;
-  const float by;  // (-infinity times 0 would be NaN)
+  const float by;
   float top[Prod::kMT], sum[Prod::kMT];
 
   __device__ __forceinline__ explicit Stats(const LogitDev &args)
-      : a(args), by(fmaxf(fabsf(args.scale2), 1e-38f)) {
+      : a(args), by(exponent_by(args.scale2)) {
 #pragma unroll
     for (int i = 0; i < Prod::kMT; ++i) top[i] = -INFINITY, sum[i] = 0.f;
   }
@@ -377,7 +385,7 @@ __device__ __forceinline__ float value(const Eight<T> &v, int k) {
 template <typename T>
 __global__ __launch_bounds__(256) void k_loss_join(const float2 *__restrict__ parts, uint32_t nparts,
                                                    uint64_t part_stride, uint32_t group, Matrix x,
-                                                   Matrix table, float scale,
+                                                   Matrix table, float scale, double to_e,
                                                    const int32_t *__restrict__ targets,
                                                    float *__restrict__ loss,
                                                    float *__restrict__ lse) {
@@ -418,10 +426,16 @@ __global__ __launch_bounds__(256) void k_loss_join(const float2 *__restrict__ pa
       float2 v = s_part[0][i];
 #pragma unroll
       for (int k = 1; k < 4; ++k) join_stats(v.x, v.y, s_part[k][i].x, s_part[k][i].y);
-      const float all = (v.x + log2f(v.y)) * kLn2;
+      // In float64, for the logits may be far above the loss.  The largest exponent gets
+      // back its logit by to_e, the inverse of by (Stats) with by's rounding; the sum's
+      // exponents keep that rounding, 2^-24 of how far the logits lie below the largest.
+      int power;
+      const float part = frexpf(v.y, &power);
+      const double all = (v.x == -INFINITY ? -INFINITY : v.x * to_e) +
+                         (power + (double)log2f(part)) * 0.693147180559945309417;
       if (own == 0) {
-        lse[token] = all;
-        loss[token] = target < table.rows ? all - scale * dot : 0.f;
+        lse[token] = (float)all;
+        loss[token] = target < table.rows ? (float)(all - (double)scale * dot) : 0.f;
       }
     }
     __syncthreads();
@@ -444,7 +458,7 @@ struct Derivatives {
 #pragma unroll
     for (int i = 0; i < Prod::kMT; ++i) {
       const uint32_t token = token0 + 16 * i, at = a.weights.in(token);
-      const float lse = a.lse[at] * kLog2e,
+      const float lse = (float)(a.lse[at] * a.to_2),
                   own = a.weights.dloss[at] * a.weights.scale / reference;
       counts[i] = a.weights.counts(token);
       lse2[i] = counts[i] ? lse : 0.f;
@@ -917,6 +931,7 @@ LogitDev logits(const nsfps_loss_args &a, const Matrix &x, const Matrix &e, uint
   d.e = e;
   d.tiles = tiling(x_rows, e_rows, tile);
   d.scale2 = a.scale * kLog2e;
+  d.to_2 = std::fabs(a.scale) < 1e-30f ? kLog2e : (double)d.scale2 / a.scale;
   d.row0 = (uint32_t)row0;
   d.lse = a.d_lse;
   return d;
@@ -1192,6 +1207,7 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
       });
     LAUNCH(rc);
   }
+  const double to_e = std::fabs((double)a.scale) / exponent_by(a.scale * kLog2e);
   const auto join = [&](auto t) {
     // as many workgroups as fill the chip (us of 7 tokens x 262,144 rows 30, 46 with
     // 16 tokens a workgroup; with gradient 16,384 x 8,192 x 64 220, 235 with one)
@@ -1200,7 +1216,7 @@ hipError_t launch_loss(const nsfps_loss_args &a, hipStream_t st) {
     const uint32_t grid = (uint32_t)std::min<uint64_t>(1u << 16, host_ceil_div(a.tokens, group));
     k_loss_join<decltype(t)><<<grid, 256, 0, st>>>(
         (const float2 *)(ws + p.parts), (uint32_t)p.nparts, stride, group, x_of(a),
-        table_of(a, 0, a.rows), a.scale, a.d_targets, a.d_loss, a.d_lse);
+        table_of(a, 0, a.rows), a.scale, to_e, a.d_targets, a.d_loss, a.d_lse);
     return hipGetLastError();
   };
   return a.dtype == NSFPS_F32 ? join(float()) : join(bf16());
