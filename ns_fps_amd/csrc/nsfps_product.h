@@ -110,11 +110,12 @@ struct Feed {
     const uint64_t base = (uint64_t)from;
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-      // (m0 is set where it is used, here and by the compiler; a scalar register that
-      // the vector unit wrote may be read five states later)
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+      // (the compiler sets m0 itself, so that it knows what is there, but counts no
+      // waits into these instructions: a scalar register that the vector unit wrote may
+      // be read five states later, m0 one)
+      asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
                    :
-                   : "v"(at[i]), "s"(base), "s"(to + 16 * kThreads * i)
+                   : "v"(at[i]), "s"(base), "{m0}"(to + 16 * kThreads * i)
                    : "memory");
   }
 };
