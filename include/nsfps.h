@@ -534,7 +534,8 @@ nsfps_status nsfps_dropout_device(const nsfps_dropout_args *args, void *stream);
  * products in bfloat16 where the result is bfloat16, with 16 bits for a float32
  * table gradient of bfloat16 inputs, with 24 in float32 calls.
  *
- * A row of the table that is not finite spoils every token.  At most 2^30
+ * scale and scale * log2(e) have to be finite.  A row of the table that is not
+ * finite spoils every token.  At most 2^30
  * tokens, 2^31 - 1 rows, width at most 65,536.  The gradient takes the
  * vocabulary in pieces, whose products live in the workspace, beside copies of
  * rows that the kernels cannot take as they are; its size goes by sizes and types

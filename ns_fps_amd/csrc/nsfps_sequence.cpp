@@ -430,7 +430,9 @@ nsfps_status check_row_stride(uint64_t stride, uint64_t rows, uint64_t width, co
 
 nsfps_status check_loss(const nsfps_loss_args *a, bool grad) {
   TRY(check_loss_sizes(a));
-  if (!std::isfinite(a->scale)) return fail(NSFPS_EINVAL, "scale must be finite");
+  // (logits are found in powers of two)
+  if (!std::isfinite(a->scale) || !std::isfinite(a->scale * 1.44269504f))
+    return fail(NSFPS_EINVAL, "scale and scale * log2(e) must be finite");
   TRY(check_row_stride(a->x_stride, a->tokens, a->width, "x_stride"));
   TRY(check_row_stride(a->table_stride, a->rows, a->width, "table_stride"));
   if (a->rows) TRY(check_pointer(a->d_table, size_of(a->dtype), "d_table"));
