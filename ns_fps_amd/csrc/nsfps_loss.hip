@@ -312,7 +312,7 @@ struct Stats {
   __device__ __forceinline__ bool plain(uint32_t tile) const {
     return (tile + 1) * Prod::kN <= a.e.rows && a.scale2 >= 0.f;
   }
-  __device__ __forceinline__ void part(const typename Prod::Sum &z, uint32_t, int i) {
+  __device__ __forceinline__ void part(const typename Prod::Sum &z, int i) {
     float m = z[i][0][0];
 #pragma unroll
     for (int j = 0; j < Prod::kNT; ++j)
@@ -341,7 +341,7 @@ struct Stats {
           }
     }
 #pragma unroll
-    for (int i = 0; i < Prod::kMT; ++i) part(z, tile, i);
+    for (int i = 0; i < Prod::kMT; ++i) part(z, i);
   }
 };
 
@@ -495,11 +495,6 @@ struct Derivatives {
       for (int q = 0; q < V; ++q) o[q] = d[k + q];
       store_f32<D, V>(out + Prod::column(k / 4), o);
     }
-  }
-  __device__ __forceinline__ void part(const typename Prod::Sum &z, uint32_t tile, int i) const {
-    float d[4 * Prod::kNT];
-    values(z, i, d);
-    store(tile, i, d);
   }
   __device__ __forceinline__ void whole(const typename Prod::Sum &z, uint32_t tile) const {
     const bool simple = plain(tile);

@@ -5,7 +5,7 @@
 //
 // Operands in LDS are bfloat16; a float32 value is there as up to three terms
 // whose sum it is, in planes, and its products are those of the planes that
-// matter (kPasses).  Rows of a tile have no padding; the 16-byte pieces of a row
+// matter (Passes).  Rows of a tile have no padding; the 16-byte pieces of a row
 // are exchanged instead, by a number that the row gives (the turn), so that rows
 // which lanes read at once lie in different banks.  Reads of a Col tile transpose
 // on the way.
