@@ -9,8 +9,8 @@
 // the vector rate for products would else weigh more than the memory.
 //
 // Memory is the bound: 64 x 4,096 rows of 640 bfloat16, three quarters of them
-// inside, onto a residual and its gradient: 288 us together, 5.0 TB/s read and
-// written.
+// inside, onto a residual 150 us, its gradient 132, one after the other 286: 5.0 TB/s
+// read and written.
 #include "nsfps_launch.h"
 #include "nsfps_seq_device.h"
 
@@ -71,7 +71,7 @@ __device__ __forceinline__ float dropped(float x, float r, bool keep, float fact
 
 // A lane writes the places that it has read: y may be the rows of x or residual.
 // kWideRows: a lane has a block of eight values, in 16-byte accesses (the case above
-// 287 us, 684 the other way).  Else a wave makes the masks of 64 blocks, a lane each,
+// 286 us, 684 the other way).  Else a wave makes the masks of 64 blocks, a lane each,
 // and takes their 512 values 64 neighbours at a time, each lane asking for the mask of
 // its value's block (16,384 rows of 323 float32: 10.8 us, 3.9 TB/s).
 template <typename T, bool kWideRows>

@@ -14,16 +14,21 @@
 // terms that reach 24 bits.  d is rounded to one term (8 bits) where the
 // products' results are bfloat16, to two for a float32 table gradient of
 // bfloat16 inputs, to three in float32 calls.  Sums are float32 everywhere.
+// (Two terms for bfloat16 results too, through registers: the error against 64 bits
+// goes from 0.0019 to 0.0017 of the norm at 77 tokens x 313 rows, where probabilities
+// are not small, from 0.00165 to 0.00164 at 30 x 19,106; the time from 24.5 to 24.5
+// and from 67 to 76 us, at 46 x 241,327 x 79 from 130 to 163.  One is what a result of
+// 8 bits is worth.)
 //
 // The matrix cores bound large calls: the statistics of 16,384 tokens, 262,144
 // rows of 256 bfloat16 take 1.96 ms, 1.12 PFLOP/s, as fast as a plain product of
-// 8,192^3 (1.13).  Their gradient takes 64 pieces of 4,096 rows: d 62 us (30 of
-// them the product, 18 the 134 MB that it writes, the rest the start of its
-// workgroups), the two products that read it 70 us (0.98 PFLOP/s), the sums' rows
-// 5.6 us.  64 million values of d a piece: 32, 128 and 256 million were no faster,
+// 8,192^3 (1.13).  Their gradient takes 64 pieces of 4,096 rows: d 62 to 64 us by card
+// (its product alone would take 30 at that rate, the 134 MB that it writes 26 at a
+// copy's), the two products that read it 70 to 76 us (0.98 to 0.92 PFLOP/s), the sums'
+// rows 5.5 us.  64 million values of d a piece: 32, 128 and 256 million were no faster,
 // and more than 128 million would not stay in the memory-side cache.  A float32
 // call's six products a product: 16,384 tokens, 8,192 rows, width 383 in 2.3 ms,
-// where float32 matrix instructions would need 2.7.  A table's one reading bounds
+// (2.4 on a slower card), where float32 matrix instructions would need 2.7.  A table's one reading bounds
 // calls of few tokens: 7 tokens, 262,144 rows of 256 bfloat16 26 us, 5.1 TB/s.
 #include "nsfps_launch.h"
 #include "nsfps_product.h"
@@ -290,8 +295,8 @@ __device__ __forceinline__ void join_stats(float &m, float &s, float m2, float s
   m = top;
 }
 
-// What exponents are, in powers of two, of a logit without its scale (not 0: -infinity
-// times 0 would be NaN).
+// The factor that makes a power of two's exponent of a logit without its scale, and
+// without its sign.  (Not 0: -infinity times 0 would be NaN.)
 __host__ __device__ __forceinline__ float exponent_by(float scale2) {
   return fmaxf(fabsf(scale2), 1e-38f);
 }

@@ -13,9 +13,9 @@
 // others: outputs may be the inputs' own rows.
 //
 // Memory is the bound: 64 x 4,096 rows of 2 x 8 heads of 64, bfloat16, three
-// quarters of them inside their sequences: norms 208 us (4.5 TB/s read and
-// written), gradient 330 us (4.1 TB/s).  One token of 512 requests: 5.0 us, mostly
-// the launch.
+// quarters of them inside their sequences: norms 210 us (4.5 TB/s read and
+// written), gradient 306 us (4.4 TB/s), one after the other 518.  One token of 512
+// requests: 5.1 us, mostly the launch.
 #include "nsfps_launch.h"
 #include "nsfps_seq_device.h"
 
@@ -466,7 +466,7 @@ NormDev norm_dev(const nsfps_norm_args &a) {
 }
 
 // Slots of a vector: as many as the rotation, the head and every address keep
-// aligned, at most 16 bytes (us of norms and gradient of the case above: 520 with 8
+// aligned, at most 16 bytes (us of norms and gradient of the case above: 518 with 8
 // bfloat16 values, 1,366 with single ones).
 uint32_t norm_vector(const nsfps_norm_args &a, std::initializer_list<const nsfps_rows *> rows) {
   const uint32_t size = a.dtype == NSFPS_F32 ? 4 : 2;
@@ -491,7 +491,7 @@ void norm_split(NormDev &d, uint64_t tokens, uint32_t v, uint32_t most = ~0u) {
   while (lanes < 64 && lanes * v < slots) lanes *= 2;
   d.lanes = lanes;
   // heads of an item: all, so that a token's angles, in float64, are found once (us of
-  // norms and gradient of the case above 520, 831 with a head an item), unless tokens
+  // norms and gradient of the case above 518, 831 with a head an item), unless tokens
   // are too few to fill the chip (a call of one token of 64 + 64 heads of 128: 9.7,
   // 125 with all heads an item)
   constexpr uint64_t kFill = 256 * 1024;  // threads

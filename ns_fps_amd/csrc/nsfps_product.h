@@ -31,8 +31,9 @@ namespace seq {
 // read takes 16 lanes at a time, rows 0 .. 3 and 12 .. 15 of one piece and rows 4
 // .. 11 of the next one (then the other way round), over 256 bytes of banks.  One,
 // two or four rows lie in those, so the others' bits have to give the piece, and
-// with the pieces' own difference: counted, no read meets a bank twice, be its rows 0 ..
-// 15 or (kPerm) 8a + 4c + b (a, b < 4).
+// with the pieces' own difference: by count no read meets a bank twice, be its rows 0 ..
+// 15 or (kPerm) 8a + 4c + b (a, b < 4), and the hardware's counter of conflicts stays
+// at 0 in every kernel of the loss.
 template <int kTerms>
 __device__ __forceinline__ uint32_t row_turn(uint32_t r) {
   static_assert(kTerms == 128 || kTerms == 64 || kTerms == 32, "terms of a stage");
