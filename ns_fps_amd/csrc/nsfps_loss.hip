@@ -27,9 +27,9 @@
 // copy's), the two products that read it 70 to 76 us (0.98 to 0.92 PFLOP/s), the sums'
 // rows 5.5 us.  64 million values of d a piece: 32, 128 and 256 million were no faster,
 // and more than 128 million would not stay in the memory-side cache.  A float32
-// call's six products a product: 16,384 tokens, 8,192 rows, width 383 in 2.3 ms,
-// (2.4 on a slower card), where float32 matrix instructions would need 2.7.  A table's one reading bounds
-// calls of few tokens: 7 tokens, 262,144 rows of 256 bfloat16 26 us, 5.1 TB/s.
+// call's six products a product: 16,384 tokens, 8,192 rows, width 383 in 2.3 to 2.4
+// ms by card, where float32 matrix instructions would need 2.7.  A table's one reading
+// bounds calls of few tokens: 7 tokens, 262,144 rows of 256 bfloat16 27 us, 5.0 TB/s.
 #include "nsfps_launch.h"
 #include "nsfps_product.h"
 
